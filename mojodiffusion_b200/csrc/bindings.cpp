@@ -517,6 +517,126 @@ std::tuple<Tensor, Tensor, Tensor> attention_bwd(const Tensor& q, const Tensor& 
 }
 
 // ------------------------------------------------------------------------------------------
+// attention of the language models: sliding window / first tokens / sink logits, relative position buckets
+// ------------------------------------------------------------------------------------------
+// one of q, k, v, o and their gradients: bf16 [B, S, heads, Dh] with 16-byte rows. A dimension of one element takes any stride.
+void text_operand(const Tensor& t, const Tensor& like, int64_t S, int64_t heads, long long (&strides)[3], const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(0) == like.size(0) &&
+                  t.size(1) == S && t.size(2) == heads && t.size(3) == like.size(3) && t.stride(3) == 1,
+              "text attention: ", name, " must be bf16 [B, S, heads, Dh] on q's device with contiguous Dh");
+  for (int i = 0; i < 3; ++i) {
+    strides[i] = t.size(i) == 1 ? 8 : t.stride(i);
+    TORCH_CHECK(strides[i] % 8 == 0 && strides[i] > 0, "text attention: rows of ", name, " must start on 16-byte boundaries");
+  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "text attention: ", name, " must start on a 16-byte boundary");
+}
+const int* text_per_sequence(const optional<Tensor>& t, const Tensor& q, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->numel() == q.size(0),
+              "text attention: ", name, " must be [B] int32 on q's device");
+  return t->data_ptr<int>();
+}
+// masks and parameters that the forward and the backward pass share. rule: {causal, window, sinks, q_start}; buckets: {count, exact, borders ...} or empty
+void text_rule(MdbTextAttnArgs& a, const Tensor& q, const Tensor& k, double scale, const std::vector<int64_t>& rule, const optional<Tensor>& kv_len,
+               const optional<Tensor>& q_start, const optional<Tensor>& sink_logits, const optional<Tensor>& table, const std::vector<int64_t>& buckets) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) && k.size(2) > 0 && q.size(2) % k.size(2) == 0 && rule.size() == 4,
+              "text attention: q [B, Sq, H, Dh], k [B, Skv, Hkv, Dh], Dh 64 or 128, Hkv a divisor of H");
+  for (int i = 1; i < 3; ++i) TORCH_CHECK(q.size(i) < (1ll << 30) && k.size(i) < (1ll << 30), "text attention: too many rows");
+  TORCH_CHECK(q.size(0) <= 65535 && q.size(2) <= 65535, "text attention: at most 65535 sequences and heads");
+  TORCH_CHECK(rule[1] >= 1 && rule[2] >= 0, "text attention: window and sinks");
+  const int64_t far = 1 << 30;
+  a.B = (int)q.size(0); a.Sq = (int)q.size(1); a.H = (int)q.size(2); a.Dh = (int)q.size(3); a.Skv = (int)k.size(1); a.Hkv = (int)k.size(2);
+  a.causal = rule[0] != 0;
+  a.window = (int)std::min(rule[1], far);
+  a.sinks = (int)std::min(rule[2], far);
+  a.q_start = (int)std::max(std::min(rule[3], far), -far);
+  a.scale = (float)scale;
+  a.kv_len = text_per_sequence(kv_len, q, "kv_len");
+  a.q_start_ptr = text_per_sequence(q_start, q, "q_start");
+  for (const optional<Tensor>* t : {&sink_logits, &table}) {
+    if (!t->has_value() || !(*t)->defined()) continue;
+    const Tensor& p = **t;
+    const bool is_table = t == &table;
+    TORCH_CHECK(p.is_cuda() && p.device() == q.device() && p.is_contiguous() && (p.scalar_type() == at::kFloat || p.scalar_type() == at::kBFloat16) &&
+                    p.numel() == a.H * (is_table ? (buckets.empty() ? 0 : buckets[0]) : 1),
+                "text attention: ", is_table ? "table must be [buckets, H]" : "sink_logits must be [H]", ", fp32 or bf16, on q's device");
+    a.param_f32 = p.scalar_type() == at::kFloat;
+    (is_table ? a.table : a.sink_logits) = p.data_ptr();
+  }
+  TORCH_CHECK(a.table == nullptr || a.sink_logits == nullptr, "text attention: a table or sink logits");
+  if (a.table != nullptr) {
+    TORCH_CHECK(buckets.size() >= 2 && buckets[0] <= MDB_TEXT_MAX_BUCKETS && (int64_t)buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 4, "text attention: buckets");
+    a.buckets = (int)buckets[0];
+    a.exact = (int)buckets[1];
+    a.n_borders = (int)buckets.size() - 2;
+    for (int i = 0; i < a.n_borders; ++i) a.borders[i] = (int)buckets[i + 2];
+  }
+  a.status = status_ptr(q);
+}
+
+std::tuple<Tensor, Tensor> text_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, std::vector<int64_t> rule,
+                                              const optional<Tensor>& kv_len, const optional<Tensor>& q_start, const optional<Tensor>& sink_logits,
+                                              const optional<Tensor>& table, std::vector<int64_t> buckets, bool need_lse, const optional<Tensor>& out) {
+  TORCH_CHECK(q.is_cuda(), "text attention: CUDA tensors");
+  c10::cuda::CUDAGuard guard(q.device());
+  MdbTextAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  text_rule(a, q, k, scale, rule, kv_len, q_start, sink_logits, table, buckets);
+  Tensor o = out.has_value() && out->defined() ? *out : at::empty({a.B, a.Sq, a.H, a.Dh}, q.options());
+  text_operand(q, q, a.Sq, a.H, a.q_strides, "q");
+  text_operand(k, q, a.Skv, a.Hkv, a.k_strides, "k");
+  text_operand(v, q, a.Skv, a.Hkv, a.v_strides, "v");
+  text_operand(o, q, a.Sq, a.H, a.o_strides, "out");
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr();
+  Tensor lse;
+  if (need_lse) {
+    lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
+    a.lse = lse.data_ptr<float>();
+  }
+  check_rc(mdb_text_attention_fwd(&a, cur_stream()), "text_attention_fwd");
+  return {o, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> text_attention_bwd(
+    const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& dout, double scale, std::vector<int64_t> rule,
+    const optional<Tensor>& kv_len, const optional<Tensor>& q_start, const optional<Tensor>& sink_logits, const optional<Tensor>& table,
+    std::vector<int64_t> buckets, bool need_param) {
+  TORCH_CHECK(q.is_cuda(), "text attention: CUDA tensors");
+  c10::cuda::CUDAGuard guard(q.device());
+  MdbTextAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  text_rule(a, q, k, scale, rule, kv_len, q_start, sink_logits, table, buckets);
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.H * a.Sq, "text attention: lse");
+  Tensor dq = at::empty({a.B, a.Sq, a.H, a.Dh}, q.options());
+  Tensor dk = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options()), dv = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options());
+  text_operand(q, q, a.Sq, a.H, a.q_strides, "q");
+  text_operand(k, q, a.Skv, a.Hkv, a.k_strides, "k");
+  text_operand(v, q, a.Skv, a.Hkv, a.v_strides, "v");
+  text_operand(o, q, a.Sq, a.H, a.o_strides, "out");
+  text_operand(dout, q, a.Sq, a.H, a.do_strides, "the output's gradient");
+  text_operand(dq, q, a.Sq, a.H, a.dq_strides, "dq");
+  text_operand(dk, q, a.Skv, a.Hkv, a.dk_strides, "dk");
+  text_operand(dv, q, a.Skv, a.Hkv, a.dv_strides, "dv");
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr(); a.dout = dout.data_ptr();
+  a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  Tensor delta = at::empty({a.B, a.H, a.Sq}, lse.options()), dtable, dsink, ws;
+  a.delta = delta.data_ptr<float>();
+  if (need_param && a.table != nullptr) {
+    dtable = at::empty_like(*table);
+    a.d_table = dtable.data_ptr();
+    ws = at::empty({mdb_text_attention_bwd_floats(&a)}, lse.options());
+    a.table_ws = ws.data_ptr<float>();
+  }
+  if (need_param && a.sink_logits != nullptr) {
+    dsink = at::empty_like(*sink_logits);
+    a.d_sink = dsink.data_ptr();
+  }
+  check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");
+  return {dq, dk, dv, dtable, dsink};
+}
+
+// ------------------------------------------------------------------------------------------
 // norm / rope
 // ------------------------------------------------------------------------------------------
 Tensor norm_modulate_fwd(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
@@ -1313,6 +1433,8 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("pad_channels", &pad_channels);
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
+  m.def("text_attention_fwd", &text_attention_fwd);
+  m.def("text_attention_bwd", &text_attention_bwd);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);
   m.def("qk_norm_rope", &qk_norm_rope);

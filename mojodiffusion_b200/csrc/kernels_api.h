@@ -209,6 +209,36 @@ typedef struct MdbAttnBwdArgs {
 } MdbAttnBwdArgs;
 int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 
+// ---- text_attention.cu
+// q, o, dout, dq: [B, Sq, H, Dh]; k, v, dk, dv: [B, Skv, Hkv, Dh], Hkv divides H, Dh 64 or 128; strides (batch, seq, head) in elements, multiples of
+// 8, addresses multiples of 16 bytes. Key j is seen by the query at position p = q_start + row when j < kv_len and, with `causal`,
+// j <= p and (p - j < window or j < sinks). lse, delta: fp32 [B, H, Sq]; delta and table_ws are workspaces of the backward pass.
+#define MDB_TEXT_MAX_BUCKETS 128
+#define MDB_TEXT_MAX_DISTANCE 1024
+typedef struct MdbTextAttnArgs {
+  const void* q; const void* k; const void* v; void* o;
+  const void* dout; void* dq; void* dk; void* dv;
+  float* lse; float* delta;
+  const int* kv_len;          // [B] or null: all keys
+  const int* q_start_ptr;     // [B], or null: q_start for all
+  const void* sink_logits;    // [H] or null
+  const void* table;          // [buckets, H] or null
+  void* d_sink; void* d_table;
+  float* table_ws;            // mdb_text_attention_bwd_floats values when d_table is given
+  long long q_strides[3], k_strides[3], v_strides[3], o_strides[3], do_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+  int B, H, Hkv, Sq, Skv, Dh;
+  int q_start, causal, window, sinks;
+  int param_f32;              // type of sink_logits / table and their gradients: 0 bf16, 1 fp32
+  // relative position buckets: distances below `exact` have one each, distance n >= exact the bucket exact + (borders <= n); half of the buckets per direction
+  int buckets, exact, n_borders;
+  int borders[MDB_TEXT_MAX_BUCKETS / 4];
+  float scale;
+  int* status;
+} MdbTextAttnArgs;
+int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st);
+long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a);
+int mdb_text_attention_bwd(const MdbTextAttnArgs* a, cudaStream_t st);
+
 #ifdef __cplusplus
 }
 #endif

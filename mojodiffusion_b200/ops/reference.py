@@ -228,6 +228,76 @@ def attention(q, k, v, scale: Optional[float] = None, kv_len: Optional[torch.Ten
     return o
 
 
+def _grouped_softmax_attention(q, k, v, scale, seen, bias=None, sink_logits=None):
+    """Grouped-query attention over the keys that ``seen`` [B or 1, Sq, Skv] allows, plus ``bias`` [H, Sq, Skv]; ``sink_logits`` [H] take
+    part in the softmax without a value. A row without a key and without a sink logit is zero. Masked keys and values are not read."""
+    B, Sq, H, Dh = q.shape
+    Skv, G = k.shape[1], k.shape[2]
+    wide = torch.promote_types(q.dtype, torch.float32)
+    used = seen.any(1)[:, :, None, None]                              # keys that no query sees may hold anything
+    k, v = torch.where(used, k, 0).to(wide), torch.where(used, v, 0).to(wide)
+    s = torch.einsum("bqgrd,bkgd->bgrqk", q.to(wide).reshape(B, Sq, G, H // G, Dh), k).reshape(B, H, Sq, Skv) * scale
+    if bias is not None:
+        s = s + bias
+    s = s.masked_fill(~seen[:, None], float("-inf"))
+    sink = s.new_full((H,), float("-inf")) if sink_logits is None else sink_logits.to(wide)
+    s = torch.cat((s, sink[None, :, None, None].expand(B, H, Sq, 1)), -1)
+    top = s.detach().amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
+    total = e.sum(-1, keepdim=True)
+    p = (e / torch.where(total == 0, 1.0, total))[..., :-1]
+    return torch.einsum("bgrqk,bkgd->bqgrd", p.reshape(B, G, H // G, Sq, Skv), v).reshape(B, Sq, H, Dh).to(q.dtype)
+
+
+def window_attention(q, k, v, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
+                     kv_len: Optional[torch.Tensor] = None, q_start=0, sink_logits: Optional[torch.Tensor] = None):
+    """q [B, Sq, H, Dh], k / v [B, Skv, Hkv, Dh]; query row i at position p = q_start + i sees key j < kv_len when j <= p and
+    (p - j < window or j < sinks)."""
+    key = torch.arange(k.shape[1], device=q.device)
+    at = torch.arange(q.shape[1], device=q.device)
+    at = (q_start.long()[:, None] + at if isinstance(q_start, torch.Tensor) else (q_start + at)[None])[:, :, None]
+    seen = key <= at
+    if window is not None:
+        seen = seen & ((at - key < window) | (key < sinks))
+    if kv_len is not None:
+        seen = seen & (key < kv_len.long()[:, None, None])
+    return _grouped_softmax_attention(q, k, v, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), seen, None, sink_logits)
+
+
+def bucket_borders(num_buckets: int, max_distance: int):
+    """(single, borders) of the bidirectional buckets: half of the buckets per direction; distances below ``single`` have one each, the m
+    others end at distances that grow by equal factors up to ``max_distance``. A distance n >= single lies in the k-th or a later one of them
+    when floor(m log(n / single) / log(max_distance / single)) >= k, here without rounding: n^m single^k >= max_distance^k single^m."""
+    half = num_buckets // 2
+    single = half // 2
+    m = half - single
+    borders, n = [], single
+    for k in range(1, m):
+        while n ** m * single ** k < max_distance ** k * single ** m:
+            n += 1
+        borders.append(n)
+    return single, borders
+
+
+def relative_bucket(rel: torch.Tensor, num_buckets: int, max_distance: int) -> torch.Tensor:
+    """Bucket of every relative position (key minus query)."""
+    single, borders = bucket_borders(num_buckets, max_distance)
+    n = rel.abs()
+    far = single + torch.bucketize(n, torch.tensor(borders, dtype=n.dtype, device=n.device), right=True)
+    return torch.where(n < single, n, far) + torch.where(rel > 0, num_buckets // 2, 0)
+
+
+def relative_attention(q, k, v, table, max_distance: int = 128, scale: float = 1.0, kv_len: Optional[torch.Tensor] = None):
+    """q [B, Sq, H, Dh], k / v [B, Skv, Hkv, Dh], table [buckets, H]: score + table[bucket(j - i), h] over the keys j < kv_len."""
+    Sq, Skv = q.shape[1], k.shape[1]
+    key = torch.arange(Skv, device=q.device)
+    which = relative_bucket(key[None, :] - torch.arange(Sq, device=q.device)[:, None], table.shape[0], max_distance)
+    seen = torch.ones(1, Sq, Skv, dtype=torch.bool, device=q.device)
+    if kv_len is not None:
+        seen = seen & (key < kv_len.long()[:, None, None])
+    return _grouped_softmax_attention(q, k, v, scale, seen, table.t()[:, which].to(torch.promote_types(q.dtype, torch.float32)))
+
+
 def gate_residual(x, y, gate=None, rows_per_group: int = 1, tanh_gate: bool = False):
     """x + gate[g] * y over [rows, D] (gate None: x + y)."""
     if _library_mode(x) and not tanh_gate:
