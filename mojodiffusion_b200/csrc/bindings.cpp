@@ -536,20 +536,19 @@ const int* text_per_sequence(const optional<Tensor>& t, const Tensor& q, const c
               "text attention: ", name, " must be [B] int32 on q's device");
   return t->data_ptr<int>();
 }
-// masks and parameters that the forward and the backward pass share. rule: {causal, window, sinks, q_start}; buckets: {count, exact, borders ...} or empty
+// masks and parameters that the forward and the backward pass share. rule: {window, sinks, q_start}; buckets: {count, exact, borders ...} or empty
 void text_rule(MdbTextAttnArgs& a, const Tensor& q, const Tensor& k, double scale, const std::vector<int64_t>& rule, const optional<Tensor>& kv_len,
                const optional<Tensor>& q_start, const optional<Tensor>& sink_logits, const optional<Tensor>& table, const std::vector<int64_t>& buckets) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) && k.size(2) > 0 && q.size(2) % k.size(2) == 0 && rule.size() == 4,
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) && k.size(2) > 0 && q.size(2) % k.size(2) == 0 && rule.size() == 3,
               "text attention: q [B, Sq, H, Dh], k [B, Skv, Hkv, Dh], Dh 64 or 128, Hkv a divisor of H");
   for (int i = 1; i < 3; ++i) TORCH_CHECK(q.size(i) < (1ll << 30) && k.size(i) < (1ll << 30), "text attention: too many rows");
   TORCH_CHECK(q.size(0) <= 65535 && q.size(2) <= 65535, "text attention: at most 65535 sequences and heads");
-  TORCH_CHECK(rule[1] >= 1 && rule[2] >= 0, "text attention: window and sinks");
+  TORCH_CHECK(rule[0] >= 1 && rule[1] >= 0, "text attention: window and sinks");
   const int64_t far = 1 << 30;
   a.B = (int)q.size(0); a.Sq = (int)q.size(1); a.H = (int)q.size(2); a.Dh = (int)q.size(3); a.Skv = (int)k.size(1); a.Hkv = (int)k.size(2);
-  a.causal = rule[0] != 0;
-  a.window = (int)std::min(rule[1], far);
-  a.sinks = (int)std::min(rule[2], far);
-  a.q_start = (int)std::max(std::min(rule[3], far), -far);
+  a.window = (int)std::min(rule[0], far);
+  a.sinks = (int)std::min(rule[1], far);
+  a.q_start = (int)std::max(std::min(rule[2], far), -far);
   a.scale = (float)scale;
   a.kv_len = text_per_sequence(kv_len, q, "kv_len");
   a.q_start_ptr = text_per_sequence(q_start, q, "q_start");
@@ -1402,7 +1401,7 @@ void set_wait_limit_ns(int64_t ns) {
   TORCH_CHECK(ns > 0, "set_wait_limit_ns: positive nanoseconds");
   const unsigned long long v = static_cast<unsigned long long>(ns);
   const int rc = mdb_set_wait_limit_gemm(v) | mdb_set_wait_limit_attn_fwd(v) | mdb_set_wait_limit_attn_bwd(v) |
-                 mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v);
+                 mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v) | mdb_set_wait_limit_text_fwd(v);
   TORCH_CHECK(rc == 0, "set_wait_limit_ns failed: ", rc);
 }
 

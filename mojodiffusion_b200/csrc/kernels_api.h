@@ -211,8 +211,9 @@ int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 
 // ---- text_attention.cu
 // q, o, dout, dq: [B, Sq, H, Dh]; k, v, dk, dv: [B, Skv, Hkv, Dh], Hkv divides H, Dh 64 or 128; strides (batch, seq, head) in elements, multiples of
-// 8, addresses multiples of 16 bytes. Key j is seen by the query at position p = q_start + row when j < kv_len and, with `causal`,
-// j <= p and (p - j < window or j < sinks). lse, delta: fp32 [B, H, Sq]; delta and table_ws are workspaces of the backward pass.
+// 8, addresses multiples of 16 bytes. Without a table, key j is seen by the query at position p = q_start + row when j < kv_len, j <= p and
+// (p - j < window or j < sinks); with one, when j < kv_len. scale > 0. lse (base 2; +inf: a row that saw nothing), delta: fp32 [B, H, Sq]; delta and
+// table_ws are workspaces of the backward pass.
 #define MDB_TEXT_MAX_BUCKETS 128
 #define MDB_TEXT_MAX_DISTANCE 1024
 typedef struct MdbTextAttnArgs {
@@ -227,7 +228,7 @@ typedef struct MdbTextAttnArgs {
   float* table_ws;            // mdb_text_attention_bwd_floats values when d_table is given
   long long q_strides[3], k_strides[3], v_strides[3], o_strides[3], do_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
   int B, H, Hkv, Sq, Skv, Dh;
-  int q_start, causal, window, sinks;
+  int q_start, window, sinks;
   int param_f32;              // type of sink_logits / table and their gradients: 0 bf16, 1 fp32
   // relative position buckets: distances below `exact` have one each, distance n >= exact the bucket exact + (borders <= n); half of the buckets per direction
   int buckets, exact, n_borders;

@@ -7,40 +7,11 @@
 //   dtable[b, h] = sum of ds_ij over the pairs of the bucket;  dsink[h] = -sum_i exp(sink_h - lse_i) delta_i
 //
 // This is the plain form on CUDA cores: one warp per row, all sums in fp32.
-#include "common.cuh"
-#include "kernels_api.h"
+#include "text_attention.cuh"
 
 #include <string.h>
 
 namespace mdb {
-
-constexpr int TXT_FAR = 1 << 30;
-
-__device__ __forceinline__ float load_param(const void* p, int is_f32, long long i) {
-  return is_f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-__device__ __forceinline__ int bucket_of(const MdbTextAttnArgs& a, int rel) {
-  const int n = rel < 0 ? -rel : rel;
-  int c = n;
-  if (n >= a.exact) {
-    c = a.exact;
-    for (int i = 0; i < a.n_borders; ++i) c += n >= a.borders[i];
-  }
-  return c + (rel > 0 ? a.buckets / 2 : 0);
-}
-
-// what the keys of one batch entry and the position of a query allow
-struct Sight {
-  int valid, start;
-};
-__device__ __forceinline__ Sight sight_of(const MdbTextAttnArgs& a, int b) {
-  Sight s;
-  s.valid = a.kv_len != nullptr ? min(max(a.kv_len[b], 0), a.Skv) : a.Skv;
-  s.start = a.q_start_ptr != nullptr ? a.q_start_ptr[b] : a.q_start;
-  s.start = min(max(s.start, -TXT_FAR), TXT_FAR);
-  return s;
-}
 
 template <int DH> struct Row {
   static constexpr int N = DH / 32;
@@ -82,55 +53,16 @@ __device__ __forceinline__ long long at(const long long* st, int b, int s, int h
 }
 
 template <int DH>
-__global__ void text_fwd_kernel(const MdbTextAttnArgs a) {
-  const long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= static_cast<long long>(a.B) * a.H * a.Sq) return;
-  const int i = static_cast<int>(w % a.Sq), h = static_cast<int>((w / a.Sq) % a.H), b = static_cast<int>(w / (static_cast<long long>(a.Sq) * a.H));
-  const int g = h / (a.H / a.Hkv);
-  const Sight s = sight_of(a, b);
-  const int p = s.start + i;
-  const int hi = a.causal ? min(p + 1, s.valid) : s.valid;
-  const int lo = a.causal ? max(p - a.window + 1, 0) : 0;
-  Row<DH> q, o;
-  q.load(a.q, at(a.q_strides, b, i, h), lane);
-  o.zero();
-  float m = -INFINITY, l = 0.f;
-  if (a.sink_logits != nullptr) {
-    m = load_param(a.sink_logits, a.param_f32, h);
-    l = m == -INFINITY ? 0.f : 1.f;
-  }
-  for (int j = 0; j < hi; ++j) {
-    if (j >= a.sinks && j < lo) j = lo;
-    if (j >= hi) break;
-    Row<DH> k, v;
-    k.load(a.k, at(a.k_strides, b, j, g), lane);
-    v.load(a.v, at(a.v_strides, b, j, g), lane);
-    float x = q.dot(k) * a.scale;
-    if (a.table != nullptr) x += load_param(a.table, a.param_f32, static_cast<long long>(bucket_of(a, j - i)) * a.H + h);
-    const float mn = fmaxf(m, x);
-    if (mn == -INFINITY) continue;
-    const float f = expf(m - mn), e = expf(x - mn);
-    l = l * f + e;
-    o.scale(f);
-    o.add(v, e);
-    m = mn;
-  }
-  o.store(a.o, at(a.o_strides, b, i, h), lane, l > 0.f ? 1.f / l : 0.f);
-  if (a.lse != nullptr && lane == 0) a.lse[w] = l > 0.f ? m + logf(l) : INFINITY;     // no keys: every probability comes out as zero
-}
-
-template <int DH>
 __global__ void text_dq_kernel(const MdbTextAttnArgs a) {
   const long long w = (blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (w >= static_cast<long long>(a.B) * a.H * a.Sq) return;
   const int i = static_cast<int>(w % a.Sq), h = static_cast<int>((w / a.Sq) % a.H), b = static_cast<int>(w / (static_cast<long long>(a.Sq) * a.H));
   const int g = h / (a.H / a.Hkv);
-  const Sight s = sight_of(a, b);
+  const TextSight s = text_sight(a, b);
   const int p = s.start + i;
-  const int hi = a.causal ? min(p + 1, s.valid) : s.valid;
-  const int lo = a.causal ? max(p - a.window + 1, 0) : 0;
+  const int hi = (a.table == nullptr) ? min(p + 1, s.valid) : s.valid;
+  const int lo = (a.table == nullptr) ? max(p - a.window + 1, 0) : 0;
   Row<DH> q, o, d, dq;
   q.load(a.q, at(a.q_strides, b, i, h), lane);
   o.load(a.o, at(a.o_strides, b, i, h), lane);
@@ -150,9 +82,9 @@ __global__ void text_dq_kernel(const MdbTextAttnArgs a) {
     k.load(a.k, at(a.k_strides, b, j, g), lane);
     v.load(a.v, at(a.v_strides, b, j, g), lane);
     float x = q.dot(k) * a.scale;
-    const int c = a.table != nullptr ? bucket_of(a, j - i) : 0;
-    if (a.table != nullptr) x += load_param(a.table, a.param_f32, static_cast<long long>(c) * a.H + h);
-    const float ds = expf(x - lse) * (d.dot(v) - delta);
+    const int c = a.table != nullptr ? text_bucket(a, j - i) : 0;
+    if (a.table != nullptr) x += text_param(a.table, a.param_f32, static_cast<long long>(c) * a.H + h);
+    const float ds = exp2f(x * TXT_LOG2E - lse) * (d.dot(v) - delta);
     dq.add(k, ds);
     if (part != nullptr && lane == 0) part[c] += ds;
   }
@@ -165,15 +97,15 @@ __global__ void text_dkv_kernel(const MdbTextAttnArgs a) {
   const int lane = threadIdx.x & 31;
   if (w >= static_cast<long long>(a.B) * a.Hkv * a.Skv) return;
   const int j = static_cast<int>(w % a.Skv), g = static_cast<int>((w / a.Skv) % a.Hkv), b = static_cast<int>(w / (static_cast<long long>(a.Skv) * a.Hkv));
-  const Sight s = sight_of(a, b);
+  const TextSight s = text_sight(a, b);
   Row<DH> k, v, dk, dv;
   k.load(a.k, at(a.k_strides, b, j, g), lane);
   v.load(a.v, at(a.v_strides, b, j, g), lane);
   dk.zero();
   dv.zero();
   const int rep = a.H / a.Hkv;
-  const int i0 = a.causal ? max(j - s.start, 0) : 0;
-  const int i1 = j >= s.valid ? 0 : (a.causal && j >= a.sinks) ? static_cast<int>(min(static_cast<long long>(a.Sq), static_cast<long long>(j) + a.window - s.start)) : a.Sq;
+  const int i0 = (a.table == nullptr) ? max(j - s.start, 0) : 0;
+  const int i1 = j >= s.valid ? 0 : ((a.table == nullptr) && j >= a.sinks) ? static_cast<int>(min(static_cast<long long>(a.Sq), static_cast<long long>(j) + a.window - s.start)) : a.Sq;
   for (int h = g * rep; h < (g + 1) * rep; ++h)
     for (int i = i0; i < i1; ++i) {
       Row<DH> q, d;
@@ -181,8 +113,8 @@ __global__ void text_dkv_kernel(const MdbTextAttnArgs a) {
       d.load(a.dout, at(a.do_strides, b, i, h), lane);
       const long long r = (static_cast<long long>(b) * a.H + h) * a.Sq + i;
       float x = q.dot(k) * a.scale;
-      if (a.table != nullptr) x += load_param(a.table, a.param_f32, static_cast<long long>(bucket_of(a, j - i)) * a.H + h);
-      const float e = expf(x - a.lse[r]);
+      if (a.table != nullptr) x += text_param(a.table, a.param_f32, static_cast<long long>(text_bucket(a, j - i)) * a.H + h);
+      const float e = exp2f(x * TXT_LOG2E - a.lse[r]);
       dv.add(d, e);
       dk.add(q, e * (d.dot(v) - a.delta[r]));
     }
@@ -194,11 +126,11 @@ __global__ void text_dkv_kernel(const MdbTextAttnArgs a) {
 __global__ void text_dsink_kernel(const MdbTextAttnArgs a) {
   __shared__ float part[256];
   const int h = blockIdx.x;
-  const float sink = load_param(a.sink_logits, a.param_f32, h);
+  const float sink = text_param(a.sink_logits, a.param_f32, h);
   float s = 0.f;
   for (long long r = threadIdx.x; r < static_cast<long long>(a.B) * a.Sq; r += 256) {
     const long long at_ = ((r / a.Sq) * a.H + h) * a.Sq + r % a.Sq;
-    s += expf(sink - a.lse[at_]) * a.delta[at_];
+    s += exp2f(sink * TXT_LOG2E - a.lse[at_]) * a.delta[at_];
   }
   part[threadIdx.x] = s;
   __syncthreads();
@@ -235,7 +167,7 @@ __global__ void text_dtable_kernel(const MdbTextAttnArgs a) {
 static int check_args(const MdbTextAttnArgs* a) {
   if (a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0 || a->Sq <= 0 || a->Skv <= 0) return -1;
   if (a->Dh != 64 && a->Dh != 128) return -2;
-  if (a->window < 1 || a->window > TXT_FAR || a->sinks < 0) return -5;
+  if (a->window < 1 || a->window > TXT_FAR || a->sinks < 0 || !(a->scale > 0.f)) return -5;
   if (a->table != nullptr && (a->buckets < 4 || a->buckets > MDB_TEXT_MAX_BUCKETS || a->n_borders < 0 || a->n_borders > MDB_TEXT_MAX_BUCKETS / 4 ||
                               a->exact < 1 || a->exact + a->n_borders > a->buckets / 2 - 1 || (a->n_borders == 0 && a->exact > MDB_TEXT_MAX_DISTANCE) ||
                               (a->n_borders > 0 && a->borders[a->n_borders - 1] > MDB_TEXT_MAX_DISTANCE)))
@@ -249,10 +181,7 @@ static unsigned blocks_for(long long rows) { return static_cast<unsigned>((rows 
 extern "C" int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st) {
   using namespace mdb;
   if (int r = check_args(a)) return r;
-  const unsigned n = blocks_for(static_cast<long long>(a->B) * a->H * a->Sq);
-  if (a->Dh == 128) text_fwd_kernel<128><<<n, 128, 0, st>>>(*a);
-  else text_fwd_kernel<64><<<n, 128, 0, st>>>(*a);
-  return static_cast<int>(cudaGetLastError());
+  return text_attention_prompt(*a, st);
 }
 
 extern "C" long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a) {

@@ -1,0 +1,76 @@
+// What the kernels of the language models' attention share: which keys a query sees, and the bias of a relative position.
+#pragma once
+#include "common.cuh"
+#include "kernels_api.h"
+
+namespace mdb {
+
+constexpr int TXT_FAR = 1 << 30;
+constexpr float TXT_LOG2E = 1.4426950408889634f, TXT_LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float text_param(const void* p, int is_f32, long long i) {
+  return is_f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// the keys of batch entry b end at `valid`, its query row 0 stands at position `start`
+struct TextSight {
+  int valid, start;
+};
+__device__ __forceinline__ TextSight text_sight(const MdbTextAttnArgs& a, int b) {
+  TextSight s;
+  s.valid = a.kv_len != nullptr ? min(max(a.kv_len[b], 0), a.Skv) : a.Skv;
+  s.start = a.q_start_ptr != nullptr ? a.q_start_ptr[b] : a.q_start;
+  s.start = min(max(s.start, -TXT_FAR), TXT_FAR);
+  return s;
+}
+
+// Keys that the queries at positions p_lo .. p_hi see together: [0, sinks) and [lo, end), lo >= sinks unless everything from 0 on is seen.
+// Every query sees a subset; with BIAS (no mask but the length) each sees all of them.
+struct TextKeys {
+  int sinks, lo, end;
+};
+template <bool BIAS>
+__device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const TextSight& s, int p_lo, int p_hi) {
+  TextKeys k;
+  k.end = BIAS ? s.valid : max(min(p_hi + 1, s.valid), 0);
+  k.lo = BIAS ? 0 : min(max(p_lo - a.window + 1, 0), k.end);
+  k.sinks = BIAS ? 0 : min(a.sinks, k.end);
+  if (k.sinks >= k.lo) k.sinks = k.lo = 0;
+  return k;
+}
+
+// bit i: i < n
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+// bit i: the query at position p sees key k0 + i
+__device__ __forceinline__ uint32_t text_mask(const MdbTextAttnArgs& a, int valid, int p, int k0) {
+  return bits_below(min(p + 1, valid) - k0) & (~bits_below(p - a.window + 1 - k0) | bits_below(a.sinks - k0));
+}
+
+// Distances from `near` on share one bucket per direction; text_bucket(rel) is constant beyond it on either side.
+__host__ __device__ __forceinline__ int text_near(const MdbTextAttnArgs& a) { return a.n_borders > 0 ? a.borders[a.n_borders - 1] : a.exact; }
+__device__ __forceinline__ int text_bucket(const MdbTextAttnArgs& a, int rel) {
+  const int n = rel < 0 ? -rel : rel;
+  int c = n;
+  if (n >= a.exact) {
+    c = a.exact;
+    for (int i = 0; i < a.n_borders; ++i) c += n >= a.borders[i];
+  }
+  return c + (rel > 0 ? a.buckets / 2 : 0);
+}
+
+// lets `kern` have up to `bytes` of dynamic shared memory on the current device; once for each
+constexpr int TXT_DEVICES = 64;
+template <typename K>
+inline int allow_smem(K kern, int bytes, bool (&ready)[TXT_DEVICES]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < TXT_DEVICES && ready[dev]) return 0;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < TXT_DEVICES) ready[dev] = true;
+  return 0;
+}
+
+int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st);
+
+}  // namespace mdb

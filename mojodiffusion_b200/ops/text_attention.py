@@ -100,9 +100,9 @@ def _attend(q, k, v, param, scale, rule: Sequence[int], kv_len, q_start, buckets
     return out.copy_(o) if out is not None else o
 
 
-def _native(q, k, *others) -> bool:
+def _native(q, k, scale, *others) -> bool:
     given = [t for t in others if t is not None]
-    return (native.use_native(q) and q.dtype == torch.bfloat16 and q.shape[3] in (64, 128) and q.numel() > 0 and k.numel() > 0
+    return (native.use_native(q) and 0 < scale < math.inf and q.dtype == torch.bfloat16 and q.shape[3] in (64, 128) and q.numel() > 0 and k.numel() > 0
             and max(q.shape[1], k.shape[1]) < 1 << 30 and max(q.shape[0], q.shape[2]) < 1 << 16 and native.direct(q, k, *given))
 
 
@@ -129,10 +129,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if sink_logits is not None and (sink_logits.shape != q.shape[2:3] or not sink_logits.is_floating_point() or sink_logits.device != q.device):
         raise ValueError(f"{name}: sink_logits must be [H] on q's device")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if not _native(q, k, v, kv_len, start, sink_logits) or (sink_logits is not None and sink_logits.dtype not in (torch.float32, torch.bfloat16)):
+    if not _native(q, k, scale, v, kv_len, start, sink_logits) or (sink_logits is not None and sink_logits.dtype not in (torch.float32, torch.bfloat16)):
         o = ref.window_attention(q, k, v, window, sinks, scale, kv_len, q_start, sink_logits)
         return out.copy_(o) if out is not None else o
-    rule = [1, min(window, _NO_WINDOW) if window is not None else _NO_WINDOW, min(sinks, _NO_WINDOW), 0 if start is not None else max(min(q_start, _NO_WINDOW), -_NO_WINDOW)]
+    rule = [min(window, _NO_WINDOW) if window is not None else _NO_WINDOW, min(sinks, _NO_WINDOW), 0 if start is not None else max(min(q_start, _NO_WINDOW), -_NO_WINDOW)]
     return _attend(q, k, v, sink_logits, scale, rule, kv_len, start, [], out)
 
 
@@ -157,8 +157,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
         raise ValueError(f"{name}: table must be [num_buckets, H] on q's device, num_buckets even and at least 4")
     if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
         raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
-    if (not _native(q, k, v, kv_len, table) or table.dtype not in (torch.float32, torch.bfloat16) or table.shape[0] > MAX_BUCKETS
+    if (not _native(q, k, scale, v, kv_len, table) or table.dtype not in (torch.float32, torch.bfloat16) or table.shape[0] > MAX_BUCKETS
             or max_distance > MAX_DISTANCE):
         o = ref.relative_attention(q, k, v, table, max_distance, scale, kv_len)
         return out.copy_(o) if out is not None else o
-    return _attend(q, k, v, table, float(scale), [0, _NO_WINDOW, 0, 0], kv_len, None, list(_buckets(table.shape[0], max_distance)), out)
+    return _attend(q, k, v, table, float(scale), [_NO_WINDOW, 0, 0], kv_len, None, list(_buckets(table.shape[0], max_distance)), out)

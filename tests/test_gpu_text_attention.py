@@ -381,13 +381,13 @@ def test_native_refusals():
     """What the C++ entry checks by itself, on the host, before a launch."""
     fwd = torch.ops.mdb200.text_attention_fwd
     q, k, v = _inputs(2, 8, 8, 4, 2, 64, seed=340)
-    rule = [1, 4, 0, 0]
+    rule = [4, 0, 0]
     ok = lambda **c: fwd(c.get("q", q), c.get("k", k), c.get("v", v), 1.0, c.get("rule", rule), c.get("n"), c.get("at"), c.get("sink"), c.get("table"),
                          c.get("buckets", []), False, c.get("out"))
     ok()
     table = _normal(32, 4, seed=1)
     for bad in (dict(q=q.float()), dict(k=k[:, :, :, ::2]), dict(k=k.cpu()), dict(k=_normal(2, 8, 3, 64, seed=1), v=_normal(2, 8, 3, 64, seed=1)), dict(v=v[:, :5]),
-                dict(q=_normal(2, 8, 4, 65, seed=1)[..., 1:]), dict(k=k[:1].expand(2, 8, 2, 64)), dict(rule=[1, 0, 0, 0]), dict(rule=[1, 4, -1, 0]), dict(rule=[1, 4]),
+                dict(q=_normal(2, 8, 4, 65, seed=1)[..., 1:]), dict(k=k[:1].expand(2, 8, 2, 64)), dict(rule=[0, 0, 0]), dict(rule=[4, -1, 0]), dict(rule=[4]),
                 dict(n=_ints([1])), dict(n=torch.tensor([1, 1], device=DEV)), dict(at=torch.tensor([1, 1], dtype=torch.int32)), dict(sink=_normal(3, seed=1)),
                 dict(sink=_normal(4, seed=1, dtype=torch.float16)), dict(table=table), dict(table=table, buckets=[16, 4, 9]), dict(table=table, buckets=[32, 8] + [9] * 40),
                 dict(table=table, buckets=[32, 8, 5000]), dict(sink=_normal(4, seed=1), table=table, buckets=[32, 8, 9]), dict(out=q[:, :4])):
