@@ -564,7 +564,7 @@ void text_rule(MdbTextAttnArgs& a, const Tensor& q, const Tensor& k, double scal
   }
   TORCH_CHECK(a.table == nullptr || a.sink_logits == nullptr, "text attention: a table or sink logits");
   if (a.table != nullptr) {
-    TORCH_CHECK(buckets.size() >= 2 && buckets[0] <= MDB_TEXT_MAX_BUCKETS && (int64_t)buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 4, "text attention: buckets");
+    TORCH_CHECK(buckets.size() >= 2 && buckets[0] <= MDB_TEXT_MAX_BUCKETS && (int64_t)buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 2, "text attention: buckets");
     a.buckets = (int)buckets[0];
     a.exact = (int)buckets[1];
     a.n_borders = (int)buckets.size() - 2;
@@ -1401,7 +1401,8 @@ void set_wait_limit_ns(int64_t ns) {
   TORCH_CHECK(ns > 0, "set_wait_limit_ns: positive nanoseconds");
   const unsigned long long v = static_cast<unsigned long long>(ns);
   const int rc = mdb_set_wait_limit_gemm(v) | mdb_set_wait_limit_attn_fwd(v) | mdb_set_wait_limit_attn_bwd(v) |
-                 mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v) | mdb_set_wait_limit_text_fwd(v);
+                 mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v) | mdb_set_wait_limit_text_fwd(v) |
+                 mdb_set_wait_limit_text_bwd(v);
   TORCH_CHECK(rc == 0, "set_wait_limit_ns failed: ", rc);
 }
 

@@ -214,7 +214,7 @@ int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 // 8, addresses multiples of 16 bytes. Without a table, key j is seen by the query at position p = q_start + row when j < kv_len, j <= p and
 // (p - j < window or j < sinks); with one, when j < kv_len. scale > 0. lse (base 2; +inf: a row that saw nothing), delta: fp32 [B, H, Sq]; delta and
 // table_ws are workspaces of the backward pass.
-#define MDB_TEXT_MAX_BUCKETS 128
+#define MDB_TEXT_MAX_BUCKETS 64        // at Dh 64, half as many at 128: the backward pass keeps an accumulator for each in every thread
 #define MDB_TEXT_MAX_DISTANCE 1024
 typedef struct MdbTextAttnArgs {
   const void* q; const void* k; const void* v; void* o;
@@ -223,7 +223,7 @@ typedef struct MdbTextAttnArgs {
   const int* kv_len;          // [B] or null: all keys
   const int* q_start_ptr;     // [B], or null: q_start for all
   const void* sink_logits;    // [H] or null
-  const void* table;          // [buckets, H] or null
+  const void* table;          // [buckets, H] or null; then Hkv = H
   void* d_sink; void* d_table;
   float* table_ws;            // mdb_text_attention_bwd_floats values when d_table is given
   long long q_strides[3], k_strides[3], v_strides[3], o_strides[3], do_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
@@ -232,7 +232,7 @@ typedef struct MdbTextAttnArgs {
   int param_f32;              // type of sink_logits / table and their gradients: 0 bf16, 1 fp32
   // relative position buckets: distances below `exact` have one each, distance n >= exact the bucket exact + (borders <= n); half of the buckets per direction
   int buckets, exact, n_borders;
-  int borders[MDB_TEXT_MAX_BUCKETS / 4];
+  int borders[MDB_TEXT_MAX_BUCKETS / 2];
   float scale;
   int* status;
 } MdbTextAttnArgs;

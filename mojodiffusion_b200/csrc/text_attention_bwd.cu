@@ -1,0 +1,632 @@
+// Backward pass of the language models' attention on tcgen05 / TMEM. Two launches of one kernel template and, for a learned parameter, a small sum:
+//
+//   KEYS = false (dq):     a CTA owns 128 query rows of one head and streams tiles of 64 keys:
+//       X = Q K^T, Y = dO V^T;  P = exp2(x - lse), dS = P (Y - delta);  dQ += dS K
+//   KEYS = true (dk, dv):  a CTA owns 128 keys of one key head and streams tiles of 64 queries of every head of the group, one head after the
+//       other:  X = K Q^T, Y = V dO^T;  P^T, dS^T;  dV += P^T dO, dK += dS^T Q
+//
+// The sums over a group's heads stay in the accumulators, so no two CTAs add to one output and the results do not depend on their order.
+// delta = rowsum(do o) is formed by the first launch for its own rows and read by the second.
+//
+// The 128-row operands stay in shared memory, the 64-row ones stream through a ring and serve twice: K-major for the score products and MN-major
+// for the gradient products. Score tiles are double buffered in TMEM, one buffer per math warpgroup: while one warpgroup turns its tile into
+// bf16 P / dS (over the scores, the A operand of the gradient products), the tensor core and the other one work on the next.
+//
+// Only tiles in which a pair may be visible are streamed; in those that are not visible whole, each thread makes its row's visibility bits.
+// Rows of K and V that no query of the CTA sees are zeroed in shared memory before they are multiplied (0 * NaN is not 0).
+//
+// dtable (BIAS, first launch): dS is summed by bucket, in fp32 before it is rounded. In a block of 32 rows (a warp) x 32 keys whose distances lie
+// in one bucket a thread adds its 32 values to its accumulator of that bucket. In the others, near the diagonal, it writes the running sums
+// of its 32 values to shared memory: the sum over the distances of a bucket is the difference of two of them, at places that the borders and the
+// row give. That is one addition per value and about ten instructions per bucket of the block (sums along diagonals by shuffles take about four
+// per value). Each thread has its own accumulators; they are added in a fixed order at the end.
+#include "text_attention.cuh"
+#include "gemm_api.h"
+
+#include <string.h>
+
+namespace mdb {
+
+constexpr int TB_THREADS = 320;      // warps: 0 TMA, 1 MMA issue, 2-5 and 6-9 two math warpgroups
+constexpr int TR = 128, TC = 64;     // resident rows, rows of a streamed tile
+constexpr int RUN_LD = 36;           // floats between the running sums of two rows: 16-byte stores and the skewed reads hit all banks
+
+struct alignas(64) TextBwdMaps {
+  CUtensorMap r1, r2, c1, c2;
+};
+
+template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
+  static constexpr int STAGES = (DH == 128 && BIAS && !KEYS) ? 2 : 4;      // the accumulators of dtable take the place of two
+  static constexpr int TILES = 2 * TR * DH * 2 + STAGES * 2 * TC * DH * 2 + 1024;
+  static constexpr int SUMS = (BIAS && !KEYS) ? 8 * 32 * RUN_LD * 4 : 0;
+  static __host__ __device__ int lut_bytes(int near) { return BIAS ? (2 * near + 509) * 4 : 0; }
+  static __host__ __device__ int bytes(int near, int buckets) {
+    return TILES + SUMS + lut_bytes(near) + ((BIAS && !KEYS) ? buckets * 256 * 4 + (2 * near + 4) + (buckets + 2) * 8 : 0);
+  }
+};
+
+template <int DH, bool KEYS, bool BIAS>
+__global__ void __launch_bounds__(TB_THREADS, 1)
+text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a) {
+  using Shape = TextBwdShape<DH, KEYS, BIAS>;
+  constexpr int STAGES = Shape::STAGES;
+  constexpr int DBOX = DH / 64;
+  constexpr int R_BYTES = TR * DH * 2, R_BOX = TR * 128;
+  constexpr int C_BYTES = TC * DH * 2, C_BOX = TC * 128;
+  constexpr uint32_t X_COL = 0, Y_COL = 128, ACC1_COL = 256, ACC2_COL = 384;  // X0 X1 | Y0 Y1 | dQ or dK | dV
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2], acc_full;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+  __shared__ __align__(16) float s_lse[2][TC], s_delta[2][TC];      // negated, per staged query
+
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* sR1 = smem;
+  uint8_t* sR2 = sR1 + R_BYTES;
+  uint8_t* sC = sR2 + R_BYTES;                                            // STAGES x (C1, C2)
+  const int near = BIAS ? text_near(a) : 0;
+  float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // BIAS dq: running sums [8 warps][32 rows][RUN_LD]
+  float* lut = sums + Shape::SUMS / 4;                                    // BIAS: log2(e) * bias of the distances -near - 254 .. near + 254
+  float* bins = lut + (BIAS ? 2 * near + 509 : 0);                        // BIAS dq: [buckets][256 threads]
+  // BIAS dq: the buckets in the order of their distances ("runs"): first distance and bucket of each, and the run of the distances -near .. near
+  const int run_mid = a.exact + a.n_borders, runs = 2 * run_mid + 1;
+  int* run_start = reinterpret_cast<int*>(bins + a.buckets * 256);        // [runs + 1]
+  int* run_bucket = run_start + a.buckets + 2;                            // [runs]
+  uint8_t* run_of = reinterpret_cast<uint8_t*>(run_bucket + a.buckets + 2);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int batch = blockIdx.z;
+  const int rep = a.H / a.Hkv;
+  // the rows with the most to stream start first: late queries, early keys
+  const int r0 = (KEYS || BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TR;
+  const int out_rows = KEYS ? a.Skv : a.Sq;
+  const TextSight sight = text_sight(a, batch);
+
+  // streamed tiles: keys [0, ns) and [lo, hi); queries [lo, hi) of each head of the group
+  TextKeys seen = {0, 0, 0};
+  int ns = 0, lo = 0, hi = 0;
+  if (!KEYS) {
+    seen = text_keys<BIAS>(a, sight, sight.start + r0, sight.start + min(r0 + TR, a.Sq) - 1);
+    ns = (seen.sinks + TC - 1) / TC;
+    lo = max(seen.lo / TC, ns);
+    hi = max(seen.end > seen.lo ? (seen.end + TC - 1) / TC : lo, lo);
+  } else if (r0 < sight.valid) {
+    int first = 0, end = a.Sq;
+    if (!BIAS) {
+      first = max(r0 - sight.start, 0);
+      if (r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
+    }
+    if (first < end) {
+      lo = first / TC;
+      hi = (end + TC - 1) / TC;
+    }
+  }
+  const int per_head = ns + hi - lo;
+  const int n_c = KEYS ? per_head * rep : per_head;
+  const auto tile_of = [&](int i) { return i < ns ? i : i - ns + lo; };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&r_full, 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&c_full[s], 1);
+      mbar_init(&c_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&xy_full[s], 1);
+      mbar_init(&pds_full[s], 4);
+      mbar_init(&lv_full[s], TC);
+    }
+    mbar_init(&acc_full, 1);
+    abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base_s, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&maps.r1);
+    tma_prefetch_desc(&maps.r2);
+    tma_prefetch_desc(&maps.c1);
+    tma_prefetch_desc(&maps.c2);
+  }
+  if (BIAS) {
+    // one head's bias: with a table there are as many key heads as query heads
+    for (int i = threadIdx.x; i < 2 * near + 509; i += TB_THREADS)
+      lut[i] = TXT_LOG2E * text_param(a.table, a.param_f32, static_cast<long long>(text_bucket(a, i - near - 254)) * a.H + blockIdx.y);
+    if (!KEYS && a.d_table != nullptr) {
+      for (int i = threadIdx.x; i < a.buckets * 256; i += TB_THREADS) bins[i] = 0.f;
+      for (int i = threadIdx.x; i <= 2 * near; i += TB_THREADS) {
+        const int c = text_bucket(a, i - near);
+        run_of[i] = static_cast<uint8_t>(i <= near ? run_mid - c : run_mid + c - a.buckets / 2);
+      }
+      for (int r = threadIdx.x; r < runs; r += TB_THREADS) {
+        const int c = r < run_mid ? run_mid - r : r - run_mid;                 // bucket within its direction
+        const auto reach = [&](int b) { return b <= a.exact ? b : a.borders[b - a.exact - 1]; };      // its first distance
+        run_bucket[r] = r <= run_mid ? c : c + a.buckets / 2;
+        run_start[r] = r == 0 ? -TXT_FAR : r <= run_mid ? 1 - reach(c + 1) : reach(c);
+        if (r == 0) run_start[runs] = TXT_FAR;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    // ----------------------------- TMA producer -----------------------------
+    if (n_c > 0) {
+      if (elect_one()) {
+        mbar_expect_tx(&r_full, 2 * R_BYTES);
+        for (int d = 0; d < DBOX; ++d) {
+          tma_load_4d(sR1 + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
+          tma_load_4d(sR2 + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
+        }
+      }
+      __syncwarp();
+      bool ok = true;
+      uint64_t* last_bar = &r_full;
+      uint32_t last_par = 0;
+      int head = KEYS ? blockIdx.y * rep : blockIdx.y / rep, in_head = 0;
+      for (int i = 0; i < n_c; ++i) {
+        const int st = i & (STAGES - 1);
+        const uint32_t par = (i / STAGES) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&c_empty[st], par ^ 1u, &abort_s));
+        if (!ok) {
+          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141, i);
+          break;
+        }
+        uint8_t* c1 = sC + st * 2 * C_BYTES;
+        if (elect_one()) {
+          mbar_expect_tx(&c_full[st], 2 * C_BYTES);
+          for (int d = 0; d < DBOX; ++d) {
+            tma_load_4d(c1 + d * C_BOX, &maps.c1, &c_full[st], d * 64, tile_of(in_head) * TC, head, batch);
+            tma_load_4d(c1 + C_BYTES + d * C_BOX, &maps.c2, &c_full[st], d * 64, tile_of(in_head) * TC, head, batch);
+          }
+        }
+        __syncwarp();
+        last_bar = &c_full[st];
+        last_par = par;
+        if (++in_head == per_head && KEYS) {
+          in_head = 0;
+          ++head;
+        }
+      }
+      if (!ok) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(last_bar, last_par) && globaltimer_ns() - t0 < 5000000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ----------------------------- MMA issue --------------------------------
+    if (n_c > 0) {
+      constexpr uint32_t idesc_xy = make_idesc(1, UMMA_BF16, UMMA_BF16, 0, 0, TR, TC);
+      constexpr uint32_t idesc_acc = make_idesc(1, UMMA_BF16, UMMA_BF16, 0, 1, TR, DH);
+      const uint64_t r1 = make_desc_kmajor_sw128(smem_u32(sR1)), r2 = make_desc_kmajor_sw128(smem_u32(sR2));
+      const uint64_t ck = make_desc_kmajor_sw128(smem_u32(sC)), cm = make_desc_mnmajor_sw128(smem_u32(sC), C_BOX);
+      const auto issue_xy = [&](int st, int buf) {
+        const uint64_t c1 = ck + static_cast<uint64_t>(st * (2 * C_BYTES >> 4)), c2 = c1 + (C_BYTES >> 4);
+        const uint32_t x = tmem_base + X_COL + buf * TC, y = tmem_base + Y_COL + buf * TC;
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk)
+          umma_f16_ss(x, r1 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c1 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk)
+          umma_f16_ss(y, r2 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c2 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+        umma_commit(&xy_full[buf]);
+      };
+      const auto issue_acc = [&](int st, int buf, bool first) {
+        const uint64_t c1 = cm + static_cast<uint64_t>(st * (2 * C_BYTES >> 4)), c2 = c1 + (C_BYTES >> 4);
+#pragma unroll
+        for (int kk = 0; kk < TC / 16; ++kk)
+          umma_f16_ts(tmem_base + ACC1_COL, tmem_base + Y_COL + buf * TC + kk * 8, c1 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
+        if (KEYS) {
+#pragma unroll
+          for (int kk = 0; kk < TC / 16; ++kk)
+            umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk * 8, c2 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
+        }
+      };
+      // rows of a key tile that no query of the CTA sees
+      const auto clean = [&](int i, int st) {
+        if (KEYS) return;
+        const int k0 = tile_of(i) * TC;
+        if (k0 + TC <= seen.end && (k0 >= seen.lo || k0 + TC <= seen.sinks)) return;
+        for (int r = lane; r < TC; r += 32) {
+          const int j = k0 + r;
+          if (j < seen.end && (j >= seen.lo || j < seen.sinks)) continue;
+          for (int b = 0; b < 2 * DBOX; ++b)
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(sC + st * 2 * C_BYTES + b * C_BOX + r * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&r_full, 0, &abort_s) && mbar_wait(&c_full[0], 0, &abort_s));
+      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 151, 0);
+      if (ok) {
+        tc_fence_after();
+        clean(0, 0);
+        if (elect_one()) issue_xy(0, 0);
+        __syncwarp();
+      }
+      for (int i = 0; ok && i < n_c; ++i) {
+        const int st = i & (STAGES - 1);
+        if (i + 1 < n_c) {
+          const int stn = (i + 1) & (STAGES - 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&c_full[stn], ((i + 1) / STAGES) & 1, &abort_s));
+          if (!ok) {
+            if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 152, i);
+            break;
+          }
+          tc_fence_after();
+          clean(i + 1, stn);
+          if (elect_one()) issue_xy(stn, (i + 1) & 1);
+          __syncwarp();
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&pds_full[i & 1], (i >> 1) & 1, &abort_s));
+        if (!ok) {
+          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 153, i);
+          break;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+          issue_acc(st, i & 1, i == 0);
+          umma_commit(&c_empty[st]);
+          if (i + 1 == n_c) umma_commit(&acc_full);
+        }
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------- math: warpgroup g takes the tiles of buffer g, every second one
+    const int g = (warp - 2) >> 2;
+    const int quad = warp & 3;
+    const int mt = quad * 32 + lane;  // row inside the resident tile == TMEM lane
+    const int slot = g * 128 + mt;
+    const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
+    const int row = r0 + mt;
+    const float sl2 = a.scale * TXT_LOG2E;
+    float my_nlse = -INFINITY, my_ndelta = 0.f;       // rows behind the last query: probabilities of zero
+    if (!KEYS && row < a.Sq) {
+      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
+      const uint4* o = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o) + batch * a.o_strides[0] + row * a.o_strides[1] + blockIdx.y * a.o_strides[2]);
+      const uint4* d = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dout) + batch * a.do_strides[0] + row * a.do_strides[1] + blockIdx.y * a.do_strides[2]);
+      float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < DH / 8; ++c) {
+        const uint4 u = o[c], w = d[c];
+        s = ffma2(unpack_bf16x2(u.x), unpack_bf16x2(w.x), s);
+        s = ffma2(unpack_bf16x2(u.y), unpack_bf16x2(w.y), s);
+        s = ffma2(unpack_bf16x2(u.z), unpack_bf16x2(w.z), s);
+        s = ffma2(unpack_bf16x2(u.w), unpack_bf16x2(w.w), s);
+      }
+      my_ndelta = -(s.x + s.y);
+      my_nlse = -a.lse[at];
+      if (g == 0) a.delta[at] = -my_ndelta;
+    }
+    // KEYS: thread mt < 64 stages the negated lse and delta of query mt of the warpgroup's tile, loaded one of its tiles ahead
+    float next_nlse = -INFINITY, next_ndelta = 0.f;
+    int f_head = KEYS ? blockIdx.y * rep : 0, f_tile = 0;
+    const auto fetch = [&](int ahead) {
+      f_tile += ahead;
+      while (f_tile >= per_head) {
+        f_tile -= per_head;
+        ++f_head;
+      }
+      const int q = (lo + f_tile) * TC + mt;
+      const bool in = mt < TC && q < a.Sq && f_head < (static_cast<int>(blockIdx.y) + 1) * rep;
+      const long long at = (static_cast<long long>(batch) * a.H + f_head) * a.Sq + q;
+      next_nlse = in ? -a.lse[at] : -INFINITY;
+      next_ndelta = in ? -a.delta[at] : 0.f;
+    };
+    if (KEYS && g < n_c) fetch(g);
+    bool ok = true;
+    int in_head = g;
+    const uint32_t xa = tmem_base + lane_addr + X_COL + g * TC;
+    const uint32_t ya = tmem_base + lane_addr + Y_COL + g * TC;
+    for (int i = g; i < n_c; i += 2) {
+      const uint32_t par = (i >> 1) & 1;
+      if (KEYS) {
+        while (in_head >= per_head) in_head -= per_head;
+        // the buffer was last read for tile i - 2: the warpgroup's four warps have all arrived on pds_full[g] for it
+        bool lv_ok = true;
+        if (mt < TC) {
+          if (i >= 2) lv_ok = mbar_wait(&pds_full[g], par ^ 1u, &abort_s);
+          s_lse[g][mt] = next_nlse;
+          s_delta[g][mt] = next_ndelta;
+          mbar_arrive(&lv_full[g]);
+        }
+        if (i + 2 < n_c) fetch(2);
+        lv_ok = mbar_wait(&lv_full[g], par, &abort_s) && lv_ok;
+        if (!__all_sync(0xffffffffu, lv_ok)) {
+          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 160, i);
+          ok = false;
+          break;
+        }
+      }
+      const int c0 = tile_of(in_head) * TC;          // first key (dq) or query (KEYS) of the tile
+      ok = __all_sync(0xffffffffu, mbar_wait(&xy_full[g], par, &abort_s));
+      if (!ok) {
+        if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 161, i);
+        break;
+      }
+      tc_fence_after();
+      uint32_t xr[2][32], yr[2][32];
+      float run[2][32];                              // BIAS dq: dS
+#pragma unroll
+      for (int c = 0; c < TC / 32; ++c) {
+        tmem_ld_32x32b_x32(xa + c * 32, xr[c]);
+        tmem_ld_32x32b_x32(ya + c * 32, yr[c]);
+      }
+      tmem_wait_ld();
+      bool whole;       // every pair of the tile is visible, or its row or query lies behind the last one and has a probability of zero anyway
+      if (BIAS) whole = KEYS ? r0 + TR <= sight.valid : c0 + TC <= sight.valid;
+      else if (KEYS) whole = r0 + TR <= sight.valid && r0 + TR - 1 <= sight.start + c0 && (sight.start + c0 + TC - 1 - a.window < r0 || r0 + TR <= a.sinks);
+      else whole = c0 + TC <= sight.valid && c0 + TC - 1 <= sight.start + r0 && (sight.start + r0 + TR - 1 - a.window < c0 || c0 + TC <= a.sinks);
+#pragma unroll
+      for (int c = 0; c < TC / 32; ++c) {
+        const int b0 = c0 + c * 32;
+        uint32_t see = 0xffffffffu;
+        if (!whole) {
+          if (BIAS) see = KEYS ? (row < sight.valid ? see : 0u) : bits_below(sight.valid - b0);
+          else if (KEYS) see = row < sight.valid ? ~bits_below(row - sight.start - b0) & (row < a.sinks ? see : bits_below(row + a.window - sight.start - b0)) : 0u;
+          else see = text_mask(a, sight.valid, sight.start + row, b0);
+        }
+        // BIAS: distances of the warp's 32 x 32 block lie in d0 - 31 .. d0 + 31
+        const int d0 = KEYS ? r0 + quad * 32 - b0 : b0 - (r0 + quad * 32);
+        const bool uniform = BIAS && (d0 - 31 >= near || d0 + 31 <= -near);
+        float one_bias = 0.f;
+        const float* b = nullptr;
+        if (BIAS) {
+          if (uniform) one_bias = d0 > 0 ? lut[2 * near + 508] : lut[0];
+          else b = lut + near + 254 + (KEYS ? row - b0 : b0 - row);
+        }
+        uint32_t pk[16], dk[16];
+        const float2 sl2_2 = make_float2(sl2, sl2);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float nl[4], nd[4];
+          if (KEYS) {
+            const float4 u = *reinterpret_cast<const float4*>(&s_lse[g][c * 32 + e]), w = *reinterpret_cast<const float4*>(&s_delta[g][c * 32 + e]);
+            nl[0] = u.x; nl[1] = u.y; nl[2] = u.z; nl[3] = u.w;
+            nd[0] = w.x; nd[1] = w.y; nd[2] = w.z; nd[3] = w.w;
+          } else {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              nl[m] = my_nlse;
+              nd[m] = my_ndelta;
+            }
+          }
+          if (BIAS) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) nl[m] += uniform ? one_bias : b[KEYS ? -(e + m) : e + m];
+          }
+          const float2 x01 = ffma2(make_float2(__uint_as_float(xr[c][e]), __uint_as_float(xr[c][e + 1])), sl2_2, make_float2(nl[0], nl[1]));
+          const float2 x23 = ffma2(make_float2(__uint_as_float(xr[c][e + 2]), __uint_as_float(xr[c][e + 3])), sl2_2, make_float2(nl[2], nl[3]));
+          float2 p01 = make_float2(ex2_approx(x01.x), ex2_approx(x01.y)), p23 = make_float2(ex2_approx(x23.x), ex2_approx(x23.y));
+          if (!whole) {
+            if (!(see >> e & 1u)) p01.x = 0.f;
+            if (!(see >> (e + 1) & 1u)) p01.y = 0.f;
+            if (!(see >> (e + 2) & 1u)) p23.x = 0.f;
+            if (!(see >> (e + 3) & 1u)) p23.y = 0.f;
+          }
+          const float2 d01 = fmul2(p01, fadd2(make_float2(__uint_as_float(yr[c][e]), __uint_as_float(yr[c][e + 1])), make_float2(nd[0], nd[1])));
+          const float2 d23 = fmul2(p23, fadd2(make_float2(__uint_as_float(yr[c][e + 2]), __uint_as_float(yr[c][e + 3])), make_float2(nd[2], nd[3])));
+          pk[e >> 1] = pack_bf16x2(p01.x, p01.y);
+          pk[(e >> 1) + 1] = pack_bf16x2(p23.x, p23.y);
+          dk[e >> 1] = pack_bf16x2(d01.x, d01.y);
+          dk[(e >> 1) + 1] = pack_bf16x2(d23.x, d23.y);
+          if (BIAS && !KEYS) {
+            run[c][e] = d01.x;
+            run[c][e + 1] = d01.y;
+            run[c][e + 2] = d23.x;
+            run[c][e + 3] = d23.y;
+          }
+        }
+        if (KEYS) tmem_st_32x32b_x16(xa + c * 16, pk);
+        tmem_st_32x32b_x16(ya + c * 16, dk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pds_full[g]);
+      if (BIAS && !KEYS && a.d_table != nullptr) {
+        // with the tile's products under way
+#pragma unroll
+        for (int c = 0; c < TC / 32; ++c) {
+          const int b0 = c0 + c * 32, d0 = b0 - (r0 + quad * 32);
+          const int first = run_of[min(max(d0 - 31 + near, 0), 2 * near)], last = run_of[min(max(d0 + 31 + near, 0), 2 * near)];
+          if (first == last) {
+            float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) s = fadd2(s, make_float2(run[c][e], run[c][e + 1]));
+            bins[run_bucket[first] * 256 + slot] += s.x + s.y;
+          } else {
+            // running sums of four pieces of eight, then of the whole
+            float* mine = sums + ((warp - 2) * 32 + lane) * RUN_LD;
+#pragma unroll
+            for (int e = 1; e < 8; ++e)
+#pragma unroll
+              for (int m = 0; m < 32; m += 8) run[c][m + e] += run[c][m + e - 1];
+#pragma unroll
+            for (int m = 8; m < 32; m += 8) {
+              const float base = run[c][m - 1];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) run[c][m + e] += base;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(mine + e) = make_float4(run[c][e], run[c][e + 1], run[c][e + 2], run[c][e + 3]);
+            float before = 0.f;
+            for (int r = first; r <= last; ++r) {
+              const int end = min(max(run_start[r + 1] + row - b0, 0), 32);
+              const float upto = end > 0 ? mine[end - 1] : 0.f;
+              bins[run_bucket[r] * 256 + slot] += upto - before;
+              before = upto;
+            }
+          }
+        }
+      }
+      in_head += 2;
+    }
+    if (ok && n_c > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, &abort_s));
+      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 162, 0);
+    }
+    if (ok) {
+      // dq: each warpgroup stores half of the columns; KEYS: warpgroup 0 dk, warpgroup 1 dv
+      tc_fence_after();
+      bool some = n_c > 0;
+      if (KEYS) {
+        // a key that no query sees may hold anything, and its gradient is zero
+        long long first = 0, end = a.Sq;
+        if (!BIAS) {
+          first = max(row - sight.start, 0);
+          if (row >= a.sinks) end = min(end, static_cast<long long>(row) + a.window - sight.start);
+        }
+        some = some && row < sight.valid && first < end;
+      }
+      const bool second = KEYS && g == 1;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk);
+      const long long* st = !KEYS ? a.dq_strides : second ? a.dv_strides : a.dk_strides;
+      out += batch * st[0] + row * st[1] + blockIdx.y * st[2];
+      const uint32_t acc = tmem_base + lane_addr + (second ? ACC2_COL : ACC1_COL);
+      const float f = second ? 1.f : a.scale;
+      constexpr int CHUNKS = KEYS ? DH / 32 : DH / 64;
+      const int first = KEYS ? 0 : g * CHUNKS;
+#pragma unroll
+      for (int c = first; c < first + CHUNKS; ++c) {
+        uint32_t r[32];
+        if (n_c > 0) {
+          tmem_ld_32x32b_x32(acc + c * 32, r);
+          tmem_wait_ld();
+        }
+        if (row < out_rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (some) {
+              w.x = pack_bf16x2(__uint_as_float(r[e + 0]) * f, __uint_as_float(r[e + 1]) * f);
+              w.y = pack_bf16x2(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
+              w.z = pack_bf16x2(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
+              w.w = pack_bf16x2(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
+            }
+            *reinterpret_cast<uint4*>(out + c * 32 + e) = w;
+          }
+        }
+      }
+    }
+    if (BIAS && !KEYS && a.d_table != nullptr) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float* part = a.table_ws + ((static_cast<long long>(batch) * a.H + blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets;
+      for (int c = warp - 2; c < a.buckets; c += 8) {
+        float s = 0.f;
+#pragma unroll
+        for (int m = 0; m < 256; m += 32) s += bins[c * 256 + m + lane];
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+        if (lane == 0) part[c] = s;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// dsink of one head per block; the order of the sum is fixed by the launch shape
+__global__ void text_dsink_kernel(const __grid_constant__ MdbTextAttnArgs a) {
+  __shared__ float part[256];
+  const int h = blockIdx.x;
+  const float sink = TXT_LOG2E * text_param(a.sink_logits, a.param_f32, h);
+  float s = 0.f;
+  for (int b = 0; b < a.B; ++b) {
+    const long long at = (static_cast<long long>(b) * a.H + h) * a.Sq;
+    for (int i = threadIdx.x; i < a.Sq; i += 256) s += exp2f(sink - a.lse[at + i]) * a.delta[at + i];
+  }
+  part[threadIdx.x] = s;
+  __syncthreads();
+  for (int n = 128; n > 0; n >>= 1) {
+    if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    if (a.param_f32) static_cast<float*>(a.d_sink)[h] = -part[0];
+    else static_cast<__nv_bfloat16*>(a.d_sink)[h] = __float2bfloat16_rn(-part[0]);
+  }
+}
+
+// dtable[:, h]: the parts of all row blocks and sequences, in a fixed order
+__global__ void text_dtable_kernel(const __grid_constant__ MdbTextAttnArgs a, const int blocks) {
+  __shared__ float part[256];
+  const int h = blockIdx.x, c = threadIdx.x % a.buckets, group = threadIdx.x / a.buckets, groups = 256 / a.buckets;
+  float s = 0.f;
+  if (group < groups)
+    for (int r = group; r < a.B * blocks; r += groups)
+      s += a.table_ws[((static_cast<long long>(r / blocks) * a.H + h) * blocks + r % blocks) * a.buckets + c];
+  part[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < a.buckets) {
+    for (int n = 1; n < groups; ++n) s += part[n * a.buckets + c];
+    const long long to = static_cast<long long>(c) * a.H + h;
+    if (a.param_f32) static_cast<float*>(a.d_table)[to] = s;
+    else static_cast<__nv_bfloat16*>(a.d_table)[to] = __float2bfloat16_rn(s);
+  }
+}
+
+static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh, const long long* strides, int rows) {
+  int64_t ext[4] = {Dh, S, H, B};
+  int64_t str[4] = {2, strides[1] * 2, strides[2] * 2, strides[0] * 2};
+  int box[4] = {64, rows, 1, 1};
+  return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
+}
+
+template <int DH, bool KEYS, bool BIAS>
+static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, cudaStream_t st) {
+  using Shape = TextBwdShape<DH, KEYS, BIAS>;
+  constexpr int MOST = 225 * 1024;                 // beside what the kernel declares itself
+  const int smem = BIAS ? Shape::bytes(text_near(a), a.buckets) : Shape::bytes(0, 0);
+  if (smem > MOST) return -6;
+  auto kern = text_bwd_kernel<DH, KEYS, BIAS>;
+  static bool ready[TXT_DEVICES];
+  if (int r = allow_smem(kern, MOST, ready)) return r;
+  kern<<<dim3(((KEYS ? a.Skv : a.Sq) + TR - 1) / TR, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <int DH>
+static int text_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
+  TextBwdMaps maps;
+  int r;
+  if ((r = bwd_map(&maps.r1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TR))) return 1000 + r;
+  if ((r = bwd_map(&maps.r2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TR))) return 1100 + r;
+  if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
+  if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
+  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, st) : launch_text_bwd<DH, false, false>(maps, a, st))) return r;
+  if ((r = bwd_map(&maps.r1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
+  if ((r = bwd_map(&maps.r2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
+  if ((r = bwd_map(&maps.c1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
+  if ((r = bwd_map(&maps.c2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
+  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, st) : launch_text_bwd<DH, true, false>(maps, a, st);
+}
+
+int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
+  if (int r = a.Dh == 128 ? text_backward<128>(a, st) : text_backward<64>(a, st)) return r;
+  if (a.d_sink != nullptr) text_dsink_kernel<<<a.H, 256, 0, st>>>(a);
+  if (a.d_table != nullptr) text_dtable_kernel<<<a.H, 256, 0, st>>>(a, (a.Sq + TR - 1) / TR);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace mdb
+
+MDB_DEFINE_WAIT_LIMIT_SETTER(mdb_set_wait_limit_text_bwd)

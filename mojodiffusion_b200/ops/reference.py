@@ -288,7 +288,7 @@ def relative_bucket(rel: torch.Tensor, num_buckets: int, max_distance: int) -> t
 
 
 def relative_attention(q, k, v, table, max_distance: int = 128, scale: float = 1.0, kv_len: Optional[torch.Tensor] = None):
-    """q [B, Sq, H, Dh], k / v [B, Skv, Hkv, Dh], table [buckets, H]: score + table[bucket(j - i), h] over the keys j < kv_len."""
+    """q [B, Sq, H, Dh], k / v [B, Skv, H, Dh], table [buckets, H]: score + table[bucket(j - i), h] over the keys j < kv_len."""
     Sq, Skv = q.shape[1], k.shape[1]
     key = torch.arange(Skv, device=q.device)
     which = relative_bucket(key[None, :] - torch.arange(Sq, device=q.device)[:, None], table.shape[0], max_distance)

@@ -18,8 +18,8 @@ import torch
 from . import native, reference as ref
 
 _NO_WINDOW = 1 << 30
-#: buckets and distances that the kernels' tables hold
-MAX_BUCKETS, MAX_DISTANCE = 128, 1024
+#: buckets (by head width) and distances that the kernels' tables hold; beyond them the torch statement runs
+MAX_BUCKETS, MAX_DISTANCE = {64: 64, 128: 32}, 1024
 
 
 def _ops():
@@ -144,7 +144,7 @@ def _buckets(num_buckets: int, max_distance: int):
 
 def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int = 128, scale: float = 1.0,
                        kv_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Bidirectional attention with a learned bias: q [B, Sq, H, Dh], k / v [B, Skv, Hkv, Dh] (any strides) -> [B, Sq, H, Dh].
+    """Bidirectional attention with a learned bias: q [B, Sq, H, Dh], k / v [B, Skv, H, Dh] (any strides) -> [B, Sq, H, Dh].
 
     ``table`` [num_buckets, H] (an even number, at least 4; the weight of the encoders' ``relative_attention_bias``) is added to the score of query i and
     key j at the bucket of j - i: half of the buckets per direction, single distances first, then distances that grow by equal factors up to
@@ -153,11 +153,13 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     """
     name = "relative_attention"
     _check(name, q, k, v, kv_len, out)
+    if k.shape[2] != q.shape[2]:
+        raise ValueError(f"{name}: q, k and v with the same heads")
     if table.dim() != 2 or table.shape[1] != q.shape[2] or table.shape[0] < 4 or table.shape[0] % 2 or not table.is_floating_point() or table.device != q.device:
         raise ValueError(f"{name}: table must be [num_buckets, H] on q's device, num_buckets even and at least 4")
     if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
         raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
-    if (not _native(q, k, scale, v, kv_len, table) or table.dtype not in (torch.float32, torch.bfloat16) or table.shape[0] > MAX_BUCKETS
+    if (not _native(q, k, scale, v, kv_len, table) or table.dtype not in (torch.float32, torch.bfloat16) or table.shape[0] > MAX_BUCKETS[q.shape[3]]
             or max_distance > MAX_DISTANCE):
         o = ref.relative_attention(q, k, v, table, max_distance, scale, kv_len)
         return out.copy_(o) if out is not None else o

@@ -44,8 +44,8 @@ def test_window_attention_and_its_gradients(case):
 
 @pytest.mark.parametrize("buckets,distance,kv_len", [(32, 128, None), (8, 10, [30, 7]), (4, 3, [0, 30])])
 def test_relative_attention_and_its_gradients(buckets, distance, kv_len):
-    B, S, H, G = 2, 30, 4, 2
-    q, k, v = (_normal(B, S, h, 8, seed=i).requires_grad_() for i, h in enumerate((H, G, G)))
+    B, S, H = 2, 30, 4
+    q, k, v = (_normal(B, S, H, 8, seed=i).requires_grad_() for i in range(3))
     table, grad = _normal(buckets, H, seed=5).requires_grad_(), _normal(B, S, H, 8, seed=6)
     n = torch.tensor(kv_len, dtype=torch.int32) if kv_len is not None else None
     value, _ = oracle(q, k, v, 0.5, seen_by(S, S, B, kv_len=n, causal=False), grad, table=table, max_distance=distance)
@@ -83,7 +83,7 @@ def test_outputs_and_empty_inputs():
     table = _normal(32, 4, seed=3, dtype=torch.bfloat16)
     out = torch.empty_like(q)
     assert O.window_attention(q, k, k, 2, out=out) is out and torch.equal(out, O.window_attention(q, k, k, 2))
-    assert O.relative_attention(q, k, k, table, out=out) is out and torch.equal(out, O.relative_attention(q, k, k, table))
+    assert O.relative_attention(q, q, q, table, out=out) is out and torch.equal(out, O.relative_attention(q, q, q, table))
     assert O.window_attention(q[:0], k[:0], k[:0]).shape == (0, 5, 4, 8)
     assert O.window_attention(q[:, :0], k, k).shape == (2, 0, 4, 8)
     assert float(O.window_attention(q, k[:, :0], k[:, :0]).abs().max()) == 0
@@ -100,7 +100,7 @@ def test_refusals():
                  lambda: w(q, k, k, q_start=ints(1, 2, 3)), lambda: w(q, k, k, q_start=1.0), lambda: w(q, k, k, q_start=torch.tensor([1, 2])),
                  lambda: w(q, k, k, sink_logits=_normal(2, seed=1)), lambda: w(q, k, k, sink_logits=torch.ones(4, dtype=torch.long)), lambda: w(q, k, k, out=q[:, :2]),
                  lambda: w(q, k, k, out=torch.empty_like(q, dtype=torch.float64)), lambda: w(q, k[:, :, :0], k[:, :, :0]),
-                 lambda: r(q, k, k, table[:, :3]), lambda: r(q, k, k, table[:31]), lambda: r(q, k, k, table[:2]), lambda: r(q, k, k, table[0]), lambda: r(q, k, k, table.long()),
-                 lambda: r(q, k, k, table, 8), lambda: r(q, k, k, table, 100.0), lambda: r(q, k, k, table, kv_len=ints(1)), lambda: r(q, k, k, table, out=q[:1])):
+                 lambda: r(q, q, q, table[:, :3]), lambda: r(q, q, q, table[:31]), lambda: r(q, q, q, table[:2]), lambda: r(q, q, q, table[0]), lambda: r(q, q, q, table.long()),
+                 lambda: r(q, q, q, table, 8), lambda: r(q, q, q, table, 100.0), lambda: r(q, q, q, table, kv_len=ints(1)), lambda: r(q, q, q, table, out=q[:1]), lambda: r(q, k, k, table)):
         with pytest.raises(ValueError):
             call()

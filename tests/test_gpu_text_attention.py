@@ -81,18 +81,21 @@ def test_window_attention_gradients(case):
     check(dict(zip(("out", "dq", "dk", "dv", "dsink"), (out, *got))), value, bound, str(case))
 
 
-# B, S, H, Hkv, Dh, buckets, max_distance, kv_len, fp32 table
+# B, S, H, H, Dh, buckets, max_distance, kv_len, fp32 table
 RELATIVE = [
     (1, 1, 4, 4, 64, 32, 128, None, False),
     (2, 77, 4, 4, 64, 32, 128, [77, 40], False),
     (1, 128, 3, 3, 64, 32, 128, None, False),
     (1, 300, 2, 2, 128, 32, 128, None, True),
     (3, 257, 2, 2, 64, 32, 128, [257, 0, 129], False),
-    (1, 600, 4, 2, 64, 32, 128, None, False),
+    (1, 600, 4, 4, 64, 32, 128, None, False),
     (2, 190, 2, 2, 64, 64, 200, [11, 190], False),
-    (1, 333, 2, 1, 128, 8, 3, None, False),
+    (1, 333, 2, 2, 128, 8, 3, None, False),
     (1, 150, 2, 2, 64, 4, 100, None, True),
-    (1, 700, 1, 1, 64, 128, 1024, None, False),
+    (1, 700, 1, 1, 64, 64, 1024, None, False),
+    (1, 260, 2, 2, 128, 32, 1000, [259], False),
+    (1, 260, 2, 2, 64, 32, 9, None, False),             # all borders at one distance
+    (1, 200, 2, 2, 64, 66, 128, None, False),           # more buckets than the kernels keep: the torch statement
 ]
 
 
@@ -201,6 +204,7 @@ def test_layouts(layout, Sq):
     value, bound = oracle(q, k, v, D ** -0.5, seen_by(Sq, Skv, B, 40, 3, None, at))
     check(dict(out=O.window_attention(q, k, v, 40, 3, q_start=at)), value, bound, layout)
     table = _normal(32, 2 * H, seed=93)[:, ::2]
+    k, v = make(B, Skv, H, D, 94), make(B, Skv, H, D, 95)
     value, bound = oracle(q, k, v, D ** -0.5, seen_by(Sq, Skv, B, causal=False), table=table)
     check(dict(out=O.relative_attention(q, k, v, table, scale=D ** -0.5)), value, bound, layout)
 
@@ -243,12 +247,13 @@ def test_out_buffers():
 
 def test_the_same_bits_every_time():
     q, k, v = (t.requires_grad_() for t in _inputs(2, 700, 700, 8, 2, 64, seed=120))
+    q2, k2 = (_normal(2, 700, 8, 64, seed=i).requires_grad_() for i in (127, 128))
     grad, table, sink = _normal(2, 700, 8, 64, seed=124), _normal(32, 8, seed=125).requires_grad_(), _normal(8, seed=126).requires_grad_()
 
     def both():
         a = O.window_attention(q, k, v, 100, 4, sink_logits=sink)
-        b = O.relative_attention(q, k, v, table, scale=0.125)
-        return [a, b, *torch.autograd.grad(a, [q, k, v, sink], grad), *torch.autograd.grad(b, [q, k, v, table], grad)]
+        b = O.relative_attention(q, q2, k2, table, scale=0.125)
+        return [a, b, *torch.autograd.grad(a, [q, k, v, sink], grad), *torch.autograd.grad(b, [q, q2, k2, table], grad)]
 
     first = both()
     for _ in range(3):
@@ -363,8 +368,8 @@ def test_other_types_and_widths_take_the_torch_statement():
         value, _ = oracle(q, k, v, D ** -0.5, seen_by(20, 20, 1, 6, 1))
         assert float((O.window_attention(q, k, v, 6, 1).double() - value["out"]).abs().max()) < tol
         table = _normal(16, 4, seed=330, dtype=dtype)
-        value, _ = oracle(q, k, v, 0.1, seen_by(20, 20, 1, causal=False), table=table, max_distance=20)
-        assert float((O.relative_attention(q, k, v, table, 20, 0.1).double() - value["out"]).abs().max()) < tol
+        value, _ = oracle(q, q, q, 0.1, seen_by(20, 20, 1, causal=False), table=table, max_distance=20)
+        assert float((O.relative_attention(q, q, q, table, 20, 0.1).double() - value["out"]).abs().max()) < tol
 
 
 def test_nothing_to_do():
@@ -374,6 +379,7 @@ def test_nothing_to_do():
     assert O.window_attention(q, k, k).shape == (1, 0, 4, 64)
     q, k = _normal(1, 3, 4, 64, seed=1), _normal(1, 0, 2, 64, seed=1)
     assert float(O.window_attention(q, k, k).abs().max()) == 0
+    k = _normal(1, 0, 4, 64, seed=1)
     assert float(O.relative_attention(q, k, k, _normal(32, 4, seed=2)).abs().max()) == 0
 
 
@@ -390,6 +396,7 @@ def test_native_refusals():
                 dict(q=_normal(2, 8, 4, 65, seed=1)[..., 1:]), dict(k=k[:1].expand(2, 8, 2, 64)), dict(rule=[0, 0, 0]), dict(rule=[4, -1, 0]), dict(rule=[4]),
                 dict(n=_ints([1])), dict(n=torch.tensor([1, 1], device=DEV)), dict(at=torch.tensor([1, 1], dtype=torch.int32)), dict(sink=_normal(3, seed=1)),
                 dict(sink=_normal(4, seed=1, dtype=torch.float16)), dict(table=table), dict(table=table, buckets=[16, 4, 9]), dict(table=table, buckets=[32, 8] + [9] * 40),
-                dict(table=table, buckets=[32, 8, 5000]), dict(sink=_normal(4, seed=1), table=table, buckets=[32, 8, 9]), dict(out=q[:, :4])):
+                dict(table=table, buckets=[32, 8, 9], k=q, v=q, at=None, rule=[4]), dict(table=table, buckets=[32, 8, 9]), dict(table=table, buckets=[32, 8, 5000], k=q, v=q),
+                dict(table=table, buckets=[32, 8, 20, 10], k=q, v=q), dict(table=table, buckets=[32, 16], k=q, v=q), dict(sink=_normal(4, seed=1), table=table, buckets=[32, 8, 9]), dict(out=q[:, :4])):
         with pytest.raises(RuntimeError):
             ok(**bad)
