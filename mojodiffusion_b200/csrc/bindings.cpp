@@ -1402,7 +1402,7 @@ void set_wait_limit_ns(int64_t ns) {
   const unsigned long long v = static_cast<unsigned long long>(ns);
   const int rc = mdb_set_wait_limit_gemm(v) | mdb_set_wait_limit_attn_fwd(v) | mdb_set_wait_limit_attn_bwd(v) |
                  mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v) | mdb_set_wait_limit_text_fwd(v) |
-                 mdb_set_wait_limit_text_bwd(v);
+                 mdb_set_wait_limit_text_bwd(v) | mdb_set_wait_limit_text_step(v);
   TORCH_CHECK(rc == 0, "set_wait_limit_ns failed: ", rc);
 }
 

@@ -59,6 +59,7 @@ int mdb_set_wait_limit_comm(unsigned long long ns);
 int mdb_set_wait_limit_mxfp8(unsigned long long ns);
 int mdb_set_wait_limit_text_fwd(unsigned long long ns);
 int mdb_set_wait_limit_text_bwd(unsigned long long ns);
+int mdb_set_wait_limit_text_step(unsigned long long ns);
 
 #ifdef __cplusplus
 }

@@ -29,7 +29,7 @@ static int check_args(const MdbTextAttnArgs* a) {
 
 extern "C" int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st) {
   if (int r = mdb::check_args(a)) return r;
-  return mdb::text_attention_prompt(*a, st);
+  return mdb::text_attention_is_step(*a) ? mdb::text_attention_step(*a, st) : mdb::text_attention_prompt(*a, st);
 }
 
 extern "C" long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a) {
