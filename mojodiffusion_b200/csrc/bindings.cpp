@@ -7,7 +7,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <string>
@@ -519,120 +521,166 @@ std::tuple<Tensor, Tensor, Tensor> attention_bwd(const Tensor& q, const Tensor& 
 // ------------------------------------------------------------------------------------------
 // attention of the language models: sliding window / first tokens / sink logits, relative position buckets
 // ------------------------------------------------------------------------------------------
-// one of q, k, v, o and their gradients: bf16 [B, S, heads, Dh] with 16-byte rows. A dimension of one element takes any stride.
-void text_operand(const Tensor& t, const Tensor& like, int64_t S, int64_t heads, long long (&strides)[3], const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(0) == like.size(0) &&
-                  t.size(1) == S && t.size(2) == heads && t.size(3) == like.size(3) && t.stride(3) == 1,
-              "text attention: ", name, " must be bf16 [B, S, heads, Dh] on q's device with contiguous Dh");
-  for (int i = 0; i < 3; ++i) {
-    strides[i] = t.size(i) == 1 ? 8 : t.stride(i);
-    TORCH_CHECK(strides[i] % 8 == 0 && strides[i] > 0, "text attention: rows of ", name, " must start on 16-byte boundaries");
-  }
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "text attention: ", name, " must start on a 16-byte boundary");
+// A refused argument raises ValueError, as the Python layer's own checks do.
+#define TEXT_CHECK(cond, ...) TORCH_CHECK_VALUE(cond, "text attention: ", __VA_ARGS__)
+
+// whether the kernels read and write this layout: contiguous Dh, other strides positive multiples of 8 elements, a 16-byte address
+bool text_layout(const Tensor& t) {
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  return ok;
 }
-const int* text_per_sequence(const optional<Tensor>& t, const Tensor& q, const char* name) {
-  if (!t.has_value() || !t->defined()) return nullptr;
-  TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->numel() == q.size(0),
-              "text attention: ", name, " must be [B] int32 on q's device");
-  return t->data_ptr<int>();
+// one of q, k, v, o and their gradients, bf16 [B, S, heads, Dh], copied where its layout is another one
+Tensor text_rows(const Tensor& t, const Tensor& like, int64_t S, int64_t heads, long long (&strides)[3], const char* name) {
+  TEXT_CHECK(t.device() == like.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(0) == like.size(0) && t.size(1) == S && t.size(2) == heads &&
+                 t.size(3) == like.size(3), name, " must be bf16 [B, S, heads, Dh] with the sizes of the others, on q's device");
+  Tensor r = text_layout(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+  for (int i = 0; i < 3; ++i) strides[i] = r.size(i) == 1 ? 8 : r.stride(i);      // a dimension of one element takes any stride
+  return r;
 }
-// masks and parameters that the forward and the backward pass share. rule: {window, sinks, q_start}; buckets: {count, exact, borders ...} or empty
-void text_rule(MdbTextAttnArgs& a, const Tensor& q, const Tensor& k, double scale, const std::vector<int64_t>& rule, const optional<Tensor>& kv_len,
-               const optional<Tensor>& q_start, const optional<Tensor>& sink_logits, const optional<Tensor>& table, const std::vector<int64_t>& buckets) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128) && k.size(2) > 0 && q.size(2) % k.size(2) == 0 && rule.size() == 3,
-              "text attention: q [B, Sq, H, Dh], k [B, Skv, Hkv, Dh], Dh 64 or 128, Hkv a divisor of H");
-  for (int i = 1; i < 3; ++i) TORCH_CHECK(q.size(i) < (1ll << 30) && k.size(i) < (1ll << 30), "text attention: too many rows");
-  TORCH_CHECK(q.size(0) <= 65535 && q.size(2) <= 65535, "text attention: at most 65535 sequences and heads");
-  TORCH_CHECK(rule[0] >= 1 && rule[1] >= 0, "text attention: window and sinks");
+// whether the call may write `out` in place: the kernels' layout, every element once, and no memory that the call reads
+bool text_writable(const Tensor& out, std::initializer_list<const Tensor*> read) {
+  if (!text_layout(out)) return false;
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int i = 0; i < 4; ++i)
+    if (out.size(i) > 1) dims.emplace_back(out.stride(i), out.size(i));
+  std::sort(dims.begin(), dims.end());
+  for (size_t i = 1; i < dims.size(); ++i)
+    if (dims[i].first < dims[i - 1].first * dims[i - 1].second) return false;
+  for (const Tensor* t : read)
+    if (t->defined() && t->is_alias_of(out)) return false;
+  return true;
+}
+Tensor text_per_sequence(const optional<Tensor>& t, const Tensor& q, const char* name) {
+  if (!t.has_value() || !t->defined()) return Tensor();
+  TEXT_CHECK(t->device() == q.device() && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == q.size(0), name, " must be int32 [B] on q's device");
+  return t->contiguous();
+}
+// One call's operands: the arguments of the launch and what owns the memory that they name.
+struct TextCall {
+  MdbTextAttnArgs a;
+  Tensor q, k, v, kv_len, q_start, param;
+};
+// buckets: {count, exact, borders ...} and a table, or empty and sink logits (or no parameter)
+TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int64_t window, int64_t sinks, const optional<Tensor>& kv_len, int64_t q_start,
+                   const optional<Tensor>& q_starts, const optional<Tensor>& param, const std::vector<int64_t>& buckets) {
+  TextCall c;
+  MdbTextAttnArgs& a = c.a;
+  memset(&a, 0, sizeof(a));
+  TEXT_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128), "q [B, Sq, H, Dh] and k [B, Skv, Hkv, Dh] on a GPU, Dh 64 or 128");
+  TEXT_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "k and v need a number of heads that divides q's");
+  for (int i = 0; i < 3; ++i) TEXT_CHECK(q.size(i) < (i == 1 ? 1ll << 30 : 65536) && k.size(i) < (i == 1 ? 1ll << 30 : 65536), "fewer than 2^30 rows, 65536 sequences and heads");
+  TEXT_CHECK(window >= 1 && sinks >= 0, "window of at least 1, sinks of at least 0");
+  TEXT_CHECK(scale > 0 && std::isfinite(scale), "a positive scale");
   const int64_t far = 1 << 30;
   a.B = (int)q.size(0); a.Sq = (int)q.size(1); a.H = (int)q.size(2); a.Dh = (int)q.size(3); a.Skv = (int)k.size(1); a.Hkv = (int)k.size(2);
-  a.window = (int)std::min(rule[0], far);
-  a.sinks = (int)std::min(rule[1], far);
-  a.q_start = (int)std::max(std::min(rule[2], far), -far);
+  a.window = (int)std::min(window, far);
+  a.sinks = (int)std::min(sinks, far);
+  a.q_start = (int)std::max(std::min(q_start, far), -far);
   a.scale = (float)scale;
-  a.kv_len = text_per_sequence(kv_len, q, "kv_len");
-  a.q_start_ptr = text_per_sequence(q_start, q, "q_start");
-  for (const optional<Tensor>* t : {&sink_logits, &table}) {
-    if (!t->has_value() || !(*t)->defined()) continue;
-    const Tensor& p = **t;
-    const bool is_table = t == &table;
-    TORCH_CHECK(p.is_cuda() && p.device() == q.device() && p.is_contiguous() && (p.scalar_type() == at::kFloat || p.scalar_type() == at::kBFloat16) &&
-                    p.numel() == a.H * (is_table ? (buckets.empty() ? 0 : buckets[0]) : 1),
-                "text attention: ", is_table ? "table must be [buckets, H]" : "sink_logits must be [H]", ", fp32 or bf16, on q's device");
-    a.param_f32 = p.scalar_type() == at::kFloat;
-    (is_table ? a.table : a.sink_logits) = p.data_ptr();
+  c.kv_len = text_per_sequence(kv_len, q, "kv_len");
+  c.q_start = text_per_sequence(q_starts, q, "q_start");
+  if (c.kv_len.defined()) a.kv_len = c.kv_len.data_ptr<int>();
+  if (c.q_start.defined()) a.q_start_ptr = c.q_start.data_ptr<int>();
+  if (param.has_value() && param->defined()) {
+    const bool table = !buckets.empty();
+    TEXT_CHECK(param->device() == q.device() && (param->scalar_type() == at::kFloat || param->scalar_type() == at::kBFloat16) && param->dim() == (table ? 2 : 1) &&
+                   param->size(-1) == a.H && (!table || param->size(0) == buckets[0]),
+               table ? "table must be [buckets, H]" : "sink_logits must be [H]", ", fp32 or bf16, on q's device");
+    c.param = param->contiguous();
+    a.param_f32 = c.param.scalar_type() == at::kFloat;
+    (table ? a.table : a.sink_logits) = c.param.data_ptr();
   }
-  TORCH_CHECK(a.table == nullptr || a.sink_logits == nullptr, "text attention: a table or sink logits");
-  if (a.table != nullptr) {
-    TORCH_CHECK(buckets.size() >= 2 && buckets[0] <= MDB_TEXT_MAX_BUCKETS && (int64_t)buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 2, "text attention: buckets");
+  if (!buckets.empty()) {
+    TEXT_CHECK(a.table != nullptr && a.Hkv == a.H && buckets.size() >= 2 && buckets[0] * a.Dh <= MDB_TEXT_MAX_BUCKETS * 64 && buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 2 &&
+                   buckets.back() <= MDB_TEXT_MAX_DISTANCE, "buckets");
     a.buckets = (int)buckets[0];
     a.exact = (int)buckets[1];
     a.n_borders = (int)buckets.size() - 2;
     for (int i = 0; i < a.n_borders; ++i) a.borders[i] = (int)buckets[i + 2];
   }
+  c.q = text_rows(q, q, a.Sq, a.H, a.q_strides, "q");
+  c.k = text_rows(k, q, a.Skv, a.Hkv, a.k_strides, "k");
+  c.v = text_rows(v, q, a.Skv, a.Hkv, a.v_strides, "v");
+  a.q = c.q.data_ptr(); a.k = c.k.data_ptr(); a.v = c.v.data_ptr();
   a.status = status_ptr(q);
+  return c;
+}
+Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse) {
+  MdbTextAttnArgs& a = c.a;
+  const bool given = out.has_value() && out->defined();
+  if (given) TEXT_CHECK(out->sizes() == c.q.sizes() && out->scalar_type() == at::kBFloat16 && out->device() == c.q.device(), "out must have q's shape, type and device");
+  Tensor o = given && text_writable(*out, {&c.q, &c.k, &c.v, &c.param, &c.kv_len, &c.q_start}) ? *out : at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
+  if (lse != nullptr) *lse = at::empty({a.B, a.H, a.Sq}, c.q.options().dtype(at::kFloat));
+  if (c.q.numel() > 0 && c.k.numel() > 0) {
+    for (int i = 0; i < 3; ++i) a.o_strides[i] = o.size(i) == 1 ? 8 : o.stride(i);
+    a.o = o.data_ptr();
+    if (lse != nullptr) a.lse = lse->data_ptr<float>();
+    check_rc(mdb_text_attention_fwd(&a, cur_stream()), "text_attention_fwd");
+  } else {
+    o.zero_();
+    if (lse != nullptr) lse->fill_(INFINITY);
+  }
+  if (!given || o.is_same(*out)) return o;
+  Tensor to = *out;
+  to.copy_(o);
+  return to;
 }
 
-std::tuple<Tensor, Tensor> text_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, double scale, std::vector<int64_t> rule,
-                                              const optional<Tensor>& kv_len, const optional<Tensor>& q_start, const optional<Tensor>& sink_logits,
-                                              const optional<Tensor>& table, std::vector<int64_t> buckets, bool need_lse, const optional<Tensor>& out) {
-  TORCH_CHECK(q.is_cuda(), "text attention: CUDA tensors");
-  c10::cuda::CUDAGuard guard(q.device());
-  MdbTextAttnArgs a;
-  memset(&a, 0, sizeof(a));
-  text_rule(a, q, k, scale, rule, kv_len, q_start, sink_logits, table, buckets);
-  Tensor o = out.has_value() && out->defined() ? *out : at::empty({a.B, a.Sq, a.H, a.Dh}, q.options());
-  text_operand(q, q, a.Sq, a.H, a.q_strides, "q");
-  text_operand(k, q, a.Skv, a.Hkv, a.k_strides, "k");
-  text_operand(v, q, a.Skv, a.Hkv, a.v_strides, "v");
-  text_operand(o, q, a.Sq, a.H, a.o_strides, "out");
-  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr();
-  Tensor lse;
-  if (need_lse) {
-    lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
-    a.lse = lse.data_ptr<float>();
-  }
-  check_rc(mdb_text_attention_fwd(&a, cur_stream()), "text_attention_fwd");
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, const optional<Tensor>& kv_len, int64_t q_start,
+                        const optional<Tensor>& q_starts, const optional<Tensor>& sink_logits, const optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, sink_logits, {});
+  return text_forward(c, out, nullptr);
+}
+Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, std::vector<int64_t> buckets, double scale, const optional<Tensor>& kv_len,
+                          const optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  TextCall c = text_call(q, k, v, scale, 1 << 30, 0, kv_len, 0, {}, table, buckets);
+  return text_forward(c, out, nullptr);
+}
+// the two passes of the autograd node
+std::tuple<Tensor, Tensor> text_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale, int64_t window, int64_t sinks,
+                                              const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts, std::vector<int64_t> buckets) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
+  Tensor lse, o = text_forward(c, {}, &lse);
   return {o, lse};
 }
-
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> text_attention_bwd(
-    const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse, const Tensor& dout, double scale, std::vector<int64_t> rule,
-    const optional<Tensor>& kv_len, const optional<Tensor>& q_start, const optional<Tensor>& sink_logits, const optional<Tensor>& table,
-    std::vector<int64_t> buckets, bool need_param) {
-  TORCH_CHECK(q.is_cuda(), "text attention: CUDA tensors");
-  c10::cuda::CUDAGuard guard(q.device());
-  MdbTextAttnArgs a;
-  memset(&a, 0, sizeof(a));
-  text_rule(a, q, k, scale, rule, kv_len, q_start, sink_logits, table, buckets);
-  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.H * a.Sq, "text attention: lse");
-  Tensor dq = at::empty({a.B, a.Sq, a.H, a.Dh}, q.options());
-  Tensor dk = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options()), dv = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options());
-  text_operand(q, q, a.Sq, a.H, a.q_strides, "q");
-  text_operand(k, q, a.Skv, a.Hkv, a.k_strides, "k");
-  text_operand(v, q, a.Skv, a.Hkv, a.v_strides, "v");
-  text_operand(o, q, a.Sq, a.H, a.o_strides, "out");
-  text_operand(dout, q, a.Sq, a.H, a.do_strides, "the output's gradient");
-  text_operand(dq, q, a.Sq, a.H, a.dq_strides, "dq");
-  text_operand(dk, q, a.Skv, a.Hkv, a.dk_strides, "dk");
-  text_operand(dv, q, a.Skv, a.Hkv, a.dv_strides, "dv");
-  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr(); a.dout = dout.data_ptr();
+std::tuple<Tensor, Tensor, Tensor, Tensor> text_attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, const Tensor& o,
+                                                              const Tensor& lse, const Tensor& dout, double scale, int64_t window, int64_t sinks,
+                                                              const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts,
+                                                              std::vector<int64_t> buckets, bool need_param) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
+  MdbTextAttnArgs& a = c.a;
+  TEXT_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.H * a.Sq, "lse");
+  Tensor o_ = text_rows(o, q, a.Sq, a.H, a.o_strides, "the output"), d = text_rows(dout, q, a.Sq, a.H, a.do_strides, "the output's gradient");
+  Tensor dq = at::empty({a.B, a.Sq, a.H, a.Dh}, q.options()), dk = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options()), dv = at::empty_like(dk), dparam, ws;
+  if (need_param && c.param.defined()) dparam = at::empty_like(c.param);
+  if (c.q.numel() == 0 || c.k.numel() == 0) {
+    for (Tensor* t : {&dq, &dk, &dv, &dparam})
+      if (t->defined()) t->zero_();
+    return {dq, dk, dv, dparam};
+  }
+  text_rows(dq, q, a.Sq, a.H, a.dq_strides, "dq");
+  text_rows(dk, q, a.Skv, a.Hkv, a.dk_strides, "dk");
+  text_rows(dv, q, a.Skv, a.Hkv, a.dv_strides, "dv");
+  a.o = o_.data_ptr(); a.dout = d.data_ptr();
   a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
   a.lse = lse.data_ptr<float>();
-  Tensor delta = at::empty({a.B, a.H, a.Sq}, lse.options()), dtable, dsink, ws;
+  Tensor delta = at::empty({a.B, a.H, a.Sq}, lse.options());
   a.delta = delta.data_ptr<float>();
-  if (need_param && a.table != nullptr) {
-    dtable = at::empty_like(*table);
-    a.d_table = dtable.data_ptr();
+  if (dparam.defined() && a.table != nullptr) {
+    a.d_table = dparam.data_ptr();
     ws = at::empty({mdb_text_attention_bwd_floats(&a)}, lse.options());
     a.table_ws = ws.data_ptr<float>();
+  } else if (dparam.defined()) {
+    a.d_sink = dparam.data_ptr();
   }
-  if (need_param && a.sink_logits != nullptr) {
-    dsink = at::empty_like(*sink_logits);
-    a.d_sink = dsink.data_ptr();
-  }
+  g_launches.fetch_add(dparam.defined() ? 2 : 1, std::memory_order_relaxed);
   check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");
-  return {dq, dk, dv, dtable, dsink};
+  return {dq, dk, dv, dparam};
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1433,6 +1481,8 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("pad_channels", &pad_channels);
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
+  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor? out) -> Tensor", &window_attention);
+  m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor? out) -> Tensor", &relative_attention);
   m.def("text_attention_fwd", &text_attention_fwd);
   m.def("text_attention_bwd", &text_attention_bwd);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);

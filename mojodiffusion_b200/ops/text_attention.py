@@ -4,14 +4,14 @@
 sink logits are those of serenitymojo/models/text_encoder/gpt_oss_encoder.mojo:14-44), ``relative_attention`` the bidirectional encoders
 whose layers add a learned bias for buckets of relative positions (serenitymojo/models/text_encoder/t5_encoder.mojo).
 
-bf16 tensors with heads of 64 or 128 on a GPU run the kernels of ``csrc/text_attention.cu``, forward and backward; other types, other
+bf16 tensors with heads of 64 or 128 on a GPU run the kernels of ``csrc/text_attention*.cu``, forward and backward; other types, other
 head widths and the CPU run the torch statements of ``ops.reference``. Keys and values that no query sees are not read: they may hold anything.
 """
 from __future__ import annotations
 
 import functools
 import math
-from typing import Optional, Sequence, Union
+from typing import Optional, Union
 
 import torch
 
@@ -22,48 +22,25 @@ _NO_WINDOW = 1 << 30
 MAX_BUCKETS, MAX_DISTANCE = {64: 64, 128: 32}, 1024
 
 
-def _ops():
-    return native.ops()
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """[B, S, heads, Dh] as the kernels read it: contiguous Dh, other strides positive multiples of 8 elements, a 16-byte address."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride())):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _writable(out: torch.Tensor, *read: torch.Tensor) -> bool:
-    """Whether the kernels can write ``out`` in place: rows as they store them, each element once, and no memory that the call reads."""
-    if _rows16(out) is not out:
-        return False
-    dims = sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1)
-    if any(s1 < s0 * n0 for (s0, n0), (s1, _) in zip(dims, dims[1:])):
-        return False
-    mine = out.untyped_storage().data_ptr()
-    return all(t.untyped_storage().data_ptr() != mine for t in read)
-
-
 class _TextAttentionFn(torch.autograd.Function):
     """One node for both operators: ``param`` is the table of position buckets (``buckets`` not empty) or the sink logits, or None."""
 
     @staticmethod
-    def forward(ctx, q, k, v, param, scale, rule, kv_len, q_start, buckets):
-        sink, table = (None, param) if buckets else (param, None)
-        o, lse = _ops().text_attention_fwd(q, k, v, scale, rule, kv_len, q_start, sink, table, buckets, True, None)
-        ctx.save_for_backward(q, k, v, o, lse, param, kv_len, q_start)
-        ctx.cfg = (scale, rule, buckets)
+    def forward(ctx, q, k, v, param, scale, window, sinks, kv_len, q_start, buckets):
+        start, starts = (0, q_start) if isinstance(q_start, torch.Tensor) else (q_start, None)
+        o, lse = native.ops().text_attention_fwd(q, k, v, param, scale, window, sinks, kv_len, start, starts, buckets)
+        ctx.save_for_backward(q, k, v, param, o, lse, kv_len, starts)
+        ctx.cfg = (scale, window, sinks, start, buckets)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, param, kv_len, q_start = ctx.saved_tensors
-        scale, rule, buckets = ctx.cfg
-        sink, table = (None, param) if buckets else (param, None)
-        dq, dk, dv, dtable, dsink = _ops().text_attention_bwd(q, k, v, o, lse, _rows16(do), scale, rule, kv_len, q_start, sink, table, buckets,
-                                                              param is not None and ctx.needs_input_grad[3])
-        return dq, dk, dv, dtable if buckets else dsink, None, None, None, None, None
+        q, k, v, param, o, lse, kv_len, starts = ctx.saved_tensors
+        scale, window, sinks, start, buckets = ctx.cfg
+        need = param is not None and ctx.needs_input_grad[3]
+        dq, dk, dv, dp = native.ops().text_attention_bwd(q, k, v, param, o, lse, do, scale, window, sinks, kv_len, start, starts, buckets, need)
+        return dq, dk, dv, dp if need else None, None, None, None, None, None, None
 
 
 def _check(name, q, k, v, kv_len, out):
@@ -85,25 +62,17 @@ def _per_sequence(name, what, t, q):
         raise ValueError(f"{name}: {what} must be int32 [B] on q's device")
 
 
-def _attend(q, k, v, param, scale, rule: Sequence[int], kv_len, q_start, buckets: Sequence[int], out):
-    """The kernels' call: with a gradient the autograd node, else the forward pass alone, into ``out`` where that can be written."""
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    param, kv_len, q_start = (t.contiguous() if t is not None else None for t in (param, kv_len, q_start))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, param)):
-        o = _TextAttentionFn.apply(q, k, v, param, scale, rule, kv_len, q_start, buckets)
-    else:
-        sink, table = (None, param) if buckets else (param, None)
-        direct = out is not None and _writable(out, *(t for t in (q, k, v, param, kv_len, q_start) if t is not None))
-        o, _ = _ops().text_attention_fwd(q, k, v, scale, rule, kv_len, q_start, sink, table, buckets, False, out if direct else None)
-        if direct:
-            return out
-    return out.copy_(o) if out is not None else o
+def _kernels(q, k, v, scale, param, kv_len, q_start, out) -> bool:
+    """Whether the kernels cover the call. They check shapes, types and devices themselves, which costs a short call less."""
+    if not (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 4 and q.shape[3] in (64, 128) and 0 < scale < math.inf):
+        return False
+    if param is not None and param.dtype is not torch.bfloat16 and param.dtype is not torch.float32:
+        return False
+    return native.use_native(q) and native.direct(*(t for t in (q, k, v, param, kv_len, q_start, out) if t is not None))
 
 
-def _native(q, k, scale, *others) -> bool:
-    given = [t for t in others if t is not None]
-    return (native.use_native(q) and 0 < scale < math.inf and q.dtype == torch.bfloat16 and q.shape[3] in (64, 128) and q.numel() > 0 and k.numel() > 0
-            and max(q.shape[1], k.shape[1]) < 1 << 30 and max(q.shape[0], q.shape[2]) < 1 << 16 and native.direct(q, k, *given))
+def _wants_grad(q, k, v, param) -> bool:
+    return torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (param is not None and param.requires_grad))
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
@@ -117,29 +86,38 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     and carry no value. A row that sees no key is zero and has no gradient. Differentiable in q, k, v and sink_logits, once.
     """
     name = "window_attention"
-    _check(name, q, k, v, kv_len, out)
-    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
+    if window is None:
+        window = _NO_WINDOW
+    elif isinstance(window, bool) or not isinstance(window, int) or window < 1:
         raise ValueError(f"{name}: window must be a positive int or None")
     if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
         raise ValueError(f"{name}: sinks must be an int of at least 0")
-    start = q_start if isinstance(q_start, torch.Tensor) else None
-    if start is None and (isinstance(q_start, bool) or not isinstance(q_start, int)):
+    starts = q_start if isinstance(q_start, torch.Tensor) else None
+    if starts is None and (isinstance(q_start, bool) or not isinstance(q_start, int)):
         raise ValueError(f"{name}: q_start must be an int or int32 [B]")
-    _per_sequence(name, "q_start", start, q)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    window, sinks = min(window, _NO_WINDOW), min(sinks, _NO_WINDOW)
+    start = 0 if starts is not None else max(min(q_start, _NO_WINDOW), -_NO_WINDOW)
+    kernels = _kernels(q, k, v, scale, sink_logits, kv_len, starts, out)
+    if kernels:
+        if not _wants_grad(q, k, v, sink_logits):
+            return native.ops().window_attention(q, k, v, window, sinks, scale, kv_len, start, starts, sink_logits, out)
+        o = _TextAttentionFn.apply(q, k, v, sink_logits, scale, window, sinks, kv_len, starts if starts is not None else start, [])
+        if out is None:
+            return o
+    _check(name, q, k, v, kv_len, out)
+    _per_sequence(name, "q_start", starts, q)
     if sink_logits is not None and (sink_logits.shape != q.shape[2:3] or not sink_logits.is_floating_point() or sink_logits.device != q.device):
         raise ValueError(f"{name}: sink_logits must be [H] on q's device")
-    scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    if not _native(q, k, scale, v, kv_len, start, sink_logits) or (sink_logits is not None and sink_logits.dtype not in (torch.float32, torch.bfloat16)):
-        o = ref.window_attention(q, k, v, window, sinks, scale, kv_len, q_start, sink_logits)
-        return out.copy_(o) if out is not None else o
-    rule = [min(window, _NO_WINDOW) if window is not None else _NO_WINDOW, min(sinks, _NO_WINDOW), 0 if start is not None else max(min(q_start, _NO_WINDOW), -_NO_WINDOW)]
-    return _attend(q, k, v, sink_logits, scale, rule, kv_len, start, [], out)
+    if not kernels:
+        o = ref.window_attention(q, k, v, window, sinks, scale, kv_len, starts if starts is not None else start, sink_logits)
+    return out.copy_(o) if out is not None else o
 
 
 @functools.lru_cache(maxsize=64)
 def _buckets(num_buckets: int, max_distance: int):
     single, borders = ref.bucket_borders(num_buckets, max_distance)
-    return (num_buckets, single, *borders)
+    return [num_buckets, single, *borders]
 
 
 def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, max_distance: int = 128, scale: float = 1.0,
@@ -152,15 +130,24 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     switches a bucket off; a row that sees no key is zero and has no gradient. Differentiable in q, k, v and table, once.
     """
     name = "relative_attention"
+    if table.dim() != 2 or table.shape[0] < 4 or table.shape[0] % 2:
+        raise ValueError(f"{name}: table must be [num_buckets, H], num_buckets even and at least 4")
+    if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
+        raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
+    scale = float(scale)
+    kernels = (_kernels(q, k, v, scale, table, kv_len, None, out) and table.shape[0] <= MAX_BUCKETS[q.shape[3]] and max_distance <= MAX_DISTANCE)
+    if kernels:
+        buckets = _buckets(table.shape[0], max_distance)
+        if not _wants_grad(q, k, v, table):
+            return native.ops().relative_attention(q, k, v, table, buckets, scale, kv_len, out)
+        o = _TextAttentionFn.apply(q, k, v, table, scale, _NO_WINDOW, 0, kv_len, 0, buckets)
+        if out is None:
+            return o
     _check(name, q, k, v, kv_len, out)
     if k.shape[2] != q.shape[2]:
         raise ValueError(f"{name}: q, k and v with the same heads")
-    if table.dim() != 2 or table.shape[1] != q.shape[2] or table.shape[0] < 4 or table.shape[0] % 2 or not table.is_floating_point() or table.device != q.device:
-        raise ValueError(f"{name}: table must be [num_buckets, H] on q's device, num_buckets even and at least 4")
-    if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
-        raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
-    if (not _native(q, k, scale, v, kv_len, table) or table.dtype not in (torch.float32, torch.bfloat16) or table.shape[0] > MAX_BUCKETS[q.shape[3]]
-            or max_distance > MAX_DISTANCE):
+    if table.shape[1] != q.shape[2] or not table.is_floating_point() or table.device != q.device:
+        raise ValueError(f"{name}: table must be [num_buckets, H] on q's device")
+    if not kernels:
         o = ref.relative_attention(q, k, v, table, max_distance, scale, kv_len)
-        return out.copy_(o) if out is not None else o
-    return _attend(q, k, v, table, float(scale), [_NO_WINDOW, 0, 0], kv_len, None, list(_buckets(table.shape[0], max_distance)), out)
+    return out.copy_(o) if out is not None else o

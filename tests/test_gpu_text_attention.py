@@ -372,6 +372,17 @@ def test_other_types_and_widths_take_the_torch_statement():
         assert float((O.relative_attention(q, q, q, table, 20, 0.1).double() - value["out"]).abs().max()) < tol
 
 
+def test_scales_the_kernels_do_not_take():
+    """Zero and negative scales: the torch statement."""
+    q, k, v = _inputs(1, 20, 20, 4, 4, 64, seed=335)
+    table = _normal(32, 4, seed=336)
+    for scale in (0.0, -0.2):
+        value, bound = oracle(q, k, v, scale, seen_by(20, 20, 1, 6, 1))
+        check(dict(out=O.window_attention(q, k, v, 6, 1, scale)), value, bound, "window")
+        value, bound = oracle(q, k, v, scale, seen_by(20, 20, 1, causal=False), table=table)
+        check(dict(out=O.relative_attention(q, k, v, table, scale=scale)), value, bound, "relative")
+
+
 def test_nothing_to_do():
     q, k = _normal(0, 3, 4, 64, seed=1), _normal(0, 3, 2, 64, seed=1)
     assert O.window_attention(q, k, k).shape == (0, 3, 4, 64)
@@ -380,23 +391,52 @@ def test_nothing_to_do():
     q, k = _normal(1, 3, 4, 64, seed=1), _normal(1, 0, 2, 64, seed=1)
     assert float(O.window_attention(q, k, k).abs().max()) == 0
     k = _normal(1, 0, 4, 64, seed=1)
-    assert float(O.relative_attention(q, k, k, _normal(32, 4, seed=2)).abs().max()) == 0
+    table = _normal(32, 4, seed=2)
+    assert float(O.relative_attention(q, k, k, table).abs().max()) == 0
+    leaves = [t.requires_grad_() for t in (q, k, table)]
+    got = torch.autograd.grad(O.relative_attention(q, k, k, table).sum(), leaves)
+    assert [g.shape for g in got] == [t.shape for t in leaves] and all(float(g.abs().sum()) == 0 for g in got)
+
+
+def test_refusals():
+    q, k = _normal(2, 5, 4, 64, seed=1), _normal(2, 5, 2, 64, seed=2)
+    table = _normal(32, 4, seed=3)
+    w, r = O.window_attention, O.relative_attention
+    leaf = lambda t: t.clone().requires_grad_()
+    calls = [lambda q, k: w(q[0], k, k), lambda q, k: w(q, k, k[:, :4]), lambda q, k: w(q, k[:1], k[:1]), lambda q, k: w(q, k[..., :32], k[..., :32]),
+             lambda q, k: w(q[:, :, :3], k, k), lambda q, k: w(q, k.float(), k.float()), lambda q, k: w(q, k.cpu(), k.cpu()), lambda q, k: w(q, k, k, 0),
+             lambda q, k: w(q, k, k, 2.0), lambda q, k: w(q, k, k, 2, -1), lambda q, k: w(q, k, k, kv_len=_ints([1])), lambda q, k: w(q, k, k, kv_len=_ints([1, 2]).long()),
+             lambda q, k: w(q, k, k, kv_len=_ints([1, 2]).cpu()), lambda q, k: w(q, k, k, q_start=_ints([1, 2, 3])), lambda q, k: w(q, k, k, q_start=1.0),
+             lambda q, k: w(q, k, k, q_start=_ints([1, 2]).long()), lambda q, k: w(q, k, k, sink_logits=_normal(2, seed=1)),
+             lambda q, k: w(q, k, k, sink_logits=torch.ones(4, dtype=torch.long, device=DEV)), lambda q, k: w(q, k, k, sink_logits=_normal(4, seed=1).cpu()),
+             lambda q, k: w(q, k, k, out=torch.empty_like(q)[:, :2]), lambda q, k: w(q, k, k, out=torch.empty_like(q, dtype=torch.float32)),
+             lambda q, k: w(q, k, k, out=torch.empty_like(q, device="cpu")), lambda q, k: w(q, k[:, :, :0], k[:, :, :0]),
+             lambda q, k: r(q, q, q, table[:, :3]), lambda q, k: r(q, q, q, table[:31]), lambda q, k: r(q, q, q, table[:2]), lambda q, k: r(q, q, q, table[0]),
+             lambda q, k: r(q, q, q, table.long()), lambda q, k: r(q, q, q, table.cpu()), lambda q, k: r(q, q, q, table, 8), lambda q, k: r(q, q, q, table, 100.0),
+             lambda q, k: r(q, q, q, table, kv_len=_ints([1])), lambda q, k: r(q, q, q, table, out=torch.empty_like(q)[:1]), lambda q, k: r(q, k, k, table)]
+    for i, call in enumerate(calls):
+        for grad in (False, True):
+            with pytest.raises(ValueError):
+                call(leaf(q), leaf(k)) if grad else call(q, k)
+                pytest.fail(f"call {i} went through")
+    o = w(leaf(q), k, k)
+    g, = torch.autograd.grad(o, [o.grad_fn.next_functions[0][0].variable], torch.ones_like(o), create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()                       # differentiable once
 
 
 def test_native_refusals():
-    """What the C++ entry checks by itself, on the host, before a launch."""
-    fwd = torch.ops.mdb200.text_attention_fwd
+    """What the C++ entries check by themselves, on the host, before a launch."""
     q, k, v = _inputs(2, 8, 8, 4, 2, 64, seed=340)
-    rule = [4, 0, 0]
-    ok = lambda **c: fwd(c.get("q", q), c.get("k", k), c.get("v", v), 1.0, c.get("rule", rule), c.get("n"), c.get("at"), c.get("sink"), c.get("table"),
-                         c.get("buckets", []), False, c.get("out"))
-    ok()
     table = _normal(32, 4, seed=1)
-    for bad in (dict(q=q.float()), dict(k=k[:, :, :, ::2]), dict(k=k.cpu()), dict(k=_normal(2, 8, 3, 64, seed=1), v=_normal(2, 8, 3, 64, seed=1)), dict(v=v[:, :5]),
-                dict(q=_normal(2, 8, 4, 65, seed=1)[..., 1:]), dict(k=k[:1].expand(2, 8, 2, 64)), dict(rule=[0, 0, 0]), dict(rule=[4, -1, 0]), dict(rule=[4]),
-                dict(n=_ints([1])), dict(n=torch.tensor([1, 1], device=DEV)), dict(at=torch.tensor([1, 1], dtype=torch.int32)), dict(sink=_normal(3, seed=1)),
-                dict(sink=_normal(4, seed=1, dtype=torch.float16)), dict(table=table), dict(table=table, buckets=[16, 4, 9]), dict(table=table, buckets=[32, 8] + [9] * 40),
-                dict(table=table, buckets=[32, 8, 9], k=q, v=q, at=None, rule=[4]), dict(table=table, buckets=[32, 8, 9]), dict(table=table, buckets=[32, 8, 5000], k=q, v=q),
-                dict(table=table, buckets=[32, 8, 20, 10], k=q, v=q), dict(table=table, buckets=[32, 16], k=q, v=q), dict(sink=_normal(4, seed=1), table=table, buckets=[32, 8, 9]), dict(out=q[:, :4])):
-        with pytest.raises(RuntimeError):
-            ok(**bad)
+    relative = lambda b, k=q, t=table: torch.ops.mdb200.relative_attention(q, k, k, t, b, 1.0, None, None)
+    relative([32, 8, 9])
+    for bad in (lambda: relative([32, 8, 9], k), lambda: relative([16, 4, 9]), lambda: relative([32]), lambda: relative([32, 8] + [9] * 40), lambda: relative([32, 8, 5000]),
+                lambda: relative([32, 8, 20, 10]), lambda: relative([32, 16]), lambda: relative([32, 0, 9]), lambda: relative([66, 8, 9], t=_normal(66, 4, seed=1)),
+                lambda: relative([32, 8, 9], t=_normal(32, 4, seed=1, dtype=torch.float16)),
+                lambda: torch.ops.mdb200.window_attention(q, k, v, 0, 0, 1.0, None, 0, None, None, None),
+                lambda: torch.ops.mdb200.window_attention(q, k, v, 4, -1, 1.0, None, 0, None, None, None),
+                lambda: torch.ops.mdb200.window_attention(q, k, v, 4, 0, 0.0, None, 0, None, None, None),
+                lambda: torch.ops.mdb200.window_attention(q, k, v, 4, 0, math.nan, None, 0, None, None, None)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bad()
