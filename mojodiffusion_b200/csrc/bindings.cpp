@@ -592,8 +592,8 @@ TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, double sca
     (table ? a.table : a.sink_logits) = c.param.data_ptr();
   }
   if (!buckets.empty()) {
-    TEXT_CHECK(a.table != nullptr && a.Hkv == a.H && buckets.size() >= 2 && buckets[0] * a.Dh <= MDB_TEXT_MAX_BUCKETS * 64 && buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 2 &&
-                   buckets.back() <= MDB_TEXT_MAX_DISTANCE, "buckets");
+    TEXT_CHECK(a.table != nullptr && a.Hkv == a.H && buckets.size() >= 2 && buckets[0] * a.Dh <= MDB_TEXT_MAX_BUCKETS * 64 && buckets.size() - 2 <= MDB_TEXT_MAX_BUCKETS / 2,
+               "a table for as many key heads as query heads, and buckets of a number that the kernels keep");
     a.buckets = (int)buckets[0];
     a.exact = (int)buckets[1];
     a.n_borders = (int)buckets.size() - 2;

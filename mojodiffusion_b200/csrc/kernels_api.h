@@ -215,7 +215,8 @@ int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 // (p - j < window or j < sinks); with one, when j < kv_len. scale > 0. lse (base 2; +inf: a row that saw nothing), delta: fp32 [B, H, Sq]; delta and
 // table_ws are workspaces of the backward pass.
 #define MDB_TEXT_MAX_BUCKETS 64        // at Dh 64, half as many at 128: the backward pass keeps an accumulator for each in every thread
-#define MDB_TEXT_MAX_DISTANCE 1024
+#define MDB_TEXT_MAX_NEAR_64 512        // last border, by head width: the tables of biases by distance share the shared memory with the tiles
+#define MDB_TEXT_MAX_NEAR_128 240
 typedef struct MdbTextAttnArgs {
   const void* q; const void* k; const void* v; void* o;
   const void* dout; void* dq; void* dk; void* dv;

@@ -22,7 +22,7 @@ static int check_args(const MdbTextAttnArgs* a) {
     if (a->borders[i] < last) return -6;
     last = a->borders[i];
   }
-  return last > MDB_TEXT_MAX_DISTANCE ? -6 : 0;
+  return last > (a->Dh == 64 ? MDB_TEXT_MAX_NEAR_64 : MDB_TEXT_MAX_NEAR_128) ? -6 : 0;
 }
 
 }  // namespace mdb

@@ -58,6 +58,41 @@ __device__ __forceinline__ int text_bucket(const MdbTextAttnArgs& a, int rel) {
   return c + (rel > 0 ? a.buckets / 2 : 0);
 }
 
+// The bias of one head by distance, for the distances -near - 254 .. near + 254 (all that a tile near the diagonal meets), in shared memory. Four
+// copies, shifted by an element each: a thread reads four neighbours with one aligned 16-byte load, whatever its row; the distance between the
+// copies lets 8 lanes of consecutive rows hit all banks.
+struct TextLut {
+  static __host__ __device__ __forceinline__ int entries(int near) { return 2 * near + 509; }
+  static __host__ __device__ __forceinline__ int copy_floats(int near) { return (entries(near) + 3 + 31) / 32 * 32 + 8; }
+  static __host__ __device__ __forceinline__ int bytes(int near) { return 4 * copy_floats(near) * 4 + (entries(near) + 15) / 16 * 16; }      // copies, buckets
+
+  float* copies;
+  uint8_t* buckets;
+  int near, ld;
+  __device__ __forceinline__ TextLut(void* smem, int near_) : copies(static_cast<float*>(smem)), near(near_), ld(copy_floats(near_)) {
+    buckets = reinterpret_cast<uint8_t*>(copies + 4 * ld);
+  }
+  // once
+  __device__ __forceinline__ void set_buckets(const MdbTextAttnArgs& a, int thread, int threads) const {
+    for (int i = thread; i < entries(near); i += threads) buckets[i] = static_cast<uint8_t>(text_bucket(a, i - near - 254));
+  }
+  // for each head, after all threads have set the buckets and read the head before
+  __device__ __forceinline__ void set_head(const MdbTextAttnArgs& a, int head, int thread, int threads) const {
+    for (int i = thread; i < entries(near); i += threads) {
+      const float v = TXT_LOG2E * text_param(a.table, a.param_f32, static_cast<long long>(buckets[i]) * a.H + head);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copies[j * ld + i + j] = v;
+    }
+  }
+  __device__ __forceinline__ float before() const { return copies[0]; }                       // key far before the query, and behind it
+  __device__ __forceinline__ float behind() const { return copies[entries(near) - 1]; }
+  // where the biases of the distances d, d + 1, ... lie: 16-byte loads at multiples of four
+  __device__ __forceinline__ const float* from(int d) const {
+    const int i = near + 254 + d, j = -i & 3;
+    return copies + j * ld + i + j;
+  }
+};
+
 // lets `kern` have up to `bytes` of dynamic shared memory on the current device; once for each
 constexpr int TXT_DEVICES = 64;
 template <typename K>

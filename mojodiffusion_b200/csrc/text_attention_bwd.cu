@@ -39,7 +39,7 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
   static constexpr int STAGES = (DH == 128 && BIAS && !KEYS) ? 2 : 4;      // the accumulators of dtable take the place of two
   static constexpr int TILES = 2 * TR * DH * 2 + STAGES * 2 * TC * DH * 2 + 1024;
   static constexpr int SUMS = (BIAS && !KEYS) ? 8 * 32 * RUN_LD * 4 : 0;
-  static __host__ __device__ int lut_bytes(int near) { return BIAS ? (2 * near + 509) * 4 : 0; }
+  static __host__ __device__ int lut_bytes(int near) { return BIAS ? TextLut::bytes(near) : 0; }
   static __host__ __device__ int bytes(int near, int buckets) {
     return TILES + SUMS + lut_bytes(near) + ((BIAS && !KEYS) ? buckets * 256 * 4 + (2 * near + 4) + (buckets + 2) * 8 : 0);
   }
@@ -68,8 +68,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   uint8_t* sC = sR2 + R_BYTES;                                            // STAGES x (C1, C2)
   const int near = BIAS ? text_near(a) : 0;
   float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // BIAS dq: running sums [8 warps][32 rows][RUN_LD]
-  float* lut = sums + Shape::SUMS / 4;                                    // BIAS: log2(e) * bias of the distances -near - 254 .. near + 254
-  float* bins = lut + (BIAS ? 2 * near + 509 : 0);                        // BIAS dq: [buckets][256 threads]
+  const TextLut lut(sums + Shape::SUMS / 4, near);                        // BIAS
+  float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // BIAS dq: [buckets][256 threads]
   // BIAS dq: the buckets in the order of their distances ("runs"): first distance and bucket of each, and the run of the distances -near .. near
   const int run_mid = a.exact + a.n_borders, runs = 2 * run_mid + 1;
   int* run_start = reinterpret_cast<int*>(bins + a.buckets * 256);        // [runs + 1]
@@ -135,8 +135,9 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   }
   if (BIAS) {
     // one head's bias: with a table there are as many key heads as query heads
-    for (int i = threadIdx.x; i < 2 * near + 509; i += TB_THREADS)
-      lut[i] = TXT_LOG2E * text_param(a.table, a.param_f32, static_cast<long long>(text_bucket(a, i - near - 254)) * a.H + blockIdx.y);
+    lut.set_buckets(a, threadIdx.x, TB_THREADS);
+    __syncthreads();
+    lut.set_head(a, blockIdx.y, threadIdx.x, TB_THREADS);
     if (!KEYS && a.d_table != nullptr) {
       for (int i = threadIdx.x; i < a.buckets * 256; i += TB_THREADS) bins[i] = 0.f;
       for (int i = threadIdx.x; i <= 2 * near; i += TB_THREADS) {
@@ -385,8 +386,9 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         float one_bias = 0.f;
         const float* b = nullptr;
         if (BIAS) {
-          if (uniform) one_bias = d0 > 0 ? lut[2 * near + 508] : lut[0];
-          else b = lut + near + 254 + (KEYS ? row - b0 : b0 - row);
+          // four neighbours in one load: distances grow along the keys, and fall along the queries
+          if (uniform) one_bias = d0 > 0 ? lut.behind() : lut.before();
+          else b = lut.from(KEYS ? row - b0 - 3 : b0 - row);
         }
         uint32_t pk[16], dk[16];
         const float2 sl2_2 = make_float2(sl2, sl2);
@@ -405,8 +407,12 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             }
           }
           if (BIAS) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) nl[m] += uniform ? one_bias : b[KEYS ? -(e + m) : e + m];
+            float4 u = make_float4(one_bias, one_bias, one_bias, one_bias);
+            if (!uniform) u = *reinterpret_cast<const float4*>(b + (KEYS ? -e : e));
+            nl[0] += KEYS ? u.w : u.x;
+            nl[1] += KEYS ? u.z : u.y;
+            nl[2] += KEYS ? u.y : u.z;
+            nl[3] += KEYS ? u.x : u.w;
           }
           const float2 x01 = ffma2(make_float2(__uint_as_float(xr[c][e]), __uint_as_float(xr[c][e + 1])), sl2_2, make_float2(nl[0], nl[1]));
           const float2 x23 = ffma2(make_float2(__uint_as_float(xr[c][e + 2]), __uint_as_float(xr[c][e + 3])), sl2_2, make_float2(nl[2], nl[3]));

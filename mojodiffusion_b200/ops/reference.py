@@ -5,6 +5,7 @@ tests run a kernel and compare against the function of the same name here evalua
 """
 from __future__ import annotations
 
+import bisect
 import math
 import os
 from typing import Optional, Sequence
@@ -268,14 +269,10 @@ def bucket_borders(num_buckets: int, max_distance: int):
     """(single, borders) of the bidirectional buckets: half of the buckets per direction; distances below ``single`` have one each, the m
     others end at distances that grow by equal factors up to ``max_distance``. A distance n >= single lies in the k-th or a later one of them
     when floor(m log(n / single) / log(max_distance / single)) >= k, here without rounding: n^m single^k >= max_distance^k single^m."""
-    half = num_buckets // 2
-    single = half // 2
-    m = half - single
-    borders, n = [], single
-    for k in range(1, m):
-        while n ** m * single ** k < max_distance ** k * single ** m:
-            n += 1
-        borders.append(n)
+    single = num_buckets // 4
+    m = num_buckets // 2 - single
+    reached = lambda n, k: n ** m * single ** k >= max_distance ** k * single ** m
+    borders = [bisect.bisect_left(range(max_distance + 1), True, lo=single, key=lambda n: reached(n, k)) for k in range(1, m)]
     return single, borders
 
 

@@ -18,8 +18,8 @@ import torch
 from . import native, reference as ref
 
 _NO_WINDOW = 1 << 30
-#: buckets (by head width) and distances that the kernels' tables hold; beyond them the torch statement runs
-MAX_BUCKETS, MAX_DISTANCE = {64: 64, 128: 32}, 1024
+#: by head width, the buckets that the kernels' tables hold and the distance at which the last one may begin; beyond them the torch statement runs
+MAX_BUCKETS, MAX_NEAR = {64: 64, 128: 32}, {64: 512, 128: 240}
 
 
 class _TextAttentionFn(torch.autograd.Function):
@@ -135,9 +135,9 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
         raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
     scale = float(scale)
-    kernels = (_kernels(q, k, v, scale, table, kv_len, None, out) and table.shape[0] <= MAX_BUCKETS[q.shape[3]] and max_distance <= MAX_DISTANCE)
+    buckets = _buckets(table.shape[0], max_distance)
+    kernels = _kernels(q, k, v, scale, table, kv_len, None, out) and table.shape[0] <= MAX_BUCKETS[q.shape[3]] and buckets[-1] <= MAX_NEAR[q.shape[3]]
     if kernels:
-        buckets = _buckets(table.shape[0], max_distance)
         if not _wants_grad(q, k, v, table):
             return native.ops().relative_attention(q, k, v, table, buckets, scale, kv_len, out)
         o = _TextAttentionFn.apply(q, k, v, table, scale, _NO_WINDOW, 0, kv_len, 0, buckets)

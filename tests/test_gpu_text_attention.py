@@ -92,8 +92,9 @@ RELATIVE = [
     (2, 190, 2, 2, 64, 64, 200, [11, 190], False),
     (1, 333, 2, 2, 128, 8, 3, None, False),
     (1, 150, 2, 2, 64, 4, 100, None, True),
-    (1, 700, 1, 1, 64, 64, 1024, None, False),
-    (1, 260, 2, 2, 128, 32, 1000, [259], False),
+    (1, 1300, 1, 1, 64, 64, 560, None, False),          # the last bucket begins at 502
+    (1, 520, 2, 2, 128, 32, 385, [519], False),         # at 238
+    (1, 200, 2, 2, 128, 32, 1000, None, False),         # at 547: the torch statement
     (1, 260, 2, 2, 64, 32, 9, None, False),             # all borders at one distance
     (1, 200, 2, 2, 64, 66, 128, None, False),           # more buckets than the kernels keep: the torch statement
 ]
