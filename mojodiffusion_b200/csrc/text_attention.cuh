@@ -64,24 +64,26 @@ __device__ __forceinline__ int text_bucket(const MdbTextAttnArgs& a, int rel) {
 struct TextLut {
   static __host__ __device__ __forceinline__ int entries(int near) { return 2 * near + 509; }
   static __host__ __device__ __forceinline__ int copy_floats(int near) { return (entries(near) + 3 + 31) / 32 * 32 + 8; }
-  static __host__ __device__ __forceinline__ int bytes(int near) { return 4 * copy_floats(near) * 4 + (entries(near) + 15) / 16 * 16; }      // copies, buckets
+  static __host__ __device__ __forceinline__ int bytes(int near) { return 4 * copy_floats(near) * 4; }
 
   float* copies;
-  uint8_t* buckets;
   int near, ld;
-  __device__ __forceinline__ TextLut(void* smem, int near_) : copies(static_cast<float*>(smem)), near(near_), ld(copy_floats(near_)) {
-    buckets = reinterpret_cast<uint8_t*>(copies + 4 * ld);
-  }
-  // once
-  __device__ __forceinline__ void set_buckets(const MdbTextAttnArgs& a, int thread, int threads) const {
-    for (int i = thread; i < entries(near); i += threads) buckets[i] = static_cast<uint8_t>(text_bucket(a, i - near - 254));
-  }
-  // for each head, after all threads have set the buckets and read the head before
-  __device__ __forceinline__ void set_head(const MdbTextAttnArgs& a, int head, int thread, int threads) const {
-    for (int i = thread; i < entries(near); i += threads) {
-      const float v = TXT_LOG2E * text_param(a.table, a.param_f32, static_cast<long long>(buckets[i]) * a.H + head);
+  __device__ __forceinline__ TextLut(void* smem, int near_) : copies(static_cast<float*>(smem)), near(near_), ld(copy_floats(near_)) {}
+  // By `warps` whole warps; the caller synchronises. Every warp takes some of the buckets, in the order of their distances, with one load for their
+  // values, and stores each over its distances.
+  __device__ __forceinline__ void set(const MdbTextAttnArgs& a, int head, int warp, int warps) const {
+    const int mid = a.exact + a.n_borders, n = entries(near), lane = threadIdx.x & 31;
+    const auto reach = [&](int c) { return c <= a.exact ? c : a.borders[c - a.exact - 1]; };      // first distance of a bucket of either direction
+    const auto start = [&](int r) { return r <= 0 ? -near - 254 : r <= mid ? 1 - reach(mid - r + 1) : reach(r - mid); };
+    const int mine = warp + lane * warps;
+    float v = 0.f;
+    if (mine <= 2 * mid) v = TXT_LOG2E * text_param(a.table, a.param_f32, static_cast<long long>(mine <= mid ? mid - mine : mine - mid + a.buckets / 2) * a.H + head);
+    for (int k = 0, r = warp; r <= 2 * mid; ++k, r += warps) {
+      const float u = __shfl_sync(0xffffffffu, v, k);
+      const int lo = start(r) + near + 254, hi = r == 2 * mid ? n : start(r + 1) + near + 254;
+      for (int i = lo + lane; i < hi; i += 32)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) copies[j * ld + i + j] = v;
+        for (int j = 0; j < 4; ++j) copies[j * ld + i + j] = u;
     }
   }
   __device__ __forceinline__ float before() const { return copies[0]; }                       // key far before the query, and behind it

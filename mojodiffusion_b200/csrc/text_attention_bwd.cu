@@ -135,9 +135,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   }
   if (BIAS) {
     // one head's bias: with a table there are as many key heads as query heads
-    lut.set_buckets(a, threadIdx.x, TB_THREADS);
-    __syncthreads();
-    lut.set_head(a, blockIdx.y, threadIdx.x, TB_THREADS);
+    lut.set(a, blockIdx.y, warp, TB_THREADS / 32);
     if (!KEYS && a.d_table != nullptr) {
       for (int i = threadIdx.x; i < a.buckets * 256; i += TB_THREADS) bins[i] = 0.f;
       for (int i = threadIdx.x; i <= 2 * near; i += TB_THREADS) {

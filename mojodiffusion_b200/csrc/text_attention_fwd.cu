@@ -2,15 +2,15 @@
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp2(x_ij - m_i) / l_i,  x_ij = log2(e) (scale q_i . k_j + bias(j - i)),  m_i a running reference of x_ij
 //
-// A CTA owns up to 256 / Dh * 64 query rows, in tiles of 128, that read the same keys and values: the same rows of several heads of one group where the
-// group's size allows (they visit the same key tiles, whatever the window), else consecutive rows of one head. Every tile has its softmax
-// warpgroup, one thread per row: it turns the scores S = Q K^T (fp32 in TMEM) into probabilities, bf16, written into TMEM over the scores they came
-// from and read from there as the A operand of O += P V, while the tensor core works for the other tiles. K and V arrive by TMA.
-// Heads of 128: 2 tiles with 128 keys at a time fill the 512 columns of TMEM. Heads of 64: 4 tiles with 64 keys; exponentials bound them, and
-// four softmax warps per scheduler instead of two hide their latencies (8 x 512 x 64 x 64 with position buckets: 2 tiles of 128 keys 117 us).
+// A CTA owns two tiles of 128 query rows that read the same keys and values: the same rows of two heads of one group where the group's size is even
+// (they visit the same key tiles, whatever the window), else 256 consecutive rows of one head. Either tile has its softmax warpgroup, one thread
+// per row: it turns the scores S = Q K^T (fp32 in TMEM) into probabilities, bf16, written into TMEM over the scores they came from and read from
+// there as the A operand of O += P V, while the tensor core works for the other tile. K and V arrive by TMA.
 //
-// A CTA works through several such items. Its loads and the first scores of the next item run under the epilogue of this one, which needs only O:
-// with a window an item has few key tiles, and the start and end of a CTA would be a third of its time.
+// Heads of 128: 128 keys at a time, which fills TMEM and most of the shared memory with one CTA. It works through several such items: the loads and
+// the first scores of the next one run under the epilogue, which needs only O (with a window an item has few key tiles).
+// Heads of 64: 64 keys at a time and half of TMEM, so that two CTAs share an SM. There the exponentials and their latencies bound: four softmax warps
+// per scheduler instead of two, and the start and the epilogue of one CTA run under the other's work.
 //
 // Key tiles are visited only where a row of the CTA may see a key: the tiles of the first `sinks` keys, then those of the windows. Pieces of 32 keys
 // that none of a warp's 32 rows sees are not exponentiated, those that all of them see are not masked; in the others each thread makes
@@ -29,14 +29,16 @@ namespace mdb {
 constexpr int TQ = 128;                              // rows of a query tile
 
 template <int DH> struct FwdShape {
-  static constexpr int NT = DH == 64 ? 4 : 2;        // query tiles
   static constexpr int TK = DH == 64 ? 64 : 128;     // keys of a key tile
-  static constexpr int STAGES = DH == 64 ? 4 : 2;    // of K and of V
-  static constexpr int THREADS = 128 + NT * 128;     // warps 0: TMA, 1 (and 2 with four tiles): MMA issue for two tiles each; four per query tile
-  static constexpr int CTRL_REGS = DH == 64 ? 56 : 88, SOFT_REGS = DH == 64 ? 104 : 208;      // 128 ctrl + 128 NT soft <= THREADS * (96, 168)
+  static constexpr int STAGES = DH == 64 ? 3 : 2;    // of K and of V
+  static constexpr int CTAS = DH == 64 ? 2 : 1;      // per SM
+  // warps 0: TMA, 1: MMA issue; from SOFT on four per query tile. One CTA per SM has registers to move from a first warpgroup (of which two warps idle).
+  static constexpr int SOFT = DH == 64 ? 2 : 4, THREADS = (SOFT + 8) * 32;
+  static constexpr int CTRL_REGS = 88, SOFT_REGS = 208;      // 128 ctrl + 256 soft <= 384 * 168
+  static constexpr int TMEM = 2 * TK + 2 * DH;       // tile t's scores from t * TK on, its output from 2 * TK + t * DH on
   static constexpr int Q_BYTES = TQ * DH * 2, K_BYTES = TK * DH * 2;
   static constexpr int Q_BOX = TQ * 128, K_BOX = TK * 128;      // 64 columns of a tile
-  static constexpr int BYTES = NT * Q_BYTES + STAGES * 2 * K_BYTES + NT * 4 * 2048 + 1024;
+  static constexpr int BYTES = 2 * Q_BYTES + STAGES * 2 * K_BYTES + 8 * 2048 + 1024;
 };
 
 struct alignas(64) TextMaps {
@@ -48,15 +50,15 @@ template <int REGS> __device__ __forceinline__ void regs_down() { asm volatile("
 
 // How the query tiles of an item lie: `heads` heads (a divisor of the group's) x `blocks` blocks of rows, both powers of two
 struct TextTiles {
-  int heads, heads_log, blocks;          // per item
+  int heads, heads_log, blocks;          // per item: two heads, two blocks, or one of each
   int row_items, items;       // items along the rows; in all
 };
 
 // One work item, seen by a whole warp: its query tiles, and the key tiles that any of them visits: [0, ns) and then [lo, lo + n_kv - ns).
-// Lane l looks at query tile l % NT.
+// Lane l looks at query tile l % 2.
 template <int DH, bool BIAS> struct TextItem {
   using Shape = FwdShape<DH>;
-  static constexpr int NT = Shape::NT, TK = Shape::TK;
+  static constexpr int TK = Shape::TK;
   int batch, head, q0;        // of the first tile
   TextSight sight;
   TextKeys all;               // keys that any row sees
@@ -65,9 +67,11 @@ template <int DH, bool BIAS> struct TextItem {
 
   static __device__ __forceinline__ int tile_head(int head, int t, const TextTiles& l) { return head + (t & (l.heads - 1)); }
   static __device__ __forceinline__ int tile_q0(int q0, int t, const TextTiles& l) { return q0 + (t >> l.heads_log) * TQ; }
+  // the order of the items with BIAS: those of a head follow one another, so that its bias table is made once
+  static __device__ __forceinline__ int head_of(const MdbTextAttnArgs& a, int item, const TextTiles& l) { return item / l.row_items / a.B; }
   __device__ __forceinline__ void set(const MdbTextAttnArgs& a, int item, const TextTiles& l) {
     int block;
-    if (BIAS) {                 // the items of a head follow one another, so that its bias table is made once
+    if (BIAS) {
       const int rest = item / l.row_items;
       block = item - rest * l.row_items;
       head = rest / a.B;
@@ -81,7 +85,7 @@ template <int DH, bool BIAS> struct TextItem {
     }
     q0 = block * l.blocks * TQ;
     sight = text_sight(a, batch);
-    const int t = threadIdx.x & (NT - 1), first = tile_q0(q0, t, l);
+    const int t = threadIdx.x & 1, first = tile_q0(q0, t, l);
     TextKeys k = {0, 0, 0};
     if (t < l.heads * l.blocks && first < a.Sq) k = text_keys<BIAS>(a, sight, sight.start + first, sight.start + min(first + TQ, a.Sq) - 1);
     const int n_sinks = (k.sinks + TK - 1) / TK;
@@ -106,131 +110,147 @@ template <int N> struct Int {
 };
 
 template <int DH, bool BIAS>
-__global__ void __launch_bounds__(FwdShape<DH>::THREADS, 1)
+__global__ void __launch_bounds__(FwdShape<DH>::THREADS, FwdShape<DH>::CTAS)
 text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextTiles tiles) {
   using Shape = FwdShape<DH>;
-  constexpr int NT = Shape::NT, TK = Shape::TK, STAGES = Shape::STAGES, PIECES = TK / 32, PARTS = TK / 64;      // parts: P is published 64 keys at a time
+  constexpr int TK = Shape::TK, STAGES = Shape::STAGES, PIECES = TK / 32, PARTS = TK / 64;      // parts: P is published 64 keys at a time
   constexpr int DBOX = DH / 64;
-  constexpr uint32_t S_COL = 0, O_COL = NT * TK;        // both 256 columns: tile t's scores from t * TK on, its output from 256 + t * DH on
-  static_assert(NT * TK == 256 && NT * DH == 256, "TMEM columns");
+  constexpr uint32_t O_COL = 2 * TK;
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-  __shared__ uint64_t s_full[NT], p_full[NT][PARTS], o_full[NT], o_empty[NT];
+  __shared__ uint64_t s_full[2], p_full[2][PARTS], o_full[2], o_empty[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
 
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + NT * Shape::Q_BYTES;
+  uint8_t* sK = sQ + 2 * Shape::Q_BYTES;
   uint8_t* sV = sK + STAGES * Shape::K_BYTES;
   uint8_t* sO = sV + STAGES * Shape::K_BYTES;        // 2 KB per softmax warp: 32 columns of its 32 output rows
-  const TextLut lut(sO + NT * 4 * 2048, BIAS ? text_near(a) : 0);
+  const TextLut lut(sO + 8 * 2048, BIAS ? text_near(a) : 0);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // BIAS: a range of items, else every gridDim.x-th
-  const int first = BIAS ? static_cast<int>(static_cast<long long>(tiles.items) * blockIdx.x / gridDim.x) : blockIdx.x;
-  const int last = BIAS ? static_cast<int>(static_cast<long long>(tiles.items) * (blockIdx.x + 1) / gridDim.x) : tiles.items;
-  const int step = BIAS ? 1 : gridDim.x;
+  // one item to a CTA where two share an SM (the next one starts wherever a CTA ends); else a range of them with BIAS, or every gridDim.x-th
+  constexpr bool ONE = Shape::CTAS == 2, RANGE = BIAS && !ONE;
+  const int first = RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * blockIdx.x / gridDim.x) : blockIdx.x;
+  const int last = ONE ? first + 1 : RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * (blockIdx.x + 1) / gridDim.x) : tiles.items;
+  const int step = ONE || RANGE ? 1 : gridDim.x;
   TextItem<DH, BIAS> w;
 
-  if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
-    mbar_init(&q_empty, NT / 2);
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], NT / 2);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], NT / 2);
+  // The TMA warp makes the barriers and starts loading while the others get ready: nobody else touches either before __syncthreads.
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&maps.q);
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+      mbar_init(&q_full, 1);
+      mbar_init(&q_empty, 1);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 1);
+        mbar_init(&v_full[s], 1);
+        mbar_init(&v_empty[s], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&s_full[t], 1);
+        for (int h = 0; h < PARTS; ++h) mbar_init(&p_full[t][h], 4);
+        mbar_init(&o_full[t], 1);
+        mbar_init(&o_empty[t], 4);
+      }
+      abort_s = 0;
+      fence_mbar_init();
     }
-    for (int t = 0; t < NT; ++t) {
-      mbar_init(&s_full[t], 1);
-      for (int h = 0; h < PARTS; ++h) mbar_init(&p_full[t][h], 4);
-      mbar_init(&o_full[t], 1);
-      mbar_init(&o_empty[t], 4);
-    }
-    abort_s = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(&tmem_base_s, 512);
+    __syncwarp();
+  } else if (warp == 1) {
+    tmem_alloc(&tmem_base_s, Shape::TMEM);
     tmem_relinquish();
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&maps.q);
-    tma_prefetch_desc(&maps.k);
-    tma_prefetch_desc(&maps.v);
+  const auto load_q = [&]() {
+    const int n_q = tiles.heads * tiles.blocks;
+    if (elect_one()) {
+      mbar_expect_tx(&q_full, n_q * Shape::Q_BYTES);
+      for (int t = 0; t < n_q; ++t)
+        for (int d = 0; d < DBOX; ++d)
+          tma_load_4d(sQ + t * Shape::Q_BYTES + d * Shape::Q_BOX, &maps.q, &q_full, d * 64, w.tile_q0(w.q0, t, tiles), w.tile_head(w.head, t, tiles), w.batch);
+    }
+    __syncwarp();
+  };
+  const auto load_kv = [&](int kv, int st, int i, int kv_head) {
+    uint64_t* full = kv ? &v_full[st] : &k_full[st];
+    if (elect_one()) {
+      mbar_expect_tx(full, Shape::K_BYTES);
+      for (int d = 0; d < DBOX; ++d)
+        tma_load_4d((kv ? sV : sK) + st * Shape::K_BYTES + d * Shape::K_BOX, kv ? &maps.v : &maps.k, full, d * 64, w.key_tile(i) * TK, kv_head, w.batch);
+    }
+    __syncwarp();
+  };
+  const int rep = a.H / a.Hkv;
+  int early = 0;              // key tiles of the first item that are on their way
+  if (warp == 0 && first < last) {
+    w.set(a, first, tiles);
+    if (w.n_kv > 0) {
+      load_q();
+      for (; early < STAGES && early < w.n_kv; ++early)
+        for (int kv = 0; kv < 2; ++kv) load_kv(kv, early, early, w.head / rep);
+    }
   }
-  if (BIAS) lut.set_buckets(a, threadIdx.x, Shape::THREADS);
+  if (BIAS && ONE && warp != 0) lut.set(a, w.head_of(a, first, tiles), warp - 1, Shape::THREADS / 32 - 1);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
-  if (warp < 4) {
-    regs_down<Shape::CTRL_REGS>();
+  if (warp < Shape::SOFT) {
+    if (Shape::CTAS == 1) regs_down<Shape::CTRL_REGS>();
     if (warp == 0) {
       // ----------------------------- TMA producer -----------------------------
-      const int rep = a.H / a.Hkv, n_q = tiles.heads * tiles.blocks;
       bool ok = true;
-      uint64_t* last_bar = nullptr;
+      uint64_t* last_bar = &v_full[max(early - 1, 0)];
       uint32_t last_par = 0;
       int n_items = 0, n_tiles = 0;           // that have keys; key tiles so far
       for (int item = first; ok && item < last; item += step) {
-        w.set(a, item, tiles);
+        if (item != first) w.set(a, item, tiles);
         if (w.n_kv == 0) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(&q_empty, (n_items & 1) ^ 1u, &abort_s));
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 110, item);
-          break;
+        if (item != first) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&q_empty, (n_items & 1) ^ 1u, &abort_s));
+          if (!ok) {
+            if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 110, item);
+            break;
+          }
+          load_q();
         }
-        if (elect_one()) {
-          mbar_expect_tx(&q_full, n_q * Shape::Q_BYTES);
-          for (int t = 0; t < n_q; ++t)
-            for (int d = 0; d < DBOX; ++d)
-              tma_load_4d(sQ + t * Shape::Q_BYTES + d * Shape::Q_BOX, &maps.q, &q_full, d * 64, w.tile_q0(w.q0, t, tiles), w.tile_head(w.head, t, tiles), w.batch);
-        }
-        __syncwarp();
-        last_bar = &q_full;
-        last_par = n_items & 1;
         ++n_items;
         const int kv_head = w.head / rep;
         for (int i = 0; ok && i < w.n_kv; ++i, ++n_tiles) {
+          if (n_tiles < early) continue;
           const int st = n_tiles % STAGES;
           const uint32_t par = (n_tiles / STAGES) & 1;
           for (int kv = 0; kv < 2; ++kv) {
-            uint64_t* empty = kv ? &v_empty[st] : &k_empty[st];
-            uint64_t* full = kv ? &v_full[st] : &k_full[st];
-            ok = __all_sync(0xffffffffu, mbar_wait(empty, par ^ 1u, &abort_s));
+            ok = __all_sync(0xffffffffu, mbar_wait(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s));
             if (!ok) {
               if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 111 + kv, i);
               break;
             }
-            if (elect_one()) {
-              mbar_expect_tx(full, Shape::K_BYTES);
-              for (int d = 0; d < DBOX; ++d)
-                tma_load_4d((kv ? sV : sK) + st * Shape::K_BYTES + d * Shape::K_BOX, kv ? &maps.v : &maps.k, full, d * 64, w.key_tile(i) * TK, kv_head, w.batch);
-            }
-            __syncwarp();
-            last_bar = full;
+            load_kv(kv, st, i, kv_head);
+            last_bar = kv ? &v_full[st] : &k_full[st];
             last_par = par;
           }
         }
       }
-      if (!ok && last_bar != nullptr) {
+      if (!ok) {
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(last_bar, last_par) && globaltimer_ns() - t0 < 5000000ull) {
         }
       }
-    } else if (warp <= NT / 2) {
-      // ----------------------------- MMA issue: query tiles t0 and t0 + 1 -----
+    } else if (warp == 1) {
+      // ----------------------------- MMA issue --------------------------------
       // The order of the tensor core's work is this warp's: P V of a tile, then its next S, in turn with the other tile. What a turn takes
       // beside its MMAs delays both, so everything that does not change within an item is at hand.
-      const int t0 = (warp - 1) * 2;
-      const uint32_t s_col = tmem_base + S_COL + t0 * TK, o_col = tmem_base + O_COL + t0 * DH;
-      const uint64_t q_desc = make_desc_kmajor_sw128(smem_u32(sQ + t0 * Shape::Q_BYTES)), k_desc = make_desc_kmajor_sw128(smem_u32(sK));
+      const uint32_t s_col = tmem_base, o_col = tmem_base + O_COL;
+      const uint64_t q_desc = make_desc_kmajor_sw128(smem_u32(sQ)), k_desc = make_desc_kmajor_sw128(smem_u32(sK));
       const uint64_t v_desc = make_desc_mnmajor_sw128(smem_u32(sV), Shape::K_BOX);
       constexpr uint32_t idesc_s = make_idesc(1, UMMA_BF16, UMMA_BF16, 0, 0, TQ, TK), idesc_pv = make_idesc(1, UMMA_BF16, UMMA_BF16, 0, 1, TQ, DH);
       const auto issue_s = [&](int u, int st) {
@@ -239,7 +259,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           const uint32_t q_off = u * Shape::Q_BYTES + (kk / 4) * Shape::Q_BOX + (kk % 4) * 32, k_off = (kk / 4) * Shape::K_BOX + (kk % 4) * 32;
           umma_f16_ss(s_col + u * TK, q_desc + (q_off >> 4), k_desc + ((st * Shape::K_BYTES + k_off) >> 4), idesc_s, kk != 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[t0 + u]);
+        umma_commit(&s_full[u]);
       };
       const auto issue_pv = [&](int u, int st, int part, uint32_t more) {
 #pragma unroll
@@ -257,8 +277,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         int t_lo[2], t_hi[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          t_lo[u] = __shfl_sync(0xffffffffu, w.t_lo, t0 + u);
-          t_hi[u] = __shfl_sync(0xffffffffu, w.t_hi, t0 + u);
+          t_lo[u] = __shfl_sync(0xffffffffu, w.t_lo, u);
+          t_hi[u] = __shfl_sync(0xffffffffu, w.t_hi, u);
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&q_full, n_items & 1, &abort_s) && mbar_wait(&k_full[n_tiles % STAGES], (n_tiles / STAGES) & 1, &abort_s));
         if (!ok) {
@@ -278,7 +298,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         // the epilogue of the item before has read the tiles' O
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (ok && t_hi[u] > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_empty[t0 + u], (outs[u]++ & 1) ^ 1u, &abort_s));
+          if (ok && t_hi[u] > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_empty[u], (outs[u]++ & 1) ^ 1u, &abort_s));
         if (!ok) {
           if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 122, item);
           break;
@@ -312,16 +332,16 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             if (w.sees(t_lo[u], t_hi[u], i)) {
 #pragma unroll
               for (int part = 0; part < PARTS; ++part) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&p_full[t0 + u][part], done[u] & 1, &abort_s));
+                ok = __all_sync(0xffffffffu, mbar_wait(&p_full[u][part], done[u] & 1, &abort_s));
                 if (!ok) {
-                  if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 124 + t0 + u, i);
+                  if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 124 + u, i);
                   return;
                 }
                 tc_fence_after();
                 if (elect_one()) {
                   issue_pv(u, st, part, begun[u]);
                   if (part == PARTS - 1) {
-                    umma_commit(&o_full[t0 + u]);
+                    umma_commit(&o_full[u]);
                     if (next) issue_s(u, st_n);
                   }
                 }
@@ -350,30 +370,31 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     __syncwarp();
   } else {
     // ------------------------------- softmax: one thread per query row -----------------------
-    regs_up<Shape::SOFT_REGS>();
-    const int t = (warp - 4) >> 2;
+    if (Shape::CTAS == 1) regs_up<Shape::SOFT_REGS>();
+    const int t = (warp - Shape::SOFT) >> 2;
     const int quad = warp & 3;
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_tile = tmem_base + lane_addr + S_COL + t * TK;
+    const uint32_t s_tile = tmem_base + lane_addr + t * TK;
     const uint32_t o_addr = tmem_base + lane_addr + O_COL + t * DH;
     const float sl2 = a.scale * TXT_LOG2E;
-    const int near = lut.near;
-    uint8_t* stage = sO + (warp - 4) * 2048;
+    uint8_t* stage = sO + (warp - Shape::SOFT) * 2048;
     bool ok = true;
     int done = 0, lut_head = -1;
 
     for (int item = first; item < last; item += step) {
       w.set(a, item, tiles);
       const int head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
-      if (BIAS && head != lut_head) {
-        asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");           // nobody reads the head before
-        lut.set_head(a, head, threadIdx.x - 128, NT * 128);
-        asm volatile("bar.sync 1, %0;" ::"n"(NT * 128) : "memory");
+      if (BIAS && !ONE && head != lut_head) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");           // nobody reads the head before
+        lut.set(a, head, warp - Shape::SOFT, 8);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         lut_head = head;
       }
       if (!ok || t >= tiles.heads * tiles.blocks || row0 - quad * 32 >= a.Sq) continue;
       const int my_lo = __shfl_sync(0xffffffffu, w.t_lo, t), my_hi = __shfl_sync(0xffffffffu, w.t_hi, t);
       const int p0 = w.sight.start + row0;        // position of the warp's first row
+      // key tiles from whole_lo (or below the first keys' end) to whole_hi are seen whole by the warp's rows
+      const int valid = w.sight.valid, whole_hi = BIAS ? valid - TK : min(p0 + 1, valid) - TK, whole_lo = BIAS ? 0 : p0 + 32 - a.window;
       // The reference m and the divisor l; a sink logit is the first member of the sum.
       float m_used = -INFINITY, l_run = 0.f;
       if (!BIAS && a.sink_logits != nullptr) {
@@ -382,9 +403,9 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       }
       bool fresh = true;
 
-      for (int i = 0; ok && i < w.n_kv; ++i) {
-        if (!w.sees(my_lo, my_hi, i)) continue;
-        const int k0 = w.key_tile(i) * TK;
+      for (int i = 0, kt = w.key_tile(0); i < w.n_kv; ++i, kt = i == w.ns ? w.lo : kt + 1) {
+        if (kt >= my_hi || (kt < my_lo && kt >= w.ns)) continue;
+        const int k0 = kt * TK;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], done & 1, &abort_s));
         if (!ok) {
           if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, i);
@@ -398,8 +419,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         float mul = sl2, add = 0.f;           // exponent = mul * score + add - m
         if (BIAS) {
           const int d = k0 - row0;
-          if (d - 31 >= near) add = lut.behind();
-          else if (d + TK - 1 <= -near) add = lut.before();
+          if (d - 31 >= lut.near) add = lut.behind();
+          else if (d + TK - 1 <= -lut.near) add = lut.before();
           else {
             const float* b = lut.from(d - lane);
             mul = 1.f;
@@ -417,10 +438,10 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
               }
           }
         }
-        if (BIAS ? k0 + TK > w.sight.valid : !(k0 + TK - 1 <= p0 && k0 + TK <= w.sight.valid && (k0 > p0 + 31 - a.window || k0 + TK <= a.sinks))) {
+        if (k0 > whole_hi || (!BIAS && k0 < whole_lo && k0 + TK > a.sinks)) {
 #pragma unroll
           for (int c = 0; c < PIECES; ++c) {
-            const uint32_t see = BIAS ? bits_below(w.sight.valid - k0 - c * 32) : text_mask(a, w.sight.valid, p0 + lane, k0 + c * 32);
+            const uint32_t see = BIAS ? bits_below(valid - k0 - c * 32) : text_mask(a, valid, p0 + lane, k0 + c * 32);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(see >> e & 1u)) sv[c][e] = 0xff800000u;        // -inf
@@ -474,12 +495,13 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            // half of every second group of four exponentials runs on the FMA pipe: the special-function unit bounds the rest
+            // Half of every second group of four exponentials runs on the FMA pipe, the rest on the special-function unit (1 x 4096 x 37 x 64, all keys
+            // visible: 208 us, 216 without). Beside the biases of heads of 64 instructions are scarcer: all on the unit (232 us, 249 with).
             const float2 x01 = ffma2(make_float2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), mul2, nm2);
             const float2 x23 = ffma2(make_float2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), mul2, nm2);
             const float2 u = make_float2(ex2_approx(x01.x), ex2_approx(x23.x));
             float2 v;
-            if ((e >> 2) % 2 == 1) v = ex2_poly2(make_float2(x01.y, x23.y), -127.f);
+            if (!(DH == 64 && BIAS) && (e >> 2) % 2 == 1) v = ex2_poly2(make_float2(x01.y, x23.y), -127.f);
             else v = make_float2(ex2_approx(x01.y), ex2_approx(x23.y));
             sum_a = fadd2(sum_a, u);
             sum_b = fadd2(sum_b, v);
@@ -550,7 +572,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    tmem_dealloc(tmem_base, Shape::TMEM);
   }
 }
 
@@ -577,11 +599,11 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
   if ((r = allow_smem(kern, MOST, ready))) return r;
   const int smem = Shape::BYTES + (BIAS ? TextLut::bytes(text_near(a)) : 0);
   if (smem > MOST) return -6;
-  // As many tiles to an item as leave an item for every SM, heads of a group before blocks of rows. The bias table in shared memory is one head's.
-  const int row_blocks = (a.Sq + TQ - 1) / TQ, sms = device_sm_count();
+  // Two tiles to an item unless one leaves fewer SMs idle, heads of a group before blocks of rows. The bias table in shared memory is one head's.
+  const int row_blocks = (a.Sq + TQ - 1) / TQ, slots = Shape::CTAS * device_sm_count();
   TextTiles l;
   long long items = 0;
-  for (int n = Shape::NT; n >= 1; n /= 2) {
+  for (int n = 2; n >= 1; n /= 2) {
     l.heads = 1;
     l.heads_log = 0;
     while (!BIAS && 2 * l.heads <= n && (a.H / a.Hkv) % (2 * l.heads) == 0) {
@@ -591,11 +613,11 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
     l.blocks = n / l.heads;
     l.row_items = (row_blocks + l.blocks - 1) / l.blocks;
     items = static_cast<long long>(l.row_items) * (a.H / l.heads) * a.B;
-    if (items >= sms) break;
+    if (items >= slots) break;
   }
   if (items > 0x7fffffff) return -8;
   l.items = static_cast<int>(items);
-  kern<<<static_cast<unsigned>(items < sms ? items : sms), Shape::THREADS, smem, st>>>(maps, a, l);
+  kern<<<static_cast<unsigned>(Shape::CTAS == 2 || items < slots ? items : slots), Shape::THREADS, smem, st>>>(maps, a, l);
   return static_cast<int>(cudaGetLastError());
 }
 
