@@ -319,7 +319,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             for (int r = lane; r < TK; r += 32) {
               const int j = k0 + r;
               if (j < w.all.end && (j >= w.all.lo || j < w.all.sinks)) continue;
-#pragma unroll 1
+#pragma unroll
               for (int c = 0; c < 8 * DBOX; ++c)
                 *reinterpret_cast<uint4*>(sV + st * Shape::K_BYTES + (c >> 3) * Shape::K_BOX + r * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -381,16 +381,19 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     bool ok = true;
     int done = 0, lut_head = -1;
 
+    if (first < last) w.set(a, first, tiles);
     for (int item = first; item < last; item += step) {
-      w.set(a, item, tiles);
-      const int head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
+      const int batch = w.batch, head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
       if (BIAS && !ONE && head != lut_head) {
         asm volatile("bar.sync 1, 256;" ::: "memory");           // nobody reads the head before
         lut.set(a, head, warp - Shape::SOFT, 8);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         lut_head = head;
       }
-      if (!ok || t >= tiles.heads * tiles.blocks || row0 - quad * 32 >= a.Sq) continue;
+      if (!ok || t >= tiles.heads * tiles.blocks || row0 - quad * 32 >= a.Sq) {
+        if (item + step < last) w.set(a, item + step, tiles);
+        continue;
+      }
       const int my_lo = __shfl_sync(0xffffffffu, w.t_lo, t), my_hi = __shfl_sync(0xffffffffu, w.t_hi, t);
       const int p0 = w.sight.start + row0;        // position of the warp's first row
       // key tiles from whole_lo (or below the first keys' end) to whole_hi are seen whole by the warp's rows
@@ -442,6 +445,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
 #pragma unroll
           for (int c = 0; c < PIECES; ++c) {
             const uint32_t see = BIAS ? bits_below(valid - k0 - c * 32) : text_mask(a, valid, p0 + lane, k0 + c * 32);
+            if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (!(see >> e & 1u)) sv[c][e] = 0xff800000u;        // -inf
@@ -520,16 +524,17 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         ++done;
         fresh = false;
       }
+      if (item + step < last) w.set(a, item + step, tiles);      // while the last products run
       if (ok && !fresh) {
         ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], (done - 1) & 1, &abort_s));
-        if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 135 + t, w.n_kv);
+        if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 135 + t, item);
       }
       if (!ok) continue;
       tc_fence_after();
       const uint32_t keep = m_used == -INFINITY ? 0u : 0xffffffffu;      // a row without keys is zero whatever O holds
       const float inv_l = 1.f / l_run;
       // 32 columns at a time through shared memory, so that a store covers 64 bytes of eight rows instead of 16 of 32
-      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + w.batch * a.o_strides[0] + head * a.o_strides[2] + (row0 + (lane >> 2)) * a.o_strides[1] + (lane & 3) * 8;
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + batch * a.o_strides[0] + head * a.o_strides[2] + (row0 + (lane >> 2)) * a.o_strides[1] + (lane & 3) * 8;
       const int left = a.Sq - row0 - (lane >> 2);                        // rows of this lane from its first one on
       uint4* mine = reinterpret_cast<uint4*>(stage + lane * 64);
       const uint4* theirs = reinterpret_cast<const uint4*>(stage + (lane >> 2) * 64) + ((lane & 3) ^ (lane >> 3 & 3));
@@ -564,7 +569,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       __syncwarp();
       // +inf where a row saw nothing: the backward pass then finds probabilities of zero
       if (a.lse != nullptr && row0 + lane < a.Sq)
-        a.lse[(static_cast<long long>(w.batch) * a.H + head) * a.Sq + row0 + lane] = l_run > 0.f && m_used != -INFINITY ? m_used + log2f(l_run) : INFINITY;
+        a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + row0 + lane] = l_run > 0.f && m_used != -INFINITY ? m_used + log2f(l_run) : INFINITY;
     }
   }
 
