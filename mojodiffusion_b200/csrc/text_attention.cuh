@@ -39,6 +39,25 @@ __device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const Te
   return k;
 }
 
+// mbar_wait in fewer instructions, by a whole warp: these kernels wait at many places, and what they do in between must stay in the instruction cache
+__device__ __forceinline__ bool text_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint64_t since = 0;
+  uint32_t spins = 0;
+  bool ok = true;
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 63u) != 0) continue;
+    const uint64_t now = globaltimer_ns();
+    if (since == 0) since = now;
+    if (now - since > MDB_WAIT_LIMIT_NS || *abort_flag) {
+      *abort_flag = 1;
+      ok = false;
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // bit i: i < n
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 // bit i: the query at position p sees key k0 + i

@@ -172,6 +172,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     const int n_q = tiles.heads * tiles.blocks;
     if (elect_one()) {
       mbar_expect_tx(&q_full, n_q * Shape::Q_BYTES);
+#pragma unroll 1
       for (int t = 0; t < n_q; ++t)
         for (int d = 0; d < DBOX; ++d)
           tma_load_4d(sQ + t * Shape::Q_BYTES + d * Shape::Q_BOX, &maps.q, &q_full, d * 64, w.tile_q0(w.q0, t, tiles), w.tile_head(w.head, t, tiles), w.batch);
@@ -193,7 +194,9 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     w.set(a, first, tiles);
     if (w.n_kv > 0) {
       load_q();
+#pragma unroll 1
       for (; early < STAGES && early < w.n_kv; ++early)
+#pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) load_kv(kv, early, early, w.head / rep);
     }
   }
@@ -215,11 +218,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         if (item != first) w.set(a, item, tiles);
         if (w.n_kv == 0) continue;
         if (item != first) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&q_empty, (n_items & 1) ^ 1u, &abort_s));
-          if (!ok) {
-            if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 110, item);
-            break;
-          }
+          ok = text_wait(&q_empty, (n_items & 1) ^ 1u, &abort_s);
+          if (!ok) break;
           load_q();
         }
         ++n_items;
@@ -228,12 +228,10 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           if (n_tiles < early) continue;
           const int st = n_tiles % STAGES;
           const uint32_t par = (n_tiles / STAGES) & 1;
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
-            ok = __all_sync(0xffffffffu, mbar_wait(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s));
-            if (!ok) {
-              if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 111 + kv, i);
-              break;
-            }
+            ok = text_wait(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s);
+            if (!ok) break;
             load_kv(kv, st, i, kv_head);
             last_bar = kv ? &v_full[st] : &k_full[st];
             last_par = par;
@@ -241,6 +239,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         }
       }
       if (!ok) {
+        if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 111, n_tiles);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(last_bar, last_par) && globaltimer_ns() - t0 < 5000000ull) {
         }
@@ -280,11 +279,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           t_lo[u] = __shfl_sync(0xffffffffu, w.t_lo, u);
           t_hi[u] = __shfl_sync(0xffffffffu, w.t_hi, u);
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&q_full, n_items & 1, &abort_s) && mbar_wait(&k_full[n_tiles % STAGES], (n_tiles / STAGES) & 1, &abort_s));
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 121, item);
-          break;
-        }
+        ok = text_wait(&q_full, n_items & 1, &abort_s) && text_wait(&k_full[n_tiles % STAGES], (n_tiles / STAGES) & 1, &abort_s);
+        if (!ok) break;
         ++n_items;
         tc_fence_after();
         if (elect_one()) {
@@ -298,21 +294,14 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         // the epilogue of the item before has read the tiles' O
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (ok && t_hi[u] > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_empty[u], (outs[u]++ & 1) ^ 1u, &abort_s));
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 122, item);
-          break;
-        }
+          if (ok && !ONE && t_hi[u] > 0) ok = text_wait(&o_empty[u], (outs[u]++ & 1) ^ 1u, &abort_s);
+        if (!ok) break;
         uint32_t begun[2] = {0, 0};
         for (int i = 0; i < w.n_kv; ++i, ++n_tiles) {
           const int st = n_tiles % STAGES, st_n = (n_tiles + 1) % STAGES;
           const bool more = i + 1 < w.n_kv;
-          ok = __all_sync(0xffffffffu, mbar_wait(&v_full[st], (n_tiles / STAGES) & 1, &abort_s) &&
-                                           (!more || mbar_wait(&k_full[st_n], ((n_tiles + 1) / STAGES) & 1, &abort_s)));
-          if (!ok) {
-            if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 123, i);
-            break;
-          }
+          ok = text_wait(&v_full[st], (n_tiles / STAGES) & 1, &abort_s) && (!more || text_wait(&k_full[st_n], ((n_tiles + 1) / STAGES) & 1, &abort_s));
+          if (!ok) break;
           const int k0 = w.key_tile(i) * TK;
           if (k0 + TK > w.all.end || (k0 < w.all.lo && k0 + TK > w.all.sinks)) {
 #pragma unroll 1
@@ -332,11 +321,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             if (w.sees(t_lo[u], t_hi[u], i)) {
 #pragma unroll
               for (int part = 0; part < PARTS; ++part) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&p_full[u][part], done[u] & 1, &abort_s));
-                if (!ok) {
-                  if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 124 + u, i);
-                  return;
-                }
+                ok = text_wait(&p_full[u][part], done[u] & 1, &abort_s);
+                if (!ok) return;
                 tc_fence_after();
                 if (elect_one()) {
                   issue_pv(u, st, part, begun[u]);
@@ -366,6 +352,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           __syncwarp();
         }
       }
+      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 121, n_tiles);
     }
     __syncwarp();
   } else {
@@ -409,11 +396,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       for (int i = 0, kt = w.key_tile(0); i < w.n_kv; ++i, kt = i == w.ns ? w.lo : kt + 1) {
         if (kt >= my_hi || (kt < my_lo && kt >= w.ns)) continue;
         const int k0 = kt * TK;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], done & 1, &abort_s));
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, i);
-          break;
-        }
+        ok = text_wait(&s_full[t], done & 1, &abort_s);
+        if (!ok) break;
         tc_fence_after();
         uint32_t sv[PIECES][32];
 #pragma unroll
@@ -470,11 +454,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           // The reference is raised when a row has outgrown it by more than 2^8, and with the first key that a row sees.
           const bool need = mx > m_used + 8.0f;
           if (__any_sync(0xffffffffu, need)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], (done - 1) & 1, &abort_s));
-            if (!ok) {
-              if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141 + t, i);
-              break;
-            }
+            ok = text_wait(&o_full[t], (done - 1) & 1, &abort_s);
+            if (!ok) break;
             tc_fence_after();
             const float alpha = need ? exp2f(m_used - mx) : 1.0f;
             if (need) m_used = mx;
@@ -526,8 +507,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       }
       if (item + step < last) w.set(a, item + step, tiles);      // while the last products run
       if (ok && !fresh) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], (done - 1) & 1, &abort_s));
-        if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 135 + t, item);
+        ok = text_wait(&o_full[t], (done - 1) & 1, &abort_s);
       }
       if (!ok) continue;
       tc_fence_after();
@@ -551,7 +531,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         tmem_wait_ld();
         if (c == DH / 32 - 1) tc_fence_before();
         __syncwarp();
-        if (c == DH / 32 - 1 && lane == 0) mbar_arrive(&o_empty[t]);      // the next item's products may have O
+        if (!ONE && c == DH / 32 - 1 && lane == 0) mbar_arrive(&o_empty[t]);      // the next item's products may have O
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint4 v;
@@ -571,6 +551,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       if (a.lse != nullptr && row0 + lane < a.Sq)
         a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + row0 + lane] = l_run > 0.f && m_used != -INFINITY ? m_used + log2f(l_run) : INFINITY;
     }
+    if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, done);
   }
 
   tc_fence_before();
