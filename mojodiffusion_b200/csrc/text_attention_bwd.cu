@@ -36,52 +36,61 @@ struct alignas(64) TextBwdMaps {
 };
 
 template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
-  static constexpr int STAGES = (DH == 128 && BIAS && !KEYS) ? 2 : 4;      // the accumulators of dtable take the place of two
-  static constexpr int TILES = 2 * TR * DH * 2 + STAGES * 2 * TC * DH * 2 + 1024;
-  static constexpr int SUMS = (BIAS && !KEYS) ? 8 * 32 * RUN_LD * 4 : 0;
+  static constexpr bool SUMMED = BIAS && !KEYS;                            // dtable is formed
+  // Heads of 64: two CTAs to an SM, each with one buffer of X and Y whose columns the two warpgroups share. The accumulators of dtable leave room for
+  // one CTA, heads of 128 need all of TMEM: there two buffers, one for either warpgroup.
+  static constexpr int CTAS = DH == 64 && !SUMMED ? 2 : 1, BUFS = CTAS == 2 ? 1 : 2;
+  static constexpr int TMEM = CTAS == 2 ? 256 : 512;
+  static constexpr int STAGES = 4;
+  static constexpr int TILES = (KEYS ? 2 * TR * DH * 2 : 0) + STAGES * 2 * TC * DH * 2 + 1024;
+  static constexpr int SUMS = SUMMED ? 8 * 32 * RUN_LD * 4 : 0;
   static __host__ __device__ int lut_bytes(int near) { return BIAS ? TextLut::bytes(near) : 0; }
   static __host__ __device__ int bytes(int near, int buckets) {
-    return TILES + SUMS + lut_bytes(near) + ((BIAS && !KEYS) ? buckets * 256 * 4 + (2 * near + 4) + (buckets + 2) * 8 : 0);
+    return TILES + SUMS + lut_bytes(near) + (SUMMED ? buckets * 256 * 4 + buckets * 4 + (2 * near + 4) : 0);
   }
 };
 
 template <int DH, bool KEYS, bool BIAS>
-__global__ void __launch_bounds__(TB_THREADS, 1)
-text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a) {
+__global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
+text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const int ranks) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
-  constexpr int STAGES = Shape::STAGES;
+  constexpr int STAGES = Shape::STAGES, BUFS = Shape::BUFS;
+  constexpr bool SUMMED = Shape::SUMMED;
   constexpr int DBOX = DH / 64;
   constexpr int R_BYTES = TR * DH * 2, R_BOX = TR * 128;
   constexpr int C_BYTES = TC * DH * 2, C_BOX = TC * 128;
-  constexpr uint32_t X_COL = 0, Y_COL = 128, ACC1_COL = 256, ACC2_COL = 384;  // X0 X1 | Y0 Y1 | dQ or dK | dV
+  constexpr uint32_t X_COL = 0, Y_COL = BUFS * TC, ACC1_COL = 2 * BUFS * TC, ACC2_COL = ACC1_COL + DH;      // X buffers | Y buffers | dQ or dK | dV
+  constexpr uint32_t AQ_COL = ACC1_COL + DH, AD_COL = AQ_COL + DH / 2;                                 // dq: Q | dO, bf16 pairs
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2], acc_full;
+  __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2], acc_full, a_full;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
-  __shared__ __align__(16) float s_lse[2][TC], s_delta[2][TC];      // negated, per staged query
+  __shared__ uint32_t has_part;
+  __shared__ __align__(16) float s_lse[2][TC], s_delta[2][TC];      // negated, per staged query: of either buffer, or of either warpgroup's columns, twice
 
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
   uint8_t* sR1 = smem;
   uint8_t* sR2 = sR1 + R_BYTES;
-  uint8_t* sC = sR2 + R_BYTES;                                            // STAGES x (C1, C2)
+  uint8_t* sC = KEYS ? sR2 + R_BYTES : smem;                              // STAGES x (C1, C2)
   const int near = BIAS ? text_near(a) : 0;
-  float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // BIAS dq: running sums [8 warps][32 rows][RUN_LD]
+  float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // SUMMED: running sums [8 warps][32 rows][RUN_LD]
   const TextLut lut(sums + Shape::SUMS / 4, near);                        // BIAS
-  float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // BIAS dq: [buckets][256 threads]
-  // BIAS dq: the buckets in the order of their distances ("runs"): first distance and bucket of each, and the run of the distances -near .. near
+  float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // SUMMED: [buckets][256 threads]: dS of a row before its first key of each run
+  // SUMMED: the buckets in the order of their distances ("runs"): first distance of each, and the run of the distances -near .. near
   const int run_mid = a.exact + a.n_borders, runs = 2 * run_mid + 1;
-  int* run_start = reinterpret_cast<int*>(bins + a.buckets * 256);        // [runs + 1]
-  int* run_bucket = run_start + a.buckets + 2;                            // [runs]
-  uint8_t* run_of = reinterpret_cast<uint8_t*>(run_bucket + a.buckets + 2);
+  int* run_start = reinterpret_cast<int*>(bins + a.buckets * 256);        // [runs]
+  uint8_t* run_of = reinterpret_cast<uint8_t*>(run_start + a.buckets);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int batch = blockIdx.z;
   const int rep = a.H / a.Hkv;
   // the rows with the most to stream start first: late queries, early keys
-  const int r0 = (KEYS || BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TR;
+  // KEYS: the CTAs of a cluster share what is streamed for one block of keys
+  const int rank = KEYS ? blockIdx.x % ranks : 0;
+  const int r0 = (KEYS ? blockIdx.x / ranks : BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TR;
   const int out_rows = KEYS ? a.Skv : a.Sq;
   const TextSight sight = text_sight(a, batch);
 
@@ -105,8 +114,18 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
   const int per_head = ns + hi - lo;
-  const int n_c = KEYS ? per_head * rep : per_head;
+  const int n_all = KEYS ? per_head * rep : per_head;
+  const int i_first = KEYS ? static_cast<int>(static_cast<long long>(n_all) * rank / ranks) : 0;
+  const int n_c = KEYS ? static_cast<int>(static_cast<long long>(n_all) * (rank + 1) / ranks) - i_first : n_all;
   const auto tile_of = [&](int i) { return i < ns ? i : i - ns + lo; };
+  const auto key_seen = [&](int key) {
+    long long first = 0, end = a.Sq;
+    if (!BIAS) {
+      first = max(key - sight.start, 0);
+      if (key >= a.sinks) end = min(end, static_cast<long long>(key) + a.window - sight.start);
+    }
+    return key < sight.valid && first < end;
+  };
 
   if (threadIdx.x == 0) {
     mbar_init(&r_full, 1);
@@ -116,20 +135,23 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&xy_full[s], 1);
-      mbar_init(&pds_full[s], 4);
-      mbar_init(&lv_full[s], TC);
+      mbar_init(&pds_full[s], BUFS == 1 ? 8 : 4);
+      mbar_init(&lv_full[s], BUFS == 1 ? 32 : TC);
     }
     mbar_init(&acc_full, 1);
+    mbar_init(&a_full, 8);
     abort_s = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base_s, 512);
+    tmem_alloc(&tmem_base_s, Shape::TMEM);
     tmem_relinquish();
   }
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&maps.r1);
-    tma_prefetch_desc(&maps.r2);
+    if (KEYS) {
+      tma_prefetch_desc(&maps.r1);
+      tma_prefetch_desc(&maps.r2);
+    }
     tma_prefetch_desc(&maps.c1);
     tma_prefetch_desc(&maps.c2);
   }
@@ -145,9 +167,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       for (int r = threadIdx.x; r < runs; r += TB_THREADS) {
         const int c = r < run_mid ? run_mid - r : r - run_mid;                 // bucket within its direction
         const auto reach = [&](int b) { return b <= a.exact ? b : a.borders[b - a.exact - 1]; };      // its first distance
-        run_bucket[r] = r <= run_mid ? c : c + a.buckets / 2;
         run_start[r] = r == 0 ? -TXT_FAR : r <= run_mid ? 1 - reach(c + 1) : reach(c);
-        if (r == 0) run_start[runs] = TXT_FAR;
       }
     }
   }
@@ -159,7 +179,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   if (warp == 0) {
     // ----------------------------- TMA producer -----------------------------
     if (n_c > 0) {
-      if (elect_one()) {
+      if (KEYS && elect_one()) {
         mbar_expect_tx(&r_full, 2 * R_BYTES);
         for (int d = 0; d < DBOX; ++d) {
           tma_load_4d(sR1 + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
@@ -168,13 +188,13 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       }
       __syncwarp();
       bool ok = true;
-      uint64_t* last_bar = &r_full;
+      uint64_t* last_bar = KEYS ? &r_full : &c_full[0];
       uint32_t last_par = 0;
-      int head = KEYS ? blockIdx.y * rep : blockIdx.y / rep, in_head = 0;
+      int head = KEYS ? blockIdx.y * rep + i_first / max(per_head, 1) : blockIdx.y / rep, in_head = KEYS ? i_first % max(per_head, 1) : 0;
       for (int i = 0; i < n_c; ++i) {
         const int st = i & (STAGES - 1);
         const uint32_t par = (i / STAGES) & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&c_empty[st], par ^ 1u, &abort_s));
+        ok = text_wait(&c_empty[st], par ^ 1u, &abort_s);
         if (!ok) {
           if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141, i);
           break;
@@ -214,21 +234,23 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         const uint32_t x = tmem_base + X_COL + buf * TC, y = tmem_base + Y_COL + buf * TC;
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk)
-          umma_f16_ss(x, r1 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c1 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+          if (KEYS) umma_f16_ss(x, r1 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c1 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+          else umma_f16_ts(x, tmem_base + AQ_COL + kk * 8, c1 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk)
-          umma_f16_ss(y, r2 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c2 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+          if (KEYS) umma_f16_ss(y, r2 + (((kk / 4) * R_BOX + (kk % 4) * 32) >> 4), c2 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
+          else umma_f16_ts(y, tmem_base + AD_COL + kk * 8, c2 + (((kk / 4) * C_BOX + (kk % 4) * 32) >> 4), idesc_xy, kk != 0 ? 1u : 0u);
         umma_commit(&xy_full[buf]);
       };
       const auto issue_acc = [&](int st, int buf, bool first) {
         const uint64_t c1 = cm + static_cast<uint64_t>(st * (2 * C_BYTES >> 4)), c2 = c1 + (C_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < TC / 16; ++kk)
-          umma_f16_ts(tmem_base + ACC1_COL, tmem_base + Y_COL + buf * TC + kk * 8, c1 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
+          umma_f16_ts(tmem_base + ACC1_COL, tmem_base + Y_COL + buf * TC + kk / 2 * 32 + kk % 2 * 8, c1 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
         if (KEYS) {
 #pragma unroll
           for (int kk = 0; kk < TC / 16; ++kk)
-            umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk * 8, c2 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
+            umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk / 2 * 32 + kk % 2 * 8, c2 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
         }
       };
       // rows of a key tile that no query of the CTA sees
@@ -246,8 +268,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         fence_proxy_async_smem();
         __syncwarp();
       };
-      bool ok = __all_sync(0xffffffffu, mbar_wait(&r_full, 0, &abort_s) && mbar_wait(&c_full[0], 0, &abort_s));
-      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 151, 0);
+      bool ok = text_wait(KEYS ? &r_full : &a_full, 0, &abort_s) && text_wait(&c_full[0], 0, &abort_s);
       if (ok) {
         tc_fence_after();
         clean(0, 0);
@@ -255,36 +276,35 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         __syncwarp();
       }
       for (int i = 0; ok && i < n_c; ++i) {
-        const int st = i & (STAGES - 1);
-        if (i + 1 < n_c) {
-          const int stn = (i + 1) & (STAGES - 1);
-          ok = __all_sync(0xffffffffu, mbar_wait(&c_full[stn], ((i + 1) / STAGES) & 1, &abort_s));
-          if (!ok) {
-            if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 152, i);
-            break;
-          }
+        const int st = i & (STAGES - 1), stn = (i + 1) & (STAGES - 1);
+        const bool more = i + 1 < n_c;
+        if (more) {
+          ok = text_wait(&c_full[stn], ((i + 1) / STAGES) & 1, &abort_s);
+          if (!ok) break;
           tc_fence_after();
           clean(i + 1, stn);
-          if (elect_one()) issue_xy(stn, (i + 1) & 1);
-          __syncwarp();
+          if (BUFS == 2) {
+            if (elect_one()) issue_xy(stn, (i + 1) & 1);
+            __syncwarp();
+          }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&pds_full[i & 1], (i >> 1) & 1, &abort_s));
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 153, i);
-          break;
-        }
+        ok = text_wait(&pds_full[BUFS == 2 ? i & 1 : 0], (BUFS == 2 ? i >> 1 : i) & 1, &abort_s);
+        if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_acc(st, i & 1, i == 0);
+          issue_acc(st, BUFS == 2 ? i & 1 : 0, i == 0);
           umma_commit(&c_empty[st]);
-          if (i + 1 == n_c) umma_commit(&acc_full);
+          if (more && BUFS == 1) issue_xy(stn, 0);        // over scores that the products before have read
+          if (!more) umma_commit(&acc_full);
         }
         __syncwarp();
       }
+      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 151, n_c);
     }
     __syncwarp();
   } else {
     // ------------------------------- math: warpgroup g takes the tiles of buffer g, every second one
+    // (with one buffer: 32 columns of every tile)
     const int g = (warp - 2) >> 2;
     const int quad = warp & 3;
     const int mt = quad * 32 + lane;  // row inside the resident tile == TMEM lane
@@ -293,76 +313,106 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     const int row = r0 + mt;
     const float sl2 = a.scale * TXT_LOG2E;
     float my_nlse = -INFINITY, my_ndelta = 0.f;       // rows behind the last query: probabilities of zero
-    if (!KEYS && row < a.Sq) {
-      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
-      const uint4* o = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o) + batch * a.o_strides[0] + row * a.o_strides[1] + blockIdx.y * a.o_strides[2]);
-      const uint4* d = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dout) + batch * a.do_strides[0] + row * a.do_strides[1] + blockIdx.y * a.do_strides[2]);
-      float2 s = make_float2(0.f, 0.f);
+    if (!KEYS) {
+      // Q (warpgroup 0) and dO (1) become A operands in TMEM: with 64 columns of B, A from shared memory would cost the score products 48 cycles for
+      // every 32. On the way warpgroup 1 forms delta.
+      const long long* st = g == 0 ? a.q_strides : a.do_strides;
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(g == 0 ? a.q : a.dout) + batch * st[0] + row * st[1] + blockIdx.y * st[2]);
+      const uint4* out = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o) + batch * a.o_strides[0] + row * a.o_strides[1] + blockIdx.y * a.o_strides[2]);
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < DH / 8; ++c) {
-        const uint4 u = o[c], w = d[c];
-        s = ffma2(unpack_bf16x2(u.x), unpack_bf16x2(w.x), s);
-        s = ffma2(unpack_bf16x2(u.y), unpack_bf16x2(w.y), s);
-        s = ffma2(unpack_bf16x2(u.z), unpack_bf16x2(w.z), s);
-        s = ffma2(unpack_bf16x2(u.w), unpack_bf16x2(w.w), s);
+      for (int c = 0; c < DH / 64; ++c) {
+        uint32_t r[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 u = row < a.Sq ? src[c * 8 + e] : make_uint4(0, 0, 0, 0);
+          r[4 * e] = u.x;
+          r[4 * e + 1] = u.y;
+          r[4 * e + 2] = u.z;
+          r[4 * e + 3] = u.w;
+        }
+        if (g == 1 && row < a.Sq) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 w = out[c * 8 + e];
+            sum = ffma2(unpack_bf16x2(r[4 * e]), unpack_bf16x2(w.x), sum);
+            sum = ffma2(unpack_bf16x2(r[4 * e + 1]), unpack_bf16x2(w.y), sum);
+            sum = ffma2(unpack_bf16x2(r[4 * e + 2]), unpack_bf16x2(w.z), sum);
+            sum = ffma2(unpack_bf16x2(r[4 * e + 3]), unpack_bf16x2(w.w), sum);
+          }
+        }
+        tmem_st_32x32b_x32(tmem_base + lane_addr + (g == 0 ? AQ_COL : AD_COL) + c * 32, r);
       }
-      my_ndelta = -(s.x + s.y);
-      my_nlse = -a.lse[at];
-      if (g == 0) a.delta[at] = -my_ndelta;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full);
+      float* deltas = &s_delta[0][0];          // [128]
+      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
+      if (row < a.Sq) my_nlse = -a.lse[at];
+      if (g == 1) {
+        deltas[mt] = sum.x + sum.y;
+        if (row < a.Sq) a.delta[at] = sum.x + sum.y;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      my_ndelta = -deltas[mt];
     }
     // KEYS: thread mt < 64 stages the negated lse and delta of query mt of the warpgroup's tile, loaded one of its tiles ahead
     float next_nlse = -INFINITY, next_ndelta = 0.f;
-    int f_head = KEYS ? blockIdx.y * rep : 0, f_tile = 0;
+    constexpr int STAGERS = BUFS == 1 ? 32 : TC;          // threads of a warpgroup that stage, and queries that they stage
+    int f_head = KEYS ? blockIdx.y * rep + i_first / max(per_head, 1) : 0, f_tile = KEYS ? i_first % max(per_head, 1) : 0;
     const auto fetch = [&](int ahead) {
       f_tile += ahead;
       while (f_tile >= per_head) {
         f_tile -= per_head;
         ++f_head;
       }
-      const int q = (lo + f_tile) * TC + mt;
-      const bool in = mt < TC && q < a.Sq && f_head < (static_cast<int>(blockIdx.y) + 1) * rep;
+      const int q = (lo + f_tile) * TC + (BUFS == 1 ? g * 32 : 0) + mt;
+      const bool in = q < a.Sq && f_head < (static_cast<int>(blockIdx.y) + 1) * rep;
       const long long at = (static_cast<long long>(batch) * a.H + f_head) * a.Sq + q;
       next_nlse = in ? -a.lse[at] : -INFINITY;
       next_ndelta = in ? -a.delta[at] : 0.f;
     };
-    if (KEYS && g < n_c) fetch(g);
+    const int i_begin = BUFS == 2 ? g : 0;
+    const bool stager = mt < STAGERS;                    // the same in a whole warp
+    if (KEYS && stager && i_begin < n_c) fetch(i_begin);
+    float sum_all = 0.f;      // SUMMED: dS of this row and warpgroup so far, which ends before key sum_end
+    int sum_end = 0;
     bool ok = true;
-    int in_head = g;
-    const uint32_t xa = tmem_base + lane_addr + X_COL + g * TC;
-    const uint32_t ya = tmem_base + lane_addr + Y_COL + g * TC;
-    for (int i = g; i < n_c; i += 2) {
-      const uint32_t par = (i >> 1) & 1;
+    int in_head = (KEYS ? i_first % max(per_head, 1) : 0) + i_begin;
+    const uint32_t xa = tmem_base + lane_addr + X_COL + (BUFS == 2 ? g * TC : 0);
+    const uint32_t ya = tmem_base + lane_addr + Y_COL + (BUFS == 2 ? g * TC : 0);
+    for (int i = i_begin; i < n_c; i += BUFS) {
+      const uint32_t par = (BUFS == 2 ? i >> 1 : i) & 1;
+      const int half = BUFS == 1 ? (i & 1) * 32 : 0;      // where this tile's queries are staged
       if (KEYS) {
         while (in_head >= per_head) in_head -= per_head;
-        // the buffer was last read for tile i - 2: the warpgroup's four warps have all arrived on pds_full[g] for it
+        // Two buffers: the place was last read for tile i - 2, and the warpgroup's four warps have all arrived on pds_full[g] for it. One buffer: also for
+        // tile i - 2, and the scores of tile i - 1, which this warp has seen, were only formed after all warps had arrived for it.
         bool lv_ok = true;
-        if (mt < TC) {
-          if (i >= 2) lv_ok = mbar_wait(&pds_full[g], par ^ 1u, &abort_s);
-          s_lse[g][mt] = next_nlse;
-          s_delta[g][mt] = next_ndelta;
+        if (stager) {
+          if (BUFS == 2 && i >= 2) lv_ok = mbar_wait(&pds_full[g], par ^ 1u, &abort_s);
+          s_lse[g][half + mt] = next_nlse;
+          s_delta[g][half + mt] = next_ndelta;
           mbar_arrive(&lv_full[g]);
         }
-        if (i + 2 < n_c) fetch(2);
-        lv_ok = mbar_wait(&lv_full[g], par, &abort_s) && lv_ok;
-        if (!__all_sync(0xffffffffu, lv_ok)) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 160, i);
-          ok = false;
-          break;
-        }
+        if (stager && i + BUFS < n_c) fetch(BUFS);
+        ok = text_wait(&lv_full[g], par, &abort_s);
+        ok = __all_sync(0xffffffffu, ok && lv_ok);
+        if (!ok) break;
       }
       const int c0 = tile_of(in_head) * TC;          // first key (dq) or query (KEYS) of the tile
-      ok = __all_sync(0xffffffffu, mbar_wait(&xy_full[g], par, &abort_s));
-      if (!ok) {
-        if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 161, i);
-        break;
-      }
+      ok = text_wait(&xy_full[BUFS == 2 ? g : 0], par, &abort_s);
+      if (!ok) break;
       tc_fence_after();
-      uint32_t xr[2][32], yr[2][32];
-      float run[2][32];                              // BIAS dq: dS
+      constexpr int NC = BUFS;                       // pieces of 32 columns of a thread: all of the tile's, or one
+      const int piece0 = BUFS == 1 ? g : 0;
+      uint32_t xr[NC][32], yr[NC][32];
+      float run[NC][32];                             // BIAS dq: dS
 #pragma unroll
-      for (int c = 0; c < TC / 32; ++c) {
-        tmem_ld_32x32b_x32(xa + c * 32, xr[c]);
-        tmem_ld_32x32b_x32(ya + c * 32, yr[c]);
+      for (int c = 0; c < NC; ++c) {
+        tmem_ld_32x32b_x32(xa + (piece0 + c) * 32, xr[c]);
+        tmem_ld_32x32b_x32(ya + (piece0 + c) * 32, yr[c]);
       }
       tmem_wait_ld();
       bool whole;       // every pair of the tile is visible, or its row or query lies behind the last one and has a probability of zero anyway
@@ -370,8 +420,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       else if (KEYS) whole = r0 + TR <= sight.valid && r0 + TR - 1 <= sight.start + c0 && (sight.start + c0 + TC - 1 - a.window < r0 || r0 + TR <= a.sinks);
       else whole = c0 + TC <= sight.valid && c0 + TC - 1 <= sight.start + r0 && (sight.start + r0 + TR - 1 - a.window < c0 || c0 + TC <= a.sinks);
 #pragma unroll
-      for (int c = 0; c < TC / 32; ++c) {
-        const int b0 = c0 + c * 32;
+      for (int c = 0; c < NC; ++c) {
+        const int b0 = c0 + (piece0 + c) * 32;
         uint32_t see = 0xffffffffu;
         if (!whole) {
           if (BIAS) see = KEYS ? (row < sight.valid ? see : 0u) : bits_below(sight.valid - b0);
@@ -394,7 +444,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         for (int e = 0; e < 32; e += 4) {
           float nl[4], nd[4];
           if (KEYS) {
-            const float4 u = *reinterpret_cast<const float4*>(&s_lse[g][c * 32 + e]), w = *reinterpret_cast<const float4*>(&s_delta[g][c * 32 + e]);
+            const float4 u = *reinterpret_cast<const float4*>(&s_lse[g][half + c * 32 + e]), w = *reinterpret_cast<const float4*>(&s_delta[g][half + c * 32 + e]);
             nl[0] = u.x; nl[1] = u.y; nl[2] = u.z; nl[3] = u.w;
             nd[0] = w.x; nd[1] = w.y; nd[2] = w.z; nd[3] = w.w;
           } else {
@@ -434,67 +484,74 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             run[c][e + 3] = d23.y;
           }
         }
-        if (KEYS) tmem_st_32x32b_x16(xa + c * 16, pk);
-        tmem_st_32x32b_x16(ya + c * 16, dk);
+        if (KEYS) tmem_st_32x32b_x16(xa + (piece0 + c) * 32, pk);      // over scores of this piece: they are in registers by now
+        tmem_st_32x32b_x16(ya + (piece0 + c) * 32, dk);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&pds_full[g]);
-      if (BIAS && !KEYS && a.d_table != nullptr) {
+      if (lane == 0) mbar_arrive(&pds_full[BUFS == 2 ? g : 0]);
+      if (SUMMED && a.d_table != nullptr) {
         // with the tile's products under way
 #pragma unroll
-        for (int c = 0; c < TC / 32; ++c) {
+        for (int c = 0; c < NC; ++c) {
           const int b0 = c0 + c * 32, d0 = b0 - (r0 + quad * 32);
-          const int first = run_of[min(max(d0 - 31 + near, 0), 2 * near)], last = run_of[min(max(d0 + 31 + near, 0), 2 * near)];
-          if (first == last) {
-            float2 s = make_float2(0.f, 0.f);
+          const int r_lo = run_of[min(max(sum_end - (r0 + quad * 32) - 32 + near, 0), 2 * near)], r_hi = run_of[min(max(d0 + 31 + near, 0), 2 * near)];
+          // running sums of four pieces of eight, then of the whole
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) s = fadd2(s, make_float2(run[c][e], run[c][e + 1]));
-            bins[run_bucket[first] * 256 + slot] += s.x + s.y;
-          } else {
-            // running sums of four pieces of eight, then of the whole
-            float* mine = sums + ((warp - 2) * 32 + lane) * RUN_LD;
+          for (int e = 1; e < 8; ++e)
 #pragma unroll
-            for (int e = 1; e < 8; ++e)
+            for (int m = 0; m < 32; m += 8) run[c][m + e] += run[c][m + e - 1];
 #pragma unroll
-              for (int m = 0; m < 32; m += 8) run[c][m + e] += run[c][m + e - 1];
-#pragma unroll
-            for (int m = 8; m < 32; m += 8) {
-              const float base = run[c][m - 1];
+          for (int m = 8; m < 32; m += 8) {
+            const float base = run[c][m - 1];
+            if (r_lo == r_hi) {
+              run[c][m + 7] += base;
+            } else {
 #pragma unroll
               for (int e = 0; e < 8; ++e) run[c][m + e] += base;
             }
+          }
+          if (r_lo != r_hi) {
+            float* mine = sums + ((warp - 2) * 32 + lane) * RUN_LD;
 #pragma unroll
             for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(mine + e) = make_float4(run[c][e], run[c][e + 1], run[c][e + 2], run[c][e + 3]);
-            float before = 0.f;
-            for (int r = first; r <= last; ++r) {
-              const int end = min(max(run_start[r + 1] + row - b0, 0), 32);
-              const float upto = end > 0 ? mine[end - 1] : 0.f;
-              bins[run_bucket[r] * 256 + slot] += upto - before;
-              before = upto;
+            // Bucket r + 1 of this row begins at key `at`: what came before it. Where that key lies in a tile of the other warpgroup, the sum so far.
+#pragma unroll 4
+            for (int r = r_lo; r < r_hi; ++r) {
+              const int at = run_start[r + 1] + row;
+              const float upto = at > b0 ? mine[min(at - b0, 32) - 1] : 0.f;
+              if (at >= sum_end && at < b0 + 32) bins[(r + 1) * 256 + slot] = sum_all + upto;
             }
           }
+          sum_all += run[c][31];
+          sum_end = b0 + 32;
         }
       }
-      in_head += 2;
+      in_head += BUFS;
     }
-    if (ok && n_c > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, &abort_s));
-      if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 162, 0);
-    }
-    if (ok) {
+    if (ok && n_c > 0) ok = text_wait(&acc_full, 0, &abort_s);
+    if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 161, n_c);
+    if (ok && KEYS && ranks > 1 && n_c > 0) {
+      // the parts of dk (warpgroup 0) and dv (1) of this CTA, fp32 [2][128][DH], over the tiles, which nothing reads any more
+      tc_fence_after();
+      float4* part = reinterpret_cast<float4*>(smem) + (g * TR + mt) * (DH / 4);
+      const uint32_t acc = tmem_base + lane_addr + (g == 1 ? ACC2_COL : ACC1_COL);
+#pragma unroll 1
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(acc + c * 32, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          part[(c * 8 + e) ^ (mt & 7)] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
+      }
+    } else if (ok && (!KEYS || ranks == 1)) {
       // dq: each warpgroup stores half of the columns; KEYS: warpgroup 0 dk, warpgroup 1 dv
       tc_fence_after();
       bool some = n_c > 0;
       if (KEYS) {
-        // a key that no query sees may hold anything, and its gradient is zero
-        long long first = 0, end = a.Sq;
-        if (!BIAS) {
-          first = max(row - sight.start, 0);
-          if (row >= a.sinks) end = min(end, static_cast<long long>(row) + a.window - sight.start);
-        }
-        some = some && row < sight.valid && first < end;
+        some = some && key_seen(row);      // a key that no query sees may hold anything, and its gradient is zero
       }
       const bool second = KEYS && g == 1;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk);
@@ -526,13 +583,20 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         }
       }
     }
-    if (BIAS && !KEYS && a.d_table != nullptr) {
+    if (SUMMED && a.d_table != nullptr) {
+      // runs that begin behind the last key, and the end of the last one
+      for (int r = 1; r < runs; ++r)
+        if (run_start[r] + row >= sum_end) bins[r * 256 + slot] = sum_all;
+      bins[runs * 256 + slot] = sum_all;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       float* part = a.table_ws + ((static_cast<long long>(batch) * a.H + blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets;
       for (int c = warp - 2; c < a.buckets; c += 8) {
+        const int side = c < a.buckets / 2 ? c : c - a.buckets / 2, r = c < a.buckets / 2 ? run_mid - c : run_mid + side;
         float s = 0.f;
+        if (side <= run_mid && (c < a.buckets / 2 || side > 0)) {
 #pragma unroll
-        for (int m = 0; m < 256; m += 32) s += bins[c * 256 + m + lane];
+          for (int m = 0; m < 256; m += 32) s += bins[(r + 1) * 256 + m + lane] - bins[r * 256 + m + lane];
+        }
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
         if (lane == 0) part[c] = s;
@@ -540,11 +604,48 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
 
+  if (KEYS && ranks > 1) {
+    // the cluster's parts, added in the order of their ranks; every CTA stores its share of the rows
+    if (threadIdx.x == 0) has_part = n_c > 0 ? 1u : 0u;
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const int share = TR / ranks;
+    uint32_t parts = 0;
+    for (int k = 0; k < ranks; ++k) parts |= ld_cluster_u32(mapa_shared(smem_u32(&has_part), k)) << k;
+    for (int e = threadIdx.x; e < 2 * share * (DH / 8); e += TB_THREADS) {
+      const int c = e % (DH / 8), m = e / (DH / 8) / share, rr = rank * share + e / (DH / 8) % share, key = r0 + rr;
+      if (key >= out_rows) continue;
+      float4 x[4], y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!(parts >> k & 1u)) continue;
+        const uint32_t at = mapa_shared(smem_u32(smem), k) + (m * TR + rr) * (DH * 4);
+        x[k] = ld_cluster_f32x4(at + (((2 * c) ^ (rr & 7)) << 4));
+        y[k] = ld_cluster_f32x4(at + (((2 * c + 1) ^ (rr & 7)) << 4));
+      }
+      float4 u = x[0], v = y[0];
+#pragma unroll
+      for (int k = 1; k < 4; ++k) {
+        u.x += x[k].x; u.y += x[k].y; u.z += x[k].z; u.w += x[k].w;
+        v.x += y[k].x; v.y += y[k].y; v.z += y[k].z; v.w += y[k].w;
+      }
+      const float f = m == 0 ? a.scale : 1.f;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (key_seen(key)) w = make_uint4(pack_bf16x2(u.x * f, u.y * f), pack_bf16x2(u.z * f, u.w * f), pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+      const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + blockIdx.y * st[2] + c * 8) = w;
+    }
+    __syncwarp();
+    cluster_arrive();      // no CTA leaves while another one reads its part
+    cluster_wait();
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    tmem_dealloc(tmem_base, Shape::TMEM);
   }
 }
 
@@ -595,6 +696,19 @@ static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh,
   return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
 }
 
+// CTAs that share what one block of keys streams. The first keys stream every query, the others those of a window: more CTAs per block while there are few
+// blocks for the SMs, or while the first block alone takes half as long as all work spread over them, and at least four tiles are left to each.
+// (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: 1 / 2 / 4 CTAs)
+static int key_ranks(const MdbTextAttnArgs& a, int blocks, int slots) {
+  const double rep = a.H / a.Hkv, all = rep * ((a.Sq + TC - 1) / TC);
+  const double usual = a.table != nullptr ? all : rep * ((static_cast<double>(a.window < a.Sq ? a.window : a.Sq) + TR) / TC);
+  const double most = a.table == nullptr && a.sinks > 0 ? all : usual, each = most < usual ? most : usual;
+  const double groups = static_cast<double>(a.Hkv) * a.B, per_slot = groups * (most + (blocks - 1) * each) / slots;
+  int ranks = 1;
+  while (ranks < 4 && each >= 8 * ranks && (groups * blocks * ranks < 2 * slots || most / ranks > 0.5 * per_slot)) ranks *= 2;
+  return ranks;
+}
+
 template <int DH, bool KEYS, bool BIAS>
 static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, cudaStream_t st) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
@@ -604,16 +718,27 @@ static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, cu
   auto kern = text_bwd_kernel<DH, KEYS, BIAS>;
   static bool ready[TXT_DEVICES];
   if (int r = allow_smem(kern, MOST, ready)) return r;
-  kern<<<dim3(((KEYS ? a.Skv : a.Sq) + TR - 1) / TR, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a);
-  return static_cast<int>(cudaGetLastError());
+  const int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR, ranks = KEYS ? key_ranks(a, blocks, Shape::CTAS * device_sm_count()) : 1;
+  cudaLaunchConfig_t c;
+  memset(&c, 0, sizeof(c));
+  c.gridDim = dim3(blocks * ranks, KEYS ? a.Hkv : a.H, a.B);
+  c.blockDim = dim3(TB_THREADS);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = ranks;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&c, kern, maps, a, ranks));
 }
 
 template <int DH>
 static int text_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
-  TextBwdMaps maps;
+  TextBwdMaps maps;      // the first pass has no R tiles in shared memory
+  memset(&maps, 0, sizeof(maps));
   int r;
-  if ((r = bwd_map(&maps.r1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TR))) return 1000 + r;
-  if ((r = bwd_map(&maps.r2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TR))) return 1100 + r;
   if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
   if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
   if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, st) : launch_text_bwd<DH, false, false>(maps, a, st))) return r;
