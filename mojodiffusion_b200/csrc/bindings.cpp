@@ -673,10 +673,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> text_attention_bwd(const Tensor& q, c
   a.delta = delta.data_ptr<float>();
   if (dparam.defined() && a.table != nullptr) {
     a.d_table = dparam.data_ptr();
-    ws = at::empty({mdb_text_attention_bwd_floats(&a)}, lse.options());
-    a.table_ws = ws.data_ptr<float>();
   } else if (dparam.defined()) {
     a.d_sink = dparam.data_ptr();
+  }
+  if (const long long n = mdb_text_attention_bwd_floats(&a)) {
+    ws = at::empty({n}, lse.options());
+    a.ws = ws.data_ptr<float>();
   }
   g_launches.fetch_add(dparam.defined() ? 2 : 1, std::memory_order_relaxed);
   check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");

@@ -213,7 +213,7 @@ int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 // q, o, dout, dq: [B, Sq, H, Dh]; k, v, dk, dv: [B, Skv, Hkv, Dh], Hkv divides H, Dh 64 or 128; strides (batch, seq, head) in elements, multiples of
 // 8, addresses multiples of 16 bytes. Without a table, key j is seen by the query at position p = q_start + row when j < kv_len, j <= p and
 // (p - j < window or j < sinks); with one, when j < kv_len. scale > 0. lse (base 2; +inf: a row that saw nothing), delta: fp32 [B, H, Sq]; delta and
-// table_ws are workspaces of the backward pass.
+// ws are workspaces of the backward pass.
 #define MDB_TEXT_MAX_BUCKETS 64        // at Dh 64, half as many at 128: the backward pass keeps an accumulator for each in every thread
 #define MDB_TEXT_MAX_NEAR_64 512        // last border, by head width: the tables of biases by distance share the shared memory with the tiles
 #define MDB_TEXT_MAX_NEAR_128 240
@@ -226,7 +226,7 @@ typedef struct MdbTextAttnArgs {
   const void* sink_logits;    // [H] or null
   const void* table;          // [buckets, H] or null; then Hkv = H
   void* d_sink; void* d_table;
-  float* table_ws;            // mdb_text_attention_bwd_floats values when d_table is given
+  float* ws;                  // mdb_text_attention_bwd_floats values, none of which need be set
   long long q_strides[3], k_strides[3], v_strides[3], o_strides[3], do_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
   int B, H, Hkv, Sq, Skv, Dh;
   int q_start, window, sinks;

@@ -33,7 +33,7 @@ extern "C" int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st)
 }
 
 extern "C" long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a) {
-  return static_cast<long long>(a->B) * a->H * ((a->Sq + 127) / 128) * a->buckets;
+  return mdb::check_args(a) ? 0 : mdb::text_attention_backward_floats(*a);
 }
 
 extern "C" int mdb_text_attention_bwd(const MdbTextAttnArgs* a, cudaStream_t st) {

@@ -143,6 +143,7 @@ inline int allow_smem(K kern, int bytes, bool (&ready)[TXT_DEVICES]) {
 int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st);
 bool text_attention_is_step(const MdbTextAttnArgs& a);
 int text_attention_step(const MdbTextAttnArgs& a, cudaStream_t st);
+long long text_attention_backward_floats(const MdbTextAttnArgs& a);
 int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st);
 
 }  // namespace mdb

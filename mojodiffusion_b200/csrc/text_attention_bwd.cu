@@ -23,6 +23,7 @@
 #include "text_attention.cuh"
 #include "gemm_api.h"
 
+#include <algorithm>
 #include <string.h>
 
 namespace mdb {
@@ -33,6 +34,14 @@ constexpr int RUN_LD = 36;           // floats between the running sums of two r
 
 struct alignas(64) TextBwdMaps {
   CUtensorMap r1, r2, c1, c2;
+};
+
+// The blocks of the first keys, which every query may see. Their CTAs take the queries of a window, as the others do; the rest of what they stream is
+// shared by `slices` more CTAs each. Their parts of dk and dv (of the first keys' rows alone) are added by a kernel of their own: fp32
+// [B, Hkv, blocks, 1 + slices, 2, TR, DH].
+struct TextFirst {
+  int blocks, slices;
+  float* ws;
 };
 
 template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
@@ -52,7 +61,7 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
 
 template <int DH, bool KEYS, bool BIAS>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
-text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const int ranks) {
+text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextFirst fk) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int STAGES = Shape::STAGES, BUFS = Shape::BUFS;
   constexpr bool SUMMED = Shape::SUMMED;
@@ -66,7 +75,6 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2], acc_full, a_full;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
-  __shared__ uint32_t has_part;
   __shared__ __align__(16) float s_lse[2][TC], s_delta[2][TC];      // negated, per staged query: of either buffer, or of either warpgroup's columns, twice
 
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -88,9 +96,11 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   const int batch = blockIdx.z;
   const int rep = a.H / a.Hkv;
   // the rows with the most to stream start first: late queries, early keys
-  // KEYS: the CTAs of a cluster share what is streamed for one block of keys
-  const int rank = KEYS ? blockIdx.x % ranks : 0;
-  const int r0 = (KEYS ? blockIdx.x / ranks : BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) * TR;
+  // KEYS: blocks of keys, then the slices of the first ones
+  const int key_blocks = (a.Skv + TR - 1) / TR, extra = KEYS ? static_cast<int>(blockIdx.x) - key_blocks : -1;
+  const int part = extra >= 0 ? 1 + extra % fk.slices : 0;
+  const int block = !KEYS ? (BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) : extra >= 0 ? extra / fk.slices : blockIdx.x;
+  const int r0 = block * TR;
   const int out_rows = KEYS ? a.Skv : a.Sq;
   const TextSight sight = text_sight(a, batch);
 
@@ -106,17 +116,21 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     int first = 0, end = a.Sq;
     if (!BIAS) {
       first = max(r0 - sight.start, 0);
-      if (r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
+      if (block < fk.blocks || r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
     }
     if (first < end) {
       lo = first / TC;
       hi = (end + TC - 1) / TC;
     }
+    if (part > 0) {                 // the queries behind the window's
+      lo = max(first / TC, hi);
+      hi = max((a.Sq + TC - 1) / TC, lo);
+    }
   }
   const int per_head = ns + hi - lo;
   const int n_all = KEYS ? per_head * rep : per_head;
-  const int i_first = KEYS ? static_cast<int>(static_cast<long long>(n_all) * rank / ranks) : 0;
-  const int n_c = KEYS ? static_cast<int>(static_cast<long long>(n_all) * (rank + 1) / ranks) - i_first : n_all;
+  const int i_first = part > 0 ? static_cast<int>(static_cast<long long>(n_all) * (part - 1) / fk.slices) : 0;
+  const int n_c = part > 0 ? static_cast<int>(static_cast<long long>(n_all) * part / fk.slices) - i_first : n_all;
   const auto tile_of = [&](int i) { return i < ns ? i : i - ns + lo; };
   const auto key_seen = [&](int key) {
     long long first = 0, end = a.Sq;
@@ -532,21 +546,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
     if (ok && n_c > 0) ok = text_wait(&acc_full, 0, &abort_s);
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 161, n_c);
-    if (ok && KEYS && ranks > 1 && n_c > 0) {
-      // the parts of dk (warpgroup 0) and dv (1) of this CTA, fp32 [2][128][DH], over the tiles, which nothing reads any more
-      tc_fence_after();
-      float4* part = reinterpret_cast<float4*>(smem) + (g * TR + mt) * (DH / 4);
-      const uint32_t acc = tmem_base + lane_addr + (g == 1 ? ACC2_COL : ACC1_COL);
-#pragma unroll 1
-      for (int c = 0; c < DH / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(acc + c * 32, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          part[(c * 8 + e) ^ (mt & 7)] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
-      }
-    } else if (ok && (!KEYS || ranks == 1)) {
+    if (ok) {
       // dq: each warpgroup stores half of the columns; KEYS: warpgroup 0 dk, warpgroup 1 dv
       tc_fence_after();
       bool some = n_c > 0;
@@ -559,6 +559,9 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       out += batch * st[0] + row * st[1] + blockIdx.y * st[2];
       const uint32_t acc = tmem_base + lane_addr + (second ? ACC2_COL : ACC1_COL);
       const float f = second ? 1.f : a.scale;
+      // rows of the first keys leave as parts, in fp32
+      const bool as_part = KEYS && block < fk.blocks && row < a.sinks;
+      float* whole = as_part ? fk.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * fk.blocks + block) * (1 + fk.slices) + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
       constexpr int CHUNKS = KEYS ? DH / 32 : DH / 64;
       const int first = KEYS ? 0 : g * CHUNKS;
 #pragma unroll
@@ -568,7 +571,11 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
           tmem_ld_32x32b_x32(acc + c * 32, r);
           tmem_wait_ld();
         }
-        if (row < out_rows) {
+        if (as_part) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(whole + c * 32 + e) = some ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]) : make_uint4(0, 0, 0, 0);
+        } else if (row < out_rows && part == 0) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint4 w = make_uint4(0, 0, 0, 0);
@@ -589,7 +596,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         if (run_start[r] + row >= sum_end) bins[r * 256 + slot] = sum_all;
       bins[runs * 256 + slot] = sum_all;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      float* part = a.table_ws + ((static_cast<long long>(batch) * a.H + blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets;
+      float* part = a.ws + ((static_cast<long long>(batch) * a.H + blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets;
       for (int c = warp - 2; c < a.buckets; c += 8) {
         const int side = c < a.buckets / 2 ? c : c - a.buckets / 2, r = c < a.buckets / 2 ? run_mid - c : run_mid + side;
         float s = 0.f;
@@ -604,43 +611,6 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
 
-  if (KEYS && ranks > 1) {
-    // the cluster's parts, added in the order of their ranks; every CTA stores its share of the rows
-    if (threadIdx.x == 0) has_part = n_c > 0 ? 1u : 0u;
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    const int share = TR / ranks;
-    uint32_t parts = 0;
-    for (int k = 0; k < ranks; ++k) parts |= ld_cluster_u32(mapa_shared(smem_u32(&has_part), k)) << k;
-    for (int e = threadIdx.x; e < 2 * share * (DH / 8); e += TB_THREADS) {
-      const int c = e % (DH / 8), m = e / (DH / 8) / share, rr = rank * share + e / (DH / 8) % share, key = r0 + rr;
-      if (key >= out_rows) continue;
-      float4 x[4], y[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!(parts >> k & 1u)) continue;
-        const uint32_t at = mapa_shared(smem_u32(smem), k) + (m * TR + rr) * (DH * 4);
-        x[k] = ld_cluster_f32x4(at + (((2 * c) ^ (rr & 7)) << 4));
-        y[k] = ld_cluster_f32x4(at + (((2 * c + 1) ^ (rr & 7)) << 4));
-      }
-      float4 u = x[0], v = y[0];
-#pragma unroll
-      for (int k = 1; k < 4; ++k) {
-        u.x += x[k].x; u.y += x[k].y; u.z += x[k].z; u.w += x[k].w;
-        v.x += y[k].x; v.y += y[k].y; v.z += y[k].z; v.w += y[k].w;
-      }
-      const float f = m == 0 ? a.scale : 1.f;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (key_seen(key)) w = make_uint4(pack_bf16x2(u.x * f, u.y * f), pack_bf16x2(u.z * f, u.w * f), pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
-      const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + blockIdx.y * st[2] + c * 8) = w;
-    }
-    __syncwarp();
-    cluster_arrive();      // no CTA leaves while another one reads its part
-    cluster_wait();
-  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -678,7 +648,7 @@ __global__ void text_dtable_kernel(const __grid_constant__ MdbTextAttnArgs a, co
   float s = 0.f;
   if (group < groups)
     for (int r = group; r < a.B * blocks; r += groups)
-      s += a.table_ws[((static_cast<long long>(r / blocks) * a.H + h) * blocks + r % blocks) * a.buckets + c];
+      s += a.ws[((static_cast<long long>(r / blocks) * a.H + h) * blocks + r % blocks) * a.buckets + c];
   part[threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.x < a.buckets) {
@@ -696,21 +666,41 @@ static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh,
   return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
 }
 
-// CTAs that share what one block of keys streams. The first keys stream every query, the others those of a window: more CTAs per block while there are few
-// blocks for the SMs, or while the first block alone takes half as long as all work spread over them, and at least four tiles are left to each.
-// (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: 1 / 2 / 4 CTAs)
-static int key_ranks(const MdbTextAttnArgs& a, int blocks, int slots) {
-  const double rep = a.H / a.Hkv, all = rep * ((a.Sq + TC - 1) / TC);
-  const double usual = a.table != nullptr ? all : rep * ((static_cast<double>(a.window < a.Sq ? a.window : a.Sq) + TR) / TC);
-  const double most = a.table == nullptr && a.sinks > 0 ? all : usual, each = most < usual ? most : usual;
-  const double groups = static_cast<double>(a.Hkv) * a.B, per_slot = groups * (most + (blocks - 1) * each) / slots;
-  int ranks = 1;
-  while (ranks < 4 && each >= 8 * ranks && (groups * blocks * ranks < 2 * slots || most / ranks > 0.5 * per_slot)) ranks *= 2;
-  return ranks;
+// Slices of about sixteen tiles of 64 queries: the start and end of a CTA take as long as four tiles.
+// (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: dk and dv without slices 215 us, SLICED)
+static TextFirst first_keys(const MdbTextAttnArgs& a) {
+  TextFirst f = {0, 0, nullptr};
+  if (a.table != nullptr || a.sinks == 0) return f;
+  const long long behind = static_cast<long long>(a.Sq) - TR - a.window;        // queries that only the first keys are streamed for, at most
+  if (behind < 4 * TC) return f;
+  f.slices = static_cast<int>(std::min<long long>((behind / TC * (a.H / a.Hkv) + 15) / 16, 64));
+  f.blocks = (std::min(a.sinks, a.Skv) + TR - 1) / TR;
+  return f;
+}
+static long long first_floats(const MdbTextAttnArgs& a, const TextFirst& f) {
+  return static_cast<long long>(a.B) * a.Hkv * f.blocks * (f.blocks > 0 ? 1 + f.slices : 0) * 2 * TR * a.Dh;
+}
+
+// dk and dv of the first keys: their parts in order. One block for a key head of a sequence and 32 rows
+__global__ void text_first_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextFirst f) {
+  const int groups = a.Dh / 8, g = blockIdx.y, batch = blockIdx.z;
+  for (int e = threadIdx.x; e < 32 * 2 * groups; e += blockDim.x) {
+    const int c = e % groups, m = e / groups % 2, key = blockIdx.x * 32 + e / groups / 2;
+    if (key >= min(a.sinks, a.Skv)) continue;
+    const float* at = f.ws + ((((static_cast<long long>(batch) * a.Hkv + g) * f.blocks + key / TR) * (1 + f.slices)) * 2 + m) * (TR * a.Dh) + key % TR * a.Dh + c * 8;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p <= f.slices; ++p, at += 2 * TR * a.Dh)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += at[i];
+    const float x = m == 0 ? a.scale : 1.f;
+    const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + g * st[2] + c * 8) =
+        make_uint4(pack_bf16x2(s[0] * x, s[1] * x), pack_bf16x2(s[2] * x, s[3] * x), pack_bf16x2(s[4] * x, s[5] * x), pack_bf16x2(s[6] * x, s[7] * x));
+  }
 }
 
 template <int DH, bool KEYS, bool BIAS>
-static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, cudaStream_t st) {
+static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, const TextFirst& fk, cudaStream_t st) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int MOST = 225 * 1024;                 // beside what the kernel declares itself
   const int smem = BIAS ? Shape::bytes(text_near(a), a.buckets) : Shape::bytes(0, 0);
@@ -718,39 +708,34 @@ static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, cu
   auto kern = text_bwd_kernel<DH, KEYS, BIAS>;
   static bool ready[TXT_DEVICES];
   if (int r = allow_smem(kern, MOST, ready)) return r;
-  const int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR, ranks = KEYS ? key_ranks(a, blocks, Shape::CTAS * device_sm_count()) : 1;
-  cudaLaunchConfig_t c;
-  memset(&c, 0, sizeof(c));
-  c.gridDim = dim3(blocks * ranks, KEYS ? a.Hkv : a.H, a.B);
-  c.blockDim = dim3(TB_THREADS);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = ranks;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  c.attrs = &at;
-  c.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&c, kern, maps, a, ranks));
+  const int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR + (KEYS ? fk.blocks * fk.slices : 0);
+  kern<<<dim3(blocks, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a, fk);
+  return static_cast<int>(cudaGetLastError());
 }
 
 template <int DH>
-static int text_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
+static int text_backward(const MdbTextAttnArgs& a, const TextFirst& fk, cudaStream_t st) {
   TextBwdMaps maps;      // the first pass has no R tiles in shared memory
   memset(&maps, 0, sizeof(maps));
   int r;
   if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
   if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
-  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, st) : launch_text_bwd<DH, false, false>(maps, a, st))) return r;
+  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, fk, st) : launch_text_bwd<DH, false, false>(maps, a, fk, st))) return r;
   if ((r = bwd_map(&maps.r1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
   if ((r = bwd_map(&maps.r2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
   if ((r = bwd_map(&maps.c1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
   if ((r = bwd_map(&maps.c2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
-  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, st) : launch_text_bwd<DH, true, false>(maps, a, st);
+  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, fk, st) : launch_text_bwd<DH, true, false>(maps, a, fk, st);
 }
 
+static long long table_floats(const MdbTextAttnArgs& a) { return a.table != nullptr ? static_cast<long long>(a.B) * a.H * ((a.Sq + TR - 1) / TR) * a.buckets : 0; }
+long long text_attention_backward_floats(const MdbTextAttnArgs& a) { return table_floats(a) + first_floats(a, first_keys(a)); }
+
 int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
-  if (int r = a.Dh == 128 ? text_backward<128>(a, st) : text_backward<64>(a, st)) return r;
+  TextFirst fk = first_keys(a);
+  fk.ws = a.ws + table_floats(a);
+  if (int r = a.Dh == 128 ? text_backward<128>(a, fk, st) : text_backward<64>(a, fk, st)) return r;
+  if (fk.blocks > 0) text_first_kernel<<<dim3((std::min(a.sinks, a.Skv) + 31) / 32, a.Hkv, a.B), 256, 0, st>>>(a, fk);
   if (a.d_sink != nullptr) text_dsink_kernel<<<a.H, 256, 0, st>>>(a);
   if (a.d_table != nullptr) text_dtable_kernel<<<a.H, 256, 0, st>>>(a, (a.Sq + TR - 1) / TR);
   return static_cast<int>(cudaGetLastError());
