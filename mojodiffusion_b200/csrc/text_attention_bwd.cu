@@ -36,11 +36,12 @@ struct alignas(64) TextBwdMaps {
   CUtensorMap r1, r2, c1, c2;
 };
 
-// The blocks of the first keys, which every query may see. Their CTAs take the queries of a window, as the others do; the rest of what they stream is
-// shared by `slices` more CTAs each. Their parts of dk and dv (of the first keys' rows alone) are added by a kernel of their own: fp32
-// [B, Hkv, blocks, 1 + slices, 2, TR, DH].
-struct TextFirst {
-  int blocks, slices;
+// What several CTAs add to dk and dv of the same keys, in fp32 parts [B, Hkv, blocks, count, 2, TR, DH] that the last kernel adds in order.
+//   slices > 0: the first `blocks` blocks hold keys that every query may see. Their first part comes from the queries of a window, like the sums of the
+//               other blocks; the rest of what they stream is shared by `slices` more CTAs each. Only rows of first keys are parts.
+//   slices = 0, count > 1: few blocks for the SMs: `count` CTAs share what each of them streams.
+struct TextParts {
+  int blocks, slices, count;
   float* ws;
 };
 
@@ -61,7 +62,7 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
 
 template <int DH, bool KEYS, bool BIAS>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
-text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextFirst fk) {
+text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextParts parts) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int STAGES = Shape::STAGES, BUFS = Shape::BUFS;
   constexpr bool SUMMED = Shape::SUMMED;
@@ -96,10 +97,11 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   const int batch = blockIdx.z;
   const int rep = a.H / a.Hkv;
   // the rows with the most to stream start first: late queries, early keys
-  // KEYS: blocks of keys, then the slices of the first ones
-  const int key_blocks = (a.Skv + TR - 1) / TR, extra = KEYS ? static_cast<int>(blockIdx.x) - key_blocks : -1;
-  const int part = extra >= 0 ? 1 + extra % fk.slices : 0;
-  const int block = !KEYS ? (BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) : extra >= 0 ? extra / fk.slices : blockIdx.x;
+  // KEYS: blocks of keys in turn with their parts, or blocks and then the slices of the first ones
+  const int key_blocks = (a.Skv + TR - 1) / TR, extra = KEYS && parts.slices > 0 ? static_cast<int>(blockIdx.x) - key_blocks : -1;
+  const bool shared = KEYS && parts.slices == 0 && parts.count > 1;
+  const int part = extra >= 0 ? 1 + extra % parts.slices : shared ? blockIdx.x % parts.count : 0;
+  const int block = !KEYS ? (BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) : extra >= 0 ? extra / parts.slices : shared ? blockIdx.x / parts.count : blockIdx.x;
   const int r0 = block * TR;
   const int out_rows = KEYS ? a.Skv : a.Sq;
   const TextSight sight = text_sight(a, batch);
@@ -116,21 +118,22 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     int first = 0, end = a.Sq;
     if (!BIAS) {
       first = max(r0 - sight.start, 0);
-      if (block < fk.blocks || r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
+      if ((parts.slices > 0 && block < parts.blocks) || r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
     }
     if (first < end) {
       lo = first / TC;
       hi = (end + TC - 1) / TC;
     }
-    if (part > 0) {                 // the queries behind the window's
+    if (extra >= 0) {               // the queries behind the window's
       lo = max(first / TC, hi);
       hi = max((a.Sq + TC - 1) / TC, lo);
     }
   }
   const int per_head = ns + hi - lo;
   const int n_all = KEYS ? per_head * rep : per_head;
-  const int i_first = part > 0 ? static_cast<int>(static_cast<long long>(n_all) * (part - 1) / fk.slices) : 0;
-  const int n_c = part > 0 ? static_cast<int>(static_cast<long long>(n_all) * part / fk.slices) - i_first : n_all;
+  const int share = extra >= 0 ? part - 1 : part, shares = extra >= 0 ? parts.slices : shared ? parts.count : 1;
+  const int i_first = KEYS ? static_cast<int>(static_cast<long long>(n_all) * share / shares) : 0;
+  const int n_c = KEYS ? static_cast<int>(static_cast<long long>(n_all) * (share + 1) / shares) - i_first : n_all;
   const auto tile_of = [&](int i) { return i < ns ? i : i - ns + lo; };
   const auto key_seen = [&](int key) {
     long long first = 0, end = a.Sq;
@@ -141,33 +144,57 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     return key < sight.valid && first < end;
   };
 
-  if (threadIdx.x == 0) {
-    mbar_init(&r_full, 1);
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&c_full[s], 1);
-      mbar_init(&c_empty[s], 1);
+  // The TMA warp makes the barriers and starts loading while the others get ready: nobody else touches either before __syncthreads.
+  const int kv_head0 = KEYS ? blockIdx.y * rep + i_first / max(per_head, 1) : blockIdx.y / rep;
+  int load_head = kv_head0, load_tile = KEYS ? i_first % max(per_head, 1) : 0;
+  const auto load_c = [&](int st) {
+    uint8_t* c1 = sC + st * 2 * C_BYTES;
+    if (elect_one()) {
+      mbar_expect_tx(&c_full[st], 2 * C_BYTES);
+      for (int d = 0; d < DBOX; ++d) {
+        tma_load_4d(c1 + d * C_BOX, &maps.c1, &c_full[st], d * 64, tile_of(load_tile) * TC, load_head, batch);
+        tma_load_4d(c1 + C_BYTES + d * C_BOX, &maps.c2, &c_full[st], d * 64, tile_of(load_tile) * TC, load_head, batch);
+      }
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&xy_full[s], 1);
-      mbar_init(&pds_full[s], BUFS == 1 ? 8 : 4);
-      mbar_init(&lv_full[s], BUFS == 1 ? 32 : TC);
+    __syncwarp();
+    if (++load_tile == per_head && KEYS) {
+      load_tile = 0;
+      ++load_head;
     }
-    mbar_init(&acc_full, 1);
-    mbar_init(&a_full, 8);
-    abort_s = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(&r_full, 1);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&c_full[s], 1);
+        mbar_init(&c_empty[s], 1);
+      }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&xy_full[s], 1);
+        mbar_init(&pds_full[s], BUFS == 1 ? 8 : 4);
+        mbar_init(&lv_full[s], BUFS == 1 ? 32 : TC);
+      }
+      mbar_init(&acc_full, 1);
+      mbar_init(&a_full, 8);
+      abort_s = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    if (n_c > 0) {
+      if (KEYS && elect_one()) {
+        mbar_expect_tx(&r_full, 2 * R_BYTES);
+        for (int d = 0; d < DBOX; ++d) {
+          tma_load_4d(sR1 + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
+          tma_load_4d(sR2 + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
+        }
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < STAGES && i < n_c; ++i) load_c(i);
+    }
+  } else if (warp == 1) {
     tmem_alloc(&tmem_base_s, Shape::TMEM);
     tmem_relinquish();
-  }
-  if (warp == 0 && lane == 0) {
-    if (KEYS) {
-      tma_prefetch_desc(&maps.r1);
-      tma_prefetch_desc(&maps.r2);
-    }
-    tma_prefetch_desc(&maps.c1);
-    tma_prefetch_desc(&maps.c2);
   }
   if (BIAS) {
     // one head's bias: with a table there are as many key heads as query heads
@@ -192,46 +219,20 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
 
   if (warp == 0) {
     // ----------------------------- TMA producer -----------------------------
-    if (n_c > 0) {
-      if (KEYS && elect_one()) {
-        mbar_expect_tx(&r_full, 2 * R_BYTES);
-        for (int d = 0; d < DBOX; ++d) {
-          tma_load_4d(sR1 + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
-          tma_load_4d(sR2 + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
-        }
-      }
-      __syncwarp();
-      bool ok = true;
-      uint64_t* last_bar = KEYS ? &r_full : &c_full[0];
-      uint32_t last_par = 0;
-      int head = KEYS ? blockIdx.y * rep + i_first / max(per_head, 1) : blockIdx.y / rep, in_head = KEYS ? i_first % max(per_head, 1) : 0;
-      for (int i = 0; i < n_c; ++i) {
-        const int st = i & (STAGES - 1);
-        const uint32_t par = (i / STAGES) & 1;
-        ok = text_wait(&c_empty[st], par ^ 1u, &abort_s);
-        if (!ok) {
-          if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141, i);
-          break;
-        }
-        uint8_t* c1 = sC + st * 2 * C_BYTES;
-        if (elect_one()) {
-          mbar_expect_tx(&c_full[st], 2 * C_BYTES);
-          for (int d = 0; d < DBOX; ++d) {
-            tma_load_4d(c1 + d * C_BOX, &maps.c1, &c_full[st], d * 64, tile_of(in_head) * TC, head, batch);
-            tma_load_4d(c1 + C_BYTES + d * C_BOX, &maps.c2, &c_full[st], d * 64, tile_of(in_head) * TC, head, batch);
-          }
-        }
-        __syncwarp();
-        last_bar = &c_full[st];
-        last_par = par;
-        if (++in_head == per_head && KEYS) {
-          in_head = 0;
-          ++head;
-        }
-      }
-      if (!ok) {
+    bool ok = true;
+    int i = STAGES;
+    for (; i < n_c; ++i) {
+      const int st = i & (STAGES - 1);
+      ok = text_wait(&c_empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s);
+      if (!ok) break;
+      load_c(st);
+    }
+    if (!ok) {
+      if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141, i);
+      // the copies on the way land before the memory is given up
+      for (int j = i - STAGES; j < i; ++j) {
         const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(last_bar, last_par) && globaltimer_ns() - t0 < 5000000ull) {
+        while (!mbar_try_wait(&c_full[j & (STAGES - 1)], (j / STAGES) & 1) && globaltimer_ns() - t0 < 5000000ull) {
         }
       }
     }
@@ -374,7 +375,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     // KEYS: thread mt < 64 stages the negated lse and delta of query mt of the warpgroup's tile, loaded one of its tiles ahead
     float next_nlse = -INFINITY, next_ndelta = 0.f;
     constexpr int STAGERS = BUFS == 1 ? 32 : TC;          // threads of a warpgroup that stage, and queries that they stage
-    int f_head = KEYS ? blockIdx.y * rep + i_first / max(per_head, 1) : 0, f_tile = KEYS ? i_first % max(per_head, 1) : 0;
+    int f_head = kv_head0, f_tile = KEYS ? i_first % max(per_head, 1) : 0;
     const auto fetch = [&](int ahead) {
       f_tile += ahead;
       while (f_tile >= per_head) {
@@ -559,9 +560,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       out += batch * st[0] + row * st[1] + blockIdx.y * st[2];
       const uint32_t acc = tmem_base + lane_addr + (second ? ACC2_COL : ACC1_COL);
       const float f = second ? 1.f : a.scale;
-      // rows of the first keys leave as parts, in fp32
-      const bool as_part = KEYS && block < fk.blocks && row < a.sinks;
-      float* whole = as_part ? fk.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * fk.blocks + block) * (1 + fk.slices) + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
+      const bool as_part = shared || (KEYS && parts.slices > 0 && block < parts.blocks && row < a.sinks);
+      float* whole = as_part ? parts.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * parts.blocks + block) * parts.count + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
       constexpr int CHUNKS = KEYS ? DH / 32 : DH / 64;
       const int first = KEYS ? 0 : g * CHUNKS;
 #pragma unroll
@@ -575,7 +575,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             *reinterpret_cast<uint4*>(whole + c * 32 + e) = some ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]) : make_uint4(0, 0, 0, 0);
-        } else if (row < out_rows && part == 0) {
+        } else if (row < out_rows && extra < 0) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint4 w = make_uint4(0, 0, 0, 0);
@@ -619,44 +619,62 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   }
 }
 
-// dsink of one head per block; the order of the sum is fixed by the launch shape
-__global__ void text_dsink_kernel(const __grid_constant__ MdbTextAttnArgs a) {
-  __shared__ float part[256];
-  const int h = blockIdx.x;
-  const float sink = TXT_LOG2E * text_param(a.sink_logits, a.param_f32, h);
+// What is left, in one launch: blocks [0, adders) add the parts of dk and dv, 32 rows of a key head of a sequence each; the others form the gradient of
+// one head's sink logit, -sum of exp2(sink - lse) delta, or of its column of the table, from the sums of all row blocks and sequences. All in a fixed order.
+__global__ void __launch_bounds__(256)
+text_finish_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextParts parts, const int part_rows, const int adders, const int row_blocks) {
+  __shared__ float sums[256];
+  if (static_cast<int>(blockIdx.x) < adders) {
+    const int groups = a.Dh / 8, lines = (part_rows + 31) / 32;
+    const int line = blockIdx.x % lines, g = blockIdx.x / lines % a.Hkv, batch = blockIdx.x / lines / a.Hkv;
+    for (int e = threadIdx.x; e < 32 * 2 * groups; e += 256) {
+      const int c = e % groups, m = e / groups % 2, key = line * 32 + e / groups / 2;
+      if (key >= part_rows) continue;
+      const float* at = parts.ws + ((((static_cast<long long>(batch) * a.Hkv + g) * parts.blocks + key / TR) * parts.count) * 2 + m) * (TR * a.Dh) + key % TR * a.Dh + c * 8;
+      float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int p = 0; p < parts.count; ++p) {
+        const float4 u = *reinterpret_cast<const float4*>(at + static_cast<long long>(p) * 2 * TR * a.Dh), v = *reinterpret_cast<const float4*>(at + static_cast<long long>(p) * 2 * TR * a.Dh + 4);
+        s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+        s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+      }
+      const float x = m == 0 ? a.scale : 1.f;
+      const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + g * st[2] + c * 8) =
+          make_uint4(pack_bf16x2(s[0] * x, s[1] * x), pack_bf16x2(s[2] * x, s[3] * x), pack_bf16x2(s[4] * x, s[5] * x), pack_bf16x2(s[6] * x, s[7] * x));
+    }
+    return;
+  }
+  const int h = blockIdx.x - adders, t = threadIdx.x;
+  const auto store = [&](void* to, long long at, float v) {
+    if (a.param_f32) static_cast<float*>(to)[at] = v;
+    else static_cast<__nv_bfloat16*>(to)[at] = __float2bfloat16_rn(v);
+  };
   float s = 0.f;
+  if (a.d_table != nullptr) {
+    const int c = t % a.buckets, group = t / a.buckets, groups = 256 / a.buckets;
+    if (group < groups)
+      for (int r = group; r < a.B * row_blocks; r += groups) s += a.ws[((static_cast<long long>(r / row_blocks) * a.H + h) * row_blocks + r % row_blocks) * a.buckets + c];
+    sums[t] = s;
+    __syncthreads();
+    if (t >= a.buckets) return;
+    for (int n = 1; n < groups; ++n) s += sums[n * a.buckets + c];
+    store(a.d_table, static_cast<long long>(c) * a.H + h, s);
+    return;
+  }
+  const float sink = TXT_LOG2E * text_param(a.sink_logits, a.param_f32, h);
   for (int b = 0; b < a.B; ++b) {
     const long long at = (static_cast<long long>(b) * a.H + h) * a.Sq;
-    for (int i = threadIdx.x; i < a.Sq; i += 256) s += exp2f(sink - a.lse[at + i]) * a.delta[at + i];
+#pragma unroll 4
+    for (int i = t; i < a.Sq; i += 256) s += exp2f(sink - a.lse[at + i]) * a.delta[at + i];
   }
-  part[threadIdx.x] = s;
+  sums[t] = s;
   __syncthreads();
   for (int n = 128; n > 0; n >>= 1) {
-    if (threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+    if (t < n) sums[t] += sums[t + n];
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    if (a.param_f32) static_cast<float*>(a.d_sink)[h] = -part[0];
-    else static_cast<__nv_bfloat16*>(a.d_sink)[h] = __float2bfloat16_rn(-part[0]);
-  }
-}
-
-// dtable[:, h]: the parts of all row blocks and sequences, in a fixed order
-__global__ void text_dtable_kernel(const __grid_constant__ MdbTextAttnArgs a, const int blocks) {
-  __shared__ float part[256];
-  const int h = blockIdx.x, c = threadIdx.x % a.buckets, group = threadIdx.x / a.buckets, groups = 256 / a.buckets;
-  float s = 0.f;
-  if (group < groups)
-    for (int r = group; r < a.B * blocks; r += groups)
-      s += a.ws[((static_cast<long long>(r / blocks) * a.H + h) * blocks + r % blocks) * a.buckets + c];
-  part[threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.x < a.buckets) {
-    for (int n = 1; n < groups; ++n) s += part[n * a.buckets + c];
-    const long long to = static_cast<long long>(c) * a.H + h;
-    if (a.param_f32) static_cast<float*>(a.d_table)[to] = s;
-    else static_cast<__nv_bfloat16*>(a.d_table)[to] = __float2bfloat16_rn(s);
-  }
+  if (t == 0) store(a.d_sink, h, -sums[0]);
 }
 
 static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh, const long long* strides, int rows) {
@@ -666,41 +684,30 @@ static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh,
   return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
 }
 
-// Slices of about sixteen tiles of 64 queries: the start and end of a CTA take as long as four tiles.
-// (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: dk and dv without slices 215 us, SLICED)
-static TextFirst first_keys(const MdbTextAttnArgs& a) {
-  TextFirst f = {0, 0, nullptr};
-  if (a.table != nullptr || a.sinks == 0) return f;
+// The start and end of a CTA take as long as about four tiles of 64 queries: slices of sixteen (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: dk and dv
+// without slices 215 us, with them 132), and parts of eight at least where few blocks leave SMs idle.
+static TextParts text_parts(const MdbTextAttnArgs& a) {
+  TextParts p = {0, 0, 1, nullptr};
+  const long long rep = a.H / a.Hkv, blocks = (a.Skv + TR - 1) / TR;
   const long long behind = static_cast<long long>(a.Sq) - TR - a.window;        // queries that only the first keys are streamed for, at most
-  if (behind < 4 * TC) return f;
-  f.slices = static_cast<int>(std::min<long long>((behind / TC * (a.H / a.Hkv) + 15) / 16, 64));
-  f.blocks = (std::min(a.sinks, a.Skv) + TR - 1) / TR;
-  return f;
-}
-static long long first_floats(const MdbTextAttnArgs& a, const TextFirst& f) {
-  return static_cast<long long>(a.B) * a.Hkv * f.blocks * (f.blocks > 0 ? 1 + f.slices : 0) * 2 * TR * a.Dh;
-}
-
-// dk and dv of the first keys: their parts in order. One block for a key head of a sequence and 32 rows
-__global__ void text_first_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextFirst f) {
-  const int groups = a.Dh / 8, g = blockIdx.y, batch = blockIdx.z;
-  for (int e = threadIdx.x; e < 32 * 2 * groups; e += blockDim.x) {
-    const int c = e % groups, m = e / groups % 2, key = blockIdx.x * 32 + e / groups / 2;
-    if (key >= min(a.sinks, a.Skv)) continue;
-    const float* at = f.ws + ((((static_cast<long long>(batch) * a.Hkv + g) * f.blocks + key / TR) * (1 + f.slices)) * 2 + m) * (TR * a.Dh) + key % TR * a.Dh + c * 8;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p <= f.slices; ++p, at += 2 * TR * a.Dh)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] += at[i];
-    const float x = m == 0 ? a.scale : 1.f;
-    const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + g * st[2] + c * 8) =
-        make_uint4(pack_bf16x2(s[0] * x, s[1] * x), pack_bf16x2(s[2] * x, s[3] * x), pack_bf16x2(s[4] * x, s[5] * x), pack_bf16x2(s[6] * x, s[7] * x));
+  if (a.table == nullptr && a.sinks > 0 && behind >= 4 * TC) {
+    p.slices = static_cast<int>(std::min<long long>((behind / TC * rep + 15) / 16, 64));
+    p.blocks = (std::min(a.sinks, a.Skv) + TR - 1) / TR;
+    p.count = 1 + p.slices;
+    return p;
   }
+  const long long tiles = rep * ((std::min<long long>(a.Sq, a.table != nullptr ? a.Sq : static_cast<long long>(a.window) + TR) + TC - 1) / TC);
+  const long long slots = (a.Dh == 64 ? 2 : 1) * device_sm_count();
+  p.count = static_cast<int>(std::max<long long>(1, std::min({slots / (blocks * a.Hkv * a.B), tiles / 8, 8ll})));
+  if (p.count > 1) p.blocks = static_cast<int>(blocks);
+  return p;
+}
+static long long part_floats(const MdbTextAttnArgs& a, const TextParts& p) {
+  return static_cast<long long>(a.B) * a.Hkv * p.blocks * p.count * 2 * TR * a.Dh;
 }
 
 template <int DH, bool KEYS, bool BIAS>
-static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, const TextFirst& fk, cudaStream_t st) {
+static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int MOST = 225 * 1024;                 // beside what the kernel declares itself
   const int smem = BIAS ? Shape::bytes(text_near(a), a.buckets) : Shape::bytes(0, 0);
@@ -708,36 +715,39 @@ static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, co
   auto kern = text_bwd_kernel<DH, KEYS, BIAS>;
   static bool ready[TXT_DEVICES];
   if (int r = allow_smem(kern, MOST, ready)) return r;
-  const int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR + (KEYS ? fk.blocks * fk.slices : 0);
-  kern<<<dim3(blocks, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a, fk);
+  int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR;
+  if (KEYS) blocks = parts.slices > 0 ? blocks + parts.blocks * parts.slices : blocks * parts.count;
+  kern<<<dim3(blocks, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a, parts);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <int DH>
-static int text_backward(const MdbTextAttnArgs& a, const TextFirst& fk, cudaStream_t st) {
+static int text_backward(const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
   TextBwdMaps maps;      // the first pass has no R tiles in shared memory
   memset(&maps, 0, sizeof(maps));
   int r;
   if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
   if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
-  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, fk, st) : launch_text_bwd<DH, false, false>(maps, a, fk, st))) return r;
+  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, parts, st) : launch_text_bwd<DH, false, false>(maps, a, parts, st))) return r;
   if ((r = bwd_map(&maps.r1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
   if ((r = bwd_map(&maps.r2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
   if ((r = bwd_map(&maps.c1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
   if ((r = bwd_map(&maps.c2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
-  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, fk, st) : launch_text_bwd<DH, true, false>(maps, a, fk, st);
+  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, parts, st) : launch_text_bwd<DH, true, false>(maps, a, parts, st);
 }
 
 static long long table_floats(const MdbTextAttnArgs& a) { return a.table != nullptr ? static_cast<long long>(a.B) * a.H * ((a.Sq + TR - 1) / TR) * a.buckets : 0; }
-long long text_attention_backward_floats(const MdbTextAttnArgs& a) { return table_floats(a) + first_floats(a, first_keys(a)); }
+long long text_attention_backward_floats(const MdbTextAttnArgs& a) { return table_floats(a) + part_floats(a, text_parts(a)); }
 
 int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
-  TextFirst fk = first_keys(a);
-  fk.ws = a.ws + table_floats(a);
-  if (int r = a.Dh == 128 ? text_backward<128>(a, fk, st) : text_backward<64>(a, fk, st)) return r;
-  if (fk.blocks > 0) text_first_kernel<<<dim3((std::min(a.sinks, a.Skv) + 31) / 32, a.Hkv, a.B), 256, 0, st>>>(a, fk);
-  if (a.d_sink != nullptr) text_dsink_kernel<<<a.H, 256, 0, st>>>(a);
-  if (a.d_table != nullptr) text_dtable_kernel<<<a.H, 256, 0, st>>>(a, (a.Sq + TR - 1) / TR);
+  TextParts parts = text_parts(a);
+  parts.ws = a.ws + table_floats(a);
+  if (int r = a.Dh == 128 ? text_backward<128>(a, parts, st) : text_backward<64>(a, parts, st)) return r;
+  const int part_rows = parts.slices > 0 ? std::min(a.sinks, a.Skv) : parts.count > 1 ? a.Skv : 0;
+  const long long adders = static_cast<long long>((part_rows + 31) / 32) * a.Hkv * a.B, params = a.d_sink != nullptr || a.d_table != nullptr ? a.H : 0;
+  if (adders + params > 0x7fffffff) return -8;
+  if (adders + params > 0)
+    text_finish_kernel<<<static_cast<unsigned>(adders + params), 256, 0, st>>>(a, parts, part_rows, static_cast<int>(adders), (a.Sq + TR - 1) / TR);
   return static_cast<int>(cudaGetLastError());
 }
 
