@@ -47,16 +47,16 @@ struct TextParts {
 
 template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
   static constexpr bool SUMMED = BIAS && !KEYS;                            // dtable is formed
-  // Heads of 64: two CTAs to an SM, each with one buffer of X and Y whose columns the two warpgroups share. The accumulators of dtable leave room for
-  // one CTA, heads of 128 need all of TMEM: there two buffers, one for either warpgroup.
-  static constexpr int CTAS = DH == 64 && !SUMMED ? 2 : 1, BUFS = CTAS == 2 ? 1 : 2;
+  // Heads of 64: two CTAs to an SM, each with one buffer of X and Y whose columns the two warpgroups share (with dtable where its tables leave the room,
+  // as for 32 buckets of distances up to 128). Heads of 128 need all of TMEM: there two buffers, one for either warpgroup.
+  static constexpr int CTAS = DH == 64 ? 2 : 1, BUFS = CTAS == 2 ? 1 : 2;
   static constexpr int TMEM = CTAS == 2 ? 256 : 512;
-  static constexpr int STAGES = 4;
+  static constexpr int STAGES = DH == 64 && SUMMED ? 2 : 4;
   static constexpr int TILES = (KEYS ? 2 * TR * DH * 2 : 0) + STAGES * 2 * TC * DH * 2 + 1024;
   static constexpr int SUMS = SUMMED ? 8 * 32 * RUN_LD * 4 : 0;
   static __host__ __device__ int lut_bytes(int near) { return BIAS ? TextLut::bytes(near) : 0; }
   static __host__ __device__ int bytes(int near, int buckets) {
-    return TILES + SUMS + lut_bytes(near) + (SUMMED ? buckets * 256 * 4 + buckets * 4 + (2 * near + 4) : 0);
+    return TILES + SUMS + lut_bytes(near) + (SUMMED ? (buckets - 1) * 256 * 4 + buckets * 4 + (2 * near + 4) : 0);
   }
 };
 
@@ -86,10 +86,10 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   const int near = BIAS ? text_near(a) : 0;
   float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // SUMMED: running sums [8 warps][32 rows][RUN_LD]
   const TextLut lut(sums + Shape::SUMS / 4, near);                        // BIAS
-  float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // SUMMED: [buckets][256 threads]: dS of a row before its first key of each run
+  float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // SUMMED: [buckets - 1][256 threads]: dS of a row before its first key of the second run, the third, ... and in all
   // SUMMED: the buckets in the order of their distances ("runs"): first distance of each, and the run of the distances -near .. near
   const int run_mid = a.exact + a.n_borders, runs = 2 * run_mid + 1;
-  int* run_start = reinterpret_cast<int*>(bins + a.buckets * 256);        // [runs]
+  int* run_start = reinterpret_cast<int*>(bins + (a.buckets - 1) * 256);        // [runs]
   uint8_t* run_of = reinterpret_cast<uint8_t*>(run_start + a.buckets);
 
   const int warp = threadIdx.x >> 5;
@@ -200,7 +200,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     // one head's bias: with a table there are as many key heads as query heads
     lut.set(a, blockIdx.y, warp, TB_THREADS / 32);
     if (!KEYS && a.d_table != nullptr) {
-      for (int i = threadIdx.x; i < a.buckets * 256; i += TB_THREADS) bins[i] = 0.f;
+      for (int i = threadIdx.x; i < (a.buckets - 1) * 256; i += TB_THREADS) bins[i] = 0.f;
       for (int i = threadIdx.x; i <= 2 * near; i += TB_THREADS) {
         const int c = text_bucket(a, i - near);
         run_of[i] = static_cast<uint8_t>(i <= near ? run_mid - c : run_mid + c - a.buckets / 2);
@@ -510,7 +510,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         // with the tile's products under way
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int b0 = c0 + c * 32, d0 = b0 - (r0 + quad * 32);
+          const int b0 = c0 + (piece0 + c) * 32, d0 = b0 - (r0 + quad * 32);
           const int r_lo = run_of[min(max(sum_end - (r0 + quad * 32) - 32 + near, 0), 2 * near)], r_hi = run_of[min(max(d0 + 31 + near, 0), 2 * near)];
           // running sums of four pieces of eight, then of the whole
 #pragma unroll
@@ -536,7 +536,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             for (int r = r_lo; r < r_hi; ++r) {
               const int at = run_start[r + 1] + row;
               const float upto = at > b0 ? mine[min(at - b0, 32) - 1] : 0.f;
-              if (at >= sum_end && at < b0 + 32) bins[(r + 1) * 256 + slot] = sum_all + upto;
+              if (at >= sum_end && at < b0 + 32) bins[r * 256 + slot] = sum_all + upto;
             }
           }
           sum_all += run[c][31];
@@ -593,8 +593,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     if (SUMMED && a.d_table != nullptr) {
       // runs that begin behind the last key, and the end of the last one
       for (int r = 1; r < runs; ++r)
-        if (run_start[r] + row >= sum_end) bins[r * 256 + slot] = sum_all;
-      bins[runs * 256 + slot] = sum_all;
+        if (run_start[r] + row >= sum_end) bins[(r - 1) * 256 + slot] = sum_all;
+      bins[(runs - 1) * 256 + slot] = sum_all;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       float* part = a.ws + ((static_cast<long long>(batch) * a.H + blockIdx.y) * gridDim.x + blockIdx.x) * a.buckets;
       for (int c = warp - 2; c < a.buckets; c += 8) {
@@ -602,7 +602,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         float s = 0.f;
         if (side <= run_mid && (c < a.buckets / 2 || side > 0)) {
 #pragma unroll
-          for (int m = 0; m < 256; m += 32) s += bins[(r + 1) * 256 + m + lane] - bins[r * 256 + m + lane];
+          for (int m = 0; m < 256; m += 32) s += bins[r * 256 + m + lane] - (r > 0 ? bins[(r - 1) * 256 + m + lane] : 0.f);
         }
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
