@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -606,20 +607,27 @@ TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, double sca
   a.status = status_ptr(q);
   return c;
 }
-Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse) {
+// lse and low (what the rounding of the output left): for a backward pass, or null
+Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tensor* low) {
   MdbTextAttnArgs& a = c.a;
   const bool given = out.has_value() && out->defined();
   if (given) TEXT_CHECK(out->sizes() == c.q.sizes() && out->scalar_type() == at::kBFloat16 && out->device() == c.q.device(), "out must have q's shape, type and device");
   Tensor o = given && text_writable(*out, {&c.q, &c.k, &c.v, &c.param, &c.kv_len, &c.q_start}) ? *out : at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
-  if (lse != nullptr) *lse = at::empty({a.B, a.H, a.Sq}, c.q.options().dtype(at::kFloat));
+  if (lse != nullptr) {
+    *lse = at::empty({a.B, a.H, a.Sq}, c.q.options().dtype(at::kFloat));
+    // where rows have few keys (see text_attention_bwd.cu); with more it is far below the other roundings, and a pass over memory each way
+    if (std::min<int64_t>(a.Skv, (int64_t)a.window + a.sinks) <= 256) *low = at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
+  }
   if (c.q.numel() > 0 && c.k.numel() > 0) {
     for (int i = 0; i < 3; ++i) a.o_strides[i] = o.size(i) == 1 ? 8 : o.stride(i);
     a.o = o.data_ptr();
-    if (lse != nullptr) a.lse = lse->data_ptr<float>();
+    if (lse != nullptr) {
+      a.lse = lse->data_ptr<float>();
+      if (low->defined()) a.o_low = low->data_ptr();
+    }
     check_rc(mdb_text_attention_fwd(&a, cur_stream()), "text_attention_fwd");
   } else {
     o.zero_();
-    if (lse != nullptr) lse->fill_(INFINITY);
   }
   if (!given || o.is_same(*out)) return o;
   Tensor to = *out;
@@ -631,58 +639,80 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
                         const optional<Tensor>& q_starts, const optional<Tensor>& sink_logits, const optional<Tensor>& out) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
   TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, sink_logits, {});
-  return text_forward(c, out, nullptr);
+  return text_forward(c, out, nullptr, nullptr);
 }
 Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, std::vector<int64_t> buckets, double scale, const optional<Tensor>& kv_len,
                           const optional<Tensor>& out) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
   TextCall c = text_call(q, k, v, scale, 1 << 30, 0, kv_len, 0, {}, table, buckets);
-  return text_forward(c, out, nullptr);
+  return text_forward(c, out, nullptr, nullptr);
 }
-// the two passes of the autograd node
-std::tuple<Tensor, Tensor> text_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale, int64_t window, int64_t sinks,
-                                              const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts, std::vector<int64_t> buckets) {
-  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
-  TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
-  Tensor lse, o = text_forward(c, {}, &lse);
-  return {o, lse};
-}
-std::tuple<Tensor, Tensor, Tensor, Tensor> text_attention_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, const Tensor& o,
-                                                              const Tensor& lse, const Tensor& dout, double scale, int64_t window, int64_t sinks,
-                                                              const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts,
-                                                              std::vector<int64_t> buckets, bool need_param) {
-  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
-  TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
-  MdbTextAttnArgs& a = c.a;
-  TEXT_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == (int64_t)a.B * a.H * a.Sq, "lse");
-  Tensor o_ = text_rows(o, q, a.Sq, a.H, a.o_strides, "the output"), d = text_rows(dout, q, a.Sq, a.H, a.do_strides, "the output's gradient");
-  Tensor dq = at::empty({a.B, a.Sq, a.H, a.Dh}, q.options()), dk = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options()), dv = at::empty_like(dk), dparam, ws;
-  if (need_param && c.param.defined()) dparam = at::empty_like(c.param);
-  if (c.q.numel() == 0 || c.k.numel() == 0) {
-    for (Tensor* t : {&dq, &dk, &dv, &dparam})
-      if (t->defined()) t->zero_();
-    return {dq, dk, dv, dparam};
+// The node of either operator: `param` is the table of position buckets (`buckets` not empty) or the sink logits, or absent.
+struct TextAttention : public torch::autograd::Function<TextAttention> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale,
+                        int64_t window, int64_t sinks, const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts,
+                        const std::vector<int64_t>& buckets) {
+    c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+    TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
+    Tensor lse, low, o = text_forward(c, {}, &lse, &low);
+    ctx->save_for_backward({q, k, v, c.param, c.kv_len, c.q_start, o, low, lse});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["rule"] = std::vector<int64_t>{window, sinks, q_start};
+    ctx->saved_data["buckets"] = buckets;
+    return o;
   }
-  text_rows(dq, q, a.Sq, a.H, a.dq_strides, "dq");
-  text_rows(dk, q, a.Skv, a.Hkv, a.dk_strides, "dk");
-  text_rows(dv, q, a.Skv, a.Hkv, a.dv_strides, "dv");
-  a.o = o_.data_ptr(); a.dout = d.data_ptr();
-  a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
-  a.lse = lse.data_ptr<float>();
-  Tensor delta = at::empty({a.B, a.H, a.Sq}, lse.options());
-  a.delta = delta.data_ptr<float>();
-  if (dparam.defined() && a.table != nullptr) {
-    a.d_table = dparam.data_ptr();
-  } else if (dparam.defined()) {
-    a.d_sink = dparam.data_ptr();
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &param = saved[3], &kv_len = saved[4], &q_starts = saved[5], &o = saved[6], &low = saved[7], &lse = saved[8];
+    const auto rule = ctx->saved_data["rule"].toIntVector(), buckets = ctx->saved_data["buckets"].toIntVector();
+    torch::autograd::variable_list d(11);
+    {
+      at::NoGradGuard none;
+      c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+      TextCall c = text_call(q, k, v, ctx->saved_data["scale"].toDouble(), rule[0], rule[1], kv_len, rule[2], q_starts, param, buckets);
+      MdbTextAttnArgs& a = c.a;
+      const bool need_param = param.defined() && ctx->needs_input_grad(3);
+      Tensor dout = text_rows(grads[0], q, a.Sq, a.H, a.do_strides, "the output's gradient");
+      d[0] = at::empty({a.B, a.Sq, a.H, a.Dh}, q.options());
+      d[1] = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options());
+      d[2] = at::empty({a.B, a.Skv, a.Hkv, a.Dh}, q.options());
+      if (need_param) d[3] = at::empty_like(c.param);
+      if (c.q.numel() == 0 || c.k.numel() == 0) {
+        for (int i = 0; i < 4; ++i)
+          if (d[i].defined()) d[i].zero_();
+      } else {
+        text_rows(o, q, a.Sq, a.H, a.o_strides, "the output");
+        text_rows(d[0], q, a.Sq, a.H, a.dq_strides, "dq");
+        text_rows(d[1], q, a.Skv, a.Hkv, a.dk_strides, "dk");
+        text_rows(d[2], q, a.Skv, a.Hkv, a.dv_strides, "dv");
+        a.o = o.data_ptr(); a.o_low = low.defined() ? low.data_ptr() : nullptr; a.dout = dout.data_ptr();
+        a.dq = d[0].data_ptr(); a.dk = d[1].data_ptr(); a.dv = d[2].data_ptr();
+        a.lse = lse.data_ptr<float>();
+        if (need_param) (a.table != nullptr ? a.d_table : a.d_sink) = d[3].data_ptr();
+        // delta and what the launches leave for one another
+        const int64_t rows = (lse.numel() + 3) / 4 * 4;
+        Tensor ws = at::empty({rows + mdb_text_attention_bwd_floats(&a)}, lse.options());
+        a.delta = ws.data_ptr<float>();
+        a.ws = a.delta + rows;
+        g_launches.fetch_add(need_param ? 2 : 1, std::memory_order_relaxed);
+        check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");
+      }
+    }
+    if (at::GradMode::is_enabled()) {      // a graph of the gradients is wanted: it ends here, with an error where it is walked
+      torch::autograd::variable_list leaves;
+      for (int i = 0; i < 4; ++i)
+        if (d[i].defined()) leaves.push_back(d[i].detach().set_requires_grad(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>("window_attention and relative_attention are differentiable once", (int64_t)leaves.size());
+      leaves = (*error)(std::move(leaves));
+      for (int i = 0, n = 0; i < 4; ++i)
+        if (d[i].defined()) d[i] = leaves[n++];
+    }
+    return d;
   }
-  if (const long long n = mdb_text_attention_bwd_floats(&a)) {
-    ws = at::empty({n}, lse.options());
-    a.ws = ws.data_ptr<float>();
-  }
-  g_launches.fetch_add(dparam.defined() ? 2 : 1, std::memory_order_relaxed);
-  check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");
-  return {dq, dk, dv, dparam};
+};
+Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale, int64_t window, int64_t sinks,
+                      const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts, std::vector<int64_t> buckets) {
+  return TextAttention::apply(q, k, v, param, scale, window, sinks, kv_len, q_start, q_starts, buckets);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1485,8 +1515,7 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("attention_bwd", &attention_bwd);
   m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor? out) -> Tensor", &window_attention);
   m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor? out) -> Tensor", &relative_attention);
-  m.def("text_attention_fwd", &text_attention_fwd);
-  m.def("text_attention_bwd", &text_attention_bwd);
+  m.def("text_attention", &text_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);
   m.def("qk_norm_rope", &qk_norm_rope);

@@ -219,6 +219,7 @@ int mdb_attention_bwd(const MdbAttnBwdArgs* a, cudaStream_t st);
 #define MDB_TEXT_MAX_NEAR_128 240
 typedef struct MdbTextAttnArgs {
   const void* q; const void* k; const void* v; void* o;
+  void* o_low;                // what the rounding of o left, bf16 with o's strides, or null; the backward pass adds it to o in delta
   const void* dout; void* dq; void* dk; void* dv;
   float* lse; float* delta;
   const int* kv_len;          // [B] or null: all keys

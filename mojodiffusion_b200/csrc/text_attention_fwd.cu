@@ -524,7 +524,10 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         if (fresh) {
 #pragma unroll
           for (int n = 0; n < 4; ++n)
-            if (n * 8 < left) *reinterpret_cast<uint4*>(o + n * 8 * a.o_strides[1]) = make_uint4(0, 0, 0, 0);
+            if (n * 8 < left) {
+              *reinterpret_cast<uint4*>(o + n * 8 * a.o_strides[1]) = make_uint4(0, 0, 0, 0);
+              if (a.o_low != nullptr) *reinterpret_cast<uint4*>(o + (static_cast<__nv_bfloat16*>(a.o_low) - static_cast<__nv_bfloat16*>(a.o)) + n * 8 * a.o_strides[1]) = make_uint4(0, 0, 0, 0);
+            }
           continue;
         }
         tmem_ld_32x32b_x32(o_addr + c * 32, r);
@@ -532,19 +535,30 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         if (c == DH / 32 - 1) tc_fence_before();
         __syncwarp();
         if (!ONE && c == DH / 32 - 1 && lane == 0) mbar_arrive(&o_empty[t]);      // the next item's products may have O
+        // the output, and in a second turn what its rounding left
+#pragma unroll 1
+        for (int low = 0;; ++low) {
+          uint32_t v[16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint4 v;
-          v.x = pack_bf16x2(__uint_as_float(r[8 * e + 0]) * inv_l, __uint_as_float(r[8 * e + 1]) * inv_l) & keep;
-          v.y = pack_bf16x2(__uint_as_float(r[8 * e + 2]) * inv_l, __uint_as_float(r[8 * e + 3]) * inv_l) & keep;
-          v.z = pack_bf16x2(__uint_as_float(r[8 * e + 4]) * inv_l, __uint_as_float(r[8 * e + 5]) * inv_l) & keep;
-          v.w = pack_bf16x2(__uint_as_float(r[8 * e + 6]) * inv_l, __uint_as_float(r[8 * e + 7]) * inv_l) & keep;
-          mine[e ^ (lane >> 1 & 3)] = v;
+          for (int e = 0; e < 16; ++e) {
+            const float x = __uint_as_float(r[2 * e]) * inv_l, y = __uint_as_float(r[2 * e + 1]) * inv_l;
+            v[e] = pack_bf16x2(x, y);
+            if (low) {
+              const float2 h = unpack_bf16x2(v[e]);
+              v[e] = pack_bf16x2(x - h.x, y - h.y);
+            }
+            v[e] &= keep;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine[e ^ (lane >> 1 & 3)] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          __syncwarp();
+          __nv_bfloat16* to = low ? o + (static_cast<__nv_bfloat16*>(a.o_low) - static_cast<__nv_bfloat16*>(a.o)) : o;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            if (n * 8 < left) *reinterpret_cast<uint4*>(to + n * 8 * a.o_strides[1]) = theirs[n * 32];
+          if (a.o_low == nullptr || low) break;
+          __syncwarp();
         }
-        __syncwarp();
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          if (n * 8 < left) *reinterpret_cast<uint4*>(o + n * 8 * a.o_strides[1]) = theirs[n * 32];
       }
       __syncwarp();
       // +inf where a row saw nothing: the backward pass then finds probabilities of zero

@@ -22,27 +22,6 @@ _NO_WINDOW = 1 << 30
 MAX_BUCKETS, MAX_NEAR = {64: 64, 128: 32}, {64: 512, 128: 240}
 
 
-class _TextAttentionFn(torch.autograd.Function):
-    """One node for both operators: ``param`` is the table of position buckets (``buckets`` not empty) or the sink logits, or None."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, param, scale, window, sinks, kv_len, q_start, buckets):
-        start, starts = (0, q_start) if isinstance(q_start, torch.Tensor) else (q_start, None)
-        o, lse = native.ops().text_attention_fwd(q, k, v, param, scale, window, sinks, kv_len, start, starts, buckets)
-        ctx.save_for_backward(q, k, v, param, o, lse, kv_len, starts)
-        ctx.cfg = (scale, window, sinks, start, buckets)
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, param, o, lse, kv_len, starts = ctx.saved_tensors
-        scale, window, sinks, start, buckets = ctx.cfg
-        need = param is not None and ctx.needs_input_grad[3]
-        dq, dk, dv, dp = native.ops().text_attention_bwd(q, k, v, param, o, lse, do, scale, window, sinks, kv_len, start, starts, buckets, need)
-        return dq, dk, dv, dp if need else None, None, None, None, None, None, None
-
-
 def _check(name, q, k, v, kv_len, out):
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: q [B, Sq, H, Dh], k and v [B, Skv, Hkv, Dh]")
@@ -102,7 +81,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if kernels:
         if not _wants_grad(q, k, v, sink_logits):
             return native.ops().window_attention(q, k, v, window, sinks, scale, kv_len, start, starts, sink_logits, out)
-        o = _TextAttentionFn.apply(q, k, v, sink_logits, scale, window, sinks, kv_len, starts if starts is not None else start, [])
+        o = native.ops().text_attention(q, k, v, sink_logits, scale, window, sinks, kv_len, start, starts, [])
         if out is None:
             return o
     _check(name, q, k, v, kv_len, out)
@@ -140,7 +119,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if kernels:
         if not _wants_grad(q, k, v, table):
             return native.ops().relative_attention(q, k, v, table, buckets, scale, kv_len, out)
-        o = _TextAttentionFn.apply(q, k, v, table, scale, _NO_WINDOW, 0, kv_len, 0, buckets)
+        o = native.ops().text_attention(q, k, v, table, scale, _NO_WINDOW, 0, kv_len, 0, None, buckets)
         if out is None:
             return o
     _check(name, q, k, v, kv_len, out)
