@@ -563,12 +563,13 @@ struct TextCall {
   Tensor q, k, v, kv_len, q_start, param;
 };
 // buckets: {count, exact, borders ...} and a table, or empty and sink logits (or no parameter)
-TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int64_t window, int64_t sinks, const optional<Tensor>& kv_len, int64_t q_start,
+TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, const optional<double>& given_scale, int64_t window, int64_t sinks, const optional<Tensor>& kv_len, int64_t q_start,
                    const optional<Tensor>& q_starts, const optional<Tensor>& param, const std::vector<int64_t>& buckets) {
   TextCall c;
   MdbTextAttnArgs& a = c.a;
   memset(&a, 0, sizeof(a));
   TEXT_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && (q.size(3) == 64 || q.size(3) == 128), "q [B, Sq, H, Dh] and k [B, Skv, Hkv, Dh] on a GPU, Dh 64 or 128");
+  const double scale = given_scale.has_value() ? *given_scale : 1.0 / std::sqrt((double)q.size(3));
   TEXT_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "k and v need a number of heads that divides q's");
   for (int i = 0; i < 3; ++i) TEXT_CHECK(q.size(i) < (i == 1 ? 1ll << 30 : 65536) && k.size(i) < (i == 1 ? 1ll << 30 : 65536), "fewer than 2^30 rows, 65536 sequences and heads");
   TEXT_CHECK(window >= 1 && sinks >= 0, "window of at least 1, sinks of at least 0");
@@ -635,7 +636,7 @@ Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tenso
   return to;
 }
 
-Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale, const optional<Tensor>& kv_len, int64_t q_start,
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, const optional<double>& scale, const optional<Tensor>& kv_len, int64_t q_start,
                         const optional<Tensor>& q_starts, const optional<Tensor>& sink_logits, const optional<Tensor>& out) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
   TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, sink_logits, {});
@@ -649,14 +650,14 @@ Tensor relative_attention(const Tensor& q, const Tensor& k, const Tensor& v, con
 }
 // The node of either operator: `param` is the table of position buckets (`buckets` not empty) or the sink logits, or absent.
 struct TextAttention : public torch::autograd::Function<TextAttention> {
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale,
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, const optional<double>& scale,
                         int64_t window, int64_t sinks, const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts,
                         const std::vector<int64_t>& buckets) {
     c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
     TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
     Tensor lse, low, o = text_forward(c, {}, &lse, &low);
     ctx->save_for_backward({q, k, v, c.param, c.kv_len, c.q_start, o, low, lse});
-    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["scale"] = (double)c.a.scale;
     ctx->saved_data["rule"] = std::vector<int64_t>{window, sinks, q_start};
     ctx->saved_data["buckets"] = buckets;
     return o;
@@ -710,7 +711,7 @@ struct TextAttention : public torch::autograd::Function<TextAttention> {
     return d;
   }
 };
-Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, double scale, int64_t window, int64_t sinks,
+Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& param, const optional<double>& scale, int64_t window, int64_t sinks,
                       const optional<Tensor>& kv_len, int64_t q_start, const optional<Tensor>& q_starts, std::vector<int64_t> buckets) {
   return TextAttention::apply(q, k, v, param, scale, window, sinks, kv_len, q_start, q_starts, buckets);
 }
@@ -1513,7 +1514,7 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("pad_channels", &pad_channels);
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
-  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor? out) -> Tensor", &window_attention);
+  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float? scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor? out) -> Tensor", &window_attention);
   m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor? out) -> Tensor", &relative_attention);
   m.def("text_attention", &text_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);

@@ -43,11 +43,12 @@ def _per_sequence(name, what, t, q):
 
 def _kernels(q, k, v, scale, param, kv_len, q_start, out) -> bool:
     """Whether the kernels cover the call. They check shapes, types and devices themselves, which costs a short call less."""
-    if not (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 4 and q.shape[3] in (64, 128) and 0 < scale < math.inf):
+    if not q.is_cuda or q.dtype is not torch.bfloat16 or q.dim() != 4 or not (scale is None or 0 < scale < math.inf):
         return False
-    if param is not None and param.dtype is not torch.bfloat16 and param.dtype is not torch.float32:
+    width = q.size(3)
+    if (width != 64 and width != 128) or (param is not None and param.dtype is not torch.bfloat16 and param.dtype is not torch.float32):
         return False
-    return native.use_native(q) and native.direct(*(t for t in (q, k, v, param, kv_len, q_start, out) if t is not None))
+    return native.use_native(q) and native.direct(*[t for t in (q, k, v, param, kv_len, q_start, out) if t is not None])
 
 
 def _wants_grad(q, k, v, param) -> bool:
@@ -67,16 +68,23 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     name = "window_attention"
     if window is None:
         window = _NO_WINDOW
-    elif isinstance(window, bool) or not isinstance(window, int) or window < 1:
+    elif type(window) is not int or window < 1:
         raise ValueError(f"{name}: window must be a positive int or None")
-    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+    elif window > _NO_WINDOW:
+        window = _NO_WINDOW
+    if type(sinks) is not int or sinks < 0:
         raise ValueError(f"{name}: sinks must be an int of at least 0")
-    starts = q_start if isinstance(q_start, torch.Tensor) else None
-    if starts is None and (isinstance(q_start, bool) or not isinstance(q_start, int)):
+    if sinks > _NO_WINDOW:
+        sinks = _NO_WINDOW
+    start, starts = 0, None
+    if isinstance(q_start, torch.Tensor):
+        starts = q_start
+    elif type(q_start) is not int:
         raise ValueError(f"{name}: q_start must be an int or int32 [B]")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    window, sinks = min(window, _NO_WINDOW), min(sinks, _NO_WINDOW)
-    start = 0 if starts is not None else max(min(q_start, _NO_WINDOW), -_NO_WINDOW)
+    elif q_start:
+        start = max(min(q_start, _NO_WINDOW), -_NO_WINDOW)
+    if scale is not None:
+        scale = float(scale)
     kernels = _kernels(q, k, v, scale, sink_logits, kv_len, starts, out)
     if kernels:
         if not _wants_grad(q, k, v, sink_logits):
@@ -111,7 +119,7 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     name = "relative_attention"
     if table.dim() != 2 or table.shape[0] < 4 or table.shape[0] % 2:
         raise ValueError(f"{name}: table must be [num_buckets, H], num_buckets even and at least 4")
-    if isinstance(max_distance, bool) or not isinstance(max_distance, int) or max_distance <= table.shape[0] // 4:
+    if type(max_distance) is not int or max_distance <= table.shape[0] // 4:
         raise ValueError(f"{name}: max_distance must be an int beyond the distances that have a bucket each ({table.shape[0] // 4})")
     scale = float(scale)
     buckets = _buckets(table.shape[0], max_distance)
