@@ -20,7 +20,7 @@ __device__ __forceinline__ TextSight text_sight(const MdbTextAttnArgs& a, int b)
   TextSight s;
   s.valid = a.kv_len != nullptr ? min(max(a.kv_len[b], 0), a.Skv) : a.Skv;
   s.start = a.q_start_ptr != nullptr ? a.q_start_ptr[b] : a.q_start;
-  s.start = min(max(s.start, -TXT_FAR), TXT_FAR);
+  s.start = min(max(s.start, -TXT_FAR), TXT_FAR - 1 - a.Sq);      // every position below TXT_FAR, which stands for no window
   return s;
 }
 
@@ -141,6 +141,18 @@ inline int allow_smem(K kern, int bytes, bool (&ready)[TXT_DEVICES]) {
 }
 
 int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st);
+// and clusters of up to 16 CTAs
+template <typename K>
+inline int allow_wide_clusters(K kern, bool (&ready)[TXT_DEVICES]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < TXT_DEVICES && ready[dev]) return 0;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < TXT_DEVICES) ready[dev] = true;
+  return 0;
+}
+
 bool text_attention_is_step(const MdbTextAttnArgs& a);
 int text_attention_step(const MdbTextAttnArgs& a, cudaStream_t st);
 long long text_attention_backward_floats(const MdbTextAttnArgs& a);

@@ -738,7 +738,10 @@ static int text_backward(const MdbTextAttnArgs& a, const TextParts& parts, cudaS
   return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, parts, st) : launch_text_bwd<DH, true, false>(maps, a, parts, st);
 }
 
-static long long table_floats(const MdbTextAttnArgs& a) { return a.table != nullptr ? static_cast<long long>(a.B) * a.H * ((a.Sq + TR - 1) / TR) * a.buckets : 0; }
+// sums of the table's gradient by row block, rounded up so that the parts behind them start on 16 bytes
+static long long table_floats(const MdbTextAttnArgs& a) {
+  return a.table != nullptr ? (static_cast<long long>(a.B) * a.H * ((a.Sq + TR - 1) / TR) * a.buckets + 3) / 4 * 4 : 0;
+}
 long long text_attention_backward_floats(const MdbTextAttnArgs& a) { return table_floats(a) + part_floats(a, text_parts(a)); }
 
 int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st) {

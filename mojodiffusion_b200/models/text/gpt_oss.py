@@ -49,6 +49,8 @@ class GptOssConfig:
     rope_original_max_pos: int = 4096
     swiglu_limit: float = 7.0
     swiglu_alpha: float = 1.702
+    fused_attention: bool = False       # ops.window_attention: no repeated heads, no scores of size S x S. Prompts padded on the right; other masks keep to
+                                        # the separate operations
 
 
 def yarn_inv_freq(c: GptOssConfig):
@@ -97,7 +99,7 @@ class _Attn(nn.Module):
         self.o_proj = _Lin(H * Dh, D, dtype, device)
         self.sinks = nn.Parameter(torch.zeros(H, dtype=dtype, device=device))
 
-    def forward(self, x, cos, sin, key_mask):
+    def forward(self, x, cos, sin, key_mask, kv_len=None):
         c = self.c
         B, S, _ = x.shape
         H, KV, Dh = c.num_attention_heads, c.num_key_value_heads, c.head_dim
@@ -110,6 +112,9 @@ class _Attn(nn.Module):
             return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
 
         q, k = rot(q), rot(k)
+        if c.fused_attention and (key_mask is None or kv_len is not None):
+            o = ops.window_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), self.window or None, kv_len=kv_len, sink_logits=self.sinks)
+            return self.o_proj(o.reshape(B, S, H * Dh))
         rep = H // KV
         k, v = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
         i = torch.arange(S, device=x.device)
@@ -191,8 +196,9 @@ class GptOssEncoder(nn.Module):
         ang = torch.arange(ids.shape[1], device=ids.device).float()[:, None] * inv.to(ids.device)[None]
         cos, sin = (ang.cos() * mult).to(x.dtype)[None, None], (ang.sin() * mult).to(x.dtype)[None, None]
         out = []
+        kv_len = ops.prefix_lengths(mask) if c.fused_attention and mask is not None else None
         for l in self.layers:
-            x = x + l.self_attn(l.input_layernorm(x), cos, sin, mask)
+            x = x + l.self_attn(l.input_layernorm(x), cos, sin, mask, kv_len)
             x = x + l.mlp(l.post_attention_layernorm(x))
             out.append(x)
         return out

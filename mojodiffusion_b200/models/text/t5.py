@@ -24,6 +24,8 @@ class T5Config:
     relative_attention_max_distance: int = 128
     layer_norm_epsilon: float = 1e-6
     per_layer_bias: bool = False          # UMT5: every block owns a relative_attention_bias
+    fused_attention: bool = False         # ops.relative_attention: scores, bias and probabilities in fp32 instead of bf16, nothing of size S x S. Prompts
+                                          # padded on the right; other masks keep to the separate operations
 
 
 def t5_xxl_config():
@@ -77,6 +79,13 @@ class _SelfAttention(nn.Module):
         b = relative_bucket(pos[None, :] - pos[:, None], self.c.relative_attention_num_buckets, self.c.relative_attention_max_distance)
         return self.relative_attention_bias(b).permute(2, 0, 1)[None]           # [1, H, S, S]
 
+    def attend(self, x, table, kv_len):
+        """The same with the bias by its table [buckets, H] and the padding by the prompts' lengths (or None)."""
+        B, S, _ = x.shape
+        H, dk = self.c.num_heads, self.c.d_kv
+        o = ops.relative_attention(*(p(x).view(B, S, H, dk) for p in (self.q, self.k, self.v)), table, self.c.relative_attention_max_distance, kv_len=kv_len)
+        return self.o(o.reshape(B, S, H * dk))
+
     def forward(self, x, bias):
         B, S, _ = x.shape
         H, dk = self.c.num_heads, self.c.d_kv
@@ -128,9 +137,17 @@ class T5Encoder(nn.Module):
         """ids [B, S], mask [B, S] (1 = token) -> hidden [B, S, d_model]."""
         x = self.shared(ids)
         B, S = ids.shape
-        bias = None
+        bias = table = None
+        kv_len = ops.prefix_lengths(mask) if self.cfg.fused_attention and mask is not None else None
+        fused = self.cfg.fused_attention and (mask is None or kv_len is not None)
         for blk in self.encoder.block:
             att = blk.layer[0].SelfAttention
+            if fused:
+                if hasattr(att, "relative_attention_bias"):
+                    table = att.relative_attention_bias.weight
+                x = x + att.attend(blk.layer[0].layer_norm(x), table, kv_len)
+                x = x + blk.layer[1].DenseReluDense(blk.layer[1].layer_norm(x))
+                continue
             if hasattr(att, "relative_attention_bias"):
                 bias = att.bias(S, ids.device).to(x.dtype)
                 if mask is not None:

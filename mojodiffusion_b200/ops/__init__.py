@@ -2,4 +2,4 @@
 from . import native, reference
 from .functional import *  # noqa: F401,F403
 from .native import check_status
-from .text_attention import relative_attention, window_attention
+from .text_attention import prefix_lengths, relative_attention, window_attention

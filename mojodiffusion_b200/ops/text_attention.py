@@ -22,6 +22,14 @@ _NO_WINDOW = 1 << 30
 MAX_BUCKETS, MAX_NEAR = {64: 64, 128: 32}, {64: 512, 128: 240}
 
 
+def prefix_lengths(mask: torch.Tensor) -> Optional[torch.Tensor]:
+    """``kv_len`` (int32 [B]) for a padding mask [B, S] whose rows are ones and then zeros; None for any other mask. Reads one value from the device."""
+    kept = mask != 0
+    lengths = kept.sum(1, dtype=torch.int32)
+    prefix = kept == (torch.arange(mask.shape[1], device=mask.device)[None, :] < lengths[:, None])
+    return lengths if bool(prefix.all()) else None
+
+
 def _check(name, q, k, v, kv_len, out):
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: q [B, Sq, H, Dh], k and v [B, Skv, Hkv, Dh]")

@@ -104,3 +104,45 @@ def test_refusals():
                  lambda: r(q, q, q, table, 8), lambda: r(q, q, q, table, 100.0), lambda: r(q, q, q, table, kv_len=ints(1)), lambda: r(q, q, q, table, out=q[:1]), lambda: r(q, k, k, table)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_prefix_lengths():
+    assert O.prefix_lengths(torch.tensor([[1, 1, 0], [0, 0, 0], [1, 1, 1]])).tolist() == [2, 0, 3]
+    assert O.prefix_lengths(torch.tensor([[True, False]])).dtype == torch.int32
+    assert O.prefix_lengths(torch.tensor([[0, 1]])) is None and O.prefix_lengths(torch.tensor([[1, 1], [1, 1], [0, 1]])) is None
+
+
+@pytest.mark.parametrize("per_layer", [False, True])
+def test_t5_encoder_with_fused_attention(per_layer):
+    """fp32, two layers of width 16: the separate operations and the fused one differ by fp32 roundings only (sums of at most 24 terms of size 1: 1e-5)."""
+    from mojodiffusion_b200.models.text.t5 import T5Config, T5Encoder
+
+    torch.manual_seed(0)
+    cfg = T5Config(vocab_size=50, d_model=16, d_kv=8, d_ff=24, num_layers=2, num_heads=2, relative_attention_num_buckets=8, relative_attention_max_distance=10, per_layer_bias=per_layer)
+    enc = T5Encoder(cfg)
+    ids = torch.randint(0, 50, (3, 23))
+    for mask in (None, (torch.arange(23)[None] < torch.tensor([23, 7, 15])[:, None]).long(), torch.cat((torch.zeros(3, 4), torch.ones(3, 19)), 1)):
+        cfg.fused_attention = False
+        want = enc(ids, mask)
+        cfg.fused_attention = True
+        kept = mask.bool() if mask is not None else torch.ones_like(ids, dtype=torch.bool)
+        assert float((enc(ids, mask) - want)[kept].abs().max()) < 1e-5
+
+
+def test_gpt_oss_encoder_with_fused_attention():
+    from mojodiffusion_b200.models.text.gpt_oss import GptOssConfig, GptOssEncoder
+
+    torch.manual_seed(0)
+    cfg = GptOssConfig(vocab_size=50, hidden_size=16, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=8, intermediate_size=16, num_local_experts=4,
+                       num_experts_per_tok=2, sliding_window=5)
+    enc = GptOssEncoder(cfg)
+    for l in enc.layers:
+        torch.nn.init.normal_(l.self_attn.sinks)
+    ids = torch.randint(0, 50, (2, 17))
+    for mask in (None, (torch.arange(17)[None] < torch.tensor([17, 6])[:, None]).long(), torch.cat((torch.zeros(2, 3), torch.ones(2, 14)), 1)):
+        cfg.fused_attention = False
+        want = enc.layer_states(ids, mask)
+        cfg.fused_attention = True
+        kept = mask.bool() if mask is not None else torch.ones_like(ids, dtype=torch.bool)
+        for a, b in zip(enc.layer_states(ids, mask), want):
+            assert float((a - b)[kept].abs().max()) < 1e-5

@@ -96,6 +96,8 @@ RELATIVE = [
     (1, 520, 2, 2, 128, 32, 385, [519], False),         # at 238
     (1, 200, 2, 2, 128, 32, 1000, None, False),         # at 547: the torch statement
     (1, 260, 2, 2, 64, 32, 9, None, False),             # all borders at one distance
+    (1, 1100, 1, 1, 64, 6, 60, None, False),            # shared blocks of keys behind an odd number of sums of the table
+    (1, 1100, 1, 1, 128, 10, 100, [1000], True),
     (1, 200, 2, 2, 64, 66, 128, None, False),           # more buckets than the kernels keep: the torch statement
 ]
 
@@ -123,6 +125,23 @@ def test_relative_attention_rectangle():
     leaves = [t.requires_grad_() for t in (q, k, v, table)]
     out = O.relative_attention(q, k, v, table, scale=0.7)
     check(dict(zip(("out", "dq", "dk", "dv", "dtable"), (out, *torch.autograd.grad(out, leaves, grad)))), value, bound, "rectangle")
+
+
+@pytest.mark.parametrize("Sq", [1, 90])
+def test_lengths_and_positions_out_of_range(Sq):
+    """Lengths below zero and beyond the keys, positions at the ends of 32 bits: what they say, without wrapping."""
+    B, Skv, H, G, D = 4, 200, 4, 2, 64
+    q, k, v = (t.requires_grad_() for t in _inputs(B, Sq, Skv, H, G, D, seed=50))
+    grad = _normal(B, Sq, H, D, seed=53)
+    for n, at in (([-5, 200, 2**31 - 1, -2**31], [100, 2**31 - 1, 110, 100]), ([200, 200, 150, 200], [-2**31, -2**31 + 5, 2**31 - 9, -1])):
+        near = torch.tensor(at).clamp(-2**30, 2**30)                       # the oracle counts in 64 bits; nothing changes beyond
+        for window, sinks in ((None, 0), (50, 3)):
+            seen = seen_by(Sq, Skv, B, window, sinks, torch.tensor(n), near)
+            value, bound = oracle(q, k, v, D ** -0.5, seen, grad)
+            out = O.window_attention(q, k, v, window, sinks, kv_len=_ints(n), q_start=_ints(at))
+            check(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, [q, k, v], grad)))), value, bound, f"{n} {at} {window}")
+            with torch.no_grad():
+                check(dict(out=O.window_attention(q, k, v, window, sinks, kv_len=_ints(n), q_start=_ints(at))), value, bound, f"{n} {at} {window} step")
 
 
 @pytest.mark.parametrize("Sq", [1, 90])
@@ -441,3 +460,25 @@ def test_native_refusals():
                 lambda: torch.ops.mdb200.window_attention(q, k, v, 4, 0, math.nan, None, 0, None, None, None)):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
+
+
+def test_encoders_with_fused_attention():
+    """Both text encoders in bf16: the fused form launches its kernels and gives what the separate operations give, up to the rounding of their bf16 scores,
+    bias and probabilities (2^-8 of a score of size 4 is 1.6 % of a probability: 5 % of the norm leaves room for two layers)."""
+    from mojodiffusion_b200.models.text.gpt_oss import GptOssConfig, GptOssEncoder
+    from mojodiffusion_b200.models.text.t5 import T5Config, T5Encoder
+
+    torch.manual_seed(0)
+    t5 = T5Config(vocab_size=100, d_model=256, d_ff=512, num_layers=2, num_heads=4)
+    oss = GptOssConfig(vocab_size=100, hidden_size=256, num_hidden_layers=2, num_attention_heads=8, num_key_value_heads=2, intermediate_size=128, num_local_experts=4,
+                       num_experts_per_tok=2, sliding_window=16)
+    ids = torch.randint(0, 100, (2, 70), device=DEV)
+    mask = (torch.arange(70, device=DEV)[None] < _ints([70, 31])[:, None]).long()
+    for cfg, enc in ((t5, T5Encoder(t5, torch.bfloat16, DEV)), (oss, GptOssEncoder(oss, torch.bfloat16, DEV))):
+        want = enc(ids, mask)
+        cfg.fused_attention = True
+        before = torch.ops.mdb200.launch_count()
+        got = enc(ids, mask)
+        assert torch.ops.mdb200.launch_count() > before
+        kept = mask.bool()
+        assert float((got.float() - want.float())[kept].norm() / want.float()[kept].norm()) < 0.05
