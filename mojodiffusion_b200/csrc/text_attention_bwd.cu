@@ -557,38 +557,49 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         some = some && key_seen(row);      // a key that no query sees may hold anything, and its gradient is zero
       }
       const bool second = KEYS && g == 1;
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk);
       const long long* st = !KEYS ? a.dq_strides : second ? a.dv_strides : a.dk_strides;
-      out += batch * st[0] + row * st[1] + blockIdx.y * st[2];
+      // 32 columns at a time through the tiles' memory, which no product reads any more, so that a store covers 64 bytes of eight rows: dk and dv of
+      // relative attention with 4 x 512 tokens and 64 heads of 64 columns take 86.5 us so, 93.7 with a row stored by each thread. The loop stays a loop: it runs once.
+      uint8_t* stage = sR1 + (warp - 2) * 4096;
+      const int line = r0 + quad * 32 + (lane >> 2);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk) + batch * st[0] + line * st[1] + blockIdx.y * st[2] + (lane & 3) * 8;
       const uint32_t acc = tmem_base + lane_addr + (second ? ACC2_COL : ACC1_COL);
       const float f = second ? 1.f : a.scale;
-      const bool as_part = shared || (KEYS && parts.slices > 0 && block < parts.blocks && row < a.sinks);
+      const auto leaves_as_part = [&](int row_) { return shared || (KEYS && parts.slices > 0 && block < parts.blocks && row_ < a.sinks); };
+      const bool as_part = leaves_as_part(row);
       float* whole = as_part ? parts.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * parts.blocks + block) * parts.count + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
       constexpr int CHUNKS = KEYS ? DH / 32 : DH / 64;
       const int first = KEYS ? 0 : g * CHUNKS;
-#pragma unroll
+#pragma unroll 1
       for (int c = first; c < first + CHUNKS; ++c) {
         uint32_t r[32];
         if (n_c > 0) {
           tmem_ld_32x32b_x32(acc + c * 32, r);
           tmem_wait_ld();
         }
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!some) r[e] = 0u;
         if (as_part) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(whole + c * 32 + e) = some ? make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]) : make_uint4(0, 0, 0, 0);
-        } else if (row < out_rows && extra < 0) {
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(whole + c * 32 + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+        }
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (some) {
-              w.x = pack_bf16x2(__uint_as_float(r[e + 0]) * f, __uint_as_float(r[e + 1]) * f);
-              w.y = pack_bf16x2(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
-              w.z = pack_bf16x2(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
-              w.w = pack_bf16x2(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
-            }
-            *reinterpret_cast<uint4*>(out + c * 32 + e) = w;
-          }
+        for (int e = 0; e < 4; ++e) {
+          uint4 w;
+          w.x = pack_bf16x2(__uint_as_float(r[8 * e + 0]) * f, __uint_as_float(r[8 * e + 1]) * f);
+          w.y = pack_bf16x2(__uint_as_float(r[8 * e + 2]) * f, __uint_as_float(r[8 * e + 3]) * f);
+          w.z = pack_bf16x2(__uint_as_float(r[8 * e + 4]) * f, __uint_as_float(r[8 * e + 5]) * f);
+          w.w = pack_bf16x2(__uint_as_float(r[8 * e + 6]) * f, __uint_as_float(r[8 * e + 7]) * f);
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ (lane >> 1 & 3)) << 4)) = w;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int to = line + n * 8, rl = (lane >> 2) + n * 8;
+          if (to < out_rows && extra < 0 && !leaves_as_part(to))
+            *reinterpret_cast<uint4*>(out + n * 8 * st[1] + c * 32) = *reinterpret_cast<const uint4*>(stage + rl * 64 + (((lane & 3) ^ (rl >> 1 & 3)) << 4));
         }
       }
     }
