@@ -9,9 +9,17 @@
 // delta = rowsum(do o) is formed by the first launch for its own rows and read by the second. In rows of few keys ds is a difference of nearly equal
 // terms: there the rounding of o would show (relative errors of 0.0027 in dq and dk at 20 tokens instead of 0.0024), so what it left is added.
 //
-// The 128-row operands stay in shared memory, the 64-row ones stream through a ring and serve twice: K-major for the score products and MN-major
-// for the gradient products. Score tiles are double buffered in TMEM, one buffer per math warpgroup: while one warpgroup turns its tile into
-// bf16 P / dS (over the scores, the A operand of the gradient products), the tensor core and the other one work on the next.
+// The 128-row operands stay on chip (dq: Q and dO in TMEM, KEYS: K and V in shared memory), the 64-row ones stream through a ring and serve twice:
+// K-major for the score products and MN-major for the gradient products. Heads of 128: score tiles are double buffered in TMEM, one buffer per math
+// warpgroup: while one warpgroup turns its tile into bf16 P / dS (over the scores, the A operand of the gradient products), the tensor core and the
+// other one work on the next. Heads of 64: one buffer, whose columns the warpgroups share, and a second CTA on the SM instead.
+//
+// dq's rows of Q, dO and O come by TMA, through the place of the ring, and from there into TMEM and delta: with plain loads by the thread of each
+// row a CTA began its first product 9900 of its 30000 cycles after its start, and dq of 2 x 2048 tokens, 32 / 8 heads of 128, window 512 took 127 us
+// instead of 103; with 4 x 512 tokens, 64 heads of 64 and a table 107 instead of 91.
+//
+// What bounds it: heads of 128 the turns between the products and the exponentials of a tile (about 1380 cycles for 64 streamed rows in dq and 1700 in
+// KEYS, of which the tensor core works 770 and 1020), heads of 64 the instructions of the math warps.
 //
 // Only tiles in which a pair may be visible are streamed; in those that are not visible whole, each thread makes its row's visibility bits.
 // Rows of K and V that no query of the CTA sees are zeroed in shared memory before they are multiplied (0 * NaN is not 0).
@@ -34,7 +42,8 @@ constexpr int TR = 128, TC = 64;     // resident rows, rows of a streamed tile
 constexpr int RUN_LD = 36;           // floats between the running sums of two rows: 16-byte stores and the skewed reads hit all banks
 
 struct alignas(64) TextBwdMaps {
-  CUtensorMap r1, r2, c1, c2;
+  CUtensorMap r1, r2, c1, c2;      // dq: Q, dO, K, V; KEYS: K, V, Q, dO
+  CUtensorMap o, o_low;            // dq
 };
 
 // What several CTAs add to dk and dv of the same keys, in fp32 parts [B, Hkv, blocks, count, 2, TR, DH] that the last kernel adds in order.
@@ -85,6 +94,9 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   uint8_t* sR2 = sR1 + R_BYTES;
   uint8_t* sC = KEYS ? sR2 + R_BYTES : smem;                              // STAGES x (C1, C2)
   const int near = BIAS ? text_near(a) : 0;
+  // dq: o_low, Q, dO and O of the rows come in where the stages and the running sums will be. Without o_low the first stage is loaded with them.
+  static_assert(KEYS || Shape::TILES - 1024 + Shape::SUMS >= 4 * R_BYTES);
+  const int at_once = KEYS ? STAGES : a.o_low == nullptr ? 1 : 0;
   float* sums = reinterpret_cast<float*>(sC + STAGES * 2 * C_BYTES);      // SUMMED: running sums [8 warps][32 rows][RUN_LD]
   const TextLut lut(sums + Shape::SUMS / 4, near);                        // BIAS
   float* bins = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sums) + Shape::SUMS + Shape::lut_bytes(near));      // SUMMED: [buckets - 1][256 threads]: dS of a row before its first key of the second run, the third, ... and in all
@@ -181,17 +193,20 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       fence_mbar_init();
     }
     __syncwarp();
-    if (n_c > 0) {
-      if (KEYS && elect_one()) {
-        mbar_expect_tx(&r_full, 2 * R_BYTES);
+    if (!KEYS || n_c > 0) {
+      if (elect_one()) {
+        uint8_t* to = KEYS ? sR1 : sR1 + R_BYTES;
+        mbar_expect_tx(&r_full, (KEYS ? 2 : 4 - at_once) * R_BYTES);
         for (int d = 0; d < DBOX; ++d) {
-          tma_load_4d(sR1 + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
-          tma_load_4d(sR2 + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
+          tma_load_4d(to + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
+          tma_load_4d(to + R_BYTES + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
+          if (!KEYS) tma_load_4d(to + 2 * R_BYTES + d * R_BOX, &maps.o, &r_full, d * 64, r0, blockIdx.y, batch);
+          if (!KEYS && at_once == 0) tma_load_4d(sR1 + d * R_BOX, &maps.o_low, &r_full, d * 64, r0, blockIdx.y, batch);
         }
       }
       __syncwarp();
 #pragma unroll 1
-      for (int i = 0; i < STAGES && i < n_c; ++i) load_c(i);
+      for (int i = 0; i < at_once && i < n_c; ++i) load_c(i);
     }
   } else if (warp == 1) {
     tmem_alloc(&tmem_base_s, Shape::TMEM);
@@ -221,19 +236,20 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   if (warp == 0) {
     // ----------------------------- TMA producer -----------------------------
     bool ok = true;
-    int i = STAGES;
+    int i = at_once;
     for (; i < n_c; ++i) {
       const int st = i & (STAGES - 1);
-      ok = text_wait(&c_empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s);
+      ok = !KEYS && i < STAGES ? text_wait(&a_full, 0, &abort_s) : text_wait(&c_empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s);
       if (!ok) break;
       load_c(st);
     }
     if (!ok) {
       if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 141, i);
       // the copies on the way land before the memory is given up
-      for (int j = i - STAGES; j < i; ++j) {
+      for (int j = max(i - STAGES, 0) - 1; j < i; ++j) {
+        const bool r = j < max(i - STAGES, 0);
         const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&c_full[j & (STAGES - 1)], (j / STAGES) & 1) && globaltimer_ns() - t0 < 5000000ull) {
+        while (!mbar_try_wait(r ? &r_full : &c_full[j & (STAGES - 1)], r ? 0 : (j / STAGES) & 1) && globaltimer_ns() - t0 < 5000000ull) {
         }
       }
     }
@@ -328,34 +344,38 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     const uint32_t lane_addr = static_cast<uint32_t>(quad * 32) << 16;
     const int row = r0 + mt;
     const float sl2 = a.scale * TXT_LOG2E;
+    bool ok = true;
     float my_nlse = -INFINITY, my_ndelta = 0.f;       // rows behind the last query: probabilities of zero
     if (!KEYS) {
       // Q (warpgroup 0) and dO (1) become A operands in TMEM: with 64 columns of B, A from shared memory would cost the score products 48 cycles for
       // every 32. On the way warpgroup 1 forms delta.
-      const long long* st = g == 0 ? a.q_strides : a.do_strides;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(g == 0 ? a.q : a.dout) + batch * st[0] + row * st[1] + blockIdx.y * st[2]);
-      const uint4* out = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o) + batch * a.o_strides[0] + row * a.o_strides[1] + blockIdx.y * a.o_strides[2]);
-      const uint4* out_low = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.o_low) + batch * a.o_strides[0] + row * a.o_strides[1] + blockIdx.y * a.o_strides[2]);
+      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
+      if (row < a.Sq) my_nlse = -a.lse[at];
+      ok = text_wait(&r_full, 0, &abort_s);
+      const uint8_t* mine = sR1 + (1 + g) * R_BYTES + mt * 128;
       float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < DH / 64; ++c) {
+#pragma unroll 1
+      for (int c = 0; c < DH / 64; ++c, mine += R_BOX) {
         uint32_t r[32];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint4 u = row < a.Sq ? src[c * 8 + e] : make_uint4(0, 0, 0, 0);
+          const uint4 u = *reinterpret_cast<const uint4*>(mine + ((e ^ (mt & 7)) << 4));
           r[4 * e] = u.x;
           r[4 * e + 1] = u.y;
           r[4 * e + 2] = u.z;
           r[4 * e + 3] = u.w;
         }
-        if (g == 1 && row < a.Sq) {
+        if (g == 1) {
+#pragma unroll 1
+          for (int from = R_BYTES; from >= (at_once == 0 ? -2 : 1) * R_BYTES; from -= 3 * R_BYTES) {      // O, then what its rounding left
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint4 w = out[c * 8 + e], l = a.o_low != nullptr ? out_low[c * 8 + e] : make_uint4(0, 0, 0, 0);
-            sum = ffma2(unpack_bf16x2(r[4 * e]), fadd2(unpack_bf16x2(w.x), unpack_bf16x2(l.x)), sum);
-            sum = ffma2(unpack_bf16x2(r[4 * e + 1]), fadd2(unpack_bf16x2(w.y), unpack_bf16x2(l.y)), sum);
-            sum = ffma2(unpack_bf16x2(r[4 * e + 2]), fadd2(unpack_bf16x2(w.z), unpack_bf16x2(l.z)), sum);
-            sum = ffma2(unpack_bf16x2(r[4 * e + 3]), fadd2(unpack_bf16x2(w.w), unpack_bf16x2(l.w)), sum);
+            for (int e = 0; e < 8; ++e) {
+              const uint4 w = *reinterpret_cast<const uint4*>(mine + from + ((e ^ (mt & 7)) << 4));
+              sum = ffma2(unpack_bf16x2(r[4 * e]), unpack_bf16x2(w.x), sum);
+              sum = ffma2(unpack_bf16x2(r[4 * e + 1]), unpack_bf16x2(w.y), sum);
+              sum = ffma2(unpack_bf16x2(r[4 * e + 2]), unpack_bf16x2(w.z), sum);
+              sum = ffma2(unpack_bf16x2(r[4 * e + 3]), unpack_bf16x2(w.w), sum);
+            }
           }
         }
         tmem_st_32x32b_x32(tmem_base + lane_addr + (g == 0 ? AQ_COL : AD_COL) + c * 32, r);
@@ -365,8 +385,6 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_full);
       float* deltas = &s_delta[0][0];          // [128]
-      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
-      if (row < a.Sq) my_nlse = -a.lse[at];
       if (g == 1) {
         deltas[mt] = sum.x + sum.y;
         if (row < a.Sq) a.delta[at] = sum.x + sum.y;
@@ -395,7 +413,6 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     if (KEYS && stager && i_begin < n_c) fetch(i_begin);
     float sum_all = 0.f;      // SUMMED: dS of this row and warpgroup so far, which ends before key sum_end
     int sum_end = 0;
-    bool ok = true;
     int in_head = (KEYS ? i_first % max(per_head, 1) : 0) + i_begin;
     const uint32_t xa = tmem_base + lane_addr + X_COL + (BUFS == 2 ? g * TC : 0);
     const uint32_t ya = tmem_base + lane_addr + Y_COL + (BUFS == 2 ? g * TC : 0);
@@ -736,11 +753,15 @@ static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, co
 
 template <int DH>
 static int text_backward(const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
-  TextBwdMaps maps;      // the first pass has no R tiles in shared memory
+  TextBwdMaps maps;
   memset(&maps, 0, sizeof(maps));
   int r;
   if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
   if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
+  if ((r = bwd_map(&maps.r1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TR))) return 1400 + r;
+  if ((r = bwd_map(&maps.r2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TR))) return 1500 + r;
+  if ((r = bwd_map(&maps.o, a.o, a.B, a.Sq, a.H, DH, a.o_strides, TR))) return 1600 + r;
+  if (a.o_low != nullptr && (r = bwd_map(&maps.o_low, a.o_low, a.B, a.Sq, a.H, DH, a.o_strides, TR))) return 1700 + r;
   if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, parts, st) : launch_text_bwd<DH, false, false>(maps, a, parts, st))) return r;
   if ((r = bwd_map(&maps.r1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
   if ((r = bwd_map(&maps.r2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
