@@ -39,8 +39,27 @@ __device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const Te
   return k;
 }
 
-// mbar_wait in fewer instructions, by a whole warp: these kernels wait at many places, and what they do in between must stay in the instruction cache
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred P;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 P, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, P;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait in fewer instructions, by a whole warp: these kernels wait at many places, and what they do in between must stay in the instruction cache.
+// PROBE: a look without the option to suspend comes first. Where the phase is over already that takes 40 cycles instead of 190, which the issuing warp
+// pays twice for each tile (8192 tokens, heads of 128, window 1024: 164 us, 171 without; training on 2 x 2048 tokens 280 us, 286). It is ten
+// instructions more at each place: heads of 64, whose two CTAs per SM fill each other's gaps, lose by them (a prompt of 300 tokens 11.7 us, 11.0 without).
+template <bool PROBE>
 __device__ __forceinline__ bool text_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (PROBE && __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   uint64_t since = 0;
   uint32_t spins = 0;
   bool ok = true;

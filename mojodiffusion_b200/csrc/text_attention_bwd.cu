@@ -239,7 +239,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     int i = at_once;
     for (; i < n_c; ++i) {
       const int st = i & (STAGES - 1);
-      ok = !KEYS && i < STAGES ? text_wait(&a_full, 0, &abort_s) : text_wait(&c_empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s);
+      ok = !KEYS && i < STAGES ? text_wait<DH == 128>(&a_full, 0, &abort_s) : text_wait<DH == 128>(&c_empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s);
       if (!ok) break;
       load_c(st);
     }
@@ -300,7 +300,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         fence_proxy_async_smem();
         __syncwarp();
       };
-      bool ok = text_wait(KEYS ? &r_full : &a_full, 0, &abort_s) && text_wait(&c_full[0], 0, &abort_s);
+      bool ok = text_wait<DH == 128>(KEYS ? &r_full : &a_full, 0, &abort_s) && text_wait<DH == 128>(&c_full[0], 0, &abort_s);
       if (ok) {
         tc_fence_after();
         clean(0, 0);
@@ -311,7 +311,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         const int st = i & (STAGES - 1), stn = (i + 1) & (STAGES - 1);
         const bool more = i + 1 < n_c;
         if (more) {
-          ok = text_wait(&c_full[stn], ((i + 1) / STAGES) & 1, &abort_s);
+          ok = text_wait<DH == 128>(&c_full[stn], ((i + 1) / STAGES) & 1, &abort_s);
           if (!ok) break;
           tc_fence_after();
           clean(i + 1, stn);
@@ -320,7 +320,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             __syncwarp();
           }
         }
-        ok = text_wait(&pds_full[BUFS == 2 ? i & 1 : 0], (BUFS == 2 ? i >> 1 : i) & 1, &abort_s);
+        ok = text_wait<DH == 128>(&pds_full[BUFS == 2 ? i & 1 : 0], (BUFS == 2 ? i >> 1 : i) & 1, &abort_s);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -351,7 +351,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       // every 32. On the way warpgroup 1 forms delta.
       const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
       if (row < a.Sq) my_nlse = -a.lse[at];
-      ok = text_wait(&r_full, 0, &abort_s);
+      ok = text_wait<DH == 128>(&r_full, 0, &abort_s);
       const uint8_t* mine = sR1 + (1 + g) * R_BYTES + mt * 128;
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -431,12 +431,12 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
           mbar_arrive(&lv_full[g]);
         }
         if (stager && i + BUFS < n_c) fetch(BUFS);
-        ok = text_wait(&lv_full[g], par, &abort_s);
+        ok = text_wait<DH == 128>(&lv_full[g], par, &abort_s);
         ok = __all_sync(0xffffffffu, ok && lv_ok);
         if (!ok) break;
       }
       const int c0 = tile_of(in_head) * TC;          // first key (dq) or query (KEYS) of the tile
-      ok = text_wait(&xy_full[BUFS == 2 ? g : 0], par, &abort_s);
+      ok = text_wait<DH == 128>(&xy_full[BUFS == 2 ? g : 0], par, &abort_s);
       if (!ok) break;
       tc_fence_after();
       constexpr int NC = BUFS;                       // pieces of 32 columns of a thread: all of the tile's, or one
@@ -564,7 +564,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       }
       in_head += BUFS;
     }
-    if (ok && n_c > 0) ok = text_wait(&acc_full, 0, &abort_s);
+    if (ok && n_c > 0) ok = text_wait<DH == 128>(&acc_full, 0, &abort_s);
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 161, n_c);
     if (ok) {
       // dq: each warpgroup stores half of the columns; KEYS: warpgroup 0 dk, warpgroup 1 dv

@@ -222,7 +222,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         if (item != first) w.set(a, item, tiles);
         if (w.n_kv == 0) continue;
         if (item != first) {
-          ok = text_wait(&q_empty, (n_items & 1) ^ 1u, &abort_s);
+          ok = text_wait<DH == 128>(&q_empty, (n_items & 1) ^ 1u, &abort_s);
           if (!ok) break;
           load_q();
         }
@@ -234,7 +234,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           const uint32_t par = (n_tiles / STAGES) & 1;
 #pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
-            ok = text_wait(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s);
+            ok = text_wait<DH == 128>(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s);
             if (!ok) break;
             load_kv(kv, st, i, kv_head);
             last_bar = kv ? &v_full[st] : &k_full[st];
@@ -283,7 +283,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           t_lo[u] = __shfl_sync(0xffffffffu, w.t_lo, u);
           t_hi[u] = __shfl_sync(0xffffffffu, w.t_hi, u);
         }
-        ok = text_wait(&q_full, n_items & 1, &abort_s) && text_wait(&k_full[n_tiles % STAGES], (n_tiles / STAGES) & 1, &abort_s);
+        ok = text_wait<DH == 128>(&q_full, n_items & 1, &abort_s) && text_wait<DH == 128>(&k_full[n_tiles % STAGES], (n_tiles / STAGES) & 1, &abort_s);
         if (!ok) break;
         ++n_items;
         tc_fence_after();
@@ -298,13 +298,13 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         // the epilogue of the item before has read the tiles' O
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (ok && !ONE && t_hi[u] > 0) ok = text_wait(&o_empty[u], (outs[u]++ & 1) ^ 1u, &abort_s);
+          if (ok && !ONE && t_hi[u] > 0) ok = text_wait<DH == 128>(&o_empty[u], (outs[u]++ & 1) ^ 1u, &abort_s);
         if (!ok) break;
         uint32_t begun[2] = {0, 0};
         for (int i = 0; i < w.n_kv; ++i, ++n_tiles) {
           const int st = n_tiles % STAGES, st_n = (n_tiles + 1) % STAGES;
           const bool more = i + 1 < w.n_kv;
-          ok = text_wait(&v_full[st], (n_tiles / STAGES) & 1, &abort_s) && (!more || text_wait(&k_full[st_n], ((n_tiles + 1) / STAGES) & 1, &abort_s));
+          ok = text_wait<DH == 128>(&v_full[st], (n_tiles / STAGES) & 1, &abort_s) && (!more || text_wait<DH == 128>(&k_full[st_n], ((n_tiles + 1) / STAGES) & 1, &abort_s));
           if (!ok) break;
           const int k0 = w.key_tile(i) * TK;
           if (k0 + TK > w.all.end || (k0 < w.all.lo && k0 + TK > w.all.sinks)) {
@@ -325,7 +325,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             if (w.sees(t_lo[u], t_hi[u], i)) {
 #pragma unroll
               for (int part = 0; part < PARTS; ++part) {
-                ok = text_wait(&p_full[u][part], done[u] & 1, &abort_s);
+                ok = text_wait<DH == 128>(&p_full[u][part], done[u] & 1, &abort_s);
                 if (!ok) return;
                 tc_fence_after();
                 if (elect_one()) {
@@ -400,7 +400,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       for (int i = 0, kt = w.key_tile(0); i < w.n_kv; ++i, kt = i == w.ns ? w.lo : kt + 1) {
         if (kt >= my_hi || (kt < my_lo && kt >= w.ns)) continue;
         const int k0 = kt * TK;
-        ok = text_wait(&s_full[t], done & 1, &abort_s);
+        ok = text_wait<DH == 128>(&s_full[t], done & 1, &abort_s);
         if (!ok) break;
         tc_fence_after();
         uint32_t sv[PIECES][32];
@@ -458,7 +458,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           // The reference is raised when a row has outgrown it by more than 2^8, and with the first key that a row sees.
           const bool need = mx > m_used + 8.0f;
           if (__any_sync(0xffffffffu, need)) {
-            ok = text_wait(&o_full[t], (done - 1) & 1, &abort_s);
+            ok = text_wait<DH == 128>(&o_full[t], (done - 1) & 1, &abort_s);
             if (!ok) break;
             tc_fence_after();
             const float alpha = need ? exp2f(m_used - mx) : 1.0f;
@@ -511,7 +511,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       }
       if (item + step < last) w.set(a, item + step, tiles);      // while the last products run
       if (ok && !fresh) {
-        ok = text_wait(&o_full[t], (done - 1) & 1, &abort_s);
+        ok = text_wait<DH == 128>(&o_full[t], (done - 1) & 1, &abort_s);
       }
       if (!ok) continue;
       tc_fence_after();
