@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from mojodiffusion_b200 import ops as O
-from text_attention_oracle import check, oracle, seen_by
+from text_attention_oracle import FINE, HALF, bucket, check, oracle, seen_by
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -187,6 +187,25 @@ def test_large_scores_move_the_maximum():
     out = O.window_attention(q, k, v, 300)
     # scores up to 100, so exponents up to 144 with steps of 2^-17 of fp32, from products up to 10: relative 3e-4 of a probability
     assert float((out.double() - value["out"]).abs().max()) <= (2 * 2.0 ** -8 + 1e-3) * float(v.abs().max())
+
+
+def test_table_gradient_keeps_what_rounding_the_output_left():
+    """Scores that are all equal (p = 1 before the division, also in bf16) over values whose mean no bf16 number holds: o is off by 2^-9 in every element, in
+    the same direction, so that delta = do . o would be off by 64 * 2^-9 = 0.125 in every row. The bound is what is left without that rounding: FINE for
+    the sums and exponentials in o, delta and ds each, and HALF twice for the rest of o that is kept in bf16; 0.08 of a row."""
+    S, H, D = 512, 2, 64
+    q, k = torch.zeros(1, S, H, D, device=DEV, dtype=torch.bfloat16), _normal(1, S, H, D, seed=60)
+    v = torch.where(torch.arange(S, device=DEV) % 4 == 3, 1 + 2.0 ** -7, 1.0).to(torch.bfloat16)[None, :, None, None].expand(1, S, H, D).contiguous()
+    grad = torch.ones_like(q)
+    table = torch.zeros(32, H, device=DEV, requires_grad=True)
+    got, = torch.autograd.grad(O.relative_attention(q, k, v, table), [table], grad)
+    dp = D * v[0, :, 0, 0].double()
+    delta = dp.mean()
+    ds = ((dp - delta) / S).expand(S, S)
+    off = (FINE * delta + HALF ** 2 * delta + FINE * (dp.abs() + delta + (dp - delta).abs())) / S
+    which = torch.tensor([[bucket(j - i, 32, 128) for j in range(S)] for i in range(S)], device=DEV)
+    want, bound = (torch.zeros(32, device=DEV, dtype=torch.float64).index_add_(0, which.flatten(), t.expand(S, S).flatten()) for t in (ds, off))
+    assert bool(((got.double() - want[:, None]).abs() <= bound[:, None]).all())
 
 
 def test_switched_off_buckets():
