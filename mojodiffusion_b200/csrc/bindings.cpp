@@ -609,7 +609,7 @@ TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, const opti
   return c;
 }
 // lse and low (what the rounding of the output left): for a backward pass, or null
-Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tensor* low, bool table_grad = false) {
+Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tensor* low, bool param_grad = false) {
   MdbTextAttnArgs& a = c.a;
   const bool given = out.has_value() && out->defined();
   if (given) TEXT_CHECK(out->sizes() == c.q.sizes() && out->scalar_type() == at::kBFloat16 && out->device() == c.q.device(), "out must have q's shape, type and device");
@@ -617,8 +617,8 @@ Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tenso
   if (lse != nullptr) {
     *lse = at::empty({a.B, a.H, a.Sq}, c.q.options().dtype(at::kFloat));
     // Where rows have few keys (see text_attention_bwd.cu); with more it is far below the other roundings of dq and dk, and a pass over memory each way.
-    // The table's gradient adds ds over a row's keys, where the error of delta, the same for all of them, does not average out.
-    if (table_grad || std::min<int64_t>(a.Skv, (int64_t)a.window + a.sinks) <= 256) *low = at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
+    // The table's gradient adds ds over a row's keys, where the error of delta, the same for all of them, does not average out; that of the sinks adds delta.
+    if (param_grad || std::min<int64_t>(a.Skv, (int64_t)a.window + a.sinks) <= 256) *low = at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
   }
   if (c.q.numel() > 0 && c.k.numel() > 0) {
     for (int i = 0; i < 3; ++i) a.o_strides[i] = o.size(i) == 1 ? 8 : o.stride(i);
@@ -656,7 +656,7 @@ struct TextAttention : public torch::autograd::Function<TextAttention> {
                         const std::vector<int64_t>& buckets) {
     c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
     TextCall c = text_call(q, k, v, scale, window, sinks, kv_len, q_start, q_starts, param, buckets);
-    Tensor lse, low, o = text_forward(c, {}, &lse, &low, c.a.table != nullptr && param->requires_grad());
+    Tensor lse, low, o = text_forward(c, {}, &lse, &low, c.param.defined() && param->requires_grad());
     ctx->save_for_backward({q, k, v, c.param, c.kv_len, c.q_start, o, low, lse});
     ctx->saved_data["scale"] = (double)c.a.scale;
     ctx->saved_data["rule"] = std::vector<int64_t>{window, sinks, q_start};

@@ -208,6 +208,19 @@ def test_table_gradient_keeps_what_rounding_the_output_left():
     assert bool(((got.double() - want[:, None]).abs() <= bound[:, None]).all())
 
 
+def test_sink_gradient_keeps_what_rounding_the_output_left():
+    """As above, with o off by 2^-8 (127 of 256 values are 1 + 2^-7): d_sink = -sum p_sink delta would be off by 0.0039 relative. The bound is FINE for
+    p_sink, o and delta each, and HALF twice: 0.0012."""
+    S, H, D = 512, 4, 64
+    q, k = torch.zeros(1, S, H, D, device=DEV, dtype=torch.bfloat16), _normal(1, S, 2, D, seed=61)
+    v = torch.where(torch.arange(S, device=DEV) % 256 < 127, 1 + 2.0 ** -7, 1.0).to(torch.bfloat16)[None, :, None, None].expand(1, S, 2, D).contiguous()
+    sink = torch.full((H,), -4.0, device=DEV, requires_grad=True)
+    got, = torch.autograd.grad(O.window_attention(q, k, v, q_start=S, sink_logits=sink), [sink], torch.ones_like(q))
+    others = S * math.exp(4.0)                                           # of the keys, for one of the sink
+    want = -S / (others + 1) * D * float(v[0, :, 0, 0].double().mean()) * others / (others + 1)
+    assert bool(((got.double() - want).abs() <= (3 * FINE + HALF ** 2) * abs(want)).all())
+
+
 def test_switched_off_buckets():
     q, k, v = _normal(1, 140, 2, 64, seed=80, scale=0.125), _normal(1, 140, 2, 64, seed=81), _normal(1, 140, 2, 64, seed=82)
     table, grad = _normal(32, 2, seed=83), _normal(1, 140, 2, 64, seed=84)
