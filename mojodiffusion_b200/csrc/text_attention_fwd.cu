@@ -21,7 +21,7 @@
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
 // What bounds it: the softmax of a tile and its hand-over to the tensor core and back. 8192 tokens, 32 / 8 heads of 128, window 1024 with 4 first keys:
-// 171 us, 754 TFLOP/s of visible pairs (about 0.85 PFLOP/s with the masked parts of the tiles). 8 x 512 tokens, 64 heads of 64 with a table: 79 us,
+// 163 us, 793 TFLOP/s of visible pairs (about 0.9 PFLOP/s with the masked parts of the tiles). 8 x 512 tokens, 64 heads of 64 with a table: 79 us,
 // 320 TFLOP/s; one CTA per SM and 128-key tiles took 100 there, and 199 in the former with a CTA per item instead of a loop over them.
 #include "text_attention.cuh"
 #include "gemm_api.h"
