@@ -77,6 +77,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int STAGES = Shape::STAGES, BUFS = Shape::BUFS;
   constexpr bool SUMMED = Shape::SUMMED;
+  constexpr int PLACES = 3 - BUFS;       // KEYS: where a warpgroup's queries are staged in turn, each place with a barrier of its own
   constexpr int DBOX = DH / 64;
   constexpr int R_BYTES = TR * DH * 2, R_BOX = TR * 128;
   constexpr int C_BYTES = TC * DH * 2, C_BOX = TC * 128;
@@ -84,7 +85,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   constexpr uint32_t AQ_COL = ACC1_COL + DH, AD_COL = AQ_COL + DH / 2;                                 // dq: Q | dO, bf16 pairs
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2], acc_full, a_full;
+  __shared__ uint64_t r_full, c_full[STAGES], c_empty[STAGES], xy_full[2], pds_full[2], lv_full[2][PLACES], acc_full, a_full;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   __shared__ __align__(16) float s_lse[2][TC], s_delta[2][TC];      // negated, per staged query: of either buffer, or of either warpgroup's columns, twice
@@ -186,7 +187,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       for (int s = 0; s < 2; ++s) {
         mbar_init(&xy_full[s], 1);
         mbar_init(&pds_full[s], BUFS == 1 ? 8 : 4);
-        mbar_init(&lv_full[s], BUFS == 1 ? 32 : TC);
+        for (int p = 0; p < PLACES; ++p) mbar_init(&lv_full[s][p], BUFS == 1 ? 32 : TC);
       }
       mbar_init(&acc_full, 1);
       mbar_init(&a_full, 8);
@@ -419,20 +420,23 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     const uint32_t ya = tmem_base + lane_addr + Y_COL + (BUFS == 2 ? g * TC : 0);
     for (int i = i_begin; i < n_c; i += BUFS) {
       const uint32_t par = (BUFS == 2 ? i >> 1 : i) & 1;
-      const int half = BUFS == 1 ? (i & 1) * 32 : 0;      // where this tile's queries are staged
+      const int place = i & (PLACES - 1), half = place * 32;      // where this tile's queries are staged
+      uint64_t* staged = &lv_full[g][place];
       if (KEYS) {
         while (in_head >= per_head) in_head -= per_head;
         // Two buffers: the place was last read for tile i - 2, and the warpgroup's four warps have all arrived on pds_full[g] for it. One buffer: also for
-        // tile i - 2, and the scores of tile i - 1, which this warp has seen, were only formed after all warps had arrived for it.
+        // tile i - 2, and the scores of tile i - 1, which this warp has seen, were only formed after all warps had arrived for it. By then
+        // all warps have also left their wait for the queries of tile i - 2, the place's barrier's last phase. (A barrier for both places would
+        // not do: a warp may still wait for tile i - 1's phase, and could not tell it from the one after tile i's, which has its parity.)
         bool lv_ok = true;
         if (stager) {
           if (BUFS == 2 && i >= 2) lv_ok = mbar_wait(&pds_full[g], par ^ 1u, &abort_s);
           s_lse[g][half + mt] = next_nlse;
           s_delta[g][half + mt] = next_ndelta;
-          mbar_arrive(&lv_full[g]);
+          mbar_arrive(staged);
         }
         if (stager && i + BUFS < n_c) fetch(BUFS);
-        ok = text_wait<DH == 128>(&lv_full[g], par, &abort_s);
+        ok = text_wait<DH == 128>(staged, (i >> 1) & 1, &abort_s);
         ok = __all_sync(0xffffffffu, ok && lv_ok);
         if (!ok) break;
       }
