@@ -215,9 +215,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     if (warp == 0) {
       // ----------------------------- TMA producer -----------------------------
       bool ok = true;
-      uint64_t* last_bar = &v_full[max(early - 1, 0)];
-      uint32_t last_par = 0;
-      int n_items = 0, n_tiles = 0;           // that have keys; key tiles so far
+      int n_items = 0, n_tiles = 0, loads = 2 * early;           // items that have keys; key tiles so far; loads of K and V in turn
       for (int item = first; ok && item < last; item += step) {
         if (item != first) w.set(a, item, tiles);
         if (w.n_kv == 0) continue;
@@ -237,15 +235,21 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             ok = text_wait<DH == 128>(kv ? &v_empty[st] : &k_empty[st], par ^ 1u, &abort_s);
             if (!ok) break;
             load_kv(kv, st, i, kv_head);
-            last_bar = kv ? &v_full[st] : &k_full[st];
-            last_par = par;
+            ++loads;
           }
         }
       }
       if (!ok) {
         if (lane == 0) report_status(a.status, STATUS_TIMEOUT, 111, n_tiles);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(last_bar, last_par) && globaltimer_ns() - t0 < 5000000ull) {
+        // The copies on the way land before the memory is given up: the last Q, and the last K and V of every stage. They end in any order.
+        for (int j = max(loads - 2 * STAGES, 0) - 1; j < loads; ++j) {
+          const bool q = j < max(loads - 2 * STAGES, 0);
+          if (q && n_items == 0) continue;
+          uint64_t* bar = q ? &q_full : (j & 1 ? v_full : k_full) + (j >> 1) % STAGES;
+          const uint32_t par = (q ? n_items - 1 : (j >> 1) / STAGES) & 1;
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(bar, par) && globaltimer_ns() - t0 < 5000000ull) {
+          }
         }
       }
     } else if (warp == 1) {
