@@ -53,6 +53,18 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// maxima that keep NaN: a score that is not a number makes the row's reference NaN, and with it the whole row, as in a plain softmax
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // mbar_wait in fewer instructions, by a whole warp: these kernels wait at many places, and what they do in between must stay in the instruction cache.
 // PROBE: a look without the option to suspend comes first. Where the phase is over already that takes 40 cycles instead of 190, which the issuing warp
 // pays twice for each tile (8192 tokens, heads of 128, window 1024: 164 us, 171 without; training on 2 x 2048 tokens 280 us, 286). It is ten

@@ -450,23 +450,23 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           for (int n = 0; n < 4; ++n) {
             constexpr int PER = 4 / PIECES;                 // chains in a piece
             const int c = n / PER, at = e + 2 * (n % PER);
-            mc[n] = fmax3(mc[n], __uint_as_float(sv[c][at]), __uint_as_float(sv[c][at + 1]));
+            mc[n] = max3_nan(mc[n], __uint_as_float(sv[c][at]), __uint_as_float(sv[c][at + 1]));
           }
-        const float mx = fmaf(fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])), mul, add);
+        const float mx = fmaf(max_nan(max3_nan(mc[0], mc[1], mc[2]), mc[3]), mul, add);
         if (fresh) {
-          if (mx > m_used) {
+          if (!(mx <= m_used)) {                // larger, or NaN
             l_run *= exp2f(m_used - mx);
-            m_used = mx;
+            m_used = max_nan(m_used, mx);
           }
         } else {
           // The reference is raised when a row has outgrown it by more than 2^8, and with the first key that a row sees.
-          const bool need = mx > m_used + 8.0f;
+          const bool need = !(mx <= m_used + 8.0f);      // NaN, too
           if (__any_sync(0xffffffffu, need)) {
             ok = text_wait<DH == 128>(&o_full[t], (done - 1) & 1, &abort_s);
             if (!ok) break;
             tc_fence_after();
             const float alpha = need ? exp2f(m_used - mx) : 1.0f;
-            if (need) m_used = mx;
+            if (need) m_used = max_nan(m_used, mx);
             l_run *= alpha;
 #pragma unroll 1
             for (int c = 0; c < DH / 16; ++c) {
@@ -480,7 +480,9 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
             tmem_wait_st();
           }
         }
-        const float m_now = m_used == -INFINITY ? 0.f : m_used;          // no key so far: every exponent is -inf
+        // No key so far: every exponent is -inf. A score of +inf: NaN, as the difference of two such scores; all of the row's exponents, for the
+        // polynomial takes a share of them and does not know NaN.
+        const float m_now = m_used == -INFINITY ? 0.f : m_used < INFINITY ? m_used : NAN;
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
         const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(add - m_now, add - m_now);
 #pragma unroll
@@ -571,7 +573,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       __syncwarp();
       // +inf where a row saw nothing: the backward pass then finds probabilities of zero
       if (a.lse != nullptr && row0 + lane < a.Sq)
-        a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + row0 + lane] = l_run > 0.f && m_used != -INFINITY ? m_used + log2f(l_run) : INFINITY;
+        a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + row0 + lane] = m_used == -INFINITY || l_run == 0.f ? INFINITY : m_used + log2f(l_run);
     }
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, done);
   }

@@ -1,9 +1,12 @@
-"""The language models' attention at its edges on the GPU: long streams."""
+"""The language models' attention at its edges on the GPU: long streams, scores that are not numbers."""
+import math
+
 import pytest
 import torch
 
 from mojodiffusion_b200 import ops as O
-from text_attention_oracle import check, oracle, seen_by
+from mojodiffusion_b200.ops import reference as ref
+from text_attention_oracle import FINE, HALF, check, oracle, seen_by
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -31,3 +34,71 @@ def test_gradients_of_long_streams(D):
     for _ in range(20):
         assert all(torch.equal(t, first[name]) for name, t in step().items())
     O.check_status(q)
+
+
+BAD = [("key", math.nan), ("key", math.inf), ("query", math.nan), ("query", math.inf)]
+
+
+def _with_bad_places(bad, B, Sq, Skv, H, G, D, seed):
+    """One bad element in one query or in one of sixteen neighbouring keys, a sequence of the batch for each."""
+    q, k, v = _inputs(B, Sq, Skv, H, G, D, seed=seed)
+    what, value = bad
+    for b in range(B):
+        if what == "key":
+            k[b, 20 + b, :, 5] = value
+        else:
+            q[b, b % Sq, :, 5] = value
+    return q, k, v
+
+
+def _check_bad(got, want, name):
+    """Not a number where the definition in 64 bits is not; elsewhere near it: the products' terms of size 4 and the roundings of outputs of size 1 to 4."""
+    lost = torch.isnan(want)
+    wrong = int((torch.isnan(got) != lost).sum())
+    assert int(lost.sum()) > 0 and wrong == 0, f"{name}: {wrong} values of {lost.numel()}, {int(lost.sum())} of which are lost"
+    worst = float(torch.where(lost, 0.0, got.double() - want).abs().max())
+    assert worst <= 2 * HALF * 4 + 4 * FINE, f"{name}: {worst}"
+
+
+@pytest.mark.parametrize("bad", BAD, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,starts", [(60, 10)])
+def test_window_scores_that_are_not_numbers(Sq, starts, D, bad):
+    """A query with a score of NaN or +inf among the keys that it sees has no result, and nobody else loses one."""
+    B, Skv, H, G, window = 16, 70, 4, 2, 18
+    q, k, v = _with_bad_places(bad, B, Sq, Skv, H, G, D, seed=410)
+    at = torch.arange(B, device=DEV, dtype=torch.int32) + starts - 10
+    want = ref.window_attention(q.double(), k.double(), v.double(), window, 2, q_start=at)
+    _check_bad(O.window_attention(q, k, v, window, 2, q_start=at), want, f"{bad} {Sq} {D}")
+
+
+@pytest.mark.parametrize("bad", BAD, ids=str)
+@pytest.mark.parametrize("D", [64, 128])
+def test_relative_scores_that_are_not_numbers(D, bad):
+    B, S, H = 16, 200, 2
+    q, k, v = _with_bad_places(bad, B, S, S, H, H, D, seed=420)
+    q = q * D ** -0.5
+    n = torch.tensor([17 + 5 * b for b in range(B)], dtype=torch.int32, device=DEV)      # some do not reach the bad key
+    table = _normal(32, H, seed=423)
+    want = ref.relative_attention(q.double(), k.double(), v.double(), table.double(), kv_len=n)
+    _check_bad(O.relative_attention(q, k, v, table, kv_len=n), want, f"{bad} {D}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_of_scores_that_are_not_numbers(D):
+    """The row of a bad query has no gradients, nor have the keys and values that it sees; those of other rows and of keys that no row near it sees are kept."""
+    S, H, G, window, bad = 600, 4, 2, 20, 250
+    q, k, v = _inputs(1, S, S, H, G, D, seed=430)
+    grad = _normal(1, S, H, D, seed=433)
+    clean = torch.autograd.grad(O.window_attention(*(leaves := [t.clone().requires_grad_() for t in (q, k, v)]), window), leaves, grad)
+    q[:, bad, :, 3] = math.nan
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(O.window_attention(*leaves, window), leaves, grad)
+    others = torch.arange(S, device=DEV) != bad
+    same = torch.equal(dq[:, others], clean[0][:, others])
+    assert same and bool(torch.isnan(dq[:, bad]).all())
+    for got, want in ((dk, clean[1]), (dv, clean[2])):
+        assert bool(torch.isnan(got[:, bad - window + 1:bad + 1]).all())
+        for far in (slice(0, bad - 128 - window), slice(bad + 128 + window, S)):
+            same = torch.equal(got[:, far], want[:, far])
+            assert same
