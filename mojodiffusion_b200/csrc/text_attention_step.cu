@@ -193,14 +193,14 @@ text_step_kernel(const __grid_constant__ StepMaps maps, const __grid_constant__ 
         bool raise = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float t = fmaxf(fmaxf(x[0][2 * h], x[0][2 * h + 1]), fmaxf(x[1][2 * h], x[1][2 * h + 1]));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-          // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees
+          float t = max_nan(max3_nan(x[0][2 * h], x[0][2 * h + 1], x[1][2 * h]), x[1][2 * h + 1]);
+          t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, 1));
+          t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, 2));
+          // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept
           f[h] = 1.f;
-          if (t > m[h] + 8.f) {
+          if (!(t <= m[h] + 8.f)) {
             f[h] = exp2f(m[h] - t);
-            m[h] = t;
+            m[h] = max_nan(m[h], t);
             raise = true;
           }
         }
@@ -268,7 +268,7 @@ text_step_kernel(const __grid_constant__ StepMaps maps, const __grid_constant__ 
     const int r = e / (DH / 4), w0 = (r / 16) * PER_TILE, rr = r % 16, c = e % (DH / 4) * 4;
     float top = part_m[w0][rr];
 #pragma unroll
-    for (int w = 1; w < PER_TILE; ++w) top = fmaxf(top, part_m[w0 + w][rr]);
+    for (int w = 1; w < PER_TILE; ++w) top = max_nan(top, part_m[w0 + w][rr]);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll

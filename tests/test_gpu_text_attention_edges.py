@@ -62,9 +62,9 @@ def _check_bad(got, want, name):
 
 @pytest.mark.parametrize("bad", BAD, ids=str)
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("Sq,starts", [(60, 10)])
+@pytest.mark.parametrize("Sq,starts", [(60, 10), (3, 40), (1, 35)])
 def test_window_scores_that_are_not_numbers(Sq, starts, D, bad):
-    """A query with a score of NaN or +inf among the keys that it sees has no result, and nobody else loses one."""
+    """A prompt and a few tokens over a cache: a query with a score of NaN or +inf among the keys that it sees has no result, and nobody else loses one."""
     B, Skv, H, G, window = 16, 70, 4, 2, 18
     q, k, v = _with_bad_places(bad, B, Sq, Skv, H, G, D, seed=410)
     at = torch.arange(B, device=DEV, dtype=torch.int32) + starts - 10
