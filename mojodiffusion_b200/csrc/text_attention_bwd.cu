@@ -721,19 +721,26 @@ static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh,
 
 // The start and end of a CTA take as long as about four tiles of 64 queries: slices of sixteen (2 x 2048 x 32 / 8 x 128, window 512, 4 first keys: dk and dv
 // without slices 215 us, with them 132), and parts of eight at least where few blocks leave SMs idle.
+// The slices of all first blocks are four CTAs per place on the SMs at most, and none where those blocks are as many by themselves: parts of 64 or 128 KB
+// each, so that the workspace stays below 160 MB however many first keys there are.
 static TextParts text_parts(const MdbTextAttnArgs& a) {
   TextParts p = {0, 0, 1, nullptr};
-  const long long rep = a.H / a.Hkv, blocks = (a.Skv + TR - 1) / TR;
-  const long long behind = static_cast<long long>(a.Sq) - TR - a.window;        // queries that only the first keys are streamed for, at most
-  if (a.table == nullptr && a.sinks > 0 && behind >= 4 * TC) {
-    p.slices = static_cast<int>(std::min<long long>((behind / TC * rep + 15) / 16, 64));
-    p.blocks = (std::min(a.sinks, a.Skv) + TR - 1) / TR;
-    p.count = 1 + p.slices;
-    return p;
-  }
-  const long long tiles = rep * ((std::min<long long>(a.Sq, a.table != nullptr ? a.Sq : static_cast<long long>(a.window) + TR) + TC - 1) / TC);
+  const long long rep = a.H / a.Hkv, blocks = (a.Skv + TR - 1) / TR, groups = static_cast<long long>(a.Hkv) * a.B;
   const long long slots = (a.Dh == 64 ? 2 : 1) * device_sm_count();
-  p.count = static_cast<int>(std::max<long long>(1, std::min({slots / (blocks * a.Hkv * a.B), tiles / 8, 8ll})));
+  const bool windowed = a.table == nullptr && a.sinks < a.Skv;                 // with as many first keys as keys there is no window
+  const long long reach = windowed ? std::min<long long>(a.Sq, static_cast<long long>(a.window) + TR) : a.Sq;      // queries of a block of keys, at most
+  const long long behind = a.Sq - reach;                                       // queries that only the first keys are streamed for
+  if (windowed && a.sinks > 0 && behind >= 4 * TC) {
+    const long long first = (a.sinks + TR - 1) / TR;
+    p.slices = static_cast<int>(std::min({(behind / TC * rep + 15) / 16, 4 * slots / (first * groups), 64ll}));
+    if (p.slices > 0) {
+      p.blocks = static_cast<int>(first);
+      p.count = 1 + p.slices;
+      return p;
+    }
+  }
+  const long long tiles = rep * ((reach + TC - 1) / TC);
+  p.count = static_cast<int>(std::max<long long>(1, std::min({slots / (blocks * groups), tiles / 8, 8ll})));
   if (p.count > 1) p.blocks = static_cast<int>(blocks);
   return p;
 }

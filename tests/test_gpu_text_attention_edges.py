@@ -102,3 +102,41 @@ def test_gradients_of_scores_that_are_not_numbers(D):
         for far in (slice(0, bad - 128 - window), slice(bad + 128 + window, S)):
             same = torch.equal(got[:, far], want[:, far])
             assert same
+
+
+@pytest.mark.parametrize("case", [(2, 1500, 1800, 4, 2, 64, 100, 300, [300, 100], [1800, 1300]), (2, 1500, 1800, 4, 2, 128, 100, 300, [300, 100], [1800, 1300]),
+                                  (1, 900, 1500, 6, 2, 128, 130, 700, [500], [1399]), (1, 1200, 1200, 4, 4, 64, 50, 1199, [0], [1200]),
+                                  (4, 700, 700, 32, 32, 128, 100, 600, [0, 0, 3, -9], [700, 650, 700, 0])], ids=str)
+def test_gradients_of_many_first_keys(case):
+    """Blocks of first keys whose later queries go to slices, with lengths and positions of their own; the last case has enough blocks without them."""
+    B, Sq, Skv, H, G, D, window, sinks, at, n = case
+    q, k, v = (t.requires_grad_() for t in _inputs(B, Sq, Skv, H, G, D, seed=440))
+    at, n = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in (at, n))
+    grad = _normal(B, Sq, H, D, seed=443)
+    value, bound = oracle(q, k, v, D ** -0.5, seen_by(Sq, Skv, B, window, sinks, n.cpu(), at.cpu()), grad)
+    out = O.window_attention(q, k, v, window, sinks, kv_len=n, q_start=at)
+    check(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, [q, k, v], grad)))), value, bound, str(case))
+
+
+def _backward_memory(window, sinks, B, S, H, G, D):
+    q, k, v = (t.requires_grad_() for t in _inputs(B, S, S, H, G, D, seed=450))
+    out = O.window_attention(q, k, v, window, sinks)
+    grad = _normal(B, S, H, D, seed=453)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(out, [q, k, v], grad)
+    torch.cuda.synchronize()
+    return grads, torch.cuda.max_memory_allocated() - before - sum(t.nbytes for t in grads)
+
+
+def test_workspace_of_many_first_keys():
+    """160 MB at most, beside the gradients and 4 bytes for each row of each head; and as many first keys as keys are no window at all."""
+    B, S, H, G, D = 1, 8192, 32, 8, 128
+    _, extra = _backward_memory(256, 2048, B, S, H, G, D)
+    assert extra <= 160e6 + 4 * B * S * H
+    plain, none = _backward_memory(None, 0, B, S, H, G, D)
+    for sinks in (S, 1 << 40):
+        grads, extra = _backward_memory(128, sinks, B, S, H, G, D)
+        same = all(torch.equal(a, b) for a, b in zip(grads, plain))
+        assert same and extra <= none
