@@ -539,9 +539,10 @@ Tensor text_rows(const Tensor& t, const Tensor& like, int64_t S, int64_t heads, 
   for (int i = 0; i < 3; ++i) strides[i] = r.size(i) == 1 ? 8 : r.stride(i);      // a dimension of one element takes any stride
   return r;
 }
-// whether the call may write `out` in place: the kernels' layout, every element once, and no memory that the call reads
+// whether the call may write `out` in place: the kernels' layout, every element once, no memory that the call reads, and no gradient of `out` that
+// autograd follows (a copy into it has its node, or its refusal)
 bool text_writable(const Tensor& out, std::initializer_list<const Tensor*> read) {
-  if (!text_layout(out)) return false;
+  if (!text_layout(out) || (at::GradMode::is_enabled() && out.requires_grad())) return false;
   std::vector<std::pair<int64_t, int64_t>> dims;
   for (int i = 0; i < 4; ++i)
     if (out.size(i) > 1) dims.emplace_back(out.stride(i), out.size(i));
@@ -614,6 +615,7 @@ Tensor text_forward(TextCall& c, const optional<Tensor>& out, Tensor* lse, Tenso
   const bool given = out.has_value() && out->defined();
   if (given) TEXT_CHECK(out->sizes() == c.q.sizes() && out->scalar_type() == at::kBFloat16 && out->device() == c.q.device(), "out must have q's shape, type and device");
   Tensor o = given && text_writable(*out, {&c.q, &c.k, &c.v, &c.param, &c.kv_len, &c.q_start}) ? *out : at::empty({a.B, a.Sq, a.H, a.Dh}, c.q.options());
+  if (given && o.is_same(*out)) o.unsafeGetTensorImpl()->bump_version();      // as an operation in place: nodes that saved it notice
   if (lse != nullptr) {
     *lse = at::empty({a.B, a.H, a.Sq}, c.q.options().dtype(at::kFloat));
     // Where rows have few keys (see text_attention_bwd.cu); with more it is far below the other roundings of dq and dk, and a pass over memory each way.
@@ -1515,8 +1517,8 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("pad_channels", &pad_channels);
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
-  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float? scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor? out) -> Tensor", &window_attention);
-  m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor? out) -> Tensor", &relative_attention);
+  m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float? scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor(a!)? out) -> Tensor(a!)", &window_attention);
+  m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor(a!)? out) -> Tensor(a!)", &relative_attention);
   m.def("text_attention", &text_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);

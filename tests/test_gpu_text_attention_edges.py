@@ -140,3 +140,42 @@ def test_workspace_of_many_first_keys():
         grads, extra = _backward_memory(128, sinks, B, S, H, G, D)
         same = all(torch.equal(a, b) for a, b in zip(grads, plain))
         assert same and extra <= none
+
+
+def _calls_with_out():
+    q, k, v = _inputs(2, 150, 150, 4, 2, 64, seed=460)
+    table = _normal(32, 4, seed=463)
+    few = q[:, :1].contiguous()
+    return {"prompt": (q, lambda out: O.window_attention(q, k, v, 40, 3, out=out)), "few": (few, lambda out: O.window_attention(few, k, v, 40, 3, q_start=149, out=out)),
+            "relative": (q, lambda out: O.relative_attention(q, q, q, table, scale=0.125, out=out))}
+
+
+@pytest.mark.parametrize("which", ["prompt", "few", "relative"])
+def test_an_output_buffer_is_an_in_place_operation(which):
+    """What autograd has to know: a tensor that another node saved has changed, and a leaf that requires a gradient is not written."""
+    like, call = _calls_with_out()[which]
+    want = call(torch.empty_like(like)).clone()
+    buffer, weight = torch.ones_like(like), torch.ones_like(like, requires_grad=True)
+    loss = (weight * buffer).sum()
+    version = buffer._version
+    assert call(buffer) is buffer and buffer._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    leaf = torch.ones_like(like, requires_grad=True)
+    with pytest.raises(RuntimeError, match="leaf"):
+        call(leaf)
+    assert float(leaf.detach().min()) == 1
+    with torch.no_grad():
+        assert call(leaf) is leaf
+    same = torch.equal(leaf.detach(), want)
+    assert same
+    part = (weight * 2)[:, :]                        # a view of a result with a history: its own gradient ends here
+    out = call(part)
+    grad, = torch.autograd.grad(out.sum(), weight)
+    same = torch.equal(out.detach(), want)
+    assert same and float(grad.abs().max()) == 0
+    with torch.inference_mode():
+        frozen = torch.empty_like(like)
+        call(frozen)
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        call(frozen)
