@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from ... import ops
+from ..layers import runs_as_defined
 
 
 @dataclass
@@ -137,21 +138,21 @@ class T5Encoder(nn.Module):
         """ids [B, S], mask [B, S] (1 = token) -> hidden [B, S, d_model]."""
         x = self.shared(ids)
         B, S = ids.shape
-        bias = table = None
+        bias = owner = None                             # of the blocks so far: the additive bias, once one needs it, and the module whose table it is
         kv_len = ops.prefix_lengths(mask) if self.cfg.fused_attention and mask is not None else None
         fused = self.cfg.fused_attention and (mask is None or kv_len is not None)
         for blk in self.encoder.block:
             att = blk.layer[0].SelfAttention
-            if fused:
-                if hasattr(att, "relative_attention_bias"):
-                    table = att.relative_attention_bias.weight
-                x = x + att.attend(blk.layer[0].layer_norm(x), table, kv_len)
-                x = x + blk.layer[1].DenseReluDense(blk.layer[1].layer_norm(x))
-                continue
             if hasattr(att, "relative_attention_bias"):
-                bias = att.bias(S, ids.device).to(x.dtype)
-                if mask is not None:
-                    bias = bias + (1.0 - mask[:, None, None, :].to(x.dtype)) * torch.finfo(x.dtype).min
-            x = x + att(blk.layer[0].layer_norm(x), bias)
+                bias, owner = None, att
+            # hooks, subclasses and replacements of the attention or its table see the separate operations
+            if fused and owner is not None and runs_as_defined(att, _SelfAttention) and runs_as_defined(owner.relative_attention_bias, nn.Embedding):
+                x = x + att.attend(blk.layer[0].layer_norm(x), owner.relative_attention_bias.weight, kv_len)
+            else:
+                if bias is None and owner is not None:
+                    bias = owner.bias(S, ids.device).to(x.dtype)
+                    if mask is not None:
+                        bias = bias + (1.0 - mask[:, None, None, :].to(x.dtype)) * torch.finfo(x.dtype).min
+                x = x + att(blk.layer[0].layer_norm(x), bias)
             x = x + blk.layer[1].DenseReluDense(blk.layer[1].layer_norm(x))
         return self.encoder.final_layer_norm(x)

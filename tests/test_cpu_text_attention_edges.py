@@ -4,8 +4,10 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
 import mojodiffusion_b200
+from mojodiffusion_b200 import ops as O
 
 CSRC = Path(mojodiffusion_b200.__file__).parent / "csrc"
 
@@ -101,3 +103,57 @@ int main() {
             want["kv"[j % 2], j // 2 % stages] = j // 2 // stages % 2
         got = {(kind, int(place)): int(parity) for kind, place, parity in (w.split(",") for w in waits)}
         assert len(waits) == len(got) and got == want, line
+
+
+def _t5(per_layer):
+    from mojodiffusion_b200.models.text.t5 import T5Config, T5Encoder
+
+    torch.manual_seed(0)
+    return T5Encoder(T5Config(vocab_size=50, d_model=16, d_kv=8, d_ff=24, num_layers=3, num_heads=2, relative_attention_num_buckets=8, relative_attention_max_distance=10,
+                              per_layer_bias=per_layer))
+
+
+@pytest.mark.parametrize("per_layer", [False, True])
+def test_t5_with_fused_attention_calls_what_is_hooked_or_replaced(per_layer, monkeypatch):
+    """Attention modules and tables with hooks, forwards of their own or other classes run as with the separate operations, and change the result as there."""
+    ids = torch.randint(0, 50, (3, 23), generator=torch.Generator().manual_seed(1))
+    mask = (torch.arange(23)[None] < torch.tensor([23, 7, 15])[:, None]).long()
+    kept = mask.bool()
+    fused = []
+    monkeypatch.setattr(O, "relative_attention", lambda *a, _f=O.relative_attention, **k: fused.append(1) or _f(*a, **k))
+
+    def both(enc):
+        enc.cfg.fused_attention = False
+        want = enc(ids, mask)
+        enc.cfg.fused_attention = True
+        del fused[:]
+        got = enc(ids, mask)
+        assert float((got - want)[kept].abs().max()) < 1e-5
+        return want, len(fused)
+
+    enc = _t5(per_layer)
+    plain, count = both(enc)
+    assert count == 3
+    attention = [b.layer[0].SelfAttention for b in enc.encoder.block]
+    tables = [a.relative_attention_bias for a in attention if hasattr(a, "relative_attention_bias")]
+    seen = []
+    for place, change in (("hook", lambda: attention[1].register_forward_hook(lambda m, a, out: seen.append(len(a)) or out * 2)),
+                          ("pre-hook", lambda: attention[1].register_forward_pre_hook(lambda m, a: (a[0] * 2, *a[1:]))),
+                          ("table", lambda: tables[0].register_forward_hook(lambda m, a, out: out * 3))):
+        handle = change()
+        other, count = both(enc)
+        assert float((other - plain)[kept].abs().max()) > 1e-3
+        assert count == (2 if place != "table" or per_layer else 0)
+        handle.remove()
+    assert seen == [2, 2]
+    forward = attention[2].forward
+    attention[2].forward = lambda x, bias: forward(x, bias) + 1
+    other, count = both(enc)
+    assert count == 2 and float((other - plain)[kept].abs().max()) > 1e-3
+    del attention[2].forward
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, out: None)
+    try:
+        assert both(enc)[1] == 0
+    finally:
+        handle.remove()
+    assert both(enc)[1] == 3
