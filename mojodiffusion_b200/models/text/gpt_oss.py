@@ -24,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ... import ops
+from ..layers import runs_as_defined
 
 LENS_CAPTURE_LAYERS = (5, 11, 17, 23)
 _FP4 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
@@ -198,7 +199,9 @@ class GptOssEncoder(nn.Module):
         out = []
         kv_len = ops.prefix_lengths(mask) if c.fused_attention and mask is not None else None
         for l in self.layers:
-            x = x + l.self_attn(l.input_layernorm(x), cos, sin, mask, kv_len)
+            # hooks and replacements of an attention module see the arguments of the separate operations
+            lengths = (kv_len,) if kv_len is not None and runs_as_defined(l.self_attn, _Attn) else ()
+            x = x + l.self_attn(l.input_layernorm(x), cos, sin, mask, *lengths)
             x = x + l.mlp(l.post_attention_layernorm(x))
             out.append(x)
         return out

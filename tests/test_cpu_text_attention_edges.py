@@ -157,3 +157,29 @@ def test_t5_with_fused_attention_calls_what_is_hooked_or_replaced(per_layer, mon
     finally:
         handle.remove()
     assert both(enc)[1] == 3
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_gpt_oss_attention_that_is_hooked_or_replaced(fused):
+    """The attention's arguments stay x, cos, sin and the mask for whoever looks at them or takes its place."""
+    from mojodiffusion_b200.models.text.gpt_oss import GptOssConfig, GptOssEncoder
+
+    torch.manual_seed(0)
+    cfg = GptOssConfig(vocab_size=50, hidden_size=16, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=8, intermediate_size=16, num_local_experts=4,
+                       num_experts_per_tok=2, sliding_window=5)
+    enc = GptOssEncoder(cfg)
+    ids = torch.randint(0, 50, (2, 17), generator=torch.Generator().manual_seed(1))
+    mask = (torch.arange(17)[None] < torch.tensor([17, 6])[:, None]).long()
+    want = enc(ids, mask)
+    cfg.fused_attention = fused
+    close = lambda: float((enc(ids, mask) - want)[mask.bool()].abs().max()) < 1e-5
+    args = []
+    handle = enc.layers[0].self_attn.register_forward_pre_hook(lambda m, a: args.append(len(a)))
+    assert close() and args == [4]
+    handle.remove()
+    att = enc.layers[1].self_attn
+    forward = att.forward
+    att.forward = lambda x, cos, sin, key_mask: forward(x, cos, sin, key_mask)
+    assert close()
+    del att.forward
+    assert close()
