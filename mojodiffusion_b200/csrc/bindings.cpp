@@ -574,7 +574,7 @@ TextCall text_call(const Tensor& q, const Tensor& k, const Tensor& v, const opti
   TEXT_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "k and v need a number of heads that divides q's");
   for (int i = 0; i < 3; ++i) TEXT_CHECK(q.size(i) < (i == 1 ? 1ll << 30 : 65536) && k.size(i) < (i == 1 ? 1ll << 30 : 65536), "fewer than 2^30 rows, 65536 sequences and heads");
   TEXT_CHECK(window >= 1 && sinks >= 0, "window of at least 1, sinks of at least 0");
-  TEXT_CHECK(scale > 0 && std::isfinite(scale), "a positive scale");
+  TEXT_CHECK(scale >= 0x1p-126 && scale <= 0x1p127, "a positive scale, which fp32 holds times log2(e)");
   const int64_t far = 1 << 30;
   a.B = (int)q.size(0); a.Sq = (int)q.size(1); a.H = (int)q.size(2); a.Dh = (int)q.size(3); a.Skv = (int)k.size(1); a.Hkv = (int)k.size(2);
   a.window = (int)std::min(window, far);

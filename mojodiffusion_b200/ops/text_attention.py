@@ -18,6 +18,8 @@ import torch
 from . import native, reference as ref
 
 _NO_WINDOW = 1 << 30
+#: what the kernels take, and their torch statements beyond: sequences and heads (a grid's extent), scales (normal fp32, times log2(e) too)
+_MOST_BLOCKS, _LEAST_SCALE, _MOST_SCALE = 65535, 2.0 ** -126, 2.0 ** 127
 #: by head width, the buckets that the kernels' tables hold and the distance at which the last one may begin; beyond them the torch statement runs
 MAX_BUCKETS, MAX_NEAR = {64: 64, 128: 32}, {64: 512, 128: 240}
 
@@ -51,10 +53,10 @@ def _per_sequence(name, what, t, q):
 
 def _kernels(q, k, v, scale, param, kv_len, q_start, out) -> bool:
     """Whether the kernels cover the call. They check shapes, types and devices themselves, which costs a short call less."""
-    if not q.is_cuda or q.dtype is not torch.bfloat16 or q.dim() != 4 or not (scale is None or 0 < scale < math.inf):
+    if not q.is_cuda or q.dtype is not torch.bfloat16 or q.dim() != 4 or not (scale is None or _LEAST_SCALE <= scale <= _MOST_SCALE):
         return False
-    width = q.size(3)
-    if (width != 64 and width != 128) or (param is not None and param.dtype is not torch.bfloat16 and param.dtype is not torch.float32):
+    sequences, _, heads, width = q.shape
+    if sequences > _MOST_BLOCKS or heads > _MOST_BLOCKS or (width != 64 and width != 128) or (param is not None and param.dtype is not torch.bfloat16 and param.dtype is not torch.float32):
         return False
     return native.use_native(q) and native.direct(*[t for t in (q, k, v, param, kv_len, q_start, out) if t is not None])
 

@@ -179,3 +179,50 @@ def test_an_output_buffer_is_an_in_place_operation(which):
         call(frozen)
     with pytest.raises(RuntimeError, match="[Ii]nference"):
         call(frozen)
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e-40, 2.0 ** -126, 2.0 ** 127])
+def test_scales_at_the_ends_of_fp32(scale):
+    """Scales below fp32's normal numbers go to the torch statement. Small ones make all scores equal, large ones leave the largest score's key alone."""
+    q, k, v = (t.requires_grad_() for t in _inputs(1, 70, 70, 4, 2, 64, seed=470))
+    with torch.no_grad():
+        k[..., 1:], q[..., 1:], q[..., 0] = 0, 0, 1                # scores are single numbers, all different
+        k[0, :, :, 0] = (torch.arange(70, device=DEV)[:, None] + 1.0) * (0.015625 if scale < 1 else -0.015625)
+        table = torch.zeros(32, 4, device=DEV)
+        k4 = k.repeat_interleave(2, 2)
+        for name, out in (("window", O.window_attention(q, k, v, scale=scale)), ("relative", O.relative_attention(q, k4, v.repeat_interleave(2, 2), table, scale=scale))):
+            vh = v.double().repeat_interleave(2, 2)
+            if scale < 1:
+                want = vh.cumsum(1) / torch.arange(1, 71, device=DEV)[None, :, None, None] if name == "window" else vh.mean(1, keepdim=True).expand_as(vh)
+            else:
+                want = vh[:, :1].expand_as(vh)
+            worst = float((out.double() - want).abs().max())
+            assert worst <= 2 * HALF * 4 + 4 * FINE, f"{name} {worst}"
+    out = O.window_attention(q, k, v, scale=scale)
+    assert all(bool(torch.isfinite(t).all()) for t in torch.autograd.grad(out.sum(), [q, k, v]))
+
+
+@pytest.mark.parametrize("scale", [1e39, 1e300])
+def test_scales_beyond_fp32(scale):
+    """The torch statement, whose fp32 scores are infinite."""
+    q, k, v = _inputs(1, 70, 70, 4, 4, 64, seed=475)
+    table = _normal(32, 4, seed=478)
+    for got, want in ((O.window_attention(q, k, v, 20, scale=scale), ref.window_attention(q, k, v, 20, scale=scale)),
+                      (O.relative_attention(q, k, v, table, scale=scale), ref.relative_attention(q, k, v, table, scale=scale))):
+        same = torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+        assert same
+
+
+@pytest.mark.parametrize("B,H", [(65535, 1), (65536, 1), (1, 65535), (1, 65536)])
+def test_many_sequences_and_heads(B, H):
+    """To the ends of a grid, and beyond them by the torch statement; forward and backward."""
+    q, k, v = (t.requires_grad_() for t in _inputs(B, 2, 3, H, H, 64, seed=480))
+    grad, table = _normal(B, 2, H, 64, seed=483), _normal(4, H, seed=484)
+    for call, seen in ((lambda: O.window_attention(q, k, v, 2, q_start=1), seen_by(2, 3, 1, 2, 0, None, 1)),
+                       (lambda: O.relative_attention(q, k, v, table, 2, scale=0.125), seen_by(2, 3, 1, causal=False))):
+        relative = bool(seen.all())
+        value, bound = oracle(q, k, v, 0.125, seen.expand(B, 2, 3), grad, table=table if relative else None, max_distance=2)
+        with torch.no_grad():
+            check(dict(out=call()), value, bound, "no gradient")
+        out = call()
+        check(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, [q, k, v], grad)))), value, bound, "gradients")
