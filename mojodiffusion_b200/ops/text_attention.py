@@ -107,7 +107,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     if sink_logits is not None and (sink_logits.shape != q.shape[2:3] or not sink_logits.is_floating_point() or sink_logits.device != q.device):
         raise ValueError(f"{name}: sink_logits must be [H] on q's device")
     if not kernels:
-        o = ref.window_attention(q, k, v, window, sinks, scale, kv_len, starts if starts is not None else start, sink_logits)
+        o = ref.window_attention(q, k, v, window if window < _NO_WINDOW else None, sinks, scale, kv_len, starts if starts is not None else start, sink_logits)
     return out.copy_(o) if out is not None else o
 
 

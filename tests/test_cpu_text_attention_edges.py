@@ -183,3 +183,19 @@ def test_gpt_oss_attention_that_is_hooked_or_replaced(fused):
     assert close()
     del att.forward
     assert close()
+
+
+@pytest.mark.parametrize("start", [2**30 - 1, 2**30, 2**31 - 10, -2**31, -2**30])
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_no_window_at_far_positions(start, as_tensor):
+    """Without a window, and with one beyond 32 bits, every earlier key is seen wherever the queries stand; none before the first key."""
+    q, k, v = (torch.randn(1, s, 2, 8, generator=torch.Generator().manual_seed(s)) for s in (3, 20, 21))
+    v = v[:, :20]
+    at = torch.tensor([start], dtype=torch.int32) if as_tensor else start
+    want = O.window_attention(q, k, v, q_start=20) if start > 0 else torch.zeros_like(q)
+    for window in (None, 1 << 40):
+        assert torch.equal(O.window_attention(q, k, v, window, q_start=at), want)
+    assert torch.equal(O.window_attention(q, k, v, 7, q_start=at), torch.zeros_like(q))
+    # other keys beside the two seen: another order of the 8 products of a score, 8 * 2^-24 * 20 of it and as much of a probability, over values up to 4
+    first = O.window_attention(q, k[:, :2], v[:, :2], q_start=20) if start > 0 else torch.zeros_like(q)
+    assert float((O.window_attention(q, k, v, 7, 2, q_start=at) - first).abs().max()) < 4 * 2 * 8 * 2.0 ** -24 * 20
