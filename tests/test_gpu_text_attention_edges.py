@@ -226,3 +226,16 @@ def test_many_sequences_and_heads(B, H):
             check(dict(out=call()), value, bound, "no gradient")
         out = call()
         check(dict(zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, [q, k, v], grad)))), value, bound, "gradients")
+
+
+@pytest.mark.parametrize("H,G,D,window", [(64, 8, 64, 128), (64, 8, 64, None), (4, 4, 128, 3)])
+def test_a_prompt_padded_to_other_lengths(H, G, D, window):
+    """The tokens of a prompt are the same bits whatever the length that it is padded to, with or without a gradient."""
+    q, k, v = _inputs(1, 300, 300, H, G, D, seed=490)
+    sink, n = _normal(H, seed=493), torch.tensor([5], dtype=torch.int32, device=DEV)
+    want = O.window_attention(q, k, v, window, kv_len=n, sink_logits=sink)[:, :5]
+    for S in (5, 8, 9, 64, 65, 130):
+        for grad in (False, True):
+            got = O.window_attention(q[:, :S].clone().requires_grad_(grad), k[:, :S], v[:, :S], window, kv_len=n, sink_logits=sink)[:, :5]
+            same = torch.equal(got.detach(), want)
+            assert same, f"{S} {grad}"
