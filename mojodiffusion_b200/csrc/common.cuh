@@ -515,8 +515,8 @@ __device__ __forceinline__ float ex2_approx(float x) {
 // 2^x of a pair on the FMA / integer pipes instead of the special-function unit (16 results per clock per SM), for a share of the
 // attention forward's exponentials. floor(x) comes from an add of 1.5 * 2^23 rounded toward minus infinity (the integer lands in the low
 // mantissa bits), 2^frac from a degree-3 polynomial (maximum relative error 8.6e-5, far below the bf16 rounding of the probabilities),
-// the integer part is added to the exponent field. Valid for least <= x <= 100; smaller inputs (masked scores) return what least does: about 2^-125, or with least = -127, whose
-// exponent field is 0, exactly zero.
+// the integer part is added to the exponent field. Valid for least <= x <= 100; smaller inputs (masked scores) and NaN return what least does:
+// about 2^-125, or with least = -127, whose exponent field is 0, exactly zero.
 __device__ __forceinline__ float2 ex2_poly2(float2 x, float least = -125.f) {
   x.x = fmaxf(x.x, least);
   x.y = fmaxf(x.y, least);

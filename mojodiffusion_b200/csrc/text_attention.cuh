@@ -66,9 +66,9 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 }
 
 // mbar_wait in fewer instructions, by a whole warp: these kernels wait at many places, and what they do in between must stay in the instruction cache.
-// PROBE: a look without the option to suspend comes first. Where the phase is over already that takes 40 cycles instead of 190, which the issuing warp
-// pays twice for each tile (8192 tokens, heads of 128, window 1024: 164 us, 171 without; training on 2 x 2048 tokens 280 us, 286). It is ten
-// instructions more at each place: heads of 64, whose two CTAs per SM fill each other's gaps, lose by them (a prompt of 300 tokens 11.7 us, 11.0 without).
+// PROBE: a look without the option to suspend comes first, which is shorter where the phase is over already; the issuing warp waits twice for each tile
+// (8192 tokens, heads of 128, window 1024: 164 us, 171 without; training on 2 x 2048 tokens 280 us, 286). It is ten instructions more at each
+// place: heads of 64, whose two CTAs per SM fill each other's gaps, lose by them (a prompt of 300 tokens 11.7 us, 11.0 without).
 template <bool PROBE>
 __device__ __forceinline__ bool text_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (PROBE && __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
@@ -171,7 +171,6 @@ inline int allow_smem(K kern, int bytes, bool (&ready)[TXT_DEVICES]) {
   return 0;
 }
 
-int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st);
 // and clusters of up to 16 CTAs
 template <typename K>
 inline int allow_wide_clusters(K kern, bool (&ready)[TXT_DEVICES]) {
@@ -184,6 +183,7 @@ inline int allow_wide_clusters(K kern, bool (&ready)[TXT_DEVICES]) {
   return 0;
 }
 
+int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st);
 bool text_attention_is_step(const MdbTextAttnArgs& a);
 int text_attention_step(const MdbTextAttnArgs& a, cudaStream_t st);
 long long text_attention_backward_floats(const MdbTextAttnArgs& a);

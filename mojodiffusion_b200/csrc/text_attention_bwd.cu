@@ -16,11 +16,12 @@
 // other one work on the next. Heads of 64: one buffer, whose columns the warpgroups share, and a second CTA on the SM instead.
 //
 // dq's rows of Q, dO and O come by TMA, through the place of the ring, and from there into TMEM and delta: with plain loads by the thread of each
-// row a CTA began its first product 9900 of its 30000 cycles after its start, and dq of 2 x 2048 tokens, 32 / 8 heads of 128, window 512 took 127 us
-// instead of 103; with 4 x 512 tokens, 64 heads of 64 and a table 107 instead of 91.
+// row dq of 2 x 2048 tokens, 32 / 8 heads of 128, window 512 took 127 us instead of 103; with 4 x 512 tokens, 64 heads of 64 and a table 107 instead of 91.
 //
-// What bounds it: heads of 128 the turns between the products and the exponentials of a tile (about 1380 cycles for 64 streamed rows in dq and 1700 in
-// KEYS, of which the tensor core works 770 and 1020), heads of 64 the instructions of the math warps.
+// What bounds it: the latency of the turns between the products and the exponentials of a tile. Heads of 128, the case above: tensor pipe active 33 % of the
+// cycles in dq (93 us) and 44 % in KEYS (122 us), issue slots 30 and 31 %. Heads of 64 with a table: 12 and 19 %, issue slots 46 % in both (90 and 83 us);
+// there the scores of a tile are only formed when all eight math warps are done with the one before. With short windows also the starts and ends of CTAs:
+// 1531 tokens, 64 / 8 heads of 64, window 128: dq 768 CTAs of four or five tiles, issue slots 34 %.
 //
 // Only tiles in which a pair may be visible are streamed; in those that are not visible whole, each thread makes its row's visibility bits.
 // Rows of K and V that no query of the CTA sees are zeroed in shared memory before they are multiplied (0 * NaN is not 0).

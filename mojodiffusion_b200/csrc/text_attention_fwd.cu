@@ -12,17 +12,18 @@
 // Heads of 64: 64 keys at a time and half of TMEM, so that two CTAs share an SM. There the exponentials and their latencies bound: four softmax warps
 // per scheduler instead of two, and the start and the epilogue of one CTA run under the other's work.
 //
-// Key tiles are visited only where a row of the CTA may see a key: the tiles of the first `sinks` keys, then those of the windows. Pieces of 32 keys
-// that none of a warp's 32 rows sees are not exponentiated, those that all of them see are not masked; in the others each thread makes
-// its row's 32 visibility bits from three bounds.
-// BIAS: where all distances of such a piece lie in one bucket, that bias is folded into the exponent's fused multiply-add; in the others the bias of
-// element (i, j) is element j - i of a table in shared memory (TextLut).
+// Key tiles are visited only where a row of the CTA may see a key: the tiles of the first `sinks` keys, then those of the windows. In a tile that a
+// warp's 32 rows do not see whole, each thread makes its row's 32 visibility bits of a piece of 32 keys from three bounds; a piece that all of them see
+// is left as it is. Masked pieces go through the exponentials like the others.
+// BIAS: where all distances of a warp's rows and a tile lie in one bucket, that bias is folded into the exponent's fused multiply-add; in the other
+// tiles the bias of element (i, j) is element j - i of a table in shared memory (TextLut).
 //
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
-// What bounds it: the softmax of a tile and its hand-over to the tensor core and back. 8192 tokens, 32 / 8 heads of 128, window 1024 with 4 first keys:
-// 163 us, 793 TFLOP/s of visible pairs (about 0.9 PFLOP/s with the masked parts of the tiles). 8 x 512 tokens, 64 heads of 64 with a table: 79 us,
-// 320 TFLOP/s; one CTA per SM and 128-key tiles took 100 there, and 199 in the former with a CTA per item instead of a loop over them.
+// What bounds it: the latency of a tile's way from the scores through the softmax to the next product; no unit is busy half of the time. 8192 tokens,
+// 32 / 8 heads of 128, window 1024 with 4 first keys: 162 us, 797 TFLOP/s of visible pairs, 985 with the masked 19 % of the tiles (tensor pipe active 46 % of
+// the cycles, issue slots 43 %, special-function unit 35 %). 8 x 512 tokens, 64 heads of 64 with a table: 80 us, 320 TFLOP/s (17 %, 43 %, 36 %); one CTA
+// per SM and 128-key tiles took 100 there, and 199 in the former with a CTA per item instead of a loop over them.
 #include "text_attention.cuh"
 #include "gemm_api.h"
 

@@ -1,5 +1,5 @@
 // The language models' attention for a few tokens over a cache (decoding, drafted tokens): at most 64 rows per key head, a row being one query of
-// one head of the group. No log-sum-exp is kept.
+// one head of the group, and more keys than queries. No log-sum-exp is kept.
 //
 //   o_i = sum_j exp2(x_ij - M_i) v_j / sum_j exp2(x_ij - M_i): every warp forms the sums over its keys with its own reference m, and the parts are
 //   joined with the factors exp2(m - M).
@@ -13,8 +13,9 @@
 // Visited are the tiles of the first `sinks` keys and those from the oldest key of a window on, wherever that is. Rows of V that no query sees
 // are zeroed in shared memory before the product (0 * NaN is not 0).
 //
-// 4 sequences of 70001 to 131072 keys, 8 key heads of 128: 266 us, 6.18 TB/s of keys and values; 16 of up to 16384 with window 4096: 43 us, 6.2 TB/s.
-// The smallest calls are one launch of 5 us.
+// 4 sequences of 70001 to 131072 keys, 8 key heads of 128: 256 to 276 us, 6.1 to 6.4 TB/s of keys and values, which the memory bounds. 16 of 1 to 16384 keys
+// with window 4096 and 4 first keys: 41 to 45 us for 213 to 263 MB, 5.2 to 5.8 TB/s; every sequence has the same two CTAs per key head, so that short ones
+// leave their part of the memory's rate unused. The smallest calls are one launch of 5 us.
 #include "text_attention.cuh"
 #include "gemm_api.h"
 
