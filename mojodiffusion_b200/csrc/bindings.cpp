@@ -720,6 +720,144 @@ Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const o
 }
 
 // ------------------------------------------------------------------------------------------
+// pages of keys and values
+// ------------------------------------------------------------------------------------------
+#define PAGED_CHECK(cond, ...) TORCH_CHECK_VALUE(cond, "paged cache: ", __VA_ARGS__)
+
+// The pool, which the Python layer has checked for shapes and types; `own`: what keeps copies alive
+MdbPages pages_of(const Tensor& like, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const optional<Tensor>& k_scale, const optional<Tensor>& v_scale,
+                  int64_t most, std::vector<Tensor>& own) {
+  MdbPages p;
+  memset(&p, 0, sizeof(p));
+  const int64_t least = k_pages.element_size() == 1 ? 16 : 8;      // 16 bytes
+  PAGED_CHECK(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes() && table.dim() == 2 && table.scalar_type() == at::kInt, "pages [N, Hkv, P, Dh], table int32 [B, width]");
+  const auto strides = [&](const Tensor& t, long long (&to)[2]) {
+    PAGED_CHECK(t.device() == like.device() && t.stride(3) == 1 && t.stride(2) == t.size(3) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "pages on the tensors' device, 16-byte aligned");
+    for (int i = 0; i < 2; ++i) {
+      to[i] = t.size(i) == 1 ? t.size(2) * t.size(3) : t.stride(i);
+      PAGED_CHECK(to[i] > 0 && to[i] % least == 0, "strides of pages and heads must be multiples of 16 bytes");
+    }
+  };
+  strides(k_pages, p.k_strides);
+  strides(v_pages, p.v_strides);
+  for (int i = 0; i < 4; ++i) PAGED_CHECK(k_pages.size(i) < (i == 0 ? 1ll << 31 : 65536), "fewer than 2^31 pages and 65536 heads");
+  if (k_pages.scalar_type() == at::kFloat8_e4m3fn) {
+    for (const auto* s : {&k_scale, &v_scale})
+      PAGED_CHECK(s->has_value() && (*s)->scalar_type() == at::kByte && (*s)->dim() == 2 && (*s)->size(0) == k_pages.size(0) && (*s)->size(1) == k_pages.size(1) &&
+                      ((*s)->size(1) == 1 || (*s)->stride(1) == 1) && (*s)->device() == like.device(), "scales must be uint8 [pages, Hkv], contiguous along the heads");
+    p.k_scale = k_scale->data_ptr<uint8_t>();
+    p.v_scale = v_scale->data_ptr<uint8_t>();
+    p.scale_strides[0] = k_scale->stride(0);
+    p.scale_strides[1] = v_scale->stride(0);
+  } else {
+    PAGED_CHECK(k_pages.scalar_type() == at::kBFloat16 && v_pages.scalar_type() == at::kBFloat16, "pages of bf16 or e4m3");
+  }
+  own.push_back(table.contiguous());
+  p.k = k_pages.data_ptr();
+  p.v = v_pages.data_ptr();
+  p.table = own.back().data_ptr<int>();
+  p.count = (int)k_pages.size(0); p.Hkv = (int)k_pages.size(1); p.P = (int)k_pages.size(2); p.Dh = (int)k_pages.size(3);
+  p.B = (int)table.size(0);
+  PAGED_CHECK(table.size(0) < 65536 && table.size(1) < (1ll << 30) / p.P, "fewer than 65536 sequences and 2^30 positions");
+  p.width = (int)table.size(1);
+  p.most = (int)std::min<int64_t>(most < 0 ? 1ll << 30 : most, table.size(1) * p.P);
+  p.status = status_ptr(like);
+  return p;
+}
+// rows [T, heads, Dh] in a layout that the kernels read: 16-byte pieces of a head
+const Tensor& paged_rows(const Tensor& t, long long (&strides)[2], std::vector<Tensor>& own) {
+  bool ok = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 2; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % 8 == 0);
+  own.push_back(ok ? t : t.clone(at::MemoryFormat::Contiguous));
+  for (int i = 0; i < 2; ++i) strides[i] = own.back().size(i) == 1 ? 0 : own.back().stride(i);
+  return own.back();
+}
+
+optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& start, const Tensor& cos, const Tensor& sin,
+                              const optional<Tensor>& cu, const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, const optional<Tensor>& q, const optional<Tensor>& q_norm,
+                              const optional<Tensor>& k_norm, double eps) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(k));
+  std::vector<Tensor> own;
+  own.reserve(16);
+  MdbPagedAppendArgs a;
+  memset(&a, 0, sizeof(a));
+  PAGED_CHECK(k.is_cuda() && k.dim() == 3 && k.scalar_type() == at::kBFloat16 && v.sizes() == k.sizes() && v.scalar_type() == at::kBFloat16 && k.size(0) < 1ll << 30, "k and v must be bf16 [T, Hkv, Dh], fewer than 2^30 rows");
+  a.pages = pages_of(k, k_pages, v_pages, table, k_scale, v_scale, -1, own);
+  PAGED_CHECK(k.size(1) == a.pages.Hkv && k.size(2) == a.pages.Dh && start.scalar_type() == at::kInt && start.numel() == a.pages.B && cos.sizes() == sin.sizes() && cos.size(1) * 2 == k.size(2) &&
+                  cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "k, v, start, cos or sin of another shape or type");
+  const auto whole = [&](const Tensor& t) {      // contiguous, from a 16-byte address on
+    own.push_back(t.contiguous());
+    if (reinterpret_cast<uintptr_t>(own.back().data_ptr()) % 16 != 0) own.back() = own.back().clone();
+    return own.back().data_ptr();
+  };
+  a.T = k.size(0);
+  a.k = paged_rows(k, a.k_strides, own).data_ptr();
+  a.v = paged_rows(v, a.v_strides, own).data_ptr();
+  a.start = static_cast<const int*>(whole(start));
+  a.cos = static_cast<const float*>(whole(cos));
+  a.sin = static_cast<const float*>(whole(sin));
+  a.positions = (int)std::min<int64_t>(cos.size(0), 0x7fffffff);
+  if (cu.has_value()) {
+    PAGED_CHECK(cu->scalar_type() == at::kInt && cu->numel() == a.pages.B + 1, "cu_seqlens must be int32 [B + 1]");
+    a.cu = static_cast<const int*>(whole(*cu));
+  } else {
+    PAGED_CHECK(a.T == a.pages.B, "without cu_seqlens every sequence has one row");
+  }
+  const auto weight = [&](const optional<Tensor>& w, int& f32) -> const void* {
+    if (!w.has_value()) return nullptr;
+    f32 = w->scalar_type() != at::kBFloat16;
+    return whole(f32 ? w->to(at::kFloat) : *w);
+  };
+  a.q_norm = weight(q_norm, a.q_norm_f32);
+  a.k_norm = weight(k_norm, a.k_norm_f32);
+  a.eps = (float)eps;
+  optional<Tensor> out;
+  if (q.has_value()) {
+    PAGED_CHECK(q->scalar_type() == at::kBFloat16 && q->dim() == 3 && q->size(0) == a.T && q->size(2) == k.size(2) && q->size(1) % k.size(1) == 0 && q->size(1) < 65536, "q must be bf16 [T, H, Dh]");
+    a.q = paged_rows(*q, a.q_strides, own).data_ptr();
+    a.H = (int)q->size(1);
+    out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
+    a.q_out = out->data_ptr();
+  }
+  if (a.T > 0 && a.pages.B > 0) {
+    for (const Tensor* t : {&k_pages, &v_pages}) t->unsafeGetTensorImpl()->bump_version();      // as an operation in place
+    if (k_scale.has_value())
+      for (const auto* t : {&k_scale, &v_scale}) (*t)->unsafeGetTensorImpl()->bump_version();
+    check_rc(mdb_paged_append(&a, cur_stream()), "paged_append");
+  } else if (out.has_value()) {
+    out->zero_();
+  }
+  return out;
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len, double scale, const optional<Tensor>& k_scale,
+                       const optional<Tensor>& v_scale, int64_t max_len) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  std::vector<Tensor> own;
+  own.reserve(4);
+  MdbPagedAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  PAGED_CHECK(q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kBFloat16, "q must be bf16 [B, Sq, H, Dh]");
+  a.pages = pages_of(q, k_pages, v_pages, table, k_scale, v_scale, max_len, own);
+  PAGED_CHECK(q.size(0) == a.pages.B && q.size(3) == a.pages.Dh && q.size(2) % a.pages.Hkv == 0 && q.size(1) < 1ll << 30 && q.size(2) < 65536 && kv_len.scalar_type() == at::kInt &&
+                  kv_len.numel() == a.pages.B, "q or kv_len of another shape or type");
+  Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (q.numel() == 0) return o;
+  Tensor rows = text_layout(q) ? q : q.clone(at::MemoryFormat::Contiguous), lengths = kv_len.contiguous();
+  for (int i = 0; i < 3; ++i) {
+    a.q_strides[i] = rows.size(i) == 1 ? 8 : rows.stride(i);
+    a.o_strides[i] = o.stride(i);
+  }
+  a.q = rows.data_ptr();
+  a.o = o.data_ptr();
+  a.kv_len = lengths.data_ptr<int>();
+  a.Sq = (int)q.size(1); a.H = (int)q.size(2);
+  a.scale = (float)scale;
+  check_rc(mdb_paged_attention(&a, cur_stream()), "paged_attention");
+  return o;
+}
+
+// ------------------------------------------------------------------------------------------
 // norm / rope
 // ------------------------------------------------------------------------------------------
 Tensor norm_modulate_fwd(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
@@ -1520,6 +1658,8 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float? scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor(a!)? out) -> Tensor(a!)", &window_attention);
   m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor(a!)? out) -> Tensor(a!)", &relative_attention);
   m.def("text_attention", &text_attention);
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, Tensor cos, Tensor sin, Tensor? cu_seqlens, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor? q, Tensor? q_norm, Tensor? k_norm, float eps) -> Tensor?", &paged_append);
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, float scale, Tensor? k_scale, Tensor? v_scale, int max_len) -> Tensor", &paged_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);
   m.def("qk_norm_rope", &qk_norm_rope);

@@ -242,6 +242,43 @@ int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st);
 long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a);
 int mdb_text_attention_bwd(const MdbTextAttnArgs* a, cudaStream_t st);
 
+// Pages of a key / value cache: [pages, Hkv, P, Dh], bf16 or e4m3 with a power of two per page and head. A sequence's position p lies in the page
+// table[b, p / P], slot p % P.
+typedef struct MdbPages {
+  void* k; void* v;
+  unsigned char* k_scale; unsigned char* v_scale;      // e8m0 [pages, Hkv], or null: bf16
+  const int* table;                                    // [B, width]
+  long long k_strides[2], v_strides[2];                // elements between pages and between heads; a head's [P, Dh] is contiguous
+  long long scale_strides[2];                          // between pages, of either
+  int count, width, P, Hkv, Dh, B;
+  int most;                                            // positions of a sequence, at most: width * P, or fewer
+  int* status;
+} MdbPages;
+typedef struct MdbPagedAppendArgs {
+  MdbPages pages;
+  const void* k; const void* v; const void* q;         // bf16 [T, heads, Dh]; q may be null
+  void* q_out;                                         // bf16 [T, H, Dh], contiguous
+  const int* cu;                                       // [B + 1], or null: T = B, a row each
+  const int* start;                                    // [B]: tokens in the pages before
+  const float* cos; const float* sin;                  // [positions, Dh / 2]
+  const void* q_norm; const void* k_norm;              // [Dh] or null
+  long long k_strides[2], v_strides[2], q_strides[2];  // elements between rows and between heads
+  long long T;
+  int H, positions, q_norm_f32, k_norm_f32;
+  float eps;
+} MdbPagedAppendArgs;
+int mdb_paged_append(const MdbPagedAppendArgs* a, cudaStream_t st);
+
+typedef struct MdbPagedAttnArgs {
+  MdbPages pages;
+  const void* q; void* o;                              // bf16 [B, Sq, H, Dh]
+  const int* kv_len;                                   // [B]; query row i stands at kv_len - Sq + i
+  long long q_strides[3], o_strides[3];                // elements between sequences, rows and heads
+  int Sq, H;
+  float scale;
+} MdbPagedAttnArgs;
+int mdb_paged_attention(const MdbPagedAttnArgs* a, cudaStream_t st);
+
 #ifdef __cplusplus
 }
 #endif

@@ -295,6 +295,116 @@ def relative_attention(q, k, v, table, max_distance: int = 128, scale: float = 1
     return _grouped_softmax_attention(q, k, v, scale, seen, table.t()[:, which].to(torch.promote_types(q.dtype, torch.float32)))
 
 
+def packed_attention(q, k, v, cu_seqlens, window: Optional[int] = None, scale: Optional[float] = None, sink_logits: Optional[torch.Tensor] = None):
+    """q [T, H, Dh], k / v [T, Hkv, Dh]: ``window_attention`` of each sequence, whose rows are cu_seqlens[b] .. cu_seqlens[b + 1]; the other rows are zero."""
+    ends = cu_seqlens.tolist()
+    out, at = [], 0
+    for lo, hi in zip(ends[:-1], ends[1:]):
+        if not at <= lo <= hi <= q.shape[0]:
+            raise ValueError("packed_attention: cu_seqlens must not fall, nor pass the last row")
+        out.append(q[at:lo] * 0)
+        out.append(window_attention(q[None, lo:hi], k[None, lo:hi], v[None, lo:hi], window, 0, scale, sink_logits=sink_logits)[0] if hi > lo else q[lo:hi])
+        at = hi
+    out.append(torch.zeros_like(q[at:]))
+    return torch.cat(out)
+
+
+# ---- pages of keys and values -------------------------------------------------------------------------------------------------
+E4M3_MAX = 448.0
+
+
+def page_scale_byte(most: torch.Tensor) -> torch.Tensor:
+    """The byte b of the least power of two 2^(b - 127), b >= 1, that brings ``most`` (fp32, finite) to 448 = 1.75 * 2^8 or less."""
+    mantissa, exponent = torch.frexp(most)                            # most = mantissa * 2^exponent, mantissa in [0.5, 1)
+    byte = exponent - 1 - 8 + (mantissa > 0.875) + 127
+    return torch.where(most > 0, byte, 1).clamp(min=1)
+
+
+def to_e4m3(x: torch.Tensor, byte) -> torch.Tensor:
+    """x in units of 2^(byte - 127), rounded to e4m3; infinities become NaN."""
+    x = torch.ldexp(x, 127 - torch.as_tensor(byte, device=x.device))
+    return torch.where(x.abs() == math.inf, math.nan, x).to(torch.float8_e4m3fn)
+
+
+def rotate_half_split(x, cos, sin):
+    """Halves (a, b) of the last dimension -> (a cos - b sin, b cos + a sin)."""
+    a, b = x.chunk(2, -1)
+    return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+
+
+def _pages_of(name, table, b, n, P, pages):
+    """The pages of the first n positions of sequence b."""
+    found = table[b, :(n + P - 1) // P].tolist()
+    if len(found) * P < n or any(not 0 <= p < pages for p in found):
+        raise ValueError(f"{name}: sequence {b} has a position without a page")
+    return found
+
+
+def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens=None, k_scale=None, v_scale=None, q=None, q_norm=None, k_norm=None, eps=1e-6):
+    """New rows of each sequence into its pages (in place); rotated queries or None."""
+    N, G, P, D = k_pages.shape
+    wide = torch.promote_types(k.dtype, torch.float32)
+    ends = list(range(start.numel() + 1)) if cu_seqlens is None else cu_seqlens.tolist()
+    q_out = None if q is None else torch.zeros_like(q, memory_format=torch.contiguous_format)
+
+    def turned(x, w, c, s):
+        x = x.to(wide)
+        if w is not None:
+            x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w.to(wide)
+        return rotate_half_split(x, c, s)
+
+    at = 0
+    for b, (lo, hi, first) in enumerate(zip(ends[:-1], ends[1:], start.tolist())):
+        if not at <= lo <= hi <= k.shape[0] or first < 0 or first + hi - lo > cos.shape[0]:
+            raise ValueError("paged_append: cu_seqlens must not fall, nor pass the last row; start and the positions must lie within cos and sin")
+        at = hi
+        if hi == lo:
+            continue
+        pages = _pages_of("paged_append", block_table, b, first + hi - lo, P, N)
+        c, s = (t[first:first + hi - lo, None].to(wide) for t in (cos, sin))
+        if q is not None:
+            q_out[lo:hi] = turned(q[lo:hi], q_norm, c, s).to(q.dtype)
+        for x, pool, scale in ((turned(k[lo:hi], k_norm, c, s), k_pages, k_scale), (v[lo:hi].to(wide), v_pages, v_scale)):
+            done = 0
+            while done < hi - lo:
+                page, slot = pages[(first + done) // P], (first + done) % P
+                part = x[done:done + P - slot].transpose(0, 1)                        # [G, rows, D]
+                done += part.shape[1]
+                if scale is not None:
+                    most = torch.where(part.abs() < math.inf, part.abs(), 0).amax((1, 2)).float()
+                    byte = page_scale_byte(most)
+                    if slot:
+                        before = scale[page].to(byte.dtype).clamp(max=253)
+                        byte = torch.maximum(byte, before)
+                        pool[page, :, :slot] = to_e4m3(pool[page, :, :slot].float(), (127 + byte - before)[:, None, None])
+                    scale[page] = byte.to(torch.uint8)
+                    part = to_e4m3(part, byte[:, None, None])
+                pool[page, :, slot:slot + part.shape[1]] = part.to(pool.dtype)
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, kv_len, scale=None, k_scale=None, v_scale=None, max_len=None):
+    """q [B, Sq, H, Dh] over the pages: query row i at position kv_len - Sq + i sees the keys up to its own."""
+    N, G, P, D = k_pages.shape
+    wide = torch.promote_types(q.dtype, torch.float32)
+    most = block_table.shape[1] * P if max_len is None else min(max_len, block_table.shape[1] * P)
+    out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+    for b, n in enumerate(kv_len.tolist()):
+        n = min(n, most)
+        if n <= 0 or q.shape[1] == 0:
+            continue
+        pages = _pages_of("paged_attention", block_table, b, n, P, N)
+
+        def held(pool, byte):
+            x = pool[pages].to(wide)
+            if byte is not None:
+                x = torch.ldexp(x, byte[pages].to(torch.int32)[:, :, None, None] - 127)
+            return x.transpose(1, 2).reshape(1, len(pages) * P, G, D)[:, :n]
+
+        out[b] = window_attention(q[b:b + 1].to(wide), held(k_pages, k_scale), held(v_pages, v_scale), None, 0, scale, q_start=n - q.shape[1])[0].to(q.dtype)
+    return out
+
+
 def gate_residual(x, y, gate=None, rows_per_group: int = 1, tanh_gate: bool = False):
     """x + gate[g] * y over [rows, D] (gate None: x + y)."""
     if _library_mode(x) and not tanh_gate:

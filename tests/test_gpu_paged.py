@@ -1,0 +1,202 @@
+"""Paged caches on the GPU, against their definitions in 64 bits."""
+import pytest
+import torch
+
+from mojodiffusion_b200 import ops as O
+from paged_oracle import angles, check_append, dense, pool, table_of
+from text_attention_oracle import FINE, HALF, oracle, seen_by
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _normal(*shape, seed, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dtype)
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+# starts, lengths, H, Hkv, Dh, P, 8 bits, norm, rows behind the last sequence
+APPEND = [
+    ([0], [1], 2, 1, 64, 16, True, True, 0),
+    ([300], [1], 16, 8, 128, 64, True, True, 0),
+    ([300], [1], 28, 4, 128, 64, False, True, 0),
+    (list(range(0, 130, 2)), [1] * 65, 8, 2, 128, 32, True, False, 0),
+    (list(range(0, 130, 2)), [1] * 65, 8, 2, 64, 16, True, True, 0),
+    ([5, 0, 64], [200, 1, 64], 4, 4, 128, 64, True, True, 5),
+    ([5, 0, 64], [200, 1, 64], 4, 2, 128, 128, True, False, 0),
+    ([0, 7, 3, 0], [33, 0, 20, 0], 4, 4, 64, 16, True, True, 3),
+    ([100, 127, 0], [300, 2, 128], 2, 1, 64, 128, True, True, 1),
+    ([30, 0], [70, 5], 6, 2, 64, 32, False, True, 0),
+    ([30, 0], [170, 257], 6, 2, 128, 128, False, False, 70),
+    ([15, 16, 17, 0], [1, 17, 2, 48], 2, 2, 128, 16, True, False, 1),
+    ([i % 37 for i in range(70)], [i % 5 for i in range(70)], 3, 1, 64, 16, True, True, 2),
+]
+
+
+def _append_inputs(case, seed=1):
+    start, lengths, H, G, D, P, eight, norm, spare = case
+    cu = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    T = cu[-1] + spare
+    rows = _normal(T, H + 2 * G, D, seed=seed)                  # as a projection leaves them
+    q, k, v = rows.split([H, G, G], 1)
+    q[cu[-1]:] = torch.nan                                       # rows of no sequence are not read
+    k[cu[-1]:] = torch.nan
+    ends = [a + b for a, b in zip(start, lengths)]
+    width = max(ends) // P + 2
+    pages = sum(-(-n // P) for n in ends) + 2
+    (kp, ks), (vp, vs) = pool(pages, G, P, D, eight, DEV, 2), pool(pages, G, P, D, eight, DEV, 3)
+    cos, sin = angles(max(ends) + 1, D, DEV)
+    w = [(1 + 0.2 * torch.randn(D, generator=torch.Generator().manual_seed(i))).to(torch.bfloat16) for i in range(2)] if norm else [None, None]
+    return q, k, v, cu, kp, vp, ks, vs, table_of(ends, P, pages, width), cos, sin, *w
+
+
+@pytest.mark.parametrize("case", APPEND, ids=lambda c: "-".join(str(x).replace(" ", "")[:24] for x in c))
+def test_append(case):
+    start, lengths, *_, spare = case
+    q, k, v, cu, kp, vp, ks, vs, table, cos, sin, qn, kn = _append_inputs(case)
+    before = [None if t is None else t.clone() for t in (kp, vp, ks, vs)]
+    single = lengths == [1] * len(lengths) and spare == 0
+    on = lambda w: None if w is None else w.to(DEV)
+    out = O.paged_append(k, v, kp, vp, table.to(DEV), _ints(start), cos, sin, cu_seqlens=None if single else _ints(cu), k_scale=ks, v_scale=vs, q=q, q_norm=on(qn), k_norm=on(kn))
+    check_append(before, (kp, vp, ks, vs), out, k, v, q, table, start, cu, cos, sin, qn, kn, 1e-6, str(case))
+    O.check_status()
+    if single:                                                   # the same rows, with their lengths given
+        again = [None if t is None else t.clone() for t in before]
+        out2 = O.paged_append(k, v, again[0], again[1], table.to(DEV), _ints(start), cos, sin, cu_seqlens=_ints(cu), k_scale=again[2], v_scale=again[3], q=q, q_norm=on(qn), k_norm=on(kn))
+        assert torch.equal(out, out2)
+        for a, b in zip(again, (kp, vp, ks, vs)):
+            assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    # without queries, and with weights in fp32
+    again = [None if t is None else t.clone() for t in before]
+    assert O.paged_append(k, v, again[0], again[1], table.to(DEV), _ints(start), cos, sin, cu_seqlens=_ints(cu), k_scale=again[2], v_scale=again[3], k_norm=None if kn is None else on(kn).float()) is None
+    for a, b in zip(again, (kp, vp, ks, vs)):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_append_values_that_are_not_finite_and_later_larger_ones():
+    P, D, G = 16, 64, 2
+    (kp, ks), (vp, vs) = pool(3, G, P, D, True, DEV, 0), pool(3, G, P, D, True, DEV, 1)
+    cos, sin = angles(40, D, DEV)
+    table, start = _ints([[2, 0]]), 0
+    for n, (scale, put) in enumerate([(1e-3, {}), (1.0, {3: float("inf"), 40: float("nan")}), (50.0, {0: float("-inf")}), (0.0, {}), (2e30, {}), (1e-30, {})]):
+        rows = 3 if n % 2 else 4
+        k, v = (_normal(rows, G, D, seed=10 * n + i) * scale for i in range(2))
+        for at, x in put.items():
+            v[1, 1, at] = x
+        before = [t.clone() for t in (kp, vp, ks, vs)]
+        O.paged_append(k, v, kp, vp, table, _ints([start]), cos, sin, cu_seqlens=_ints([0, rows]), k_scale=ks, v_scale=vs)
+        check_append(before, (kp, vp, ks, vs), None, k, v, None, table.cpu(), [start], [0, rows], cos, sin, None, None, 1e-6, str(n))
+        start += rows
+    O.check_status()
+
+
+# lengths, Sq, H, Hkv, Dh, P, 8 bits
+ATTENTION = [
+    ([1], 1, 2, 1, 64, 16, True),
+    ([1, 0, 16], 1, 4, 4, 128, 16, True),
+    ([300], 1, 16, 8, 128, 64, True),
+    ([300], 1, 16, 8, 128, 64, False),
+    ([5, 0, 640, 63, 64, 65], 1, 8, 2, 64, 16, True),
+    ([5, 0, 640, 63, 64, 65], 1, 8, 1, 128, 32, False),
+    ([3000, 17, 1025], 1, 28, 4, 128, 64, True),
+    ([3000, 17, 1025], 1, 12, 12, 64, 128, True),
+    ([n * 7 for n in range(70)], 1, 8, 2, 128, 32, True),
+    ([n * 7 for n in range(70)], 2, 4, 2, 64, 64, False),
+    ([4, 200, 129], 5, 16, 2, 64, 16, True),          # fewer positions than queries: rows before the first one
+    ([8, 700], 8, 64, 8, 128, 64, True),
+    ([8, 700], 7, 28, 4, 128, 16, False),
+    ([40, 300, 20], 20, 16, 2, 64, 32, True),         # parts of prompts
+    ([200, 131], 130, 6, 2, 128, 64, True),
+    ([500, 77], 70, 4, 4, 64, 16, False),
+    ([1, 0], 33, 8, 2, 128, 128, True),
+]
+
+
+def _attention_inputs(case, seed=4):
+    lengths, Sq, H, G, D, P, eight = case
+    width = max(lengths) // P + 2
+    pages = max(1, sum(-(-n // P) for n in lengths)) + 1
+    table = table_of(lengths, P, pages, width)
+    (kp, ks), (vp, vs) = pool(pages, G, P, D, eight, DEV, seed), pool(pages, G, P, D, eight, DEV, seed + 1)
+    q = _normal(len(lengths), Sq, H, D, seed=seed + 2)
+    kd, vd = (dense(p, s, table, lengths, max(lengths)) for p, s in ((kp, ks), (vp, vs)))
+    for b, n in enumerate(lengths):                              # slots behind the ends may hold anything
+        if n % P:
+            kp[int(table[b, n // P]), :, n % P:] = torch.nan
+            vp[int(table[b, n // P]), :, n % P:] = torch.nan
+    return q, kp, vp, ks, vs, table.to(DEV), kd, vd
+
+
+def check_attention(out, q, kd, vd, lengths, name):
+    """One rounding of the output, and one of the probabilities: to bf16 at most (HALF and FINE: see ``text_attention_oracle``)."""
+    B, Sq, H, D = q.shape
+    n = _ints(lengths)
+    value, bound = oracle(q, kd, vd, D ** -0.5, seen_by(Sq, max(lengths), B, None, 0, n, n - Sq))
+    assert torch.isfinite(out).all(), name
+    off = (out.double() - value["out"]).abs() - bound["out"]
+    assert float(off.max()) <= 1e-30, f"{name}: {float(off.max()):.3g} outside"
+
+
+@pytest.mark.parametrize("case", ATTENTION, ids=lambda c: "-".join(str(x).replace(" ", "")[:24] for x in c))
+def test_attention(case):
+    lengths, *_ = case
+    q, kp, vp, ks, vs, table, kd, vd = _attention_inputs(case)
+    out = O.paged_attention(q, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs)
+    check_attention(out, q, kd, vd, lengths, str(case))
+    assert torch.equal(O.paged_attention(q, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs, max_len=max(lengths)), out)
+    strided = torch.stack((q, q), 3)[:, :, :, 0]
+    assert torch.equal(O.paged_attention(strided.transpose(1, 2).contiguous().transpose(1, 2), kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs), out)
+    assert torch.equal(O.paged_attention(strided, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs), out)
+    O.check_status()
+
+
+def test_attention_max_len_cuts():
+    case = ([300, 40, 90], 1, 8, 2, 128, 32, True)
+    q, kp, vp, ks, vs, table, kd, vd = _attention_inputs(case)
+    out = O.paged_attention(q, kp, vp, table, _ints(case[0]), k_scale=ks, v_scale=vs, max_len=77)
+    check_attention(out, q, kd[:, :77], vd[:, :77], [min(n, 77) for n in case[0]], "cut")
+    assert not O.paged_attention(q, kp, vp, table, _ints(case[0]), k_scale=ks, v_scale=vs, max_len=0).any()
+
+
+def test_reports_pages_that_are_not_there():
+    """What has no page is skipped and reported; nothing else is written."""
+    P, D, G = 16, 64, 2
+    (kp, ks), (vp, vs) = pool(4, G, P, D, True, DEV, 0), pool(4, G, P, D, True, DEV, 1)
+    cos, sin = angles(64, D, DEV)
+    k, v = _normal(2, G, D, seed=2), _normal(2, G, D, seed=3)
+    before = [t.clone() for t in (kp, vp, ks, vs)]
+    O.check_status()
+    for table, start, c, s in (([[4, 1], [-1, 3]], [3, 3], cos, sin), ([[0, 1], [2, 3]], [32, 1 << 30], cos, sin), ([[0, 1], [2, 3]], [5, 9], cos[:5], sin[:5]), ([[0, 1], [2, 3]], [-1, -(1 << 31)], cos, sin)):
+        for cu in (None, _ints([0, 1, 2])):
+            out = O.paged_append(k, v, kp, vp, _ints(table), _ints(start), c, s, cu_seqlens=cu, k_scale=ks, v_scale=vs, q=k)
+            for a, b in zip(before, (kp, vp, ks, vs)):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            assert not out.any()
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+    q = _normal(2, 1, 4, D, seed=5)
+    good = O.paged_attention(q, kp, vp, _ints([[0, 1], [2, 3]]), _ints([20, 20]), k_scale=ks, v_scale=vs)
+    out = O.paged_attention(q, kp, vp, _ints([[0, 1], [2, 77]]), _ints([20, 20]), k_scale=ks, v_scale=vs)
+    assert torch.equal(out[0], good[0])
+    with pytest.raises(RuntimeError, match="BOUNDS"):
+        O.check_status()
+    O.check_status()
+
+
+def test_empty_calls():
+    P, D, G = 16, 64, 2
+    (kp, ks), (vp, vs) = pool(4, G, P, D, True, DEV, 0), pool(4, G, P, D, True, DEV, 1)
+    cos, sin = angles(8, D, DEV)
+    none = torch.empty(0, G, D, dtype=torch.bfloat16, device=DEV)
+    table0 = torch.empty(0, 3, dtype=torch.int32, device=DEV)
+    assert O.paged_append(none, none, kp, vp, table0, _ints([]), cos, sin, k_scale=ks, v_scale=vs, q=none).shape == none.shape
+    rows = torch.full((3, G, D), torch.nan, dtype=torch.bfloat16, device=DEV)
+    assert not O.paged_append(rows, rows, kp, vp, table0, _ints([]), cos, sin, cu_seqlens=_ints([0]), k_scale=ks, v_scale=vs, q=rows).any()
+    assert not O.paged_append(rows, rows, kp, vp, _ints([[0], [1]]), _ints([3, 4]), cos, sin, cu_seqlens=_ints([0, 0, 0]), k_scale=ks, v_scale=vs, q=rows).any()
+    assert O.paged_attention(torch.empty(2, 0, 4, D, dtype=torch.bfloat16, device=DEV), kp, vp, _ints([[0], [1]]), _ints([3, 4]), k_scale=ks, v_scale=vs).shape == (2, 0, 4, D)
+    assert not O.paged_attention(_normal(2, 1, 4, D, seed=0), kp, vp, _ints([[9], [9]]), _ints([0, -5]), k_scale=ks, v_scale=vs).any()
+    assert not O.paged_attention(_normal(2, 40, 4, D, seed=0), kp, vp, torch.empty(2, 0, dtype=torch.int32, device=DEV), _ints([3, 5]), k_scale=ks, v_scale=vs).any()
+    O.check_status()
