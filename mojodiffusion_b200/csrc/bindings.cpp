@@ -843,6 +843,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
                   kv_len.numel() == a.pages.B, "q or kv_len of another shape or type");
   Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   if (q.numel() == 0) return o;
+  if (a.pages.most == 0) return o.zero_();
   Tensor rows = text_layout(q) ? q : q.clone(at::MemoryFormat::Contiguous), lengths = kv_len.contiguous();
   for (int i = 0; i < 3; ++i) {
     a.q_strides[i] = rows.size(i) == 1 ? 8 : rows.stride(i);
@@ -853,6 +854,9 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.kv_len = lengths.data_ptr<int>();
   a.Sq = (int)q.size(1); a.H = (int)q.size(2);
   a.scale = (float)scale;
+  Tensor ws = at::empty({mdb_paged_attention_floats(&a)}, q.options().dtype(at::kFloat));
+  a.ws = ws.data_ptr<float>();
+  g_launches.fetch_add(1, std::memory_order_relaxed);
   check_rc(mdb_paged_attention(&a, cur_stream()), "paged_attention");
   return o;
 }
@@ -1624,7 +1628,7 @@ void set_wait_limit_ns(int64_t ns) {
   const unsigned long long v = static_cast<unsigned long long>(ns);
   const int rc = mdb_set_wait_limit_gemm(v) | mdb_set_wait_limit_attn_fwd(v) | mdb_set_wait_limit_attn_bwd(v) |
                  mdb_set_wait_limit_comm(v) | mdb_set_wait_limit_mxfp8(v) | mdb_set_wait_limit_text_fwd(v) |
-                 mdb_set_wait_limit_text_bwd(v) | mdb_set_wait_limit_text_step(v);
+                 mdb_set_wait_limit_text_bwd(v) | mdb_set_wait_limit_text_step(v) | mdb_set_wait_limit_paged(v);
   TORCH_CHECK(rc == 0, "set_wait_limit_ns failed: ", rc);
 }
 

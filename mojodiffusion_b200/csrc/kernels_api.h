@@ -276,7 +276,9 @@ typedef struct MdbPagedAttnArgs {
   long long q_strides[3], o_strides[3];                // elements between sequences, rows and heads
   int Sq, H;
   float scale;
+  float* ws;                                           // mdb_paged_attention_floats values, none of which need be set
 } MdbPagedAttnArgs;
+long long mdb_paged_attention_floats(const MdbPagedAttnArgs* a);
 int mdb_paged_attention(const MdbPagedAttnArgs* a, cudaStream_t st);
 
 #ifdef __cplusplus

@@ -1,108 +1,751 @@
 // Attention over the pages of several sequences: query row i of sequence b stands at position p = kv_len[b] - Sq + i and sees the keys up to p.
 //
-//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(s_ij - max),  s_ij = scale 2^ek q_i . k_j;  values are in units of 2^ev; ek, ev of the page and head
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp2(x_ij - m_i),  x_ij = log2(e) scale 2^ek q_i . k_j;  values are in units of 2^ev; ek, ev of the page and head
 //
-// A block of threads per query row: groups of lanes take the keys in turn, each with its own reference and sums, which meet in shared memory.
+// A few queries (at most 64 rows per key head, a row being one query of one head of the group): keys and values are read once and bound the time, so the work is split
+// over keys. All tiles of 64 keys of all sequences and key heads are one line, of which every CTA takes an equal part, wherever that begins and ends: sequences of 1 and
+// of 100000 tokens share the memory's rate. A CTA's tiles of one sequence and head ("segment") end in an output, or in a part (m, l, o) where other CTAs have tiles of
+// it too; a second, small kernel joins those in order. It is launched with the first one and waits for its end.
+//
+// A warp of its own starts the copies: it knows the pages of the next 32 places of the table and their scales, and brings K and V of a tile in by TMA, one box
+// per page. Four warps multiply, with mma.sync m16n8k16: 16 rows are all there is to multiply, a 128-row tcgen05 tile would be mostly padding.
+//
+// 8 bits: e4m3 values are exact in f16, and two of them take one conversion, so the products are f16 ones. Of a key's row a lane reads 16 bytes as they lie; which
+// of them are columns 2t, 2t + 1 of a k-step is free as long as the queries' registers use the same order, and so no byte is moved. For values ldmatrix transposes pairs of bytes,
+// one byte permutation makes two columns of them. Queries are brought to [1, 2) by a power of two per row, which leaves them exact but for those 2^-24 of the row's largest.
+// Probabilities are rounded to f16 (2^-11, where the output's rounding is 2^-8); the reference is kept 2^7 above the largest so that also those of 2^-21 of it
+// have all their bits. The powers of two of values go into the probabilities, relative to the largest met so far.
+// bf16: the products are bf16 ones; a probability goes into its product as two bf16 terms, so only the output is rounded.
+//
+// Keys behind the sequence's end are masked and their values zeroed in shared memory before the product (0 * NaN is not 0).
+#include "gemm_api.h"
 #include "paged.cuh"
+
+#include <algorithm>
+#include <string.h>
 
 namespace mdb {
 
-constexpr int PT_THREADS = 128;
+constexpr int PK = 64;                                        // keys of a tile
+constexpr int PS_WARPS = 4, PS_THREADS = (PS_WARPS + 1) * 32;
+constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
-// 16 neighbours of a key or a value
-template <bool E4M3> __device__ __forceinline__ void load16(float (&x)[16], const void* base, long long at) {
-  if (E4M3) {
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + at);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct alignas(64) PagedMaps {
+  CUtensorMap k, v;
+};
+
+template <int DH, bool E4M3> struct PagedShape {
+  static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
+  static constexpr int STAGES = 96 * 1024 / (2 * TILE);               // 96 KB, so that two CTAs share an SM
+  static constexpr int SLAB = PS_WARPS * 16 * 32 * 4;                 // 32 columns of the warps' parts
+  static constexpr int BYTES = STAGES * 2 * TILE + SLAB + 1024;
+};
+
+__device__ __forceinline__ float paged_max(float a, float b) {       // NaN stays
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void paged_ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void paged_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16> __device__ __forceinline__ void paged_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- the line of tiles: sequence after sequence, key head after key head, tile after tile ----
+__device__ __forceinline__ int paged_length(const MdbPagedAttnArgs& a, int b) { return min(max(a.kv_len[b], 0), a.pages.most); }
+__device__ __forceinline__ long long paged_tiles(const MdbPagedAttnArgs& a) {      // of one key head; by a whole warp
+  long long total = 0;
+  for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
+    const int b = b0 + (threadIdx.x & 31);
+    total += __reduce_add_sync(0xffffffffu, b < a.pages.B ? static_cast<unsigned>(paged_length(a, b) + PK - 1) / PK : 0u);
+  }
+  return total;
+}
+struct PagedPlace {
+  int b, g, t, length, tiles;
+  // of tile `at` on the line; by a whole warp
+  __device__ __forceinline__ void seek(const MdbPagedAttnArgs& a, long long at) {
+    const int lane = threadIdx.x & 31;
+    const long long target = at / a.pages.Hkv;
+    long long before = 0;
+    b = 0;
+    length = tiles = 0;
+    for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
+      const int mine = b0 + lane < a.pages.B ? paged_length(a, b0 + lane) : 0, n = (mine + PK - 1) / PK;
+      int upto = n;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 lo = e4m3x2_to_float2(static_cast<uint16_t>(w[e])), hi = e4m3x2_to_float2(static_cast<uint16_t>(w[e] >> 16));
-      x[4 * e] = lo.x; x[4 * e + 1] = lo.y; x[4 * e + 2] = hi.x; x[4 * e + 3] = hi.y;
+      for (int m = 1; m < 32; m <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, m);
+        if (lane >= m) upto += other;
+      }
+      const uint32_t behind = __ballot_sync(0xffffffffu, before + upto > target);
+      if (behind != 0) {
+        const int from = __ffs(behind) - 1;
+        b = b0 + from;
+        length = __shfl_sync(0xffffffffu, mine, from);
+        tiles = __shfl_sync(0xffffffffu, n, from);
+        before += __shfl_sync(0xffffffffu, upto, from) - tiles;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-  } else {
+    const long long rest = at - before * a.pages.Hkv;
+    g = tiles > 0 ? static_cast<int>(rest / tiles) : 0;
+    t = tiles > 0 ? static_cast<int>(rest - static_cast<long long>(g) * tiles) : 0;
+  }
+  __device__ __forceinline__ void next_segment(const MdbPagedAttnArgs& a) {
+    t = 0;
+    if (++g < a.pages.Hkv) return;
+    g = 0;
+    do {
+      if (++b >= a.pages.B) return;
+      length = paged_length(a, b);
+      tiles = (length + PK - 1) / PK;
+    } while (tiles == 0);
+  }
+};
+
+// parts: two per CTA, of the first and of the last segment of its tiles: [ctas][2][rows][DH] sums, then [ctas][2][rows][2] references and divisors
+struct PagedParts {
+  float* sums; float* tops;
+};
+
+// MT: tiles of 16 rows
+template <int DH, bool E4M3, int MT>
+__global__ void __launch_bounds__(PS_THREADS, 2)
+paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ MdbPagedAttnArgs a, const PagedParts parts) {
+  using Shape = PagedShape<DH, E4M3>;
+  constexpr int TILE = Shape::TILE, STAGES = Shape::STAGES, BOX = PK * 128;
+  constexpr int ROWS = 16 * MT, PER_TILE = PS_WARPS / MT, WK = PK / PER_TILE;      // warps that share the keys of a tile, and keys of a warp
+  constexpr int DN = DH / 8;                                                       // n-tiles of 8 columns
+  constexpr float ABOVE = E4M3 ? 7.f : 0.f;                                        // the reference stays so far below the first maximum
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uchar2 scales[STAGES][PK / 16];
+  __shared__ int abort_s;
+  __shared__ float part_m[PS_WARPS][16], part_l[PS_WARPS][16];
+  uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  float* slab = reinterpret_cast<float*>(smem + STAGES * 2 * TILE);
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const MdbPages& pg = a.pages;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], PS_WARPS);
+    }
+    abort_s = 0;
+    fence_mbar_init();
+  }
+  const long long line = paged_tiles(a) * pg.Hkv, ctas = min(static_cast<long long>(gridDim.x), line);
+  const long long line_first = blockIdx.x < ctas ? line * blockIdx.x / ctas : 0;
+  PagedPlace at;
+  at.seek(a, line_first);
+  __syncthreads();
+  if (blockIdx.x >= ctas) return;
+  const int n = static_cast<int>(line * (blockIdx.x + 1) / ctas - line_first);
+
+  if (warp == PS_WARPS) {
+    const int per_tile = max(PK / pg.P, 1), rows = min(pg.P, PK);            // boxes of a tile, keys of a box
+    const uint32_t box_bytes = rows * DH * (E4M3 ? 1 : 2);
+    int window = 0, page = -1;                                              // this lane's place of the table: window + lane
+    uint32_t sc = 0;
+    bool ok = true, fresh = true;
+    int i = 0;
+    for (; i < n; ++i) {
+      const int first_index = static_cast<int>(static_cast<long long>(at.t) * PK / pg.P);
+      if (fresh || first_index + per_tile > window + 32) {
+        window = first_index;
+        const int index = window + lane;
+        const bool needed = index < (at.length + pg.P - 1) / pg.P;
+        page = needed ? page_of(pg, at.b, index) : -1;
+        if (needed && page < 0) report_status(pg.status, STATUS_BOUNDS, 182, at.b);
+        if (E4M3) {
+          sc = 0;
+          if (page >= 0) sc = pg.k_scale[page * pg.scale_strides[0] + at.g] | pg.v_scale[page * pg.scale_strides[1] + at.g] << 8;
+        }
+        fresh = false;
+      }
+      const int st = i % STAGES;
+      ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ((i / STAGES) & 1) ^ 1u, &abort_s));
+      if (!ok) {
+        if (lane == 0) report_status(pg.status, STATUS_TIMEOUT, 183, i);
+        break;
+      }
+      const int keys = min(at.length - at.t * PK, PK), boxes = (keys + rows - 1) / rows;
+      if (E4M3) {
+        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 3) * 16) / pg.P - window) & 31);
+        if (lane < PK / 16) scales[st][lane] = make_uchar2(s & 255, s >> 8);
+      }
+      const int mine = __shfl_sync(0xffffffffu, page, (first_index - window + min(lane, per_tile - 1)) & 31);
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(&full[st], 2 * boxes * box_bytes);
+      __syncwarp();
+      if (lane < boxes) {
+        const int row = pg.P > PK ? at.t * PK % pg.P : 0;
+        uint8_t* to = smem + st * 2 * TILE;
+        if (E4M3) {
+          tma_load_4d(to + lane * box_bytes, &maps.k, &full[st], 0, row * DH / 128, at.g, mine);
+          tma_load_4d(to + TILE + lane * box_bytes, &maps.v, &full[st], 0, row * DH / 128, at.g, mine);
+        } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at + h * 8);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack_bf16x2(w[e]);
-        x[h * 8 + 2 * e] = f.x;
-        x[h * 8 + 2 * e + 1] = f.y;
+          for (int d = 0; d < DH / 64; ++d) {
+            tma_load_4d(to + d * BOX + lane * rows * 128, &maps.k, &full[st], d * 64, row, at.g, mine);
+            tma_load_4d(to + TILE + d * BOX + lane * rows * 128, &maps.v, &full[st], d * 64, row, at.g, mine);
+          }
+        }
+      }
+      __syncwarp();
+      if (++at.t == at.tiles) {
+        at.next_segment(a);
+        fresh = true;
       }
     }
+    if (!ok && lane == 0) {      // the copies on the way land before the memory is given up
+      for (int j = max(0, i - STAGES); j < i; ++j) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && globaltimer_ns() - t0 < 5000000ull) {
+        }
+      }
+    }
+    __syncwarp();
+    return;
   }
+
+  const int mt = warp / PER_TILE, part = warp % PER_TILE;
+  const int tq = lane & 3, gq = lane >> 2;                            // rows mt * 16 + gq and 8 more
+  const int rep = a.H / pg.Hkv, rows = rep * a.Sq;
+  bool ok = true;
+  for (int i = 0, segment = 0; i < n; ++segment) {
+    const int b = at.b, g = at.g, first_tile = at.t, end = at.length, start = end - a.Sq;
+    const int count = min(at.tiles - first_tile, n - i);
+    uint32_t q[DH / 16][4];
+    float sl2[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + gq + 8 * h;
+      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_strides[0] + (r / rep) * a.q_strides[1] + (g * rep + r % rep) * a.q_strides[2];
+      sl2[h] = a.scale * PAGED_LOG2E;
+      if (E4M3) {
+        // k-step 4 c + s: columns 16 (4 c + t) + 4 s .. + 3 belong to lane t
+        uint32_t w[DH / 16][2];
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < DH / 64; ++c)
+#pragma unroll
+          for (int s = 0; s < 4; s += 2) {
+            const uint4 u = r < rows ? *reinterpret_cast<const uint4*>(p + 16 * (4 * c + tq) + 4 * s) : make_uint4(0, 0, 0, 0);
+            w[4 * c + s][0] = u.x;
+            w[4 * c + s][1] = u.y;
+            w[4 * c + s + 1][0] = u.z;
+            w[4 * c + s + 1][1] = u.w;
+          }
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = unpack_bf16x2(w[kk][e]);
+            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));      // NaN and infinity come through by themselves
+          }
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 1), 253);
+        const float f = scale_inverse(e);
+        sl2[h] *= scale_value(e);
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) {
+          const float2 x = unpack_bf16x2(w[kk][0]), y = unpack_bf16x2(w[kk][1]);
+          q[kk][h] = pack_f16x2(x.x * f, x.y * f);
+          q[kk][h + 2] = pack_f16x2(y.x * f, y.y * f);
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < DH / 16; ++kk) {
+          q[kk][h] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq) : 0u;
+          q[kk][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq + 8) : 0u;
+        }
+      }
+    }
+    const int p_row[2] = {start + (mt * 16 + gq) / rep, start + (mt * 16 + gq + 8) / rep};
+    float o[DN][4];
+#pragma unroll
+    for (int d = 0; d < DN; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int unit = 0;                                                      // byte of the power of two that o is in units of
+    // key j of a group of eight lies in this row of the stage: lanes that read 16 bytes each at once then hit all banks (see the swizzle)
+    const auto key_of = [](int j) { return E4M3 && DH == 128 ? (j >> 1) + 4 * (j & 1) : j; };
+
+    for (int tile = first_tile; tile < first_tile + count; ++tile, ++i) {
+      const int st = i % STAGES;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (i / STAGES) & 1, &abort_s));
+      if (!ok) continue;
+      const uint8_t* sk = smem + st * 2 * TILE;
+      uint8_t* sv = smem + st * 2 * TILE + TILE;
+      const int k0 = tile * PK + part * WK;
+      if (k0 + WK > end) {
+        for (int r = part * WK + lane; r < part * WK + WK; r += 32)
+          if (tile * PK + r >= end) {
+            if (E4M3) {
+#pragma unroll
+              for (int c = 0; c < DH / 16; ++c) {
+                const int line_ = r * DH / 128, chunk = (r * DH % 128) / 16 + c;
+                *reinterpret_cast<uint4*>(sv + line_ * 128 + ((chunk ^ (line_ & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+              }
+            } else {
+              for (int x = 0; x < DH / 64; ++x)
+                for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(sv + x * BOX + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+        __syncwarp();
+        fence_proxy_async_smem();
+      }
+#pragma unroll
+      for (int s16 = 0; s16 < WK / 16; ++s16) {
+        const int kr = part * WK + s16 * 16, kb = tile * PK + kr;      // row in the stage, key
+        if (kb >= end) break;
+        float x[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
+          if (E4M3) {
+            const int r = kr + nt * 8 + key_of(gq), line_ = r * DH / 128;
+#pragma unroll
+            for (int c = 0; c < DH / 64; ++c) {
+              const int chunk = (r * DH % 128) / 16 + 4 * c + tq;
+              const uint4 u = *reinterpret_cast<const uint4*>(sk + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int s = 0; s < 4; ++s) paged_mma<true>(x[nt], q[4 * c + s], e4m3x2_to_f16x2(static_cast<uint16_t>(w[s])), e4m3x2_to_f16x2(static_cast<uint16_t>(w[s] >> 16)));
+            }
+          } else {
+            const int r = kr + nt * 8 + (lane & 7);
+#pragma unroll
+            for (int kk = 0; kk < DH / 16; kk += 2) {
+              uint32_t w[4];
+              const int c = (kk & 3) * 2 + (lane >> 3);
+              paged_ldsm(w, smem_u32(sk) + (kk >> 2) * BOX + r * 128 + ((c ^ (r & 7)) << 4));
+              paged_mma<false>(x[nt], q[kk], w[0], w[1]);
+              paged_mma<false>(x[nt], q[kk + 1], w[2], w[3]);
+            }
+          }
+        }
+        float mul[2] = {sl2[0], sl2[1]}, into = 1.f;
+        if (E4M3) {
+          const uchar2 sc = scales[st][kr / 16];
+          const float ks = scale_value(sc.x);
+          mul[0] *= ks;
+          mul[1] *= ks;
+          if (sc.y > unit) {                // the same in the whole warp
+            const float f = scale_inverse(127 + min(sc.y - unit, 126));
+            if (unit != 0) {
+#pragma unroll
+              for (int d = 0; d < DN; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][e] *= f;
+            }
+            unit = sc.y;
+          }
+          into = scale_inverse(127 + min(unit - sc.y, 126));
+        }
+        const bool whole = kb + 15 <= start && kb + 16 <= end;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[nt][e] *= mul[e >> 1];
+            if (!whole) {
+              const int j = kb + nt * 8 + key_of(2 * tq + (e & 1));
+              if (!(j <= p_row[e >> 1] && j < end)) x[nt][e] = -INFINITY;
+            }
+          }
+        float f[2];
+        bool raise = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = paged_max(paged_max(x[0][2 * h], x[0][2 * h + 1]), paged_max(x[1][2 * h], x[1][2 * h + 1]));
+          top = paged_max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = paged_max(top, __shfl_xor_sync(0xffffffffu, top, 2)) - ABOVE;
+          // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept
+          f[h] = 1.f;
+          if (!(top <= m[h] + 8.f)) {
+            f[h] = exp2f(m[h] - top);
+            m[h] = paged_max(m[h], top);
+            raise = true;
+          }
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          l[0] *= f[0];
+          l[1] *= f[1];
+#pragma unroll
+          for (int d = 0; d < DN; ++d) {
+            o[d][0] *= f[0];
+            o[d][1] *= f[0];
+            o[d][2] *= f[1];
+            o[d][3] *= f[1];
+          }
+        }
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float mr = m[h] == -INFINITY ? 0.f : m[h];
+            const float p0 = ex2_approx(x[nt][2 * h] - mr), p1 = ex2_approx(x[nt][2 * h + 1] - mr);
+            l[h] += p0 + p1;
+            if (E4M3) {
+              ph[nt * 2 + h] = pack_f16x2(p0 * into, p1 * into);
+            } else {
+              ph[nt * 2 + h] = pack_bf16x2(p0, p1);
+              const float2 back = unpack_bf16x2(ph[nt * 2 + h]);
+              pl[nt * 2 + h] = pack_bf16x2(p0 - back.x, p1 - back.y);
+            }
+          }
+        if (E4M3) {
+          // tiles 2 c and 2 c + 1 hold the even and the odd ones of the columns 16 c .. 16 c + 15
+          const int r = kr + (lane & 8) + key_of(lane & 7), line_ = r * DH / 128;
+#pragma unroll
+          for (int c = 0; c < DH / 16; c += 2) {
+            uint32_t w[4];
+            const int chunk = (r * DH % 128) / 16 + c + (lane >> 4);
+            paged_ldsm_t(w, smem_u32(sv) + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t b0 = __byte_perm(w[2 * y], 0, 0x3120), b1 = __byte_perm(w[2 * y + 1], 0, 0x3120);
+              paged_mma<true>(o[2 * (c + y)], ph, e4m3x2_to_f16x2(static_cast<uint16_t>(b0)), e4m3x2_to_f16x2(static_cast<uint16_t>(b1)));
+              paged_mma<true>(o[2 * (c + y) + 1], ph, e4m3x2_to_f16x2(static_cast<uint16_t>(b0 >> 16)), e4m3x2_to_f16x2(static_cast<uint16_t>(b1 >> 16)));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < DN; d += 2) {
+            uint32_t w[4];
+            const int r = kr + (lane & 15), c = (d & 7) + (lane >> 4);
+            paged_ldsm_t(w, smem_u32(sv) + (d >> 3) * BOX + r * 128 + ((c ^ (r & 7)) << 4));
+            paged_mma<false>(o[d], ph, w[0], w[1]);
+            paged_mma<false>(o[d + 1], ph, w[2], w[3]);
+            paged_mma<false>(o[d], pl, w[0], w[1]);
+            paged_mma<false>(o[d + 1], pl, w[2], w[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // the warps' parts meet in shared memory, 32 columns at a time
+    const float whole_unit = E4M3 ? scale_value(unit) : 1.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (tq == 0) {
+        part_m[warp][gq + 8 * h] = m[h];
+        part_l[warp][gq + 8 * h] = l[h];
+      }
+    }
+    const bool complete = first_tile == 0 && count == at.tiles;
+    const long long slot = 2ll * blockIdx.x + (segment > 0 ? 1 : 0);
+#pragma unroll
+    for (int c0 = 0; c0 < DH; c0 += 32) {
+      float* mine = slab + warp * 16 * 32 + gq * 32;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        if (E4M3) {
+          const int d = c0 / 8 + 2 * y;       // columns c0 + 16 y + 4 t .. + 3
+          *reinterpret_cast<float4*>(mine + 16 * y + 4 * tq) = make_float4(o[d][0] * whole_unit, o[d + 1][0] * whole_unit, o[d][1] * whole_unit, o[d + 1][1] * whole_unit);
+          *reinterpret_cast<float4*>(mine + 8 * 32 + 16 * y + 4 * tq) = make_float4(o[d][2] * whole_unit, o[d + 1][2] * whole_unit, o[d][3] * whole_unit, o[d + 1][3] * whole_unit);
+        } else {
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const int d = c0 / 8 + 2 * y + z;
+            *reinterpret_cast<float2*>(mine + 16 * y + 8 * z + 2 * tq) = make_float2(o[d][0], o[d][1]);
+            *reinterpret_cast<float2*>(mine + 8 * 32 + 16 * y + 8 * z + 2 * tq) = make_float2(o[d][2], o[d][3]);
+          }
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int e = threadIdx.x; e < rows * 8; e += 128) {
+        const int r = e >> 3, w0 = (r / 16) * PER_TILE, rr = r % 16, c = (e & 7) * 4;
+        float top = part_m[w0][rr];
+#pragma unroll
+        for (int w = 1; w < PER_TILE; ++w) top = paged_max(top, part_m[w0 + w][rr]);
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < PER_TILE; ++w) {
+          const float f = part_m[w0 + w][rr] == -INFINITY ? 0.f : exp2f(part_m[w0 + w][rr] - top);
+          const float4 v = *reinterpret_cast<const float4*>(slab + (w0 + w) * 16 * 32 + rr * 32 + c);
+          s.x += f * v.x;
+          s.y += f * v.y;
+          s.z += f * v.z;
+          s.w += f * v.w;
+          sum += f * part_l[w0 + w][rr];
+        }
+        if (!ok) continue;
+        if (complete) {
+          const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+          uint2 w;
+          w.x = pack_bf16x2(s.x * inv, s.y * inv);
+          w.y = pack_bf16x2(s.z * inv, s.w * inv);
+          if (top == -INFINITY) w = make_uint2(0, 0);
+          *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.o) + b * a.o_strides[0] + (r / rep) * a.o_strides[1] + (g * rep + r % rep) * a.o_strides[2] + c0 + c) = w;
+        } else {
+          *reinterpret_cast<float4*>(parts.sums + (slot * ROWS + r) * DH + c0 + c) = s;
+          if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(parts.tops + (slot * ROWS + r) * 2) = make_float2(top, sum);
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+    at.t = first_tile + count;
+    if (at.t == at.tiles) at.next_segment(a);
+  }
+  if (!ok && lane == 0) report_status(pg.status, STATUS_TIMEOUT, 184, n);
 }
 
-template <int DH, bool E4M3>
-__global__ void __launch_bounds__(PT_THREADS) paged_rows_kernel(const __grid_constant__ MdbPagedAttnArgs a) {
-  constexpr int LANES = DH / 16, GROUPS = PT_THREADS / LANES;
-  __shared__ float part_m[GROUPS], part_l[GROUPS], part_o[GROUPS][DH];
-  const MdbPages& p = a.pages;
-  const int l = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int h = blockIdx.x % a.H, i = blockIdx.x / a.H, b = blockIdx.y, g = h / (a.H / p.Hkv);
-  const int length = min(max(a.kv_len[b], 0), p.most), keys = max(length - a.Sq + i + 1, 0);
-  float q[16], o[16], m = -INFINITY, sum = 0.f;
-  load16<false>(q, a.q, b * a.q_strides[0] + i * a.q_strides[1] + h * a.q_strides[2] + l * 16);
-#pragma unroll
-  for (int e = 0; e < 16; ++e) o[e] = 0.f;
-  for (int j0 = 0; j0 < keys; j0 += GROUPS) {
-    const int j = j0 + group;
-    const int page = j < keys ? page_of(p, b, j / p.P) : -1;
-    if (page < 0 && j < keys) report_status(p.status, STATUS_BOUNDS, 182, b);
-    float s = 0.f, x[16];
-    if (page >= 0) {
-      load16<E4M3>(x, p.k, page * p.k_strides[0] + g * p.k_strides[1] + (j % p.P) * DH + l * 16);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s = fmaf(q[e], x[e], s);
-    }
-#pragma unroll
-    for (int n = LANES / 2; n > 0; n >>= 1) s += __shfl_xor_sync(0xffffffffu, s, n);
-    if (page < 0) continue;
-    s *= a.scale * 1.4426950408889634f;
-    if (E4M3) s *= scale_value(p.k_scale[page * p.scale_strides[0] + g]);
-    float top, w;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(m), "f"(s));
-    const float f = m == -INFINITY ? 0.f : exp2f(m - top);
-    w = top == -INFINITY ? 0.f : exp2f(s - top);
-    m = top;
-    sum = sum * f + w;
-    load16<E4M3>(x, p.v, page * p.v_strides[0] + g * p.v_strides[1] + (j % p.P) * DH + l * 16);
-    if (E4M3) w *= scale_value(p.v_scale[page * p.scale_strides[1] + g]);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = o[e] * f + w * x[e];
+// One row of one sequence per block: the parts of its key head, in order. Rows of sequences without keys are zero.
+constexpr int PJ_THREADS = 128;
+template <int DH>
+__global__ void __launch_bounds__(PJ_THREADS)
+paged_join_kernel(const __grid_constant__ MdbPagedAttnArgs a, const PagedParts parts, const int grid, const int part_rows) {
+  constexpr int LANES = DH / 4, GROUPS = PJ_THREADS / LANES;
+  __shared__ float tops[GROUPS], sums[GROUPS], slab[GROUPS][DH];
+  const int lane = threadIdx.x & 31, b = blockIdx.y, h = blockIdx.x % a.H, i = blockIdx.x / a.H, rep = a.H / a.pages.Hkv, g = h / rep, r = i * rep + h % rep;
+  const int c = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  long long before = 0, total = 0;                    // tiles of a key head before this sequence, in all
+  for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
+    const unsigned n = b0 + lane < a.pages.B ? static_cast<unsigned>(paged_length(a, b0 + lane) + PK - 1) / PK : 0u;
+    total += __reduce_add_sync(0xffffffffu, n);
+    before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0u);
   }
-  if (l == 0) {
-    part_m[group] = m;
-    part_l[group] = sum;
+  const int tiles = (paged_length(a, b) + PK - 1) / PK;
+  const long long line = total * a.pages.Hkv, u0 = before * a.pages.Hkv + static_cast<long long>(g) * tiles, u1 = u0 + tiles;
+  const long long ctas = min(static_cast<long long>(grid), line);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + b * a.o_strides[0] + i * a.o_strides[1] + h * a.o_strides[2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // by all: this kernel must not end before the one whose parts it joins
+  if (tiles == 0) {
+    for (int d = threadIdx.x; d < DH / 8; d += PJ_THREADS) *reinterpret_cast<uint4*>(out + d * 8) = make_uint4(0, 0, 0, 0);
+    return;
   }
-#pragma unroll
-  for (int e = 0; e < 16; ++e) part_o[group][l * 16 + e] = o[e];
+  // CTA k has the tiles from line k / ctas on
+  const long long first = ((u0 + 1) * ctas - 1) / line, last = (u1 * ctas - 1) / line;
+  if (first == last) return;
+  float top = -INFINITY, sum = 0.f;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (long long k = first + group; k <= last; k += GROUPS) {
+    const long long slot = 2 * k + (k == first && line * k / ctas != u0 ? 1 : 0);
+    const float2 ml = *reinterpret_cast<const float2*>(parts.tops + (slot * part_rows + r) * 2);
+    const float4 v = *reinterpret_cast<const float4*>(parts.sums + (slot * part_rows + r) * DH + c * 4);
+    if (ml.x == -INFINITY) continue;
+    const float up = paged_max(top, ml.x), f = top == -INFINITY ? 0.f : exp2f(top - up), w = exp2f(ml.x - up);
+    s.x = s.x * f + v.x * w;
+    s.y = s.y * f + v.y * w;
+    s.z = s.z * f + v.z * w;
+    s.w = s.w * f + v.w * w;
+    sum = sum * f + ml.y * w;
+    top = up;
+  }
+  if (c == 0) {
+    tops[group] = top;
+    sums[group] = sum;
+  }
+  *reinterpret_cast<float4*>(&slab[group][c * 4]) = s;
   __syncthreads();
-  for (int d = threadIdx.x; d < DH; d += PT_THREADS) {
-    float top = -INFINITY, total = 0.f, v = 0.f;
-    for (int n = 0; n < GROUPS; ++n) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(part_m[n]));
-    for (int n = 0; n < GROUPS; ++n) {
-      const float f = part_m[n] == -INFINITY ? 0.f : exp2f(part_m[n] - top);
-      total += f * part_l[n];
-      v += f * part_o[n][d];
-    }
-    static_cast<__nv_bfloat16*>(a.o)[b * a.o_strides[0] + i * a.o_strides[1] + h * a.o_strides[2] + d] = __float2bfloat16_rn(top == -INFINITY || total == 0.f ? 0.f : v / total);
+  if (group > 0) return;
+  top = tops[0];
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) top = paged_max(top, tops[k]);
+  sum = 0.f;
+  s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const float w = tops[k] == -INFINITY ? 0.f : exp2f(tops[k] - top);
+    const float4 v = *reinterpret_cast<const float4*>(&slab[k][c * 4]);
+    s.x += w * v.x;
+    s.y += w * v.y;
+    s.z += w * v.z;
+    s.w += w * v.w;
+    sum += w * sums[k];
   }
+  uint2 w = make_uint2(0, 0);
+  if (top != -INFINITY) {
+    const float inv = 1.f / sum;
+    w = make_uint2(pack_bf16x2(s.x * inv, s.y * inv), pack_bf16x2(s.z * inv, s.w * inv));
+  }
+  *reinterpret_cast<uint2*>(out + c * 4) = w;
 }
 
+static int pages_map(CUtensorMap* m, const void* pool, const MdbPages& p, const long long* strides, bool e4m3) {
+  if (e4m3) {      // lines of 128 bytes: a key of 128, two of 64
+    const int lines = p.P * p.Dh / 128;
+    int64_t ext[4] = {128, lines, p.Hkv, p.count};
+    int64_t str[4] = {1, 128, strides[1], strides[0]};
+    int box[4] = {128, std::min(p.P, PK) * p.Dh / 128, 1, 1};
+    return mdb_make_tmap(m, pool, 1, 4, ext, str, box, 1);
+  }
+  int64_t ext[4] = {p.Dh, p.P, p.Hkv, p.count};
+  int64_t str[4] = {2, p.Dh * 2, strides[1] * 2, strides[0] * 2};
+  int box[4] = {64, std::min(p.P, PK), 1, 1};
+  return mdb_make_tmap(m, pool, 2, 4, ext, str, box, 1);
+}
+
+static int step_rows(const MdbPagedAttnArgs& a) { return (a.Sq * (a.H / a.pages.Hkv) + 15) / 16 * 16; }
+// Two CTAs per SM, or one per tile where there are fewer
+static int step_ctas(const MdbPagedAttnArgs& a) {
+  const long long tiles = static_cast<long long>(a.pages.B) * a.pages.Hkv * ((a.pages.most + PK - 1) / PK);
+  return static_cast<int>(std::max(1ll, std::min(tiles, 2ll * device_sm_count())));
+}
+static int step_tiles(const MdbPagedAttnArgs& a) { return step_rows(a) <= 16 ? 1 : step_rows(a) <= 32 ? 2 : 4; }
+
+template <int DH, bool E4M3, int MT>
+static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStream_t st) {
+  auto kern = paged_step_kernel<DH, E4M3, MT>;
+  static bool ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DH, E4M3>::BYTES);
+    if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  }
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int ctas = step_ctas(a);
+  const PagedParts parts = {a.ws, a.ws + 2ll * ctas * 16 * MT * DH};
+  kern<<<ctas, PS_THREADS, PagedShape<DH, E4M3>::BYTES, st>>>(maps, a, parts);
+  if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t c;
+  memset(&c, 0, sizeof(c));
+  c.gridDim = dim3(a.Sq * a.H, a.pages.B);
+  c.blockDim = dim3(PJ_THREADS);
+  c.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&c, paged_join_kernel<DH>, a, parts, ctas, 16 * MT));
+}
 template <int DH, bool E4M3>
 static int launch_paged(const MdbPagedAttnArgs& a, cudaStream_t st) {
-  paged_rows_kernel<DH, E4M3><<<dim3(a.Sq * a.H, a.pages.B), PT_THREADS, 0, st>>>(a);
-  return static_cast<int>(cudaGetLastError());
+  PagedMaps maps;
+  int r = pages_map(&maps.k, a.pages.k, a.pages, a.pages.k_strides, E4M3);
+  if (r) return 2000 + r;
+  r = pages_map(&maps.v, a.pages.v, a.pages, a.pages.v_strides, E4M3);
+  if (r) return 3000 + r;
+  const int mt = step_tiles(a);
+  return mt == 1 ? launch_step<DH, E4M3, 1>(maps, a, st) : mt == 2 ? launch_step<DH, E4M3, 2>(maps, a, st) : launch_step<DH, E4M3, 4>(maps, a, st);
+}
+
+// ---- parts of prompts: the pages in one piece, for the kernels of whole prompts ----
+template <int DH, bool E4M3>
+__global__ void __launch_bounds__(256)
+paged_gather_kernel(const __grid_constant__ MdbPagedAttnArgs a, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v, int* __restrict__ lengths) {
+  const MdbPages& pg = a.pages;
+  constexpr int LANES = DH / 16;
+  const int b = blockIdx.y, length = paged_length(a, b), per_key = pg.Hkv * LANES;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    lengths[b] = length;
+    lengths[pg.B + b] = length - a.Sq;
+  }
+  for (long long e = blockIdx.x * 256ll + threadIdx.x; e < static_cast<long long>(length) * per_key; e += gridDim.x * 256ll) {
+    const int j = static_cast<int>(e / per_key), rest = static_cast<int>(e - static_cast<long long>(j) * per_key), g = rest / LANES, c = rest % LANES * 16;
+    const int page = page_of(pg, b, j / pg.P);
+    if (page < 0) report_status(pg.status, STATUS_BOUNDS, 185, b);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (page >= 0) {
+        const long long* s = kv ? pg.v_strides : pg.k_strides;
+        const long long from = page * s[0] + g * s[1] + (j % pg.P) * DH + c;
+        if (E4M3) {
+          const float f = scale_value((kv ? pg.v_scale : pg.k_scale)[page * pg.scale_strides[kv] + g]);
+          const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(kv ? pg.v : pg.k) + from);
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+          uint32_t* to = reinterpret_cast<uint32_t*>(u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 lo = e4m3x2_to_float2(static_cast<uint16_t>(ws[i])), hi = e4m3x2_to_float2(static_cast<uint16_t>(ws[i] >> 16));
+            to[2 * i] = pack_bf16x2(lo.x * f, lo.y * f);
+            to[2 * i + 1] = pack_bf16x2(hi.x * f, hi.y * f);
+          }
+        } else {
+          const uint4* w = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(kv ? pg.v : pg.k) + from);
+          u[0] = w[0];
+          u[1] = w[1];
+        }
+      }
+      uint4* to = reinterpret_cast<uint4*>((kv ? v : k) + ((static_cast<long long>(b) * pg.most + j) * pg.Hkv + g) * DH + c);
+      to[0] = u[0];
+      to[1] = u[1];
+    }
+  }
+}
+
+static bool is_step(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.Sq) * (a.H / a.pages.Hkv) <= 64; }
+static long long gathered(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.pages.B) * a.pages.most * a.pages.Hkv * a.pages.Dh; }      // values
+
+template <int DH, bool E4M3>
+static int launch_gathered(const MdbPagedAttnArgs& a, cudaStream_t st) {
+  const MdbPages& p = a.pages;
+  __nv_bfloat16* k = reinterpret_cast<__nv_bfloat16*>(a.ws);
+  __nv_bfloat16* v = k + gathered(a);
+  int* lengths = reinterpret_cast<int*>(v + gathered(a));
+  const long long blocks = (static_cast<long long>(p.most) * p.Hkv * (DH / 16) + 255) / 256;
+  paged_gather_kernel<DH, E4M3><<<dim3(static_cast<unsigned>(std::min(blocks, 8ll * device_sm_count())), p.B), 256, 0, st>>>(a, k, v, lengths);
+  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return static_cast<int>(e);
+  MdbTextAttnArgs t;
+  memset(&t, 0, sizeof(t));
+  t.q = a.q; t.k = k; t.v = v; t.o = a.o;
+  t.kv_len = lengths; t.q_start_ptr = lengths + p.B;
+  for (int i = 0; i < 3; ++i) {
+    t.q_strides[i] = a.q_strides[i];
+    t.o_strides[i] = a.o_strides[i];
+  }
+  t.k_strides[2] = t.v_strides[2] = DH;
+  t.k_strides[1] = t.v_strides[1] = static_cast<long long>(p.Hkv) * DH;
+  t.k_strides[0] = t.v_strides[0] = static_cast<long long>(p.most) * p.Hkv * DH;
+  t.B = p.B; t.H = a.H; t.Hkv = p.Hkv; t.Sq = a.Sq; t.Skv = p.most; t.Dh = DH;
+  t.window = 1 << 30;
+  t.scale = a.scale;
+  t.status = p.status;
+  return mdb_text_attention_fwd(&t, st);
 }
 
 }  // namespace mdb
 
+extern "C" long long mdb_paged_attention_floats(const MdbPagedAttnArgs* a) {
+  if (a->pages.most == 0) return 0;
+  if (!mdb::is_step(*a)) return mdb::gathered(*a) + 2ll * a->pages.B;
+  return 2ll * mdb::step_ctas(*a) * 16 * mdb::step_tiles(*a) * (a->pages.Dh + 2);
+}
 extern "C" int mdb_paged_attention(const MdbPagedAttnArgs* a, cudaStream_t st) {
   const MdbPages& p = a->pages;
-  if (p.B <= 0 || a->Sq <= 0 || p.Hkv <= 0 || a->H % p.Hkv != 0 || (p.P != 16 && p.P != 32 && p.P != 64 && p.P != 128)) return -1;
-  if (p.Dh == 128) return p.k_scale != nullptr ? mdb::launch_paged<128, true>(*a, st) : mdb::launch_paged<128, false>(*a, st);
-  if (p.Dh == 64) return p.k_scale != nullptr ? mdb::launch_paged<64, true>(*a, st) : mdb::launch_paged<64, false>(*a, st);
-  return -2;
+  if (p.B <= 0 || a->Sq <= 0 || p.Hkv <= 0 || p.most <= 0 || a->H % p.Hkv != 0 || (p.P != 16 && p.P != 32 && p.P != 64 && p.P != 128) || (p.Dh != 64 && p.Dh != 128)) return -1;
+  const bool e4m3 = p.k_scale != nullptr;
+  if (!mdb::is_step(*a)) {
+    if (p.Dh == 128) return e4m3 ? mdb::launch_gathered<128, true>(*a, st) : mdb::launch_gathered<128, false>(*a, st);
+    return e4m3 ? mdb::launch_gathered<64, true>(*a, st) : mdb::launch_gathered<64, false>(*a, st);
+  }
+  if (p.Dh == 128) return e4m3 ? mdb::launch_paged<128, true>(*a, st) : mdb::launch_paged<128, false>(*a, st);
+  return e4m3 ? mdb::launch_paged<64, true>(*a, st) : mdb::launch_paged<64, false>(*a, st);
 }
+
+MDB_DEFINE_WAIT_LIMIT_SETTER(mdb_set_wait_limit_paged)
