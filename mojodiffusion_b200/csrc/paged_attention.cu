@@ -3,18 +3,19 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp2(x_ij - m_i),  x_ij = log2(e) scale 2^ek q_i . k_j;  values are in units of 2^ev; ek, ev of the page and head
 //
 // A few queries (at most 64 rows per key head, a row being one query of one head of the group): keys and values are read once and bound the time, so the work is split
-// over keys. All tiles of 64 keys of all sequences and key heads are one line, of which every CTA takes an equal part, wherever that begins and ends: sequences of 1 and
+// over keys. All tiles of 128 keys of all sequences and key heads are one line, of which every CTA takes an equal part, wherever that begins and ends: sequences of 1 and
 // of 100000 tokens share the memory's rate. A CTA's tiles of one sequence and head ("segment") end in an output, or in a part (m, l, o) where other CTAs have tiles of
 // it too; a second, small kernel joins those in order. It is launched with the first one and waits for its end.
 //
 // A warp of its own starts the copies: it knows the pages of the next 32 places of the table and their scales, and brings K and V of a tile in by TMA, one box
-// per page. Four warps multiply, with mma.sync m16n8k16: 16 rows are all there is to multiply, a 128-row tcgen05 tile would be mostly padding.
+// per page. Four warps multiply, with mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the keys and the columns of V fill the 16 and the rows, of which there
+// are few, the 8. (A 128-row tcgen05 tile would be mostly padding.) Each warp has 32 keys at a time; where there are more than 16 rows the warps share out those.
 //
 // 8 bits: e4m3 values are exact in f16, and two of them take one conversion, so the products are f16 ones. Of a key's row a lane reads 16 bytes as they lie; which
 // of them are columns 2t, 2t + 1 of a k-step is free as long as the queries' registers use the same order, and so no byte is moved. For values ldmatrix transposes pairs of bytes,
-// one byte permutation makes two columns of them. Queries are brought to [1, 2) by a power of two per row, which leaves them exact but for those 2^-24 of the row's largest.
-// Probabilities are rounded to f16 (2^-11, where the output's rounding is 2^-8); the reference is kept 2^7 above the largest so that also those of 2^-21 of it
-// have all their bits. The powers of two of values go into the probabilities, relative to the largest met so far.
+// and one byte permutation makes two columns of them. Queries are brought to [1, 2) by a power of two per row, which leaves them exact but for those below 2^-14 of
+// the row's largest (2^-25 of it at most). Probabilities are rounded to f16 (2^-11, where the output's rounding is 2^-8); the reference is kept 2^7 below the first maximum, so
+// that also probabilities of 2^-21 have all their bits. The powers of two of values go into the probabilities, relative to the largest met so far.
 // bf16: the products are bf16 ones; a probability goes into its product as two bf16 terms, so only the output is rounded.
 //
 // Keys behind the sequence's end are masked and their values zeroed in shared memory before the product (0 * NaN is not 0).
@@ -26,7 +27,7 @@
 
 namespace mdb {
 
-constexpr int PK = 64;                                        // keys of a tile
+constexpr int PK = 128;                                       // keys of a tile
 constexpr int PS_WARPS = 4, PS_THREADS = (PS_WARPS + 1) * 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
@@ -37,7 +38,7 @@ struct alignas(64) PagedMaps {
 template <int DH, bool E4M3> struct PagedShape {
   static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
   static constexpr int STAGES = 96 * 1024 / (2 * TILE);               // 96 KB, so that two CTAs share an SM
-  static constexpr int SLAB = PS_WARPS * 16 * 32 * 4;                 // 32 columns of the warps' parts
+  static constexpr int SLAB = PS_WARPS * 16 * 32 * 4;                 // 32 columns of the warps' parts, at most 16 rows each
   static constexpr int BYTES = STAGES * 2 * TILE + SLAB + 1024;
 };
 
@@ -59,6 +60,11 @@ template <bool F16> __device__ __forceinline__ void paged_mma(float (&c)[4], con
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t paged_transpose(uint32_t x) {      // an 8 x 8 matrix of 16-bit elements over the warp
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -124,21 +130,21 @@ struct PagedParts {
   float* sums; float* tops;
 };
 
-// MT: tiles of 16 rows
-template <int DH, bool E4M3, int MT>
+// A warp has NT tiles of 8 rows; RG warps share the rows, and the others the keys of a tile
+template <int DH, bool E4M3, int NT, int RG>
 __global__ void __launch_bounds__(PS_THREADS, 2)
 paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ MdbPagedAttnArgs a, const PagedParts parts) {
   using Shape = PagedShape<DH, E4M3>;
   constexpr int TILE = Shape::TILE, STAGES = Shape::STAGES, BOX = PK * 128;
-  constexpr int ROWS = 16 * MT, PER_TILE = PS_WARPS / MT, WK = PK / PER_TILE;      // warps that share the keys of a tile, and keys of a warp
-  constexpr int DN = DH / 8;                                                       // n-tiles of 8 columns
-  constexpr float ABOVE = E4M3 ? 7.f : 0.f;                                        // the reference stays so far below the first maximum
+  constexpr int WR = 8 * NT, ROWS = WR * RG, PER_TILE = PS_WARPS / RG, WK = PK / PER_TILE;      // rows of a warp, of all; warps that share the keys, and keys of a warp
+  constexpr int DM = DH / 16;                                                                   // tiles of 16 columns
+  constexpr float ABOVE = E4M3 ? 7.f : 0.f;                                                     // the reference stays so far below the first maximum
 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ uchar2 scales[STAGES][PK / 16];
   __shared__ int abort_s;
-  __shared__ float part_m[PS_WARPS][16], part_l[PS_WARPS][16];
+  __shared__ float part_m[PS_WARPS][WR], part_l[PS_WARPS][WR];
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   float* slab = reinterpret_cast<float*>(smem + STAGES * 2 * TILE);
 
@@ -190,7 +196,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       }
       const int keys = min(at.length - at.t * PK, PK), boxes = (keys + rows - 1) / rows;
       if (E4M3) {
-        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 3) * 16) / pg.P - window) & 31);
+        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 7) * 16) / pg.P - window) & 31);
         if (lane < PK / 16) scales[st][lane] = make_uchar2(s & 255, s >> 8);
       }
       const int mine = __shfl_sync(0xffffffffu, page, (first_index - window + min(lane, per_tile - 1)) & 31);
@@ -228,70 +234,82 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
     return;
   }
 
-  const int mt = warp / PER_TILE, part = warp % PER_TILE;
-  const int tq = lane & 3, gq = lane >> 2;                            // rows mt * 16 + gq and 8 more
+  const int rg = warp / PER_TILE, part = warp % PER_TILE;
+  const int tq = lane & 3, gq = lane >> 2;
   const int rep = a.H / pg.Hkv, rows = rep * a.Sq;
+  // Key j of a group of eight lies in this row of the stage: with a row of 128 bytes, lanes that read 16 bytes each at once then hit all banks (see the swizzle).
+  const auto key_of = [](int j) { return E4M3 && DH == 128 ? (j >> 1) + 4 * (j & 1) : j; };
   bool ok = true;
   for (int i = 0, segment = 0; i < n; ++segment) {
     const int b = at.b, g = at.g, first_tile = at.t, end = at.length, start = end - a.Sq;
     const int count = min(at.tiles - first_tile, n - i);
-    uint32_t q[DH / 16][4];
-    float sl2[2];
+    uint32_t q[NT][DH / 16][2];
+    float sl2[NT][2];                                                   // of the rows 2 t, 2 t + 1 of a tile of 8, whose scores this lane has
+    int p_row[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = mt * 16 + gq + 8 * h;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = rg * WR + nt * 8 + gq;
       const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_strides[0] + (r / rep) * a.q_strides[1] + (g * rep + r % rep) * a.q_strides[2];
-      sl2[h] = a.scale * PAGED_LOG2E;
+      float mine = a.scale * PAGED_LOG2E;
       if (E4M3) {
         // k-step 4 c + s: columns 16 (4 c + t) + 4 s .. + 3 belong to lane t
-        uint32_t w[DH / 16][2];
         float most = 0.f;
 #pragma unroll
         for (int c = 0; c < DH / 64; ++c)
 #pragma unroll
-          for (int s = 0; s < 4; s += 2) {
-            const uint4 u = r < rows ? *reinterpret_cast<const uint4*>(p + 16 * (4 * c + tq) + 4 * s) : make_uint4(0, 0, 0, 0);
-            w[4 * c + s][0] = u.x;
-            w[4 * c + s][1] = u.y;
-            w[4 * c + s + 1][0] = u.z;
-            w[4 * c + s + 1][1] = u.w;
+          for (int x = 0; x < 4; x += 2) {
+            const uint4 u = r < rows ? *reinterpret_cast<const uint4*>(p + 16 * (4 * c + tq) + 4 * x) : make_uint4(0, 0, 0, 0);
+            q[nt][4 * c + x][0] = u.x;
+            q[nt][4 * c + x][1] = u.y;
+            q[nt][4 * c + x + 1][0] = u.z;
+            q[nt][4 * c + x + 1][1] = u.w;
           }
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float2 f = unpack_bf16x2(w[kk][e]);
+            const float2 f = unpack_bf16x2(q[nt][kk][e]);
             most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));      // NaN and infinity come through by themselves
           }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 1), 253);
         const float f = scale_inverse(e);
-        sl2[h] *= scale_value(e);
+        mine *= scale_value(e);
 #pragma unroll
-        for (int kk = 0; kk < DH / 16; ++kk) {
-          const float2 x = unpack_bf16x2(w[kk][0]), y = unpack_bf16x2(w[kk][1]);
-          q[kk][h] = pack_f16x2(x.x * f, x.y * f);
-          q[kk][h + 2] = pack_f16x2(y.x * f, y.y * f);
-        }
+        for (int kk = 0; kk < DH / 16; ++kk)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float2 x = unpack_bf16x2(q[nt][kk][y]);
+            q[nt][kk][y] = pack_f16x2(x.x * f, x.y * f);
+          }
       } else {
 #pragma unroll
         for (int kk = 0; kk < DH / 16; ++kk) {
-          q[kk][h] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq) : 0u;
-          q[kk][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq + 8) : 0u;
+          q[nt][kk][0] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq) : 0u;
+          q[nt][kk][1] = r < rows ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * tq + 8) : 0u;
         }
       }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        sl2[nt][y] = __shfl_sync(0xffffffffu, mine, 4 * (2 * tq + y));
+        p_row[nt][y] = start + (rg * WR + nt * 8 + 2 * tq + y) / rep;
+      }
     }
-    const int p_row[2] = {start + (mt * 16 + gq) / rep, start + (mt * 16 + gq + 8) / rep};
-    float o[DN][4];
+    float o[DM][NT][4];
 #pragma unroll
-    for (int d = 0; d < DN; ++d)
+    for (int d = 0; d < DM; ++d)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][nt][e] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
     int unit = 0;                                                      // byte of the power of two that o is in units of
-    // key j of a group of eight lies in this row of the stage: lanes that read 16 bytes each at once then hit all banks (see the swizzle)
-    const auto key_of = [](int j) { return E4M3 && DH == 128 ? (j >> 1) + 4 * (j & 1) : j; };
 
     for (int tile = first_tile; tile < first_tile + count; ++tile, ++i) {
       const int st = i % STAGES;
@@ -299,151 +317,179 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       if (!ok) continue;
       const uint8_t* sk = smem + st * 2 * TILE;
       uint8_t* sv = smem + st * 2 * TILE + TILE;
-      const int k0 = tile * PK + part * WK;
-      if (k0 + WK > end) {
-        for (int r = part * WK + lane; r < part * WK + WK; r += 32)
-          if (tile * PK + r >= end) {
+#pragma unroll 1
+      for (int k32 = part * WK; k32 < part * WK + WK; k32 += 32) {      // row in the stage
+        const int kb = tile * PK + k32;                                 // key
+        if (kb >= end) break;
+        if (kb + 32 > end) {
+          const int r = k32 + lane;
+          if (kb + lane >= end) {
             if (E4M3) {
+              const int line_ = r * DH / 128, chunk = (r * DH % 128) / 16;
 #pragma unroll
-              for (int c = 0; c < DH / 16; ++c) {
-                const int line_ = r * DH / 128, chunk = (r * DH % 128) / 16 + c;
-                *reinterpret_cast<uint4*>(sv + line_ * 128 + ((chunk ^ (line_ & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-              }
+              for (int c = 0; c < DH / 16; ++c) *reinterpret_cast<uint4*>(sv + line_ * 128 + (((chunk + c) ^ (line_ & 7)) << 4)) = make_uint4(0, 0, 0, 0);
             } else {
               for (int x = 0; x < DH / 64; ++x)
                 for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(sv + x * BOX + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
             }
           }
-        __syncwarp();
-        fence_proxy_async_smem();
-      }
+          __syncwarp();
+          fence_proxy_async_smem();
+        }
+        // S^T of 2 x 16 keys: this lane has keys gq and gq + 8, rows 2 t and 2 t + 1
+        float x[2][NT][4];
 #pragma unroll
-      for (int s16 = 0; s16 < WK / 16; ++s16) {
-        const int kr = part * WK + s16 * 16, kb = tile * PK + kr;      // row in the stage, key
-        if (kb >= end) break;
-        float x[2][4];
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
+            for (int e = 0; e < 4; ++e) x[s][nt][e] = 0.f;
           if (E4M3) {
-            const int r = kr + nt * 8 + key_of(gq), line_ = r * DH / 128;
 #pragma unroll
             for (int c = 0; c < DH / 64; ++c) {
-              const int chunk = (r * DH % 128) / 16 + 4 * c + tq;
-              const uint4 u = *reinterpret_cast<const uint4*>(sk + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              uint32_t w[2][4];
 #pragma unroll
-              for (int s = 0; s < 4; ++s) paged_mma<true>(x[nt], q[4 * c + s], e4m3x2_to_f16x2(static_cast<uint16_t>(w[s])), e4m3x2_to_f16x2(static_cast<uint16_t>(w[s] >> 16)));
+              for (int y = 0; y < 2; ++y) {
+                const int r = k32 + s * 16 + y * 8 + key_of(gq), line_ = r * DH / 128, chunk = (r * DH % 128) / 16 + 4 * c + tq;
+                *reinterpret_cast<uint4*>(w[y]) = *reinterpret_cast<const uint4*>(sk + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
+              }
+#pragma unroll
+              for (int z = 0; z < 4; ++z) {
+                const uint32_t k4[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(w[0][z])), e4m3x2_to_f16x2(static_cast<uint16_t>(w[1][z])),
+                                        e4m3x2_to_f16x2(static_cast<uint16_t>(w[0][z] >> 16)), e4m3x2_to_f16x2(static_cast<uint16_t>(w[1][z] >> 16))};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) paged_mma<true>(x[s][nt], k4, q[nt][4 * c + z][0], q[nt][4 * c + z][1]);
+              }
             }
           } else {
-            const int r = kr + nt * 8 + (lane & 7);
+            const int r = k32 + s * 16 + (lane & 15);
 #pragma unroll
-            for (int kk = 0; kk < DH / 16; kk += 2) {
+            for (int kk = 0; kk < DH / 16; ++kk) {
               uint32_t w[4];
-              const int c = (kk & 3) * 2 + (lane >> 3);
+              const int c = (kk & 3) * 2 + (lane >> 4);
               paged_ldsm(w, smem_u32(sk) + (kk >> 2) * BOX + r * 128 + ((c ^ (r & 7)) << 4));
-              paged_mma<false>(x[nt], q[kk], w[0], w[1]);
-              paged_mma<false>(x[nt], q[kk + 1], w[2], w[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) paged_mma<false>(x[s][nt], w, q[nt][kk][0], q[nt][kk][1]);
             }
           }
         }
-        float mul[2] = {sl2[0], sl2[1]}, into = 1.f;
+        float ks[2] = {1.f, 1.f}, into[2] = {1.f, 1.f};
         if (E4M3) {
-          const uchar2 sc = scales[st][kr / 16];
-          const float ks = scale_value(sc.x);
-          mul[0] *= ks;
-          mul[1] *= ks;
-          if (sc.y > unit) {                // the same in the whole warp
-            const float f = scale_inverse(127 + min(sc.y - unit, 126));
+          const uchar2 sc[2] = {scales[st][k32 / 16], scales[st][k32 / 16 + 1]};
+          const int top = max(sc[0].y, kb + 16 < end ? sc[1].y : 0);
+          if (top > unit) {                // the same in the whole warp
+            const float f = scale_inverse(127 + min(top - unit, 126));
             if (unit != 0) {
 #pragma unroll
-              for (int d = 0; d < DN; ++d)
+              for (int d = 0; d < DM; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[d][e] *= f;
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[d][nt][e] *= f;
             }
-            unit = sc.y;
+            unit = top;
           }
-          into = scale_inverse(127 + min(unit - sc.y, 126));
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            ks[s] = scale_value(sc[s].x);
+            into[s] = scale_inverse(127 + min(unit - sc[s].y, 126));
+          }
         }
-        const bool whole = kb + 15 <= start && kb + 16 <= end;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[nt][e] *= mul[e >> 1];
-            if (!whole) {
-              const int j = kb + nt * 8 + key_of(2 * tq + (e & 1));
-              if (!(j <= p_row[e >> 1] && j < end)) x[nt][e] = -INFINITY;
-            }
-          }
-        float f[2];
+        const bool whole = kb + 31 <= start && kb + 32 <= end;
         bool raise = false;
+        float f[NT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = paged_max(paged_max(x[0][2 * h], x[0][2 * h + 1]), paged_max(x[1][2 * h], x[1][2 * h + 1]));
-          top = paged_max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = paged_max(top, __shfl_xor_sync(0xffffffffu, top, 2)) - ABOVE;
-          // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept
-          f[h] = 1.f;
-          if (!(top <= m[h] + 8.f)) {
-            f[h] = exp2f(m[h] - top);
-            m[h] = paged_max(m[h], top);
-            raise = true;
+        for (int nt = 0; nt < NT; ++nt) {
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[s][nt][e] *= sl2[nt][e & 1] * ks[s];
+              if (!whole) {
+                const int j = kb + s * 16 + key_of(gq) + 8 * (e >> 1);
+                if (!(j <= p_row[nt][e & 1] && j < end)) x[s][nt][e] = -INFINITY;
+              }
+              top[e & 1] = paged_max(top[e & 1], x[s][nt][e]);
+            }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int z = 4; z < 32; z <<= 1) top[y] = paged_max(top[y], __shfl_xor_sync(0xffffffffu, top[y], z));
+            top[y] -= ABOVE;
+            // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept
+            f[nt][y] = 1.f;
+            if (!(top[y] <= m[nt][y] + 8.f)) {
+              f[nt][y] = exp2f(m[nt][y] - top[y]);
+              m[nt][y] = paged_max(m[nt][y], top[y]);
+              raise = true;
+            }
           }
         }
         if (__any_sync(0xffffffffu, raise)) {
-          l[0] *= f[0];
-          l[1] *= f[1];
 #pragma unroll
-          for (int d = 0; d < DN; ++d) {
-            o[d][0] *= f[0];
-            o[d][1] *= f[0];
-            o[d][2] *= f[1];
-            o[d][3] *= f[1];
+          for (int nt = 0; nt < NT; ++nt) {
+            l[nt][0] *= f[nt][0];
+            l[nt][1] *= f[nt][1];
+#pragma unroll
+            for (int d = 0; d < DM; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][nt][e] *= f[nt][e & 1];
           }
         }
-        uint32_t ph[4], pl[4];
+        // P^T as the B operand: keys 2 t, 2 t + 1 (and 8 more) of row gq, which is the transpose of what the lane has
+        uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float mr = m[h] == -INFINITY ? 0.f : m[h];
-            const float p0 = ex2_approx(x[nt][2 * h] - mr), p1 = ex2_approx(x[nt][2 * h + 1] - mr);
-            l[h] += p0 + p1;
-            if (E4M3) {
-              ph[nt * 2 + h] = pack_f16x2(p0 * into, p1 * into);
-            } else {
-              ph[nt * 2 + h] = pack_bf16x2(p0, p1);
-              const float2 back = unpack_bf16x2(ph[nt * 2 + h]);
-              pl[nt * 2 + h] = pack_bf16x2(p0 - back.x, p1 - back.y);
-            }
-          }
-        if (E4M3) {
-          // tiles 2 c and 2 c + 1 hold the even and the odd ones of the columns 16 c .. 16 c + 15
-          const int r = kr + (lane & 8) + key_of(lane & 7), line_ = r * DH / 128;
-#pragma unroll
-          for (int c = 0; c < DH / 16; c += 2) {
-            uint32_t w[4];
-            const int chunk = (r * DH % 128) / 16 + c + (lane >> 4);
-            paged_ldsm_t(w, smem_u32(sv) + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const uint32_t b0 = __byte_perm(w[2 * y], 0, 0x3120), b1 = __byte_perm(w[2 * y + 1], 0, 0x3120);
-              paged_mma<true>(o[2 * (c + y)], ph, e4m3x2_to_f16x2(static_cast<uint16_t>(b0)), e4m3x2_to_f16x2(static_cast<uint16_t>(b1)));
-              paged_mma<true>(o[2 * (c + y) + 1], ph, e4m3x2_to_f16x2(static_cast<uint16_t>(b0 >> 16)), e4m3x2_to_f16x2(static_cast<uint16_t>(b1 >> 16)));
+              const float p0 = ex2_approx(x[s][nt][2 * y] - (m[nt][0] == -INFINITY ? 0.f : m[nt][0])), p1 = ex2_approx(x[s][nt][2 * y + 1] - (m[nt][1] == -INFINITY ? 0.f : m[nt][1]));
+              l[nt][0] += p0;
+              l[nt][1] += p1;
+              if (E4M3) {
+                ph[s][nt][y] = paged_transpose(pack_f16x2(p0 * into[s], p1 * into[s]));
+              } else {
+                const uint32_t h = pack_bf16x2(p0, p1);
+                const float2 back = unpack_bf16x2(h);
+                ph[s][nt][y] = paged_transpose(h);
+                pl[s][nt][y] = paged_transpose(pack_bf16x2(p0 - back.x, p1 - back.y));
+              }
             }
-          }
-        } else {
 #pragma unroll
-          for (int d = 0; d < DN; d += 2) {
-            uint32_t w[4];
-            const int r = kr + (lane & 15), c = (d & 7) + (lane >> 4);
-            paged_ldsm_t(w, smem_u32(sv) + (d >> 3) * BOX + r * 128 + ((c ^ (r & 7)) << 4));
-            paged_mma<false>(o[d], ph, w[0], w[1]);
-            paged_mma<false>(o[d + 1], ph, w[2], w[3]);
-            paged_mma<false>(o[d], pl, w[0], w[1]);
-            paged_mma<false>(o[d + 1], pl, w[2], w[3]);
+        for (int s = 0; s < 2; ++s) {
+          const int kr = k32 + s * 16;
+          if (E4M3) {
+            // a tile's rows gq and gq + 8 are the columns 16 c + 2 gq and 16 c + 2 gq + 1
+            const int r = kr + (lane & 8) + key_of(lane & 7), line_ = r * DH / 128;
+#pragma unroll
+            for (int c = 0; c < DM; c += 2) {
+              uint32_t w[4];
+              const int chunk = (r * DH % 128) / 16 + c + (lane >> 4);
+              paged_ldsm_t(w, smem_u32(sv) + line_ * 128 + ((chunk ^ (line_ & 7)) << 4));
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t b0 = __byte_perm(w[2 * y], 0, 0x3120), b1 = __byte_perm(w[2 * y + 1], 0, 0x3120);
+                const uint32_t v4[4] = {e4m3x2_to_f16x2(static_cast<uint16_t>(b0)), e4m3x2_to_f16x2(static_cast<uint16_t>(b0 >> 16)),
+                                        e4m3x2_to_f16x2(static_cast<uint16_t>(b1)), e4m3x2_to_f16x2(static_cast<uint16_t>(b1 >> 16))};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) paged_mma<true>(o[c + y][nt], v4, ph[s][nt][0], ph[s][nt][1]);
+              }
+            }
+          } else {
+            const int r = kr + (lane & 7) + 8 * (lane >> 4);
+#pragma unroll
+            for (int c = 0; c < DM; ++c) {
+              uint32_t w[4];
+              const int chunk = (c & 3) * 2 + (lane >> 3 & 1);
+              paged_ldsm_t(w, smem_u32(sv) + (c >> 2) * BOX + r * 128 + ((chunk ^ (r & 7)) << 4));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                paged_mma<false>(o[c][nt], w, ph[s][nt][0], ph[s][nt][1]);
+                paged_mma<false>(o[c][nt], w, pl[s][nt][0], pl[s][nt][1]);
+              }
+            }
           }
         }
       }
@@ -454,37 +500,39 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
     // the warps' parts meet in shared memory, 32 columns at a time
     const float whole_unit = E4M3 ? scale_value(unit) : 1.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (tq == 0) {
-        part_m[warp][gq + 8 * h] = m[h];
-        part_l[warp][gq + 8 * h] = l[h];
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int z = 4; z < 32; z <<= 1) l[nt][y] += __shfl_xor_sync(0xffffffffu, l[nt][y], z);
+        if (gq == 0) {
+          part_m[warp][nt * 8 + 2 * tq + y] = m[nt][y];
+          part_l[warp][nt * 8 + 2 * tq + y] = l[nt][y];
+        }
       }
-    }
     const bool complete = first_tile == 0 && count == at.tiles;
     const long long slot = 2ll * blockIdx.x + (segment > 0 ? 1 : 0);
 #pragma unroll
     for (int c0 = 0; c0 < DH; c0 += 32) {
-      float* mine = slab + warp * 16 * 32 + gq * 32;
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        if (E4M3) {
-          const int d = c0 / 8 + 2 * y;       // columns c0 + 16 y + 4 t .. + 3
-          *reinterpret_cast<float4*>(mine + 16 * y + 4 * tq) = make_float4(o[d][0] * whole_unit, o[d + 1][0] * whole_unit, o[d][1] * whole_unit, o[d + 1][1] * whole_unit);
-          *reinterpret_cast<float4*>(mine + 8 * 32 + 16 * y + 4 * tq) = make_float4(o[d][2] * whole_unit, o[d + 1][2] * whole_unit, o[d][3] * whole_unit, o[d + 1][3] * whole_unit);
-        } else {
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const int d = c0 / 8 + 2 * y + z;
-            *reinterpret_cast<float2*>(mine + 16 * y + 8 * z + 2 * tq) = make_float2(o[d][0], o[d][1]);
-            *reinterpret_cast<float2*>(mine + 8 * 32 + 16 * y + 8 * z + 2 * tq) = make_float2(o[d][2], o[d][3]);
+        for (int nt = 0; nt < NT; ++nt) {
+          const float (&v)[4] = o[c0 / 16 + y][nt];
+          float* mine = slab + (warp * WR + nt * 8 + 2 * tq) * 32 + 16 * y;
+          if (E4M3) {
+            *reinterpret_cast<float2*>(mine + 2 * gq) = make_float2(v[0] * whole_unit, v[2] * whole_unit);
+            *reinterpret_cast<float2*>(mine + 32 + 2 * gq) = make_float2(v[1] * whole_unit, v[3] * whole_unit);
+          } else {
+            mine[gq] = v[0];
+            mine[gq + 8] = v[2];
+            mine[32 + gq] = v[1];
+            mine[32 + gq + 8] = v[3];
           }
         }
-      }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int e = threadIdx.x; e < rows * 8; e += 128) {
-        const int r = e >> 3, w0 = (r / 16) * PER_TILE, rr = r % 16, c = (e & 7) * 4;
+        const int r = e >> 3, w0 = (r / WR) * PER_TILE, rr = r % WR, c = (e & 7) * 4;
         float top = part_m[w0][rr];
 #pragma unroll
         for (int w = 1; w < PER_TILE; ++w) top = paged_max(top, part_m[w0 + w][rr]);
@@ -493,7 +541,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
 #pragma unroll
         for (int w = 0; w < PER_TILE; ++w) {
           const float f = part_m[w0 + w][rr] == -INFINITY ? 0.f : exp2f(part_m[w0 + w][rr] - top);
-          const float4 v = *reinterpret_cast<const float4*>(slab + (w0 + w) * 16 * 32 + rr * 32 + c);
+          const float4 v = *reinterpret_cast<const float4*>(slab + ((w0 + w) * WR + rr) * 32 + c);
           s.x += f * v.x;
           s.y += f * v.y;
           s.z += f * v.z;
@@ -608,17 +656,20 @@ static int pages_map(CUtensorMap* m, const void* pool, const MdbPages& p, const 
   return mdb_make_tmap(m, pool, 2, 4, ext, str, box, 1);
 }
 
-static int step_rows(const MdbPagedAttnArgs& a) { return (a.Sq * (a.H / a.pages.Hkv) + 15) / 16 * 16; }
+// rows that the kernel has room for: 8, 16, 32 or 64
+static int step_rows(const MdbPagedAttnArgs& a) {
+  const int rows = a.Sq * (a.H / a.pages.Hkv);
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
 // Two CTAs per SM, or one per tile where there are fewer
 static int step_ctas(const MdbPagedAttnArgs& a) {
   const long long tiles = static_cast<long long>(a.pages.B) * a.pages.Hkv * ((a.pages.most + PK - 1) / PK);
   return static_cast<int>(std::max(1ll, std::min(tiles, 2ll * device_sm_count())));
 }
-static int step_tiles(const MdbPagedAttnArgs& a) { return step_rows(a) <= 16 ? 1 : step_rows(a) <= 32 ? 2 : 4; }
 
-template <int DH, bool E4M3, int MT>
+template <int DH, bool E4M3, int NT, int RG>
 static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStream_t st) {
-  auto kern = paged_step_kernel<DH, E4M3, MT>;
+  auto kern = paged_step_kernel<DH, E4M3, NT, RG>;
   static bool ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -628,7 +679,8 @@ static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStr
   }
   if (e != cudaSuccess) return static_cast<int>(e);
   const int ctas = step_ctas(a);
-  const PagedParts parts = {a.ws, a.ws + 2ll * ctas * 16 * MT * DH};
+  constexpr int ROWS = 8 * NT * RG;
+  const PagedParts parts = {a.ws, a.ws + 2ll * ctas * ROWS * DH};
   kern<<<ctas, PS_THREADS, PagedShape<DH, E4M3>::BYTES, st>>>(maps, a, parts);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t c;
@@ -641,7 +693,7 @@ static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStr
   at.val.programmaticStreamSerializationAllowed = 1;
   c.attrs = &at;
   c.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&c, paged_join_kernel<DH>, a, parts, ctas, 16 * MT));
+  return static_cast<int>(cudaLaunchKernelEx(&c, paged_join_kernel<DH>, a, parts, ctas, ROWS));
 }
 template <int DH, bool E4M3>
 static int launch_paged(const MdbPagedAttnArgs& a, cudaStream_t st) {
@@ -650,8 +702,10 @@ static int launch_paged(const MdbPagedAttnArgs& a, cudaStream_t st) {
   if (r) return 2000 + r;
   r = pages_map(&maps.v, a.pages.v, a.pages, a.pages.v_strides, E4M3);
   if (r) return 3000 + r;
-  const int mt = step_tiles(a);
-  return mt == 1 ? launch_step<DH, E4M3, 1>(maps, a, st) : mt == 2 ? launch_step<DH, E4M3, 2>(maps, a, st) : launch_step<DH, E4M3, 4>(maps, a, st);
+  const int rows = step_rows(a);
+  if (rows == 8) return launch_step<DH, E4M3, 1, 1>(maps, a, st);
+  if (rows == 16) return launch_step<DH, E4M3, 2, 1>(maps, a, st);
+  return rows == 32 ? launch_step<DH, E4M3, 2, 2>(maps, a, st) : launch_step<DH, E4M3, 2, 4>(maps, a, st);
 }
 
 // ---- parts of prompts: the pages in one piece, for the kernels of whole prompts ----
@@ -734,7 +788,7 @@ static int launch_gathered(const MdbPagedAttnArgs& a, cudaStream_t st) {
 extern "C" long long mdb_paged_attention_floats(const MdbPagedAttnArgs* a) {
   if (a->pages.most == 0) return 0;
   if (!mdb::is_step(*a)) return mdb::gathered(*a) + 2ll * a->pages.B;
-  return 2ll * mdb::step_ctas(*a) * 16 * mdb::step_tiles(*a) * (a->pages.Dh + 2);
+  return 2ll * mdb::step_ctas(*a) * mdb::step_rows(*a) * (a->pages.Dh + 2);
 }
 extern "C" int mdb_paged_attention(const MdbPagedAttnArgs* a, cudaStream_t st) {
   const MdbPages& p = a->pages;
