@@ -724,15 +724,23 @@ Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const o
 // ------------------------------------------------------------------------------------------
 #define PAGED_CHECK(cond, ...) TORCH_CHECK_VALUE(cond, "paged cache: ", __VA_ARGS__)
 
-// The pool, which the Python layer has checked for shapes and types; `own`: what keeps copies alive
-MdbPages pages_of(const Tensor& like, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const optional<Tensor>& k_scale, const optional<Tensor>& v_scale,
+bool has(const optional<Tensor>& t) { return t.has_value() && t->defined(); }
+void paged_no_gradient(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts) PAGED_CHECK(!t->requires_grad(), "there is no gradient: call it under torch.no_grad(), or on detached tensors");
+}
+// The pool; `own`: what keeps copies alive. `most`: positions of a sequence, or -1
+MdbPages pages_of(const Tensor& like, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, int64_t B,
                   int64_t most, std::vector<Tensor>& own) {
   MdbPages p;
   memset(&p, 0, sizeof(p));
+  PAGED_CHECK(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes() && v_pages.scalar_type() == k_pages.scalar_type() && k_pages.numel() > 0 && k_pages.size(3) == like.size(-1),
+              "k_pages and v_pages must be [pages, Hkv, P, Dh] of one type, with the tensors' head width");
+  PAGED_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(0) == B && table.device() == like.device(), "block_table must be int32 [B, width] on the tensors' device");
   const int64_t least = k_pages.element_size() == 1 ? 16 : 8;      // 16 bytes
-  PAGED_CHECK(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes() && table.dim() == 2 && table.scalar_type() == at::kInt, "pages [N, Hkv, P, Dh], table int32 [B, width]");
   const auto strides = [&](const Tensor& t, long long (&to)[2]) {
-    PAGED_CHECK(t.device() == like.device() && t.stride(3) == 1 && t.stride(2) == t.size(3) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "pages on the tensors' device, 16-byte aligned");
+    PAGED_CHECK(t.device() == like.device() && t.stride(3) == 1 && t.stride(2) == t.size(3) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                "pages on the tensors' device, the [P, Dh] block of a page and head contiguous, from a 16-byte address on");
     for (int i = 0; i < 2; ++i) {
       to[i] = t.size(i) == 1 ? t.size(2) * t.size(3) : t.stride(i);
       PAGED_CHECK(to[i] > 0 && to[i] % least == 0, "strides of pages and heads must be multiples of 16 bytes");
@@ -740,25 +748,26 @@ MdbPages pages_of(const Tensor& like, const Tensor& k_pages, const Tensor& v_pag
   };
   strides(k_pages, p.k_strides);
   strides(v_pages, p.v_strides);
-  for (int i = 0; i < 4; ++i) PAGED_CHECK(k_pages.size(i) < (i == 0 ? 1ll << 31 : 65536), "fewer than 2^31 pages and 65536 heads");
+  PAGED_CHECK(k_pages.size(0) < 1ll << 31 && k_pages.size(1) < 65536, "fewer than 2^31 pages and 65536 heads");
   if (k_pages.scalar_type() == at::kFloat8_e4m3fn) {
     for (const auto* s : {&k_scale, &v_scale})
-      PAGED_CHECK(s->has_value() && (*s)->scalar_type() == at::kByte && (*s)->dim() == 2 && (*s)->size(0) == k_pages.size(0) && (*s)->size(1) == k_pages.size(1) &&
-                      ((*s)->size(1) == 1 || (*s)->stride(1) == 1) && (*s)->device() == like.device(), "scales must be uint8 [pages, Hkv], contiguous along the heads");
+      PAGED_CHECK(has(*s) && (*s)->scalar_type() == at::kByte && (*s)->dim() == 2 && (*s)->size(0) == k_pages.size(0) && (*s)->size(1) == k_pages.size(1) &&
+                      ((*s)->size(1) == 1 || (*s)->stride(1) == 1) && (*s)->device() == like.device(),
+                  "pages of 8 bits need k_scale and v_scale, uint8 [pages, Hkv], contiguous along the heads, on the tensors' device");
     p.k_scale = k_scale->data_ptr<uint8_t>();
     p.v_scale = v_scale->data_ptr<uint8_t>();
     p.scale_strides[0] = k_scale->stride(0);
     p.scale_strides[1] = v_scale->stride(0);
   } else {
-    PAGED_CHECK(k_pages.scalar_type() == at::kBFloat16 && v_pages.scalar_type() == at::kBFloat16, "pages of bf16 or e4m3");
+    PAGED_CHECK(k_pages.scalar_type() == at::kBFloat16 && !has(k_scale) && !has(v_scale), "pages of bf16 without scales, or of e4m3 with them");
   }
   own.push_back(table.contiguous());
   p.k = k_pages.data_ptr();
   p.v = v_pages.data_ptr();
   p.table = own.back().data_ptr<int>();
   p.count = (int)k_pages.size(0); p.Hkv = (int)k_pages.size(1); p.P = (int)k_pages.size(2); p.Dh = (int)k_pages.size(3);
-  p.B = (int)table.size(0);
-  PAGED_CHECK(table.size(0) < 65536 && table.size(1) < (1ll << 30) / p.P, "fewer than 65536 sequences and 2^30 positions");
+  PAGED_CHECK(B < 65536 && table.size(1) < (1ll << 30) / p.P, "fewer than 65536 sequences and 2^30 positions");
+  p.B = (int)B;
   p.width = (int)table.size(1);
   p.most = (int)std::min<int64_t>(most < 0 ? 1ll << 30 : most, table.size(1) * p.P);
   p.status = status_ptr(like);
@@ -781,10 +790,17 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   own.reserve(16);
   MdbPagedAppendArgs a;
   memset(&a, 0, sizeof(a));
-  PAGED_CHECK(k.is_cuda() && k.dim() == 3 && k.scalar_type() == at::kBFloat16 && v.sizes() == k.sizes() && v.scalar_type() == at::kBFloat16 && k.size(0) < 1ll << 30, "k and v must be bf16 [T, Hkv, Dh], fewer than 2^30 rows");
-  a.pages = pages_of(k, k_pages, v_pages, table, k_scale, v_scale, -1, own);
-  PAGED_CHECK(k.size(1) == a.pages.Hkv && k.size(2) == a.pages.Dh && start.scalar_type() == at::kInt && start.numel() == a.pages.B && cos.sizes() == sin.sizes() && cos.size(1) * 2 == k.size(2) &&
-                  cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, "k, v, start, cos or sin of another shape or type");
+  const auto on = [&](const Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.device() == k.device(); };
+  PAGED_CHECK(k.is_cuda() && k.dim() == 3 && k.scalar_type() == at::kBFloat16 && v.sizes() == k.sizes() && on(v, at::kBFloat16) && k.size(0) < 1ll << 30,
+              "k and v must be bf16 [T, Hkv, Dh] on one device, fewer than 2^30 rows");
+  PAGED_CHECK(start.dim() == 1 && on(start, at::kInt), "start must be int32 [B] on k's device");
+  a.pages = pages_of(k, k_pages, v_pages, table, k_scale, v_scale, start.size(0), -1, own);
+  PAGED_CHECK(k.size(1) == a.pages.Hkv, "the pages have other heads");
+  PAGED_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(1) * 2 == k.size(2) && on(cos, at::kFloat) && on(sin, at::kFloat), "cos and sin must be fp32 [positions, Dh / 2] on k's device");
+  PAGED_CHECK(!has(q_norm) || has(q), "q_norm without q");
+  paged_no_gradient({&k, &v, &k_pages, &v_pages});
+  for (const auto* t : {&q, &q_norm, &k_norm})
+    if (has(*t)) paged_no_gradient({&**t});
   const auto whole = [&](const Tensor& t) {      // contiguous, from a 16-byte address on
     own.push_back(t.contiguous());
     if (reinterpret_cast<uintptr_t>(own.back().data_ptr()) % 16 != 0) own.back() = own.back().clone();
@@ -797,14 +813,15 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   a.cos = static_cast<const float*>(whole(cos));
   a.sin = static_cast<const float*>(whole(sin));
   a.positions = (int)std::min<int64_t>(cos.size(0), 0x7fffffff);
-  if (cu.has_value()) {
-    PAGED_CHECK(cu->scalar_type() == at::kInt && cu->numel() == a.pages.B + 1, "cu_seqlens must be int32 [B + 1]");
+  if (has(cu)) {
+    PAGED_CHECK(on(*cu, at::kInt) && cu->dim() == 1 && cu->size(0) == a.pages.B + 1, "cu_seqlens must be int32 [B + 1] on k's device");
     a.cu = static_cast<const int*>(whole(*cu));
   } else {
     PAGED_CHECK(a.T == a.pages.B, "without cu_seqlens every sequence has one row");
   }
   const auto weight = [&](const optional<Tensor>& w, int& f32) -> const void* {
-    if (!w.has_value()) return nullptr;
+    if (!has(w)) return nullptr;
+    PAGED_CHECK(w->dim() == 1 && w->size(0) == k.size(2) && at::isFloatingType(w->scalar_type()) && w->device() == k.device(), "q_norm and k_norm must be [Dh] on k's device");
     f32 = w->scalar_type() != at::kBFloat16;
     return whole(f32 ? w->to(at::kFloat) : *w);
   };
@@ -812,8 +829,9 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   a.k_norm = weight(k_norm, a.k_norm_f32);
   a.eps = (float)eps;
   optional<Tensor> out;
-  if (q.has_value()) {
-    PAGED_CHECK(q->scalar_type() == at::kBFloat16 && q->dim() == 3 && q->size(0) == a.T && q->size(2) == k.size(2) && q->size(1) % k.size(1) == 0 && q->size(1) < 65536, "q must be bf16 [T, H, Dh]");
+  if (has(q)) {
+    PAGED_CHECK(on(*q, at::kBFloat16) && q->dim() == 3 && q->size(0) == a.T && q->size(2) == k.size(2) && q->size(1) > 0 && q->size(1) % k.size(1) == 0 && q->size(1) < 65536,
+                "q must be bf16 [T, H, Dh] on k's device, with a number of heads that k's divides");
     a.q = paged_rows(*q, a.q_strides, own).data_ptr();
     a.H = (int)q->size(1);
     out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
@@ -821,7 +839,7 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   }
   if (a.T > 0 && a.pages.B > 0) {
     for (const Tensor* t : {&k_pages, &v_pages}) t->unsafeGetTensorImpl()->bump_version();      // as an operation in place
-    if (k_scale.has_value())
+    if (has(k_scale))
       for (const auto* t : {&k_scale, &v_scale}) (*t)->unsafeGetTensorImpl()->bump_version();
     check_rc(mdb_paged_append(&a, cur_stream()), "paged_append");
   } else if (out.has_value()) {
@@ -830,17 +848,20 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   return out;
 }
 
-Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len, double scale, const optional<Tensor>& k_scale,
-                       const optional<Tensor>& v_scale, int64_t max_len) {
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len, optional<double> scale, const optional<Tensor>& k_scale,
+                       const optional<Tensor>& v_scale, optional<int64_t> max_len) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
   std::vector<Tensor> own;
   own.reserve(4);
   MdbPagedAttnArgs a;
   memset(&a, 0, sizeof(a));
-  PAGED_CHECK(q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kBFloat16, "q must be bf16 [B, Sq, H, Dh]");
-  a.pages = pages_of(q, k_pages, v_pages, table, k_scale, v_scale, max_len, own);
-  PAGED_CHECK(q.size(0) == a.pages.B && q.size(3) == a.pages.Dh && q.size(2) % a.pages.Hkv == 0 && q.size(1) < 1ll << 30 && q.size(2) < 65536 && kv_len.scalar_type() == at::kInt &&
-                  kv_len.numel() == a.pages.B, "q or kv_len of another shape or type");
+  PAGED_CHECK(q.is_cuda() && q.dim() == 4 && q.scalar_type() == at::kBFloat16 && q.size(1) < 1ll << 30 && q.size(2) < 65536 && q.size(2) > 0, "q must be bf16 [B, Sq, H, Dh]");
+  a.pages = pages_of(q, k_pages, v_pages, table, k_scale, v_scale, q.size(0), max_len.has_value() ? *max_len : -1, own);
+  PAGED_CHECK(q.size(2) % a.pages.Hkv == 0, "the pages need a number of heads that divides q's");
+  PAGED_CHECK(kv_len.scalar_type() == at::kInt && kv_len.dim() == 1 && kv_len.size(0) == a.pages.B && kv_len.device() == q.device(), "kv_len must be int32 [B] on q's device");
+  const double factor = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3));
+  PAGED_CHECK(factor >= 0x1p-126 && factor <= 0x1p126, "scale must be positive, and normal in fp32");
+  paged_no_gradient({&q, &k_pages, &v_pages});
   Tensor o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   if (q.numel() == 0) return o;
   if (a.pages.most == 0) return o.zero_();
@@ -853,7 +874,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.o = o.data_ptr();
   a.kv_len = lengths.data_ptr<int>();
   a.Sq = (int)q.size(1); a.H = (int)q.size(2);
-  a.scale = (float)scale;
+  a.scale = (float)factor;
   Tensor ws = at::empty({mdb_paged_attention_floats(&a)}, q.options().dtype(at::kFloat));
   a.ws = ws.data_ptr<float>();
   g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -1663,7 +1684,7 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor(a!)? out) -> Tensor(a!)", &relative_attention);
   m.def("text_attention", &text_attention);
   m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, Tensor cos, Tensor sin, Tensor? cu_seqlens, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor? q, Tensor? q_norm, Tensor? k_norm, float eps) -> Tensor?", &paged_append);
-  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, float scale, Tensor? k_scale, Tensor? v_scale, int max_len) -> Tensor", &paged_attention);
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, float? scale, Tensor? k_scale, Tensor? v_scale, int? max_len) -> Tensor", &paged_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);
   m.def("qk_norm_rope", &qk_norm_rope);

@@ -52,8 +52,10 @@ def _no_gradient(name, *tensors):
 
 
 def _kernels(x, k_pages, *others) -> bool:
-    return (x.dtype is torch.bfloat16 and x.shape[-1] in (64, 128) and k_pages.shape[2] in _SIZES and native.use_native(x)
-            and native.direct(x, k_pages, *[t for t in others if t is not None]))
+    """Whether the kernels cover the call. They check shapes, types and devices themselves, which costs a short call less."""
+    if not x.is_cuda or x.dtype is not torch.bfloat16 or k_pages.dim() != 4 or x.shape[-1] not in (64, 128) or k_pages.shape[2] not in _SIZES:
+        return False
+    return native.use_native(x) and native.direct(x, k_pages, *[t for t in others if t is not None])
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
@@ -69,6 +71,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     A page that gets its first token takes its scales anew, whatever it held before. Infinities in k or v become NaN in 8 bits and do not count for the scale.
     Rows behind the last sequence are not read, and zero in the result. A page that tokens go to must belong to one sequence.
     """
+    if _kernels(k, k_pages, v, q, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q_norm, k_norm):
+        return native.ops().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, eps)
     name = "paged_append"
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point() or k.shape[1] == 0 or k.device != v.device:
         raise ValueError(f"{name}: k and v must be [T, Hkv, Dh] of one floating type on one device")
@@ -94,8 +98,6 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if q is None and q_norm is not None:
         raise ValueError(f"{name}: q_norm without q")
     _no_gradient(name, k, v, q, q_norm, k_norm, k_pages, v_pages)
-    if _kernels(k, k_pages, v, q, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q_norm, k_norm):
-        return native.ops().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, float(eps))
     with torch.no_grad():
         return ref.paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, float(eps))
 
@@ -110,6 +112,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     what lies behind is not seen; parts of prompts take a workspace of this size (all that the table has room for by default). Slots behind a sequence's
     end are not read: they may hold anything.
     """
+    if max_len is not None and (type(max_len) is not int or max_len < 0):
+        raise ValueError("paged_attention: max_len must be an int of at least 0")
+    if _kernels(q, k_pages, v_pages, block_table, kv_len, k_scale, v_scale):
+        return native.ops().paged_attention(q, k_pages, v_pages, block_table, kv_len, scale, k_scale, v_scale, max_len)
     name = "paged_attention"
     if q.dim() != 4 or not q.is_floating_point() or q.shape[2] == 0:
         raise ValueError(f"{name}: q must be floating [B, Sq, H, Dh]")
@@ -118,13 +124,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"{name}: the pages need a number of heads that divides q's")
     if kv_len.dtype != torch.int32 or kv_len.shape != q.shape[:1] or kv_len.device != q.device:
         raise ValueError(f"{name}: kv_len must be int32 [B] on q's device")
-    if max_len is not None and (type(max_len) is not int or max_len < 0):
-        raise ValueError(f"{name}: max_len must be an int of at least 0")
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -126 <= scale <= 2.0 ** 126:
         raise ValueError(f"{name}: scale must be positive, and normal in fp32")
     _no_gradient(name, q, k_pages, v_pages)
-    if _kernels(q, k_pages, v_pages, block_table, kv_len, k_scale, v_scale):
-        return native.ops().paged_attention(q, k_pages, v_pages, block_table, kv_len, scale, k_scale, v_scale, -1 if max_len is None else max_len)
     with torch.no_grad():
         return ref.paged_attention(q, k_pages, v_pages, block_table, kv_len, scale, k_scale, v_scale, max_len)

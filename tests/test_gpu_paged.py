@@ -200,3 +200,29 @@ def test_empty_calls():
     assert not O.paged_attention(_normal(2, 1, 4, D, seed=0), kp, vp, _ints([[9], [9]]), _ints([0, -5]), k_scale=ks, v_scale=vs).any()
     assert not O.paged_attention(_normal(2, 40, 4, D, seed=0), kp, vp, torch.empty(2, 0, dtype=torch.int32, device=DEV), _ints([3, 5]), k_scale=ks, v_scale=vs).any()
     O.check_status()
+
+
+def test_refuses_what_the_cpu_refuses():
+    """The calls that the torch statements refuse for their arguments, and layouts that the kernels do not take."""
+    from test_cpu_paged import BAD_APPEND, BAD_ATTENTION
+
+    P, G, D, T = 16, 2, 64, 3
+    k = _normal(T, G, D, seed=0)
+    (kp, ks), (vp, vs) = pool(4, G, P, D, True, DEV, 0), pool(4, G, P, D, True, DEV, 1)
+    cos, sin = angles(64, D, DEV)
+    base = dict(k=k, v=k.clone(), k_pages=kp, v_pages=vp, block_table=_ints([[0, 1], [2, 3]]), start=_ints([0, 5]), cos=cos, sin=sin, cu_seqlens=_ints([0, 1, 3]), k_scale=ks, v_scale=vs, q=_normal(T, 4, D, seed=1))
+    O.paged_append(**base)
+    before = [t.clone() for t in (kp, vp, ks, vs)]
+    move = lambda t: t.to(DEV) if isinstance(t, torch.Tensor) else t
+    wide = torch.zeros(4, G, P, 2 * D, device=DEV).to(torch.float8_e4m3fn)
+    for bad in BAD_APPEND[:25] + [dict(k_pages=lambda a: wide[..., :D], v_pages=lambda a: wide[..., :D]), dict(start=lambda a: a["start"].cpu()), dict(q=lambda a: a["q"].cpu()), dict(cos=lambda a: a["cos"].cpu())]:
+        with pytest.raises(ValueError):
+            O.paged_append(**(base | {n: move(f(base)) if "cpu" not in f.__code__.co_names else f(base) for n, f in bad.items()}))
+    base = {n: base[n] for n in ("k_pages", "v_pages", "block_table", "k_scale", "v_scale")} | dict(q=_normal(2, 1, 4, D, seed=2), kv_len=_ints([20, 2]))
+    for i, bad in enumerate(BAD_ATTENTION):
+        if i not in (13, 14):                                # those are page numbers and lengths, not arguments
+            with pytest.raises(ValueError):
+                O.paged_attention(**(base | {n: move(f(base)) for n, f in bad.items()}))
+    for a, b in zip(before, (kp, vp, ks, vs)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    O.check_status()
