@@ -25,12 +25,10 @@ __device__ __forceinline__ int scale_byte(float most) {
 __device__ __forceinline__ float scale_value(int byte) { return __uint_as_float(static_cast<uint32_t>(byte) << 23); }
 __device__ __forceinline__ float scale_inverse(int byte) { return __uint_as_float(static_cast<uint32_t>(254 - byte) << 23); }
 
-// two values in e4m3, rounded to nearest; the first in the low byte. Infinities have no form there and become NaN
-__device__ __forceinline__ uint32_t pack_e4m3x2(float lo, float hi) {
-  lo = fabsf(lo) == INFINITY ? NAN : lo;
-  hi = fabsf(hi) == INFINITY ? NAN : hi;
+// two finite values or NaN in e4m3, rounded to nearest; the first in the low byte
+__device__ __forceinline__ uint32_t pack_e4m3x2(float2 x) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x.y), "f"(x.x));
   return r;
 }
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {      // exact

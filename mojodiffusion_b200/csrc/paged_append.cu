@@ -19,73 +19,107 @@ constexpr int PA_THREADS = 256;
 
 template <int DH> struct AppendRow {
   static constexpr int LANES = DH / 16;
-  float x[16];
+  float2 x[2][4];      // of either half
 
-  __device__ __forceinline__ void load(const __nv_bfloat16* row, int l) {
+  __device__ __forceinline__ static void fetch(uint4 (&u)[2], const __nv_bfloat16* row, int l) {
+    u[0] = *reinterpret_cast<const uint4*>(row + l * 8);
+    u[1] = *reinterpret_cast<const uint4*>(row + DH / 2 + l * 8);
+  }
+  __device__ __forceinline__ void set(const uint4 (&u)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + h * (DH / 2) + l * 8);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack_bf16x2(w[e]);
-        x[h * 8 + 2 * e] = f.x;
-        x[h * 8 + 2 * e + 1] = f.y;
-      }
+      x[h][0] = unpack_bf16x2(u[h].x);
+      x[h][1] = unpack_bf16x2(u[h].y);
+      x[h][2] = unpack_bf16x2(u[h].z);
+      x[h][3] = unpack_bf16x2(u[h].w);
     }
   }
-  __device__ __forceinline__ static float sum(float s) {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-    return s;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[h][e] = make_float2(0.f, 0.f);
   }
-  // by whole warps: the lanes of a row add up their squares
-  __device__ __forceinline__ void norm(const void* w, int f32, float eps, int l) {
-    float s = 0.f;
+  // 1 / sqrt(mean of the squares + eps); by whole warps: the lanes of a row add up theirs
+  __device__ __forceinline__ float norm(float eps) const {
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s = fmaf(x[e], x[e], s);
-    const float r = rsqrtf(sum(s) * (1.f / DH) + eps);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int d = (e >> 3) * (DH / 2) + l * 8 + (e & 7);
-      x[e] = x[e] * r * (f32 ? static_cast<const float*>(w)[d] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[d]));
+      for (int e = 0; e < 4; ++e) s = ffma2(x[h][e], x[h][e], s);
+    float t = s.x + s.y;
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+    return rsqrtf(t * (1.f / DH) + eps);
+  }
+  __device__ __forceinline__ void weigh(const void* w, int f32, float r, int l) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d = h * (DH / 2) + l * 8;
+      float2 f[4];
+      if (f32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = reinterpret_cast<const float2*>(static_cast<const float*>(w) + d)[e];
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + d);
+        f[0] = unpack_bf16x2(u.x);
+        f[1] = unpack_bf16x2(u.y);
+        f[2] = unpack_bf16x2(u.z);
+        f[3] = unpack_bf16x2(u.w);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[h][e] = fmul2(fmul2(x[h][e], make_float2(r, r)), f[e]);
     }
   }
   // products and sums are rounded one by one, as separate operations round them
-  __device__ __forceinline__ void rotate(const float* cos, const float* sin, int l) {
-    float c[8], s[8];
+  __device__ __forceinline__ void rotate(const AppendRow& angles) {      // cosines and sines
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(cos + l * 8 + e);
-      *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(sin + l * 8 + e);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = x[e], b = x[e + 8];
-      x[e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-      x[e + 8] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = x[0][e], b = x[1][e], c = angles.x[0][e], s = angles.x[1][e];
+      const float2 bs = fmul2(b, s);
+      x[0][e] = fadd2(fmul2(a, c), make_float2(-bs.x, -bs.y));
+      x[1][e] = fadd2(fmul2(b, c), fmul2(a, s));
     }
   }
-  __device__ __forceinline__ float most() const {      // of the finite values
+  __device__ __forceinline__ void set_angles(const float* cos, const float* sin, int l) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      *reinterpret_cast<float4*>(&x[0][e]) = *reinterpret_cast<const float4*>(cos + l * 8 + 2 * e);
+      *reinterpret_cast<float4*>(&x[1][e]) = *reinterpret_cast<const float4*>(sin + l * 8 + 2 * e);
+    }
+  }
+  // the largest size, infinity among them, NaN not
+  __device__ __forceinline__ float most() const {
     float m = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float a = fabsf(x[e]);
-      m = a < INFINITY ? fmaxf(m, a) : m;
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmax3(m, fabsf(x[h][e].x), fabsf(x[h][e].y));
     return m;
+  }
+  __device__ __forceinline__ void infinite_to_nan() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (fabsf(x[h][e].x) == INFINITY) x[h][e].x = NAN;
+        if (fabsf(x[h][e].y) == INFINITY) x[h][e].y = NAN;
+      }
   }
   __device__ __forceinline__ void store_bf16(__nv_bfloat16* row, int l) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<uint4*>(row + h * (DH / 2) + l * 8) = make_uint4(pack_bf16x2(x[h * 8], x[h * 8 + 1]), pack_bf16x2(x[h * 8 + 2], x[h * 8 + 3]),
-                                                                         pack_bf16x2(x[h * 8 + 4], x[h * 8 + 5]), pack_bf16x2(x[h * 8 + 6], x[h * 8 + 7]));
+      *reinterpret_cast<uint4*>(row + h * (DH / 2) + l * 8) = make_uint4(pack_bf16x2(x[h][0].x, x[h][0].y), pack_bf16x2(x[h][1].x, x[h][1].y),
+                                                                         pack_bf16x2(x[h][2].x, x[h][2].y), pack_bf16x2(x[h][3].x, x[h][3].y));
   }
   __device__ __forceinline__ void store_e4m3(uint8_t* row, int l, float f) const {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<uint2*>(row + h * (DH / 2) + l * 8) = make_uint2(pack_e4m3x2(x[h * 8] * f, x[h * 8 + 1] * f) | pack_e4m3x2(x[h * 8 + 2] * f, x[h * 8 + 3] * f) << 16,
-                                                                         pack_e4m3x2(x[h * 8 + 4] * f, x[h * 8 + 5] * f) | pack_e4m3x2(x[h * 8 + 6] * f, x[h * 8 + 7] * f) << 16);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_e4m3x2(fmul2(x[h][e], make_float2(f, f)));
+      *reinterpret_cast<uint2*>(row + h * (DH / 2) + l * 8) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    }
   }
 };
 
@@ -98,7 +132,7 @@ __device__ __forceinline__ void rescale(uint8_t* at, int bytes, int by, int t, i
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float2 lo = e4m3x2_to_float2(static_cast<uint16_t>(w[e])), hi = e4m3x2_to_float2(static_cast<uint16_t>(w[e] >> 16));
-      w[e] = pack_e4m3x2(lo.x * f, lo.y * f) | pack_e4m3x2(hi.x * f, hi.y * f) << 16;
+      w[e] = pack_e4m3x2(make_float2(lo.x * f, lo.y * f)) | pack_e4m3x2(make_float2(hi.x * f, hi.y * f)) << 16;
     }
     *reinterpret_cast<uint4*>(at + i) = u;
   }
@@ -111,8 +145,7 @@ struct AppendUnit {
 };
 // The rows of sequence b; what the lengths say is held within the T rows
 __device__ __forceinline__ void rows_of(const MdbPagedAppendArgs& a, int b, long long& first, int& length, int& start) {
-  const long long lo = a.cu == nullptr ? b : min(max(static_cast<long long>(a.cu[b]), 0ll), a.T);
-  const long long hi = a.cu == nullptr ? b + 1 : min(max(static_cast<long long>(a.cu[b + 1]), lo), a.T);
+  const long long lo = min(max(static_cast<long long>(a.cu[b]), 0ll), a.T), hi = min(max(static_cast<long long>(a.cu[b + 1]), lo), a.T);
   first = lo;
   length = static_cast<int>(hi - lo);
   start = a.start[b];
@@ -155,96 +188,213 @@ __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int
   return u;
 }
 
-// grid: units, then rows behind the last sequence; key heads; keys, values, queries of the head's group
+// grid: units, then rows behind the last sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
+// few heads, so a block has several of them. Queries are turned one row of a group of lanes after the other, two heads at a time; of keys and values a block needs a head's rows
+// of the whole unit at once, for its scale.
+struct AppendGrid {
+  int units, q_heads, kv_heads;      // heads of a block
+};
 template <int DH, bool E4M3, int ITERS>
-__global__ void __launch_bounds__(PA_THREADS)
-paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const int units) {
+__global__ void __launch_bounds__(PA_THREADS, ITERS == 4 ? 2 : 4)
+paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGrid grid) {
   using Row = AppendRow<DH>;
   constexpr int LANES = Row::LANES, GROUPS = PA_THREADS / LANES;
-  __shared__ float tops[PA_THREADS / 32];
-  const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, g = blockIdx.y, kind = blockIdx.z;
-  const int rep = a.q != nullptr ? a.H / a.pages.Hkv : 0;
-  if (static_cast<int>(blockIdx.x) >= units) {      // queries behind the last sequence come out as zeros
-    if (kind != 2) return;
-    const long long end = min(max(static_cast<long long>(a.cu[a.pages.B]), 0ll), a.T);
-    for (long long i = (static_cast<long long>(blockIdx.x) - units) * GROUPS + group; i < (a.T - end) * rep; i += static_cast<long long>(gridDim.x - units) * GROUPS) {
-      __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.q_out) + ((end + i / rep) * a.H + g * rep + i % rep) * DH;
+  __shared__ float tops[2][PA_THREADS / 32];
+  const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, G = a.pages.Hkv;
+  const int q_parts = a.q != nullptr ? (a.H + grid.q_heads - 1) / grid.q_heads : 0, kv_parts = (G + grid.kv_heads - 1) / grid.kv_heads;
+  if (static_cast<int>(blockIdx.y) < q_parts) {
+    const int h0 = blockIdx.y * grid.q_heads, hn = min(a.H, h0 + grid.q_heads);
+    if (static_cast<int>(blockIdx.x) >= grid.units) {      // queries behind the last sequence come out as zeros
+      const long long end = min(max(static_cast<long long>(a.cu[a.pages.B]), 0ll), a.T);
+      Row r;
+      r.clear();
+      for (long long t = end + (static_cast<long long>(blockIdx.x) - grid.units) * GROUPS + group; t < a.T; t += static_cast<long long>(gridDim.x - grid.units) * GROUPS)
+        for (int h = h0; h < hn; ++h) r.store_bf16(static_cast<__nv_bfloat16*>(a.q_out) + (t * a.H + h) * DH, l);
+      return;
+    }
+    const AppendUnit u = find_unit(a, blockIdx.x);
+    const bool page = u.count > 0 && page_of(a.pages, u.b, u.index) >= 0;
+    const int turned = page ? min(u.count, max(a.positions - u.position, 0)) : 0;      // rows that have a place and angles
+    for (int t0 = 0; t0 < u.count; t0 += GROUPS) {
+      const int t = t0 + group;
+      const bool in = t < u.count, placed = t < turned;
+      const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(a.q) + (u.row + t) * a.q_strides[0];
+      __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.q_out) + (u.row + t) * a.H * DH;
+      Row angles;
+      if (placed) angles.set_angles(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
+      for (int h = h0; h < hn; h += 2) {
+        uint4 raw[2][2];
+        const bool two = h + 1 < hn;
+        if (in) Row::fetch(raw[0], from + h * a.q_strides[1], l);
+        if (in && two) Row::fetch(raw[1], from + (h + 1) * a.q_strides[1], l);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<uint4*>(to + h * (DH / 2) + l * 8) = make_uint4(0, 0, 0, 0);
+        for (int y = 0; y < 2; ++y) {
+          if (y == 1 && !two) break;
+          Row r;
+          r.set(raw[y]);
+          if (a.q_norm != nullptr) r.weigh(a.q_norm, a.q_norm_f32, r.norm(a.eps), l);
+          if (placed) r.rotate(angles);
+          else r.clear();
+          if (in) r.store_bf16(to + (h + y) * DH, l);
+        }
+      }
     }
     return;
   }
+  if (static_cast<int>(blockIdx.x) >= grid.units) return;
+  const int kv = static_cast<int>(blockIdx.y) >= q_parts + kv_parts, part = blockIdx.y - q_parts - kv * kv_parts;
+  const int h0 = part * grid.kv_heads, hn = min(G, h0 + grid.kv_heads);
   const AppendUnit u = find_unit(a, blockIdx.x);
   if (u.count == 0) return;
-  const int page = page_of(a.pages, u.b, u.index), placed = page >= 0 ? min(u.count, max(a.positions - u.position, 0)) : 0;
-  if (placed < u.count && threadIdx.x == 0) report_status(a.pages.status, STATUS_BOUNDS, 181, u.b);
-  if (kind == 2) {
-    for (int i0 = 0; i0 < u.count * rep; i0 += GROUPS) {
-      const int i = i0 + group, t = i / rep, h = g * rep + i % rep;
-      const bool in = i < u.count * rep && t < placed;
-      Row r;
-      if (in) r.load(static_cast<const __nv_bfloat16*>(a.q) + (u.row + t) * a.q_strides[0] + h * a.q_strides[1], l);
-      if (a.q_norm != nullptr) r.norm(a.q_norm, a.q_norm_f32, a.eps, l);
-      if (in) r.rotate(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
-      if (i < u.count * rep && !in) {
+  const int page = page_of(a.pages, u.b, u.index), turned = page >= 0 ? min(u.count, max(a.positions - u.position, 0)) : 0;
+  if (turned < u.count && kv == 0 && part == 0 && threadIdx.x == 0) report_status(a.pages.status, STATUS_BOUNDS, 181, u.b);
+  if (turned == 0) return;
+  const long long* fs = kv ? a.v_strides : a.k_strides;
+  const long long* ps = kv ? a.pages.v_strides : a.pages.k_strides;
+  const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(kv ? a.v : a.k) + u.row * fs[0];
+  const long long at = page * ps[0] + u.slot * DH;
+#pragma unroll 1
+  for (int h = h0; h < hn; ++h) {
+    unsigned char* scale = E4M3 ? (kv ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kv] + h : nullptr;
+    const int before = E4M3 && u.slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
+    Row r[ITERS];
+    uint4 raw[ITERS][2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) r.x[e] = 0.f;
+    for (int n = 0; n < ITERS; ++n)
+      if (n * GROUPS + group < turned) Row::fetch(raw[n], from + (n * GROUPS + group) * fs[0] + h * fs[1], l);
+    float top = 0.f;
+#pragma unroll
+    for (int n = 0; n < ITERS; ++n) {
+      const int t = n * GROUPS + group;
+      r[n].set(raw[n]);
+      if (kv == 0 && a.k_norm != nullptr) r[n].weigh(a.k_norm, a.k_norm_f32, r[n].norm(a.eps), l);
+      if (t >= turned) {
+        r[n].clear();
+        continue;
       }
-      if (i < u.count * rep) r.store_bf16(static_cast<__nv_bfloat16*>(a.q_out) + ((u.row + t) * a.H + h) * DH, l);
+      if (kv == 0) {
+        Row angles;
+        angles.set_angles(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
+        r[n].rotate(angles);
+      }
+      if (!E4M3) {
+        r[n].store_bf16(static_cast<__nv_bfloat16*>(kv ? a.pages.v : a.pages.k) + at + h * ps[1] + t * DH, l);
+      } else {
+        float mine = r[n].most();
+        if (mine == INFINITY) {
+          r[n].infinite_to_nan();
+          mine = r[n].most();
+        }
+        top = fmaxf(top, mine);
+      }
     }
+    if (!E4M3) continue;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    if ((threadIdx.x & 31) == 0) tops[h & 1][threadIdx.x >> 5] = top;
+    __syncthreads();      // a head's half of `tops` is written again behind the next one's barrier
+#pragma unroll
+    for (int i = 0; i < PA_THREADS / 32; ++i) top = fmaxf(top, tops[h & 1][i]);
+    const int byte = max(scale_byte(top), before);
+    uint8_t* to = static_cast<uint8_t*>(kv ? a.pages.v : a.pages.k) + at + h * ps[1];
+    if (u.slot > 0 && byte > before) rescale(to - u.slot * DH, u.slot * DH, byte - before, threadIdx.x, PA_THREADS);
+    const float f = scale_inverse(byte);
+#pragma unroll
+    for (int n = 0; n < ITERS; ++n)
+      if (n * GROUPS + group < turned) r[n].store_e4m3(to + (n * GROUPS + group) * DH, l, f);
+    if (threadIdx.x == 0 && byte != before) *scale = static_cast<unsigned char>(byte);
+  }
+}
+
+// A row for each sequence: no page gets a second one, so a row's lanes know its scale by themselves, and heads, keys and values of all sequences are one line of
+// rows. What bounds it is the way from the length to the page, its scale and the value; a block for each page and head took 22 us for 128 tokens of 32 / 8 heads.
+constexpr int PT_THREADS = 128;
+template <int DH, bool E4M3>
+__global__ void __launch_bounds__(PT_THREADS)
+paged_append_token_kernel(const __grid_constant__ MdbPagedAppendArgs a) {
+  using Row = AppendRow<DH>;
+  constexpr int LANES = Row::LANES;
+  const int l = threadIdx.x % LANES, H = a.q != nullptr ? a.H : 0, heads = H + 2 * a.pages.Hkv;
+  const long long n = (blockIdx.x * static_cast<long long>(PT_THREADS) + threadIdx.x) / LANES;
+  const bool in = n < static_cast<long long>(a.pages.B) * heads;
+  const int b = in ? static_cast<int>(n / heads) : 0, h = in ? static_cast<int>(n - static_cast<long long>(b) * heads) : 0;
+  const bool is_q = h < H, is_v = h >= H + a.pages.Hkv;
+  const int g = is_q ? h : is_v ? h - H - a.pages.Hkv : h - H;
+  const int p = a.start[b];
+  Row r;
+  uint4 raw[2];
+  if (in) Row::fetch(raw, is_q ? static_cast<const __nv_bfloat16*>(a.q) + b * a.q_strides[0] + g * a.q_strides[1]
+                      : is_v ? static_cast<const __nv_bfloat16*>(a.v) + b * a.v_strides[0] + g * a.v_strides[1] : static_cast<const __nv_bfloat16*>(a.k) + b * a.k_strides[0] + g * a.k_strides[1], l);
+  const int page = p >= 0 && p < a.positions ? page_of(a.pages, b, p / a.pages.P) : -1, slot = p & (a.pages.P - 1);
+  unsigned char* scale = E4M3 && page >= 0 && !is_q ? (is_v ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[is_v] + g : nullptr;
+  const int before = scale != nullptr && slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
+  const void* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+  r.set(raw);
+  if (a.q_norm != nullptr || a.k_norm != nullptr) {      // by whole warps, whose rows may be of several kinds
+    const float f = r.norm(a.eps);
+    if (w != nullptr) r.weigh(w, is_q ? a.q_norm_f32 : a.k_norm_f32, f, l);
+  }
+  if (!in) return;
+  if (page >= 0 && !is_v) {
+    Row angles;
+    angles.set_angles(a.cos + p * static_cast<long long>(DH / 2), a.sin + p * static_cast<long long>(DH / 2), l);
+    r.rotate(angles);
+  }
+  if (is_q) {
+    if (page < 0) r.clear();
+    r.store_bf16(static_cast<__nv_bfloat16*>(a.q_out) + (static_cast<long long>(b) * a.H + h) * DH, l);
     return;
   }
-  if (placed == 0) return;
-  const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(kind ? a.v : a.k);
-  const long long* fs = kind ? a.v_strides : a.k_strides;
-  const long long* ps = kind ? a.pages.v_strides : a.pages.k_strides;
+  if (page < 0) {
+    if (l == 0) report_status(a.pages.status, STATUS_BOUNDS, 181, b);
+    return;
+  }
+  const long long* ps = is_v ? a.pages.v_strides : a.pages.k_strides;
   const long long at = page * ps[0] + g * ps[1];
-  Row r[ITERS];
-  float top = 0.f;
-#pragma unroll
-  for (int n = 0; n < ITERS; ++n) {
-    const int t = n * GROUPS + group;
-    if (t < placed) r[n].load(from + (u.row + t) * fs[0] + g * fs[1], l);
-    if (kind == 0 && a.k_norm != nullptr) r[n].norm(a.k_norm, a.k_norm_f32, a.eps, l);
-    if (t < placed) {
-      if (kind == 0) r[n].rotate(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
-      if (E4M3) top = fmaxf(top, r[n].most());
-      else r[n].store_bf16(static_cast<__nv_bfloat16*>(kind ? a.pages.v : a.pages.k) + at + (u.slot + t) * DH, l);
-    }
+  void* pool = is_v ? a.pages.v : a.pages.k;
+  if (!E4M3) {
+    r.store_bf16(static_cast<__nv_bfloat16*>(pool) + at + slot * DH, l);
+    return;
   }
-  if (!E4M3) return;
+  const uint32_t mine = ((1u << LANES) - 1) << ((threadIdx.x & 31) / LANES * LANES);
+  float top = r.most();
+  if (top == INFINITY) {
+    r.infinite_to_nan();
+    top = r.most();
+  }
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  unsigned char* scale = (kind ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kind] + g;
-  const int before = u.slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < PA_THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+  for (int m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(mine, top, m));
   const int byte = max(scale_byte(top), before);
-  uint8_t* to = static_cast<uint8_t*>(kind ? a.pages.v : a.pages.k) + at;
-  if (u.slot > 0 && byte > before) rescale(to, u.slot * DH, byte - before, threadIdx.x, PA_THREADS);
-  const float f = scale_inverse(byte);
-#pragma unroll
-  for (int n = 0; n < ITERS; ++n) {
-    const int t = n * GROUPS + group;
-    if (t < placed) r[n].store_e4m3(to + (u.slot + t) * DH, l, f);
-  }
-  if (threadIdx.x == 0) *scale = static_cast<unsigned char>(byte);
+  uint8_t* to = static_cast<uint8_t*>(pool) + at;
+  if (slot > 0 && byte > before) rescale(to, slot * DH, byte - before, l, LANES);
+  r.store_e4m3(to + slot * DH, l, scale_inverse(byte));
+  if (l == 0 && byte != before) *scale = static_cast<unsigned char>(byte);
 }
 
 template <int DH, bool E4M3>
 static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
+  if (a.cu == nullptr) {
+    const long long rows = static_cast<long long>(a.pages.B) * ((a.q != nullptr ? a.H : 0) + 2 * a.pages.Hkv), per = PT_THREADS / AppendRow<DH>::LANES;
+    paged_append_token_kernel<DH, E4M3><<<static_cast<unsigned>((rows + per - 1) / per), PT_THREADS, 0, st>>>(a);
+    return static_cast<int>(cudaGetLastError());
+  }
   // a sequence of n > 0 rows touches no more than (n - 1) / P + 2 pages, and no more than n
   const int B = a.pages.B, P = a.pages.P, groups = PA_THREADS / AppendRow<DH>::LANES;
-  const long long units = a.cu == nullptr ? B : std::min(a.T, a.T / P + 2ll * B);
+  const long long units = std::min(a.T, a.T / P + 2ll * B);
   if (units > 0x7ffffff0) return -8;
-  const int spare = a.cu != nullptr && a.q != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
-  const dim3 grid(static_cast<unsigned>(units) + spare, a.pages.Hkv, a.q != nullptr ? 3 : 2);
-  const int rows = a.cu == nullptr ? 1 : static_cast<int>(std::min<long long>(P, a.T));      // of a unit, at most
-  if (rows <= groups) paged_append_kernel<DH, E4M3, 1><<<grid, PA_THREADS, 0, st>>>(a, static_cast<int>(units));
-  else if (rows <= 2 * groups) paged_append_kernel<DH, E4M3, 2><<<grid, PA_THREADS, 0, st>>>(a, static_cast<int>(units));
-  else paged_append_kernel<DH, E4M3, 4><<<grid, PA_THREADS, 0, st>>>(a, static_cast<int>(units));
+  const int spare = a.q != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
+  const int rows = static_cast<int>(std::min<long long>(P, a.T)), H = a.q != nullptr ? a.H : 0, G = a.pages.Hkv;      // rows of a unit, at most
+  // heads of a block: eight and two, fewer where that leaves fewer than six blocks to an SM
+  AppendGrid grid = {static_cast<int>(units), 8, 2};
+  const auto parts = [&]() { return (H + grid.q_heads - 1) / grid.q_heads + 2 * ((G + grid.kv_heads - 1) / grid.kv_heads); };
+  while (grid.q_heads > 1 && units * parts() < 6ll * device_sm_count()) {
+    grid.q_heads /= 2;
+    grid.kv_heads = 1;
+  }
+  const dim3 blocks(static_cast<unsigned>(units) + spare, parts());
+  if (rows <= groups) paged_append_kernel<DH, E4M3, 1><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  else if (rows <= 2 * groups) paged_append_kernel<DH, E4M3, 2><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  else paged_append_kernel<DH, E4M3, 4><<<blocks, PA_THREADS, 0, st>>>(a, grid);
   return static_cast<int>(cudaGetLastError());
 }
 
