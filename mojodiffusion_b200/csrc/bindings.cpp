@@ -719,6 +719,113 @@ Tensor text_attention(const Tensor& q, const Tensor& k, const Tensor& v, const o
   return TextAttention::apply(q, k, v, param, scale, window, sinks, kv_len, q_start, q_starts, buckets);
 }
 
+// Sequences of different lengths one behind the other: q [T, H, Dh], k and v [T, Hkv, Dh] as one sequence of T rows, and where the sequences begin.
+TextCall packed_call(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, int64_t window, const optional<double>& scale, const optional<Tensor>& sink_logits, Tensor& units) {
+  TEXT_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.size(0) == q.size(0) && v.size(0) == q.size(0), "packed q must be [T, H, Dh], k and v [T, Hkv, Dh]");
+  TEXT_CHECK(cu.dim() == 1 && cu.size(0) >= 1 && cu.size(0) < 65536 && cu.scalar_type() == at::kInt && cu.device() == q.device(), "cu_seqlens must be int32 [B + 1] on q's device");
+  TextCall c = text_call(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), scale, window, 0, {}, 0, {}, sink_logits, {});
+  c.kv_len = cu.contiguous();
+  c.a.cu = c.kv_len.data_ptr<int>();
+  c.a.B = (int)cu.size(0) - 1;
+  const int64_t n = mdb_text_attention_units(&c.a);
+  if (n > 0) {
+    units = at::empty({4 * n}, c.kv_len.options());
+    c.a.units = reinterpret_cast<int4*>(units.data_ptr<int>());
+  }
+  return c;
+}
+Tensor packed_forward(TextCall& c, Tensor* lse, Tensor* low) {
+  MdbTextAttnArgs& a = c.a;
+  Tensor o = at::empty({a.Sq, a.H, a.Dh}, c.q.options());
+  if (lse != nullptr) {
+    *lse = at::empty({a.H, a.Sq}, c.q.options().dtype(at::kFloat));
+    *low = at::empty({a.Sq, a.H, a.Dh}, c.q.options());      // sequences may be short whatever T is: see text_forward
+  }
+  if (a.B == 0 || c.q.numel() == 0) {
+    if (lse != nullptr) lse->zero_(), low->zero_();
+    return o.zero_();
+  }
+  a.o_strides[0] = 8; a.o_strides[1] = (long long)a.H * a.Dh; a.o_strides[2] = a.Dh;
+  a.o = o.data_ptr();
+  if (lse != nullptr) {
+    a.lse = lse->data_ptr<float>();
+    a.o_low = low->data_ptr();
+  }
+  if (a.units != nullptr) g_launches.fetch_add(1, std::memory_order_relaxed);
+  check_rc(mdb_text_attention_fwd(&a, cur_stream()), "text_attention_fwd");
+  return o;
+}
+Tensor packed_attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, int64_t window, const optional<double>& scale, const optional<Tensor>& sink_logits) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+  Tensor units;
+  TextCall c = packed_call(q, k, v, cu, window, scale, sink_logits, units);
+  return packed_forward(c, nullptr, nullptr);
+}
+struct PackedAttention : public torch::autograd::Function<PackedAttention> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& sink_logits, const Tensor& cu, int64_t window,
+                        const optional<double>& scale) {
+    c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+    Tensor units, lse, low;
+    TextCall c = packed_call(q, k, v, cu, window, scale, sink_logits, units);
+    Tensor o = packed_forward(c, &lse, &low);
+    ctx->save_for_backward({q, k, v, c.param, c.kv_len, o, low, lse});
+    ctx->saved_data["scale"] = (double)c.a.scale;
+    ctx->saved_data["window"] = window;
+    return o;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &param = saved[3], &cu = saved[4], &o = saved[5], &low = saved[6], &lse = saved[7];
+    torch::autograd::variable_list d(7);
+    {
+      at::NoGradGuard none;
+      c10::cuda::OptionalCUDAGuard guard(at::device_of(q));
+      Tensor units;
+      TextCall c = packed_call(q, k, v, cu, ctx->saved_data["window"].toInt(), ctx->saved_data["scale"].toDouble(), param, units);
+      MdbTextAttnArgs& a = c.a;
+      const bool need_param = param.defined() && ctx->needs_input_grad(3);
+      Tensor dout = text_rows(grads[0].unsqueeze(0), c.q, a.Sq, a.H, a.do_strides, "the output's gradient");
+      d[0] = at::empty({a.Sq, a.H, a.Dh}, q.options());
+      d[1] = at::empty({a.Sq, a.Hkv, a.Dh}, q.options());
+      d[2] = at::empty({a.Sq, a.Hkv, a.Dh}, q.options());
+      if (need_param) d[3] = at::empty_like(c.param);
+      if (a.B == 0 || c.q.numel() == 0) {
+        for (int i = 0; i < 4; ++i)
+          if (d[i].defined()) d[i].zero_();
+      } else {
+        const auto rows = [&](long long (&st)[3], int heads) { st[0] = 8; st[1] = (long long)heads * a.Dh; st[2] = a.Dh; };
+        rows(a.o_strides, a.H);
+        rows(a.dq_strides, a.H);
+        rows(a.dk_strides, a.Hkv);
+        rows(a.dv_strides, a.Hkv);
+        a.o = o.data_ptr(); a.o_low = low.data_ptr(); a.dout = dout.data_ptr();
+        a.dq = d[0].data_ptr(); a.dk = d[1].data_ptr(); a.dv = d[2].data_ptr();
+        a.lse = lse.data_ptr<float>();
+        if (need_param) a.d_sink = d[3].data_ptr();
+        const int64_t floats = (lse.numel() + 3) / 4 * 4;      // delta, and behind it what the launches leave for one another
+        Tensor ws = at::empty({floats + mdb_text_attention_bwd_floats(&a)}, lse.options());
+        a.delta = ws.data_ptr<float>();
+        a.ws = a.delta + floats;
+        g_launches.fetch_add(1 + need_param + (a.units != nullptr), std::memory_order_relaxed);
+        check_rc(mdb_text_attention_bwd(&a, cur_stream()), "text_attention_bwd");
+      }
+    }
+    if (at::GradMode::is_enabled()) {      // a graph of the gradients is wanted: it ends here, with an error where it is walked
+      torch::autograd::variable_list leaves;
+      for (int i = 0; i < 4; ++i)
+        if (d[i].defined()) leaves.push_back(d[i].detach().set_requires_grad(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>("packed_attention is differentiable once", (int64_t)leaves.size());
+      leaves = (*error)(std::move(leaves));
+      for (int i = 0, n = 0; i < 4; ++i)
+        if (d[i].defined()) d[i] = leaves[n++];
+    }
+    return d;
+  }
+};
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& sink_logits, const Tensor& cu, int64_t window, const optional<double>& scale) {
+  return PackedAttention::apply(q, k, v, sink_logits, cu, window, scale);
+}
+
 // ------------------------------------------------------------------------------------------
 // pages of keys and values
 // ------------------------------------------------------------------------------------------
@@ -1683,6 +1790,8 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("window_attention(Tensor q, Tensor k, Tensor v, int window, int sinks, float? scale, Tensor? kv_len, int q_start, Tensor? q_starts, Tensor? sink_logits, Tensor(a!)? out) -> Tensor(a!)", &window_attention);
   m.def("relative_attention(Tensor q, Tensor k, Tensor v, Tensor table, int[] buckets, float scale, Tensor? kv_len, Tensor(a!)? out) -> Tensor(a!)", &relative_attention);
   m.def("text_attention", &text_attention);
+  m.def("packed_attention_fwd", &packed_attention_fwd);
+  m.def("packed_attention", &packed_attention);
   m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, Tensor cos, Tensor sin, Tensor? cu_seqlens, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor? q, Tensor? q_norm, Tensor? k_norm, float eps) -> Tensor?", &paged_append);
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, float? scale, Tensor? k_scale, Tensor? v_scale, int? max_len) -> Tensor", &paged_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);

@@ -224,6 +224,8 @@ typedef struct MdbTextAttnArgs {
   float* lse; float* delta;
   const int* kv_len;          // [B] or null: all keys
   const int* q_start_ptr;     // [B], or null: q_start for all
+  const int* cu;              // packed: [B + 1]; sequence b has the rows cu[b] .. cu[b + 1] of q, k and v [1, Sq, heads, Dh]; kv_len, q_start, sinks and table are not used
+  int4* units;                // packed, more than 32 sequences: mdb_text_attention_units places, none of which need be set
   const void* sink_logits;    // [H] or null
   const void* table;          // [buckets, H] or null; then Hkv = H
   void* d_sink; void* d_table;
@@ -239,6 +241,7 @@ typedef struct MdbTextAttnArgs {
   int* status;
 } MdbTextAttnArgs;
 int mdb_text_attention_fwd(const MdbTextAttnArgs* a, cudaStream_t st);
+long long mdb_text_attention_units(const MdbTextAttnArgs* a);
 long long mdb_text_attention_bwd_floats(const MdbTextAttnArgs* a);
 int mdb_text_attention_bwd(const MdbTextAttnArgs* a, cudaStream_t st);
 

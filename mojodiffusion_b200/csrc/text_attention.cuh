@@ -39,6 +39,50 @@ __device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const Te
   return k;
 }
 
+// Packed sequences: a unit is a block of `gran` rows of one sequence. Units stand in the order of their blocks' numbers, the last blocks, which have the most keys, of all
+// sequences first. Up to 32 sequences: a warp finds a unit from the lengths (a lane each); more: a kernel before has written down the units, sequence after sequence.
+struct TextUnit {
+  int base, rows, block;      // first row and length of the sequence; rows 0: no unit
+};
+__device__ __forceinline__ int text_first_row(const MdbTextAttnArgs& a, int b) { return min(max(a.cu[b], 0), a.Sq); }
+__device__ __forceinline__ int text_rows_of(const MdbTextAttnArgs& a, int b, int first) { return min(max(a.cu[b + 1], first), a.Sq) - first; }
+__device__ __forceinline__ TextUnit text_unit(const MdbTextAttnArgs& a, int unit, int gran) {
+  if (a.units != nullptr) {
+    const int4 u = a.units[unit];
+    return {u.x, u.y, u.z};
+  }
+  const int lane = threadIdx.x & 31;
+  const int first = lane < a.B ? text_first_row(a, lane) : 0, rows = lane < a.B ? text_rows_of(a, lane, first) : 0, n = (rows + gran - 1) / gran;
+  const auto from = [&](int level) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - level, 0)))); };      // blocks of this number or a larger one
+  int lo = 0, hi = __reduce_max_sync(0xffffffffu, n);      // from(lo) > unit >= from(hi)
+  if (unit >= from(0)) return {0, 0, 0};
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > unit) lo = mid;
+    else hi = mid;
+  }
+  const uint32_t have = __ballot_sync(0xffffffffu, n > lo);
+  const int rank = unit - from(lo + 1);
+  const int at = __ffs(__ballot_sync(0xffffffffu, n > lo && __popc(have & ((1u << lane) - 1u)) == rank)) - 1;
+  return {__shfl_sync(0xffffffffu, first, at), __shfl_sync(0xffffffffu, rows, at), lo};
+}
+// The same with the first rows, whose keys have the most queries, of all sequences first: the numbers of a sequence's blocks the other way round
+__device__ __forceinline__ TextUnit text_unit_of_keys(const MdbTextAttnArgs& a, int unit, int gran) {
+  TextUnit u = text_unit(a, unit, gran);
+  if (u.rows > 0) u.block = (u.rows + gran - 1) / gran - 1 - u.block;
+  return u;
+}
+// how many units there may be
+inline long long text_units(const MdbTextAttnArgs& a, int gran) { return a.Sq / gran + static_cast<long long>(a.B); }
+constexpr int TXT_FEW_SEQUENCES = 32;
+int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st);
+
+// rows before the first sequence and behind the last one, in turn
+template <typename F> __device__ __forceinline__ void text_rows_of_none(const MdbTextAttnArgs& a, int from, int step, F f) {
+  const int first = text_first_row(a, 0), last = max(text_first_row(a, a.B), first), n = first + a.Sq - last;
+  for (int i = from; i < n; i += step) f(i < first ? i : i - first + last);
+}
+
 __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(

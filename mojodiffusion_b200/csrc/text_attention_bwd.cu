@@ -72,7 +72,8 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
   }
 };
 
-template <int DH, bool KEYS, bool BIAS>
+// PACKED: a block is a unit of 128 rows of one sequence
+template <int DH, bool KEYS, bool BIAS, bool PACKED>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
 text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextParts parts) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
@@ -114,27 +115,32 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   const int rep = a.H / a.Hkv;
   // the rows with the most to stream start first: late queries, early keys
   // KEYS: blocks of keys in turn with their parts, or blocks and then the slices of the first ones
-  const int key_blocks = (a.Skv + TR - 1) / TR, extra = KEYS && parts.slices > 0 ? static_cast<int>(blockIdx.x) - key_blocks : -1;
+  const int key_blocks = PACKED ? 0 : (a.Skv + TR - 1) / TR, extra = KEYS && parts.slices > 0 ? static_cast<int>(blockIdx.x) - key_blocks : -1;
   const bool shared = KEYS && parts.slices == 0 && parts.count > 1;
   const int part = extra >= 0 ? 1 + extra % parts.slices : shared ? blockIdx.x % parts.count : 0;
   const int block = !KEYS ? (BIAS ? blockIdx.x : gridDim.x - 1 - blockIdx.x) : extra >= 0 ? extra / parts.slices : shared ? blockIdx.x / parts.count : blockIdx.x;
-  const int r0 = block * TR;
-  const int out_rows = KEYS ? a.Skv : a.Sq;
-  const TextSight sight = text_sight(a, batch);
+  // block, the number of a unit's block in its sequence and its first row there; the sequence's first row and length
+  const int unit = PACKED ? shared ? blockIdx.x / parts.count : static_cast<int>(blockIdx.x) : 0;
+  TextUnit of = {0, KEYS ? a.Skv : a.Sq, block};
+  if (PACKED) of = KEYS ? text_unit_of_keys(a, unit, TR) : text_unit(a, unit, TR);
+  const int base = of.base, r0 = of.block * TR, out_rows = of.rows, Sq = PACKED ? of.rows : a.Sq;
+  TextSight sight;
+  if (PACKED) sight = {of.rows, 0};
+  else sight = text_sight(a, batch);
 
   // streamed tiles: keys [0, ns) and [lo, hi); queries [lo, hi) of each head of the group
   TextKeys seen = {0, 0, 0};
   int ns = 0, lo = 0, hi = 0;
   if (!KEYS) {
-    seen = text_keys<BIAS>(a, sight, sight.start + r0, sight.start + min(r0 + TR, a.Sq) - 1);
+    seen = text_keys<BIAS>(a, sight, sight.start + r0, sight.start + min(r0 + TR, Sq) - 1);
     ns = (seen.sinks + TC - 1) / TC;
     lo = max(seen.lo / TC, ns);
     hi = max(seen.end > seen.lo ? (seen.end + TC - 1) / TC : lo, lo);
   } else if (r0 < sight.valid) {
-    int first = 0, end = a.Sq;
+    int first = 0, end = Sq;
     if (!BIAS) {
       first = max(r0 - sight.start, 0);
-      if ((parts.slices > 0 && block < parts.blocks) || r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(a.Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
+      if ((parts.slices > 0 && block < parts.blocks) || r0 >= a.sinks) end = static_cast<int>(max(min(static_cast<long long>(Sq), static_cast<long long>(r0) + TR - 1 + a.window - sight.start), 0ll));
     }
     if (first < end) {
       lo = first / TC;
@@ -142,7 +148,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
     if (extra >= 0) {               // the queries behind the window's
       lo = max(first / TC, hi);
-      hi = max((a.Sq + TC - 1) / TC, lo);
+      hi = max((Sq + TC - 1) / TC, lo);
     }
   }
   const int per_head = ns + hi - lo;
@@ -152,7 +158,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   const int n_c = KEYS ? static_cast<int>(static_cast<long long>(n_all) * (share + 1) / shares) - i_first : n_all;
   const auto tile_of = [&](int i) { return i < ns ? i : i - ns + lo; };
   const auto key_seen = [&](int key) {
-    long long first = 0, end = a.Sq;
+    long long first = 0, end = Sq;
     if (!BIAS) {
       first = max(key - sight.start, 0);
       if (key >= a.sinks) end = min(end, static_cast<long long>(key) + a.window - sight.start);
@@ -168,8 +174,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     if (elect_one()) {
       mbar_expect_tx(&c_full[st], 2 * C_BYTES);
       for (int d = 0; d < DBOX; ++d) {
-        tma_load_4d(c1 + d * C_BOX, &maps.c1, &c_full[st], d * 64, tile_of(load_tile) * TC, load_head, batch);
-        tma_load_4d(c1 + C_BYTES + d * C_BOX, &maps.c2, &c_full[st], d * 64, tile_of(load_tile) * TC, load_head, batch);
+        tma_load_4d(c1 + d * C_BOX, &maps.c1, &c_full[st], d * 64, base + tile_of(load_tile) * TC, load_head, batch);
+        tma_load_4d(c1 + C_BYTES + d * C_BOX, &maps.c2, &c_full[st], d * 64, base + tile_of(load_tile) * TC, load_head, batch);
       }
     }
     __syncwarp();
@@ -201,10 +207,10 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         uint8_t* to = KEYS ? sR1 : sR1 + R_BYTES;
         mbar_expect_tx(&r_full, (KEYS ? 2 : 4 - at_once) * R_BYTES);
         for (int d = 0; d < DBOX; ++d) {
-          tma_load_4d(to + d * R_BOX, &maps.r1, &r_full, d * 64, r0, blockIdx.y, batch);
-          tma_load_4d(to + R_BYTES + d * R_BOX, &maps.r2, &r_full, d * 64, r0, blockIdx.y, batch);
-          if (!KEYS) tma_load_4d(to + 2 * R_BYTES + d * R_BOX, &maps.o, &r_full, d * 64, r0, blockIdx.y, batch);
-          if (!KEYS && at_once == 0) tma_load_4d(sR1 + d * R_BOX, &maps.o_low, &r_full, d * 64, r0, blockIdx.y, batch);
+          tma_load_4d(to + d * R_BOX, &maps.r1, &r_full, d * 64, base + r0, blockIdx.y, batch);
+          tma_load_4d(to + R_BYTES + d * R_BOX, &maps.r2, &r_full, d * 64, base + r0, blockIdx.y, batch);
+          if (!KEYS) tma_load_4d(to + 2 * R_BYTES + d * R_BOX, &maps.o, &r_full, d * 64, base + r0, blockIdx.y, batch);
+          if (!KEYS && at_once == 0) tma_load_4d(sR1 + d * R_BOX, &maps.o_low, &r_full, d * 64, base + r0, blockIdx.y, batch);
         }
       }
       __syncwarp();
@@ -288,10 +294,11 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk / 2 * 32 + kk % 2 * 8, c2 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
         }
       };
-      // rows of a key tile that no query of the CTA sees
+      // rows of a key tile that no query of the CTA sees; packed, also rows of a query tile that belong to the next sequence
       const auto clean = [&](int i, int st) {
-        if (KEYS) return;
-        const int k0 = tile_of(i) * TC;
+        if (KEYS && !PACKED) return;
+        const int k0 = KEYS ? tile_of((i_first + i) % per_head) * TC : tile_of(i) * TC;
+        if (KEYS) seen = {0, 0, Sq};
         if (k0 + TC <= seen.end && (k0 >= seen.lo || k0 + TC <= seen.sinks)) return;
         for (int r = lane; r < TC; r += 32) {
           const int j = k0 + r;
@@ -352,8 +359,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     if (!KEYS) {
       // Q (warpgroup 0) and dO (1) become A operands in TMEM: with 64 columns of B, A from shared memory would cost the score products 48 cycles for
       // every 32. On the way warpgroup 1 forms delta.
-      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + row;
-      if (row < a.Sq) my_nlse = -a.lse[at];
+      const long long at = (static_cast<long long>(batch) * a.H + blockIdx.y) * a.Sq + base + row;
+      if (row < Sq) my_nlse = -a.lse[at];
       ok = text_wait<DH == 128>(&r_full, 0, &abort_s);
       const uint8_t* mine = sR1 + (1 + g) * R_BYTES + mt * 128;
       float2 sum = make_float2(0.f, 0.f);
@@ -390,7 +397,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       float* deltas = &s_delta[0][0];          // [128]
       if (g == 1) {
         deltas[mt] = sum.x + sum.y;
-        if (row < a.Sq) a.delta[at] = sum.x + sum.y;
+        if (row < Sq) a.delta[at] = sum.x + sum.y;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       my_ndelta = -deltas[mt];
@@ -406,8 +413,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
         ++f_head;
       }
       const int q = (lo + f_tile) * TC + (BUFS == 1 ? g * 32 : 0) + mt;
-      const bool in = q < a.Sq && f_head < (static_cast<int>(blockIdx.y) + 1) * rep;
-      const long long at = (static_cast<long long>(batch) * a.H + f_head) * a.Sq + q;
+      const bool in = q < Sq && f_head < (static_cast<int>(blockIdx.y) + 1) * rep;
+      const long long at = (static_cast<long long>(batch) * a.H + f_head) * a.Sq + base + q;
       next_nlse = in ? -a.lse[at] : -INFINITY;
       next_ndelta = in ? -a.delta[at] : 0.f;
     };
@@ -585,12 +592,12 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
       // relative attention with 4 x 512 tokens and 64 heads of 64 columns take 86.5 us so, 93.7 with a row stored by each thread. The loop stays a loop: it runs once.
       uint8_t* stage = sR1 + (warp - 2) * 4096;
       const int line = r0 + quad * 32 + (lane >> 2);
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk) + batch * st[0] + line * st[1] + blockIdx.y * st[2] + (lane & 3) * 8;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(!KEYS ? a.dq : second ? a.dv : a.dk) + batch * st[0] + (base + line) * st[1] + blockIdx.y * st[2] + (lane & 3) * 8;
       const uint32_t acc = tmem_base + lane_addr + (second ? ACC2_COL : ACC1_COL);
       const float f = second ? 1.f : a.scale;
       const auto leaves_as_part = [&](int row_) { return shared || (KEYS && parts.slices > 0 && block < parts.blocks && row_ < a.sinks); };
       const bool as_part = leaves_as_part(row);
-      float* whole = as_part ? parts.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * parts.blocks + block) * parts.count + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
+      float* whole = as_part ? parts.ws + ((((static_cast<long long>(batch) * a.Hkv + blockIdx.y) * parts.blocks + (PACKED ? unit : block)) * parts.count + part) * 2 + g) * (TR * DH) + mt * DH : nullptr;
       constexpr int CHUNKS = KEYS ? DH / 32 : DH / 64;
       const int first = KEYS ? 0 : g * CHUNKS;
 #pragma unroll 1
@@ -647,6 +654,22 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
 
+  if (PACKED && warp >= 2) {      // rows of no sequence: gradients of zero
+    const int t = threadIdx.x - 64;
+    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int line) {
+      for (int e = t; e < DH / 8; e += 256) {
+        const auto clear = [&](void* to, const long long* st) { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(to) + line * st[1] + blockIdx.y * st[2] + e * 8) = make_uint4(0, 0, 0, 0); };
+        if (!KEYS) {
+          clear(a.dq, a.dq_strides);
+          if (e == 0) a.delta[static_cast<long long>(blockIdx.y) * a.Sq + line] = 0.f;
+        } else {
+          clear(a.dk, a.dk_strides);
+          clear(a.dv, a.dv_strides);
+        }
+      }
+    });
+  }
+
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -657,15 +680,22 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
 
 // What is left, in one launch: blocks [0, adders) add the parts of dk and dv, 32 rows of a key head of a sequence each; the others form the gradient of
 // one head's sink logit, -sum of exp2(sink - lse) delta, or of its column of the table, from the sums of all row blocks and sequences. All in a fixed order.
+template <bool PACKED>
 __global__ void __launch_bounds__(256)
 text_finish_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextParts parts, const int part_rows, const int adders, const int row_blocks) {
   __shared__ float sums[256];
   if (static_cast<int>(blockIdx.x) < adders) {
     const int groups = a.Dh / 8, lines = (part_rows + 31) / 32;
     const int line = blockIdx.x % lines, g = blockIdx.x / lines % a.Hkv, batch = blockIdx.x / lines / a.Hkv;
+    TextUnit of = {0, part_rows, 0};      // packed: lines are those of the units, four of each
+    int offset = 0;
+    if (PACKED) {
+      of = text_unit_of_keys(a, line / (TR / 32), TR);
+      offset = of.block * TR - line / (TR / 32) * TR;      // from a row's place among the units' to its place in the sequence
+    }
     for (int e = threadIdx.x; e < 32 * 2 * groups; e += 256) {
       const int c = e % groups, m = e / groups % 2, key = line * 32 + e / groups / 2;
-      if (key >= part_rows) continue;
+      if (key + offset >= of.rows) continue;
       const float* at = parts.ws + ((((static_cast<long long>(batch) * a.Hkv + g) * parts.blocks + key / TR) * parts.count) * 2 + m) * (TR * a.Dh) + key % TR * a.Dh + c * 8;
       float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -676,7 +706,7 @@ text_finish_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextParts pa
       }
       const float x = m == 0 ? a.scale : 1.f;
       const long long* st = m == 0 ? a.dk_strides : a.dv_strides;
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + key * st[1] + g * st[2] + c * 8) =
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(m == 0 ? a.dk : a.dv) + batch * st[0] + (of.base + key + offset) * st[1] + g * st[2] + c * 8) =
           make_uint4(pack_bf16x2(s[0] * x, s[1] * x), pack_bf16x2(s[2] * x, s[3] * x), pack_bf16x2(s[4] * x, s[5] * x), pack_bf16x2(s[6] * x, s[7] * x));
     }
     return;
@@ -699,7 +729,7 @@ text_finish_kernel(const __grid_constant__ MdbTextAttnArgs a, const TextParts pa
     return;
   }
   const float sink = TXT_LOG2E * text_param(a.sink_logits, a.param_f32, h);
-  for (int b = 0; b < a.B; ++b) {
+  for (int b = 0; b < (PACKED ? 1 : a.B); ++b) {
     const long long at = (static_cast<long long>(b) * a.H + h) * a.Sq;
 #pragma unroll 4
     for (int i = t; i < a.Sq; i += 256) s += exp2f(sink - a.lse[at + i]) * a.delta[at + i];
@@ -726,7 +756,8 @@ static int bwd_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh,
 // each, so that the workspace stays below 160 MB however many first keys there are.
 static TextParts text_parts(const MdbTextAttnArgs& a) {
   TextParts p = {0, 0, 1, nullptr};
-  const long long rep = a.H / a.Hkv, blocks = (a.Skv + TR - 1) / TR, groups = static_cast<long long>(a.Hkv) * a.B;
+  const bool packed = a.cu != nullptr;
+  const long long rep = a.H / a.Hkv, blocks = packed ? text_units(a, TR) : (a.Skv + TR - 1) / TR, groups = static_cast<long long>(a.Hkv) * (packed ? 1 : a.B);
   const long long slots = (a.Dh == 64 ? 2 : 1) * device_sm_count();
   const bool windowed = a.table == nullptr && a.sinks < a.Skv;                 // with as many first keys as keys there is no window
   const long long reach = windowed ? std::min<long long>(a.Sq, static_cast<long long>(a.window) + TR) : a.Sq;      // queries of a block of keys, at most
@@ -746,41 +777,45 @@ static TextParts text_parts(const MdbTextAttnArgs& a) {
   return p;
 }
 static long long part_floats(const MdbTextAttnArgs& a, const TextParts& p) {
-  return static_cast<long long>(a.B) * a.Hkv * p.blocks * p.count * 2 * TR * a.Dh;
+  return static_cast<long long>(a.cu != nullptr ? 1 : a.B) * a.Hkv * p.blocks * p.count * 2 * TR * a.Dh;
 }
 
-template <int DH, bool KEYS, bool BIAS>
+template <int DH, bool KEYS, bool BIAS, bool PACKED>
 static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int MOST = 225 * 1024;                 // beside what the kernel declares itself
   const int smem = BIAS ? Shape::bytes(text_near(a), a.buckets) : Shape::bytes(0, 0);
   if (smem > MOST) return -6;
-  auto kern = text_bwd_kernel<DH, KEYS, BIAS>;
+  auto kern = text_bwd_kernel<DH, KEYS, BIAS, PACKED>;
   static bool ready[TXT_DEVICES];
   if (int r = allow_smem(kern, MOST, ready)) return r;
-  int blocks = ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR;
+  int blocks = PACKED ? static_cast<int>(text_units(a, TR)) : ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR;
   if (KEYS) blocks = parts.slices > 0 ? blocks + parts.blocks * parts.slices : blocks * parts.count;
-  kern<<<dim3(blocks, KEYS ? a.Hkv : a.H, a.B), TB_THREADS, smem, st>>>(maps, a, parts);
+  kern<<<dim3(blocks, KEYS ? a.Hkv : a.H, PACKED ? 1 : a.B), TB_THREADS, smem, st>>>(maps, a, parts);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <int DH>
 static int text_backward(const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
+  const int B = a.cu != nullptr ? 1 : a.B;
   TextBwdMaps maps;
   memset(&maps, 0, sizeof(maps));
   int r;
-  if ((r = bwd_map(&maps.c1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
-  if ((r = bwd_map(&maps.c2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
-  if ((r = bwd_map(&maps.r1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TR))) return 1400 + r;
-  if ((r = bwd_map(&maps.r2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TR))) return 1500 + r;
-  if ((r = bwd_map(&maps.o, a.o, a.B, a.Sq, a.H, DH, a.o_strides, TR))) return 1600 + r;
-  if (a.o_low != nullptr && (r = bwd_map(&maps.o_low, a.o_low, a.B, a.Sq, a.H, DH, a.o_strides, TR))) return 1700 + r;
-  if ((r = a.table != nullptr ? launch_text_bwd<DH, false, true>(maps, a, parts, st) : launch_text_bwd<DH, false, false>(maps, a, parts, st))) return r;
-  if ((r = bwd_map(&maps.r1, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
-  if ((r = bwd_map(&maps.r2, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
-  if ((r = bwd_map(&maps.c1, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
-  if ((r = bwd_map(&maps.c2, a.dout, a.B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
-  return a.table != nullptr ? launch_text_bwd<DH, true, true>(maps, a, parts, st) : launch_text_bwd<DH, true, false>(maps, a, parts, st);
+  if ((r = bwd_map(&maps.c1, a.k, B, a.Skv, a.Hkv, DH, a.k_strides, TC))) return 1200 + r;
+  if ((r = bwd_map(&maps.c2, a.v, B, a.Skv, a.Hkv, DH, a.v_strides, TC))) return 1300 + r;
+  if ((r = bwd_map(&maps.r1, a.q, B, a.Sq, a.H, DH, a.q_strides, TR))) return 1400 + r;
+  if ((r = bwd_map(&maps.r2, a.dout, B, a.Sq, a.H, DH, a.do_strides, TR))) return 1500 + r;
+  if ((r = bwd_map(&maps.o, a.o, B, a.Sq, a.H, DH, a.o_strides, TR))) return 1600 + r;
+  if (a.o_low != nullptr && (r = bwd_map(&maps.o_low, a.o_low, B, a.Sq, a.H, DH, a.o_strides, TR))) return 1700 + r;
+  if (a.cu != nullptr) r = launch_text_bwd<DH, false, false, true>(maps, a, parts, st);
+  else r = a.table != nullptr ? launch_text_bwd<DH, false, true, false>(maps, a, parts, st) : launch_text_bwd<DH, false, false, false>(maps, a, parts, st);
+  if (r) return r;
+  if ((r = bwd_map(&maps.r1, a.k, B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
+  if ((r = bwd_map(&maps.r2, a.v, B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
+  if ((r = bwd_map(&maps.c1, a.q, B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
+  if ((r = bwd_map(&maps.c2, a.dout, B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
+  if (a.cu != nullptr) return launch_text_bwd<DH, true, false, true>(maps, a, parts, st);
+  return a.table != nullptr ? launch_text_bwd<DH, true, true, false>(maps, a, parts, st) : launch_text_bwd<DH, true, false, false>(maps, a, parts, st);
 }
 
 // sums of the table's gradient by row block, rounded up so that the parts behind them start on 16 bytes
@@ -792,12 +827,15 @@ long long text_attention_backward_floats(const MdbTextAttnArgs& a) { return tabl
 int text_attention_backward(const MdbTextAttnArgs& a, cudaStream_t st) {
   TextParts parts = text_parts(a);
   parts.ws = a.ws + table_floats(a);
+  const bool packed = a.cu != nullptr;
+  if (packed)
+    if (int r = text_make_units(a, TR, st)) return r;
   if (int r = a.Dh == 128 ? text_backward<128>(a, parts, st) : text_backward<64>(a, parts, st)) return r;
-  const int part_rows = parts.slices > 0 ? std::min(a.sinks, a.Skv) : parts.count > 1 ? a.Skv : 0;
-  const long long adders = static_cast<long long>((part_rows + 31) / 32) * a.Hkv * a.B, params = a.d_sink != nullptr || a.d_table != nullptr ? a.H : 0;
+  const int part_rows = parts.slices > 0 ? std::min(a.sinks, a.Skv) : parts.count > 1 ? packed ? parts.blocks * TR : a.Skv : 0;
+  const long long adders = static_cast<long long>((part_rows + 31) / 32) * a.Hkv * (packed ? 1 : a.B), params = a.d_sink != nullptr || a.d_table != nullptr ? a.H : 0;
   if (adders + params > 0x7fffffff) return -8;
   if (adders + params > 0)
-    text_finish_kernel<<<static_cast<unsigned>(adders + params), 256, 0, st>>>(a, parts, part_rows, static_cast<int>(adders), (a.Sq + TR - 1) / TR);
+    (packed ? text_finish_kernel<true> : text_finish_kernel<false>)<<<static_cast<unsigned>(adders + params), 256, 0, st>>>(a, parts, part_rows, static_cast<int>(adders), (a.Sq + TR - 1) / TR);
   return static_cast<int>(cudaGetLastError());
 }
 

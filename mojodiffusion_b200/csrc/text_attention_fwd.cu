@@ -61,10 +61,11 @@ struct TextTiles {
 
 // One work item, seen by a whole warp: its query tiles, and the key tiles that any of them visits: [0, ns) and then [lo, lo + n_kv - ns).
 // Lane l looks at query tile l % 2.
-template <int DH, bool BIAS> struct TextItem {
+template <int DH, bool BIAS, bool PACKED> struct TextItem {
   using Shape = FwdShape<DH>;
   static constexpr int TK = Shape::TK;
   int batch, head, q0;        // of the first tile
+  int base, rows;             // packed: first row and length of the sequence; else 0 and Sq
   TextSight sight;
   TextKeys all;               // keys that any row sees
   int t_lo, t_hi;             // key tiles of this lane's query tile: [t_lo, t_hi), and of [0, ns) those below t_hi
@@ -76,7 +77,17 @@ template <int DH, bool BIAS> struct TextItem {
   static __device__ __forceinline__ int head_of(const MdbTextAttnArgs& a, int item, const TextTiles& l) { return item / l.row_items / a.B; }
   __device__ __forceinline__ void set(const MdbTextAttnArgs& a, int item, const TextTiles& l) {
     int block;
-    if (BIAS) {
+    base = 0;
+    rows = a.Sq;
+    if (PACKED) {
+      const int groups = a.H >> l.heads_log, rest = item / groups;
+      head = (item - rest * groups) << l.heads_log;
+      batch = 0;
+      const TextUnit u = text_unit(a, rest, l.blocks * TQ);
+      base = u.base;
+      rows = u.rows;
+      block = u.block;
+    } else if (BIAS) {
       const int rest = item / l.row_items;
       block = item - rest * l.row_items;
       head = rest / a.B;
@@ -89,10 +100,11 @@ template <int DH, bool BIAS> struct TextItem {
       block = l.row_items - 1 - block;
     }
     q0 = block * l.blocks * TQ;
-    sight = text_sight(a, batch);
+    if (PACKED) sight = {rows, 0};
+    else sight = text_sight(a, batch);
     const int t = threadIdx.x & 1, first = tile_q0(q0, t, l);
     TextKeys k = {0, 0, 0};
-    if (t < l.heads * l.blocks && first < a.Sq) k = text_keys<BIAS>(a, sight, sight.start + first, sight.start + min(first + TQ, a.Sq) - 1);
+    if (t < l.heads * l.blocks && first < rows) k = text_keys<BIAS>(a, sight, sight.start + first, sight.start + min(first + TQ, rows) - 1);
     const int n_sinks = (k.sinks + TK - 1) / TK;
     t_lo = k.lo / TK;
     t_hi = max(k.end > k.lo ? (k.end + TK - 1) / TK : 0, n_sinks);
@@ -114,7 +126,7 @@ template <int N> struct Int {
   static constexpr int value = N;
 };
 
-template <int DH, bool BIAS>
+template <int DH, bool BIAS, bool PACKED>
 __global__ void __launch_bounds__(FwdShape<DH>::THREADS, FwdShape<DH>::CTAS)
 text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextTiles tiles) {
   using Shape = FwdShape<DH>;
@@ -143,7 +155,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   const int first = RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * blockIdx.x / gridDim.x) : blockIdx.x;
   const int last = ONE ? first + 1 : RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * (blockIdx.x + 1) / gridDim.x) : tiles.items;
   const int step = ONE || RANGE ? 1 : gridDim.x;
-  TextItem<DH, BIAS> w;
+  TextItem<DH, BIAS, PACKED> w;
 
   // The TMA warp makes the barriers and starts loading while the others get ready: nobody else touches either before __syncthreads.
   if (warp == 0) {
@@ -180,7 +192,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
 #pragma unroll 1
       for (int t = 0; t < n_q; ++t)
         for (int d = 0; d < DBOX; ++d)
-          tma_load_4d(sQ + t * Shape::Q_BYTES + d * Shape::Q_BOX, &maps.q, &q_full, d * 64, w.tile_q0(w.q0, t, tiles), w.tile_head(w.head, t, tiles), w.batch);
+          tma_load_4d(sQ + t * Shape::Q_BYTES + d * Shape::Q_BOX, &maps.q, &q_full, d * 64, w.base + w.tile_q0(w.q0, t, tiles), w.tile_head(w.head, t, tiles), w.batch);
     }
     __syncwarp();
   };
@@ -189,7 +201,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     if (elect_one()) {
       mbar_expect_tx(full, Shape::K_BYTES);
       for (int d = 0; d < DBOX; ++d)
-        tma_load_4d((kv ? sV : sK) + st * Shape::K_BYTES + d * Shape::K_BOX, kv ? &maps.v : &maps.k, full, d * 64, w.key_tile(i) * TK, kv_head, w.batch);
+        tma_load_4d((kv ? sV : sK) + st * Shape::K_BYTES + d * Shape::K_BOX, kv ? &maps.v : &maps.k, full, d * 64, w.base + w.key_tile(i) * TK, kv_head, w.batch);
     }
     __syncwarp();
   };
@@ -380,13 +392,14 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     if (first < last) w.set(a, first, tiles);
     for (int item = first; item < last; item += step) {
       const int batch = w.batch, head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
+      const int base = w.base, rows = w.rows;
       if (BIAS && !ONE && head != lut_head) {
         asm volatile("bar.sync 1, 256;" ::: "memory");           // nobody reads the head before
         lut.set(a, head, warp - Shape::SOFT, 8);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         lut_head = head;
       }
-      if (!ok || t >= tiles.heads * tiles.blocks || row0 - quad * 32 >= a.Sq) {
+      if (!ok || t >= tiles.heads * tiles.blocks || row0 - quad * 32 >= rows) {
         if (item + step < last) w.set(a, item + step, tiles);
         continue;
       }
@@ -525,8 +538,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       const uint32_t keep = m_used == -INFINITY ? 0u : 0xffffffffu;      // a row without keys is zero whatever O holds
       const float inv_l = 1.f / l_run;
       // 32 columns at a time through shared memory, so that a store covers 64 bytes of eight rows instead of 16 of 32
-      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + batch * a.o_strides[0] + head * a.o_strides[2] + (row0 + (lane >> 2)) * a.o_strides[1] + (lane & 3) * 8;
-      const int left = a.Sq - row0 - (lane >> 2);                        // rows of this lane from its first one on
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + batch * a.o_strides[0] + head * a.o_strides[2] + (base + row0 + (lane >> 2)) * a.o_strides[1] + (lane & 3) * 8;
+      const int left = rows - row0 - (lane >> 2);                        // rows of this lane from its first one on
       uint4* mine = reinterpret_cast<uint4*>(stage + lane * 64);
       const uint4* theirs = reinterpret_cast<const uint4*>(stage + (lane >> 2) * 64) + ((lane & 3) ^ (lane >> 3 & 3));
 #pragma unroll 1
@@ -573,8 +586,19 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       }
       __syncwarp();
       // +inf where a row saw nothing: the backward pass then finds probabilities of zero
-      if (a.lse != nullptr && row0 + lane < a.Sq)
-        a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + row0 + lane] = m_used == -INFINITY || l_run == 0.f ? INFINITY : m_used + log2f(l_run);
+      if (a.lse != nullptr && row0 + lane < rows)
+        a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + base + row0 + lane] = m_used == -INFINITY || l_run == 0.f ? INFINITY : m_used + log2f(l_run);
+    }
+    if (PACKED) {      // rows of no sequence: zero, and no gradient
+      const int groups = a.H * (DH / 8);
+      text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int row) {
+        for (int e = threadIdx.x - Shape::SOFT * 32; e < groups; e += 256) {
+          const long long to = row * a.o_strides[1] + e / (DH / 8) * a.o_strides[2] + e % (DH / 8) * 8;
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + to) = make_uint4(0, 0, 0, 0);
+          if (a.o_low != nullptr) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o_low) + to) = make_uint4(0, 0, 0, 0);
+          if (a.lse != nullptr && e < a.H) a.lse[static_cast<long long>(e) * a.Sq + row] = INFINITY;
+        }
+      });
     }
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, done);
   }
@@ -594,18 +618,19 @@ static int text_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh
   return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
 }
 
-template <int DH, bool BIAS>
+template <int DH, bool BIAS, bool PACKED>
 static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
+  const int B = PACKED ? 1 : a.B;
   using Shape = FwdShape<DH>;
   TextMaps maps;
-  int r = text_map(&maps.q, a.q, a.B, a.Sq, a.H, DH, a.q_strides, TQ);
+  int r = text_map(&maps.q, a.q, B, a.Sq, a.H, DH, a.q_strides, TQ);
   if (r) return 1000 + r;
-  r = text_map(&maps.k, a.k, a.B, a.Skv, a.Hkv, DH, a.k_strides, Shape::TK);
+  r = text_map(&maps.k, a.k, B, a.Skv, a.Hkv, DH, a.k_strides, Shape::TK);
   if (r) return 2000 + r;
-  r = text_map(&maps.v, a.v, a.B, a.Skv, a.Hkv, DH, a.v_strides, Shape::TK);
+  r = text_map(&maps.v, a.v, B, a.Skv, a.Hkv, DH, a.v_strides, Shape::TK);
   if (r) return 3000 + r;
   constexpr int MOST = 226 * 1024;
-  auto kern = text_fwd_kernel<DH, BIAS>;
+  auto kern = text_fwd_kernel<DH, BIAS, PACKED>;
   static bool ready[TXT_DEVICES];
   if ((r = allow_smem(kern, MOST, ready))) return r;
   const int smem = Shape::BYTES + (BIAS ? TextLut::bytes(text_near(a)) : 0);
@@ -622,19 +647,21 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
       ++l.heads_log;
     }
     l.blocks = n / l.heads;
-    l.row_items = (row_blocks + l.blocks - 1) / l.blocks;
-    items = static_cast<long long>(l.row_items) * (a.H / l.heads) * a.B;
+    l.row_items = PACKED ? static_cast<int>(text_units(a, l.blocks * TQ)) : (row_blocks + l.blocks - 1) / l.blocks;
+    items = static_cast<long long>(l.row_items) * (a.H / l.heads) * B;
     if (items >= slots) break;
   }
   if (items > 0x7fffffff) return -8;
   l.items = static_cast<int>(items);
+  if (PACKED && (r = text_make_units(a, l.blocks * TQ, st))) return r;
   kern<<<static_cast<unsigned>(Shape::CTAS == 2 || items < slots ? items : slots), Shape::THREADS, smem, st>>>(maps, a, l);
   return static_cast<int>(cudaGetLastError());
 }
 
 int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st) {
-  if (a.table != nullptr) return a.Dh == 128 ? launch_text_fwd<128, true>(a, st) : launch_text_fwd<64, true>(a, st);
-  return a.Dh == 128 ? launch_text_fwd<128, false>(a, st) : launch_text_fwd<64, false>(a, st);
+  if (a.cu != nullptr) return a.Dh == 128 ? launch_text_fwd<128, false, true>(a, st) : launch_text_fwd<64, false, true>(a, st);
+  if (a.table != nullptr) return a.Dh == 128 ? launch_text_fwd<128, true, false>(a, st) : launch_text_fwd<64, true, false>(a, st);
+  return a.Dh == 128 ? launch_text_fwd<128, false, false>(a, st) : launch_text_fwd<64, false, false>(a, st);
 }
 
 }  // namespace mdb

@@ -3,4 +3,4 @@ from . import native, reference
 from .functional import *  # noqa: F401,F403
 from .native import check_status
 from .paged import paged_append, paged_attention
-from .text_attention import prefix_lengths, relative_attention, window_attention
+from .text_attention import packed_attention, prefix_lengths, relative_attention, window_attention

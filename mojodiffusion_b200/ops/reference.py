@@ -298,14 +298,15 @@ def relative_attention(q, k, v, table, max_distance: int = 128, scale: float = 1
 def packed_attention(q, k, v, cu_seqlens, window: Optional[int] = None, scale: Optional[float] = None, sink_logits: Optional[torch.Tensor] = None):
     """q [T, H, Dh], k / v [T, Hkv, Dh]: ``window_attention`` of each sequence, whose rows are cu_seqlens[b] .. cu_seqlens[b + 1]; the other rows are zero."""
     ends = cu_seqlens.tolist()
+    no_row = torch.zeros((), dtype=torch.bool, device=q.device)
     out, at = [], 0
     for lo, hi in zip(ends[:-1], ends[1:]):
         if not at <= lo <= hi <= q.shape[0]:
             raise ValueError("packed_attention: cu_seqlens must not fall, nor pass the last row")
-        out.append(q[at:lo] * 0)
+        out.append(torch.where(no_row, q[at:lo], 0))
         out.append(window_attention(q[None, lo:hi], k[None, lo:hi], v[None, lo:hi], window, 0, scale, sink_logits=sink_logits)[0] if hi > lo else q[lo:hi])
         at = hi
-    out.append(torch.zeros_like(q[at:]))
+    out.append(torch.where(no_row, q[at:], 0))
     return torch.cat(out)
 
 

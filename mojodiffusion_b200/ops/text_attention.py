@@ -148,3 +148,37 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     if not kernels:
         o = ref.relative_attention(q, k, v, table, max_distance, scale, kv_len)
     return out.copy_(o) if out is not None else o
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, window: Optional[int] = None, scale: Optional[float] = None,
+                     sink_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal grouped-query attention of sequences that lie one behind the other: q [T, H, Dh], k / v [T, Hkv, Dh] (any strides) -> [T, H, Dh].
+
+    Sequence b has the rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1], not falling, on the tensors' device; a length may be zero), and its row i sees its rows
+    j with ``j <= i`` and ``i - j < window`` (None: all earlier ones). Query head h reads key / value head ``h // (H // Hkv)``; ``sink_logits`` [H] take part in each row's
+    softmax and carry no value. What other sequences hold does not count, NaN neither; rows of no sequence are not read, their output is zero and has no gradient.
+    Differentiable in q, k, v and sink_logits, once.
+    """
+    name = "packed_attention"
+    if window is None:
+        window = _NO_WINDOW
+    elif type(window) is not int or window < 1:
+        raise ValueError(f"{name}: window must be a positive int or None")
+    elif window > _NO_WINDOW:
+        window = _NO_WINDOW
+    if scale is not None:
+        scale = float(scale)
+    if (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 3 and q.shape[2] in (64, 128) and q.shape[0] < _NO_WINDOW and q.shape[1] <= _MOST_BLOCKS and cu_seqlens.numel() <= _MOST_BLOCKS
+            and (scale is None or _LEAST_SCALE <= scale <= _MOST_SCALE) and (sink_logits is None or sink_logits.dtype in (torch.bfloat16, torch.float32)) and native.use_native(q)
+            and native.direct(*[t for t in (q, k, v, cu_seqlens, sink_logits) if t is not None])):
+        if not _wants_grad(q, k, v, sink_logits):
+            return native.ops().packed_attention_fwd(q, k, v, cu_seqlens, window, scale, sink_logits)
+        return native.ops().packed_attention(q, k, v, sink_logits, cu_seqlens, window, scale)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"{name}: q [T, H, Dh], k and v [T, Hkv, Dh]")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.device != q.device:
+        raise ValueError(f"{name}: cu_seqlens must be int32 [B + 1] on q's device")
+    _check(name, q[None], k[None], v[None], None, None)
+    if sink_logits is not None and (sink_logits.shape != q.shape[1:2] or not sink_logits.is_floating_point() or sink_logits.device != q.device):
+        raise ValueError(f"{name}: sink_logits must be [H] on q's device")
+    return ref.packed_attention(q, k, v, cu_seqlens, window if window < _NO_WINDOW else None, scale, sink_logits)
