@@ -889,9 +889,9 @@ const Tensor& paged_rows(const Tensor& t, long long (&strides)[2], std::vector<T
   return own.back();
 }
 
-optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& start, const Tensor& cos, const Tensor& sin,
+std::tuple<Tensor, Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& start, const Tensor& cos, const Tensor& sin,
                               const optional<Tensor>& cu, const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, const optional<Tensor>& q, const optional<Tensor>& q_norm,
-                              const optional<Tensor>& k_norm, double eps) {
+                              const optional<Tensor>& k_norm, double eps, bool keys) {
   c10::cuda::OptionalCUDAGuard guard(at::device_of(k));
   std::vector<Tensor> own;
   own.reserve(16);
@@ -935,24 +935,29 @@ optional<Tensor> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_
   a.q_norm = weight(q_norm, a.q_norm_f32);
   a.k_norm = weight(k_norm, a.k_norm_f32);
   a.eps = (float)eps;
-  optional<Tensor> out;
+  Tensor out, k_out;
   if (has(q)) {
     PAGED_CHECK(on(*q, at::kBFloat16) && q->dim() == 3 && q->size(0) == a.T && q->size(2) == k.size(2) && q->size(1) > 0 && q->size(1) % k.size(1) == 0 && q->size(1) < 65536,
                 "q must be bf16 [T, H, Dh] on k's device, with a number of heads that k's divides");
     a.q = paged_rows(*q, a.q_strides, own).data_ptr();
     a.H = (int)q->size(1);
     out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
-    a.q_out = out->data_ptr();
+    a.q_out = out.data_ptr();
+  }
+  if (keys) {
+    k_out = at::empty(k.sizes(), k.options().memory_format(at::MemoryFormat::Contiguous));
+    a.k_out = k_out.data_ptr();
   }
   if (a.T > 0 && a.pages.B > 0) {
     for (const Tensor* t : {&k_pages, &v_pages}) t->unsafeGetTensorImpl()->bump_version();      // as an operation in place
     if (has(k_scale))
       for (const auto* t : {&k_scale, &v_scale}) (*t)->unsafeGetTensorImpl()->bump_version();
     check_rc(mdb_paged_append(&a, cur_stream()), "paged_append");
-  } else if (out.has_value()) {
-    out->zero_();
+  } else {
+    for (Tensor* t : {&out, &k_out})
+      if (t->defined()) t->zero_();
   }
-  return out;
+  return {out, k_out};
 }
 
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& kv_len, optional<double> scale, const optional<Tensor>& k_scale,
@@ -1792,7 +1797,7 @@ TORCH_LIBRARY(mdb200, m) {
   m.def("text_attention", &text_attention);
   m.def("packed_attention_fwd", &packed_attention_fwd);
   m.def("packed_attention", &packed_attention);
-  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, Tensor cos, Tensor sin, Tensor? cu_seqlens, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor? q, Tensor? q_norm, Tensor? k_norm, float eps) -> Tensor?", &paged_append);
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor start, Tensor cos, Tensor sin, Tensor? cu_seqlens, Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor? q, Tensor? q_norm, Tensor? k_norm, float eps, bool keys) -> (Tensor, Tensor)", &paged_append);
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor kv_len, float? scale, Tensor? k_scale, Tensor? v_scale, int? max_len) -> Tensor", &paged_attention);
   m.def("norm_modulate_fwd", &norm_modulate_fwd);
   m.def("norm_modulate_bwd", &norm_modulate_bwd);

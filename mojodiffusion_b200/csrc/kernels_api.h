@@ -260,7 +260,7 @@ typedef struct MdbPages {
 typedef struct MdbPagedAppendArgs {
   MdbPages pages;
   const void* k; const void* v; const void* q;         // bf16 [T, heads, Dh]; q may be null
-  void* q_out;                                         // bf16 [T, H, Dh], contiguous
+  void* q_out; void* k_out;                            // bf16 [T, heads, Dh], contiguous; k_out, the turned keys, may be null
   const int* cu;                                       // [B + 1], or null: T = B, a row each
   const int* start;                                    // [B]: tokens in the pages before
   const float* cos; const float* sin;                  // [positions, Dh / 2]

@@ -188,6 +188,17 @@ __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int
   return u;
 }
 
+// Heads h0 .. hn - 1 of the rows behind the last sequence come out as zeros; by the blocks from `units` on
+template <int DH> __device__ __forceinline__ void clear_rows_of_none(const MdbPagedAppendArgs& a, int units, __nv_bfloat16* to, int heads, int h0, int hn) {
+  using Row = AppendRow<DH>;
+  constexpr int GROUPS = PA_THREADS / Row::LANES;
+  const long long end = min(max(static_cast<long long>(a.cu[a.pages.B]), 0ll), a.T);
+  Row r;
+  r.clear();
+  for (long long t = end + (static_cast<long long>(blockIdx.x) - units) * GROUPS + threadIdx.x / Row::LANES; t < a.T; t += static_cast<long long>(gridDim.x - units) * GROUPS)
+    for (int h = h0; h < hn; ++h) r.store_bf16(to + (t * heads + h) * DH, threadIdx.x % Row::LANES);
+}
+
 // grid: units, then rows behind the last sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
 // few heads, so a block has several of them. Queries are turned one row of a group of lanes after the other, two heads at a time; of keys and values a block needs a head's rows
 // of the whole unit at once, for its scale.
@@ -205,11 +216,7 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
   if (static_cast<int>(blockIdx.y) < q_parts) {
     const int h0 = blockIdx.y * grid.q_heads, hn = min(a.H, h0 + grid.q_heads);
     if (static_cast<int>(blockIdx.x) >= grid.units) {      // queries behind the last sequence come out as zeros
-      const long long end = min(max(static_cast<long long>(a.cu[a.pages.B]), 0ll), a.T);
-      Row r;
-      r.clear();
-      for (long long t = end + (static_cast<long long>(blockIdx.x) - grid.units) * GROUPS + group; t < a.T; t += static_cast<long long>(gridDim.x - grid.units) * GROUPS)
-        for (int h = h0; h < hn; ++h) r.store_bf16(static_cast<__nv_bfloat16*>(a.q_out) + (t * a.H + h) * DH, l);
+      clear_rows_of_none<DH>(a, grid.units, static_cast<__nv_bfloat16*>(a.q_out), a.H, h0, hn);
       return;
     }
     const AppendUnit u = find_unit(a, blockIdx.x);
@@ -241,22 +248,26 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
     }
     return;
   }
-  if (static_cast<int>(blockIdx.x) >= grid.units) return;
   const int kv = static_cast<int>(blockIdx.y) >= q_parts + kv_parts, part = blockIdx.y - q_parts - kv * kv_parts;
   const int h0 = part * grid.kv_heads, hn = min(G, h0 + grid.kv_heads);
+  __nv_bfloat16* k_out = kv == 0 ? static_cast<__nv_bfloat16*>(a.k_out) : nullptr;
+  if (static_cast<int>(blockIdx.x) >= grid.units) {
+    if (k_out != nullptr) clear_rows_of_none<DH>(a, grid.units, k_out, G, h0, hn);
+    return;
+  }
   const AppendUnit u = find_unit(a, blockIdx.x);
   if (u.count == 0) return;
   const int page = page_of(a.pages, u.b, u.index), turned = page >= 0 ? min(u.count, max(a.positions - u.position, 0)) : 0;
   if (turned < u.count && kv == 0 && part == 0 && threadIdx.x == 0) report_status(a.pages.status, STATUS_BOUNDS, 181, u.b);
-  if (turned == 0) return;
+  if (turned == 0 && k_out == nullptr) return;
   const long long* fs = kv ? a.v_strides : a.k_strides;
   const long long* ps = kv ? a.pages.v_strides : a.pages.k_strides;
   const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(kv ? a.v : a.k) + u.row * fs[0];
   const long long at = page * ps[0] + u.slot * DH;
 #pragma unroll 1
   for (int h = h0; h < hn; ++h) {
-    unsigned char* scale = E4M3 ? (kv ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kv] + h : nullptr;
-    const int before = E4M3 && u.slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
+    unsigned char* scale = E4M3 && page >= 0 ? (kv ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kv] + h : nullptr;
+    const int before = scale != nullptr && u.slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
     Row r[ITERS];
     uint4 raw[ITERS][2];
 #pragma unroll
@@ -270,12 +281,14 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
       if (kv == 0 && a.k_norm != nullptr) r[n].weigh(a.k_norm, a.k_norm_f32, r[n].norm(a.eps), l);
       if (t >= turned) {
         r[n].clear();
+        if (k_out != nullptr && t < u.count) r[n].store_bf16(k_out + ((u.row + t) * G + h) * DH, l);
         continue;
       }
       if (kv == 0) {
         Row angles;
         angles.set_angles(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
         r[n].rotate(angles);
+        if (k_out != nullptr) r[n].store_bf16(k_out + ((u.row + t) * G + h) * DH, l);
       }
       if (!E4M3) {
         r[n].store_bf16(static_cast<__nv_bfloat16*>(kv ? a.pages.v : a.pages.k) + at + h * ps[1] + t * DH, l);
@@ -288,7 +301,7 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
         top = fmaxf(top, mine);
       }
     }
-    if (!E4M3) continue;
+    if (!E4M3 || turned == 0) continue;
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     if ((threadIdx.x & 31) == 0) tops[h & 1][threadIdx.x >> 5] = top;
@@ -345,6 +358,8 @@ paged_append_token_kernel(const __grid_constant__ MdbPagedAppendArgs a) {
     r.store_bf16(static_cast<__nv_bfloat16*>(a.q_out) + (static_cast<long long>(b) * a.H + h) * DH, l);
     return;
   }
+  if (page < 0) r.clear();
+  if (!is_v && a.k_out != nullptr) r.store_bf16(static_cast<__nv_bfloat16*>(a.k_out) + (static_cast<long long>(b) * a.pages.Hkv + g) * DH, l);
   if (page < 0) {
     if (l == 0) report_status(a.pages.status, STATUS_BOUNDS, 181, b);
     return;
@@ -382,7 +397,7 @@ static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
   const int B = a.pages.B, P = a.pages.P, groups = PA_THREADS / AppendRow<DH>::LANES;
   const long long units = std::min(a.T, a.T / P + 2ll * B);
   if (units > 0x7ffffff0) return -8;
-  const int spare = a.q != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
+  const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
   const int rows = static_cast<int>(std::min<long long>(P, a.T)), H = a.q != nullptr ? a.H : 0, G = a.pages.Hkv;      // rows of a unit, at most
   // heads of a block: eight and two, fewer where that leaves fewer than six blocks to an SM
   AppendGrid grid = {static_cast<int>(units), 8, 2};

@@ -16,6 +16,7 @@ from .. import ops
 from ..models.layers import globally_hooked, own_parameters
 from ..models.text.qwen3 import _MLP, _Norm, _W, Qwen3Config, Qwen3Encoder, _rope
 from ..ops import native
+from .paged import PagedKVCache, paged_prefill, paged_step
 from .sampler import Rng, SamplerConfig, sample
 
 
@@ -217,3 +218,37 @@ class Qwen3Decoder:
                 break
             hidden = self.decode_step(torch.tensor([tok], dtype=torch.long, device=dev), cache)
         return out
+
+    @torch.no_grad()
+    def generate_batch(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, cfg: SamplerConfig = SamplerConfig(), eos_ids: Sequence[int] = (),
+                       device=None, cache: Optional[PagedKVCache] = None, eight_bits: bool = False) -> List[List[int]]:
+        """``generate`` for several prompts at once: a reply for each, every one with a sampler of its own that starts from ``cfg.seed``. Prompts run packed, then one token of
+        each sequence that has not ended at a time, over pages of bf16 (the model's type) or 8 bits. ``cache``: pages to take and give back, else as many as the prompts need."""
+        dev = device or next(self.enc.parameters()).device
+        if any(len(p) == 0 for p in prompts):
+            raise ValueError("generate_batch: every prompt needs a token")
+        if cache is None:
+            need = sum(-(-(len(p) + max_new_tokens) // 64) for p in prompts)
+            cache = PagedKVCache(self.cfg, max(need, 1), torch.float8_e4m3fn if eight_bits else self.enc.model.embed_tokens.weight.dtype, dev)
+        out: List[List[int]] = [[] for _ in prompts]
+        if max_new_tokens <= 0 or not prompts:
+            return out
+        first = max(cache.pages, default=-1) + 1
+        alive, rngs = list(range(len(prompts))), [Rng(cfg.seed) for _ in prompts]
+        try:
+            hidden = paged_prefill(self.enc, cache, [first + i for i in alive], prompts)
+            while True:
+                rows = self.logits(hidden).tolist()
+                for i, row in zip(alive, rows):
+                    out[i].append(sample(row, cfg, rngs[i]))
+                ended = [i for i in alive if out[i][-1] in eos_ids or len(out[i]) == max_new_tokens]
+                for i in ended:
+                    cache.release(first + i)
+                alive = [i for i in alive if i not in ended]
+                if not alive:
+                    return out
+                hidden = paged_step(self.enc, cache, [first + i for i in alive], torch.tensor([out[i][-1] for i in alive], dtype=torch.long, device=dev))
+        finally:
+            for i in range(len(prompts)):
+                if first + i in cache.pages:
+                    cache.release(first + i)

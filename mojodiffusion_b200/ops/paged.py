@@ -15,7 +15,7 @@ statements of ``ops.reference``. A page number outside the pool, or a position w
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -61,18 +61,20 @@ def _kernels(x, k_pages, *others) -> bool:
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
                  cos: torch.Tensor, sin: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
-                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Optional[torch.Tensor]:
-    """Keys and values of new tokens into the pages, in place; the rotated queries [T, H, Dh] of the same tokens where ``q`` is given.
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, keys: bool = False) -> Union[None, torch.Tensor, Tuple[Optional[torch.Tensor], torch.Tensor]]:
+    """Keys and values of new tokens into the pages, in place; the rotated queries [T, H, Dh] of the same tokens where ``q`` is given (else None). With ``keys`` a pair:
+    these and the normalised, rotated keys [T, Hkv, Dh] in k's type, for the attention of whole prompts.
 
     k, v [T, Hkv, Dh] and q [T, H, Dh] (any strides) hold the sequences' new rows one behind the other: sequence b has the rows
     cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1]; None: one row each, T = B), which take the positions start[b], start[b] + 1, ... (int32 [B]).
     Per head: root-mean-square norm with the weight ``q_norm`` / ``k_norm`` [Dh] where given (``eps`` inside the root), then the halves (a, b) become
     (a cos - b sin, b cos + a sin) with row p of ``cos`` / ``sin`` [positions, Dh / 2] (fp32) for position p; values stay as they are. All in fp32, rounded once.
     A page that gets its first token takes its scales anew, whatever it held before. Infinities in k or v become NaN in 8 bits and do not count for the scale.
-    Rows behind the last sequence are not read, and zero in the result. A page that tokens go to must belong to one sequence.
+    Rows behind the last sequence are not read, and zero in the results. A page that tokens go to must belong to one sequence.
     """
     if _kernels(k, k_pages, v, q, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q_norm, k_norm):
-        return native.ops().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, eps)
+        found = native.ops().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, eps, keys)
+        return found if keys else found[0]
     name = "paged_append"
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype or not k.is_floating_point() or k.shape[1] == 0 or k.device != v.device:
         raise ValueError(f"{name}: k and v must be [T, Hkv, Dh] of one floating type on one device")
@@ -99,7 +101,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError(f"{name}: q_norm without q")
     _no_gradient(name, k, v, q, q_norm, k_norm, k_pages, v_pages)
     with torch.no_grad():
-        return ref.paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, float(eps))
+        found = ref.paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, float(eps))
+    return found if keys else found[0]
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,

@@ -342,11 +342,12 @@ def _pages_of(name, table, b, n, P, pages):
 
 
 def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens=None, k_scale=None, v_scale=None, q=None, q_norm=None, k_norm=None, eps=1e-6):
-    """New rows of each sequence into its pages (in place); rotated queries or None."""
+    """New rows of each sequence into its pages (in place); rotated queries or None, and rotated keys."""
     N, G, P, D = k_pages.shape
     wide = torch.promote_types(k.dtype, torch.float32)
     ends = list(range(start.numel() + 1)) if cu_seqlens is None else cu_seqlens.tolist()
     q_out = None if q is None else torch.zeros_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.zeros_like(k, memory_format=torch.contiguous_format)
 
     def turned(x, w, c, s):
         x = x.to(wide)
@@ -365,7 +366,9 @@ def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlen
         c, s = (t[first:first + hi - lo, None].to(wide) for t in (cos, sin))
         if q is not None:
             q_out[lo:hi] = turned(q[lo:hi], q_norm, c, s).to(q.dtype)
-        for x, pool, scale in ((turned(k[lo:hi], k_norm, c, s), k_pages, k_scale), (v[lo:hi].to(wide), v_pages, v_scale)):
+        new = turned(k[lo:hi], k_norm, c, s)
+        k_out[lo:hi] = new.to(k.dtype)
+        for x, pool, scale in ((new, k_pages, k_scale), (v[lo:hi].to(wide), v_pages, v_scale)):
             done = 0
             while done < hi - lo:
                 page, slot = pages[(first + done) // P], (first + done) % P
@@ -381,7 +384,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlen
                     scale[page] = byte.to(torch.uint8)
                     part = to_e4m3(part, byte[:, None, None])
                 pool[page, :, slot:slot + part.shape[1]] = part.to(pool.dtype)
-    return q_out
+    return q_out, k_out
 
 
 def paged_attention(q, k_pages, v_pages, block_table, kv_len, scale=None, k_scale=None, v_scale=None, max_len=None):

@@ -48,7 +48,7 @@ def turned(x, w, cos, sin, eps):
     return torch.cat((a * c - b * s, b * c + a * s), -1), torch.cat(((a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs()), -1)
 
 
-def check_append(before, after, q_out, k, v, q, table, start, cu, cos, sin, q_norm, k_norm, eps, name=""):
+def check_append(before, after, q_out, k, v, q, table, start, cu, cos, sin, q_norm, k_norm, eps, name="", k_out=None):
     """``before`` / ``after``: (k_pages, v_pages, k_scale, v_scale) as they were and are. Sequences without pages of their own are not for here."""
     P = before[0].shape[2]
     untouched = [torch.ones(t.shape[:3], dtype=torch.bool) for t in before[:2]]
@@ -63,6 +63,9 @@ def check_append(before, after, q_out, k, v, q, table, start, cu, cos, sin, q_no
         c, s = cos[first:first + hi - lo].cpu(), sin[first:first + hi - lo].cpu()
         if q_out is not None:
             value[lo:hi], size[lo:hi] = turned(q[lo:hi].cpu(), q_norm, c, s, eps)
+        if k_out is not None:
+            y, fine = turned(k[lo:hi].cpu(), k_norm, c, s, eps)
+            assert float(((k_out[lo:hi].cpu().double() - y).abs() - (HALF16 * y.abs() + FINE * fine)).max()) <= 0, f"{name}: keys"
         for i, (x, w) in enumerate(((k, k_norm), (v, None))):
             y, fine = turned(x[lo:hi].cpu(), w, c, s, eps) if i == 0 else (x[lo:hi].cpu().double(), torch.zeros(1, dtype=torch.float64).expand(x[lo:hi].shape))
             was, now = before[i].cpu(), after[i].cpu()
@@ -106,6 +109,8 @@ def check_append(before, after, q_out, k, v, q, table, start, cu, cos, sin, q_no
         assert torch.equal(before[i].cpu().view(torch.uint8 if before[2] is not None else torch.int16)[mask], after[i].cpu().view(torch.uint8 if before[2] is not None else torch.int16)[mask]), f"{name}: a slot that no token goes to"
         if before[2] is not None:
             assert torch.equal(before[2 + i].cpu()[kept_scale], after[2 + i].cpu()[kept_scale]), f"{name}: a scale that no token goes to"
+    if k_out is not None:
+        assert not k_out[ends[-1]:].any()
     if q_out is not None:
         far = (q_out.cpu().double() - value).abs() - (HALF16 * value.abs() + FINE * size)
         assert float(far.max()) <= 0, f"{name}: q is {float(far.max()):.3g} outside its bound"

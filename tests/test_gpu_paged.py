@@ -69,9 +69,12 @@ def test_append(case):
         assert torch.equal(out, out2)
         for a, b in zip(again, (kp, vp, ks, vs)):
             assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
-    # without queries, and with weights in fp32
+    # without queries, and with weights in fp32; with the keys
     again = [None if t is None else t.clone() for t in before]
-    assert O.paged_append(k, v, again[0], again[1], table.to(DEV), _ints(start), cos, sin, cu_seqlens=_ints(cu), k_scale=again[2], v_scale=again[3], k_norm=None if kn is None else on(kn).float()) is None
+    none, keys = O.paged_append(k, v, again[0], again[1], table.to(DEV), _ints(start), cos, sin, cu_seqlens=None if single else _ints(cu), k_scale=again[2], v_scale=again[3],
+                                k_norm=None if kn is None else on(kn).float(), keys=True)
+    assert none is None
+    check_append(before, again, None, k, v, None, table, start, cu, cos, sin, None, kn, 1e-6, str(case), k_out=keys)
     for a, b in zip(again, (kp, vp, ks, vs)):
         assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
@@ -175,6 +178,9 @@ def test_reports_pages_that_are_not_there():
             for a, b in zip(before, (kp, vp, ks, vs)):
                 assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
             assert not out.any()
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+            assert not O.paged_append(k, v, kp, vp, _ints(table), _ints(start), c, s, cu_seqlens=cu, k_scale=ks, v_scale=vs, keys=True)[1].any()
             with pytest.raises(RuntimeError, match="BOUNDS"):
                 O.check_status()
     q = _normal(2, 1, 4, D, seed=5)
