@@ -987,9 +987,12 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.kv_len = lengths.data_ptr<int>();
   a.Sq = (int)q.size(1); a.H = (int)q.size(2);
   a.scale = (float)factor;
-  Tensor ws = at::empty({mdb_paged_attention_floats(&a)}, q.options().dtype(at::kFloat));
-  a.ws = ws.data_ptr<float>();
-  g_launches.fetch_add(1, std::memory_order_relaxed);
+  Tensor ws;
+  if (const int64_t floats = mdb_paged_attention_floats(&a); floats > 0) {      // two launches
+    ws = at::empty({floats}, q.options().dtype(at::kFloat));
+    a.ws = ws.data_ptr<float>();
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
   check_rc(mdb_paged_attention(&a, cur_stream()), "paged_attention");
   return o;
 }

@@ -5,7 +5,8 @@
 // A few queries (at most 64 rows per key head, a row being one query of one head of the group): keys and values are read once and bound the time, so the work is split
 // over keys. All tiles of 128 keys of all sequences and key heads are one line, of which every CTA takes an equal part, wherever that begins and ends: sequences of 1 and
 // of 100000 tokens share the memory's rate. A CTA's tiles of one sequence and head ("segment") end in an output, or in a part (m, l, o) where other CTAs have tiles of
-// it too; a second, small kernel joins those in order. It is launched with the first one and waits for its end.
+// it too; a second, small kernel joins those in order. It is launched with the first one and waits for its end. Where no sequence has more than four tiles, a CTA takes one
+// sequence and head each instead, and there is nothing to join.
 //
 // A warp of its own starts the copies: it knows the pages of the next 32 places of the table and their scales, and brings K and V of a tile in by TMA, one box
 // per page. Four warps multiply, with mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the keys and the columns of V fill the 16 and the rows, of which there
@@ -28,17 +29,21 @@
 namespace mdb {
 
 constexpr int PK = 128;                                       // keys of a tile
-constexpr int PS_WARPS = 4, PS_THREADS = (PS_WARPS + 1) * 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 struct alignas(64) PagedMaps {
   CUtensorMap k, v;
 };
 
-template <int DH, bool E4M3> struct PagedShape {
+// A warp has NT tiles of 8 rows; RG warps share the rows, and the others the keys of a tile
+template <int DH, bool E4M3, int NT, int RG> struct PagedShape {
+  static constexpr int WARPS = 4;                                     // that multiply
+  static constexpr int THREADS = (WARPS + 1) * 32;
+  static constexpr int COLS = 32;                                     // columns that the warps join at a time
   static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
-  static constexpr int STAGES = 96 * 1024 / (2 * TILE);               // 96 KB, so that two CTAs share an SM
-  static constexpr int SLAB = PS_WARPS * 16 * 32 * 4;                 // 32 columns of the warps' parts, at most 16 rows each
+  static constexpr int CTAS = NT == 1 && DH == 64 ? 3 : 2;            // per SM, with 192 KB of stages
+  static constexpr int STAGES = 192 * 1024 / CTAS / (2 * TILE);
+  static constexpr int SLAB = WARPS * 8 * NT * COLS * 4;
   static constexpr int BYTES = STAGES * 2 * TILE + SLAB + 1024;
 };
 
@@ -130,13 +135,12 @@ struct PagedParts {
   float* sums; float* tops;
 };
 
-// A warp has NT tiles of 8 rows; RG warps share the rows, and the others the keys of a tile
 template <int DH, bool E4M3, int NT, int RG>
-__global__ void __launch_bounds__(PS_THREADS, 2)
+__global__ void __launch_bounds__(PagedShape<DH, E4M3, NT, RG>::THREADS, PagedShape<DH, E4M3, NT, RG>::CTAS)
 paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ MdbPagedAttnArgs a, const PagedParts parts) {
-  using Shape = PagedShape<DH, E4M3>;
-  constexpr int TILE = Shape::TILE, STAGES = Shape::STAGES, BOX = PK * 128;
-  constexpr int WR = 8 * NT, ROWS = WR * RG, PER_TILE = PS_WARPS / RG, WK = PK / PER_TILE;      // rows of a warp, of all; warps that share the keys, and keys of a warp
+  using Shape = PagedShape<DH, E4M3, NT, RG>;
+  constexpr int TILE = Shape::TILE, STAGES = Shape::STAGES, BOX = PK * 128, WARPS = Shape::WARPS, COLS = Shape::COLS;
+  constexpr int WR = 8 * NT, ROWS = WR * RG, PER_TILE = WARPS / RG, WK = PK / PER_TILE;      // rows of a warp, of all; warps that share the keys, and keys of a warp
   constexpr int DM = DH / 16;                                                                   // tiles of 16 columns
   constexpr float ABOVE = E4M3 ? 7.f : 0.f;                                                     // the reference stays so far below the first maximum
 
@@ -144,7 +148,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
   __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ uchar2 scales[STAGES][PK / 16];
   __shared__ int abort_s;
-  __shared__ float part_m[PS_WARPS][WR], part_l[PS_WARPS][WR];
+  __shared__ float part_m[WARPS][WR], part_l[WARPS][WR];
   uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   float* slab = reinterpret_cast<float*>(smem + STAGES * 2 * TILE);
 
@@ -153,21 +157,39 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
   const MdbPages& pg = a.pages;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], PS_WARPS);
+      mbar_init(&full[s], E4M3 ? 2 : 1);      // the copies, and the scales
+      mbar_init(&empty[s], WARPS);
     }
     abort_s = 0;
     fence_mbar_init();
   }
-  const long long line = paged_tiles(a) * pg.Hkv, ctas = min(static_cast<long long>(gridDim.x), line);
-  const long long line_first = blockIdx.x < ctas ? line * blockIdx.x / ctas : 0;
   PagedPlace at;
-  at.seek(a, line_first);
-  __syncthreads();
-  if (blockIdx.x >= ctas) return;
-  const int n = static_cast<int>(line * (blockIdx.x + 1) / ctas - line_first);
+  int n;
+  if (parts.sums == nullptr) {      // one sequence and head
+    at.b = blockIdx.x / pg.Hkv;
+    at.g = blockIdx.x - at.b * pg.Hkv;
+    at.t = 0;
+    at.length = paged_length(a, at.b);
+    n = at.tiles = (at.length + PK - 1) / PK;
+    __syncthreads();
+    if (n == 0) {
+      const int rep = a.H / pg.Hkv;
+      for (int e = threadIdx.x; e < rep * a.Sq * (DH / 8); e += Shape::THREADS) {
+        const int r = e / (DH / 8);
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + at.b * a.o_strides[0] + (r / rep) * a.o_strides[1] + (at.g * rep + r % rep) * a.o_strides[2] + e % (DH / 8) * 8) = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
+  } else {
+    const long long line = paged_tiles(a) * pg.Hkv, ctas = min(static_cast<long long>(gridDim.x), line);
+    const long long line_first = blockIdx.x < ctas ? line * blockIdx.x / ctas : 0;
+    at.seek(a, line_first);
+    __syncthreads();
+    if (blockIdx.x >= ctas) return;
+    n = static_cast<int>(line * (blockIdx.x + 1) / ctas - line_first);
+  }
 
-  if (warp == PS_WARPS) {
+  if (warp == WARPS) {
     const int per_tile = max(PK / pg.P, 1), rows = min(pg.P, PK);            // boxes of a tile, keys of a box
     const uint32_t box_bytes = rows * DH * (E4M3 ? 1 : 2);
     int window = 0, page = -1;                                              // this lane's place of the table: window + lane
@@ -195,10 +217,6 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
         break;
       }
       const int keys = min(at.length - at.t * PK, PK), boxes = (keys + rows - 1) / rows;
-      if (E4M3) {
-        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 7) * 16) / pg.P - window) & 31);
-        if (lane < PK / 16) scales[st][lane] = make_uchar2(s & 255, s >> 8);
-      }
       const int mine = __shfl_sync(0xffffffffu, page, (first_index - window + min(lane, per_tile - 1)) & 31);
       __syncwarp();
       if (lane == 0) mbar_expect_tx(&full[st], 2 * boxes * box_bytes);
@@ -216,6 +234,12 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
             tma_load_4d(to + TILE + d * BOX + lane * rows * 128, &maps.v, &full[st], d * 64, row, at.g, mine);
           }
         }
+      }
+      if (E4M3) {      // behind the copies, which need not wait for them
+        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 7) * 16) / pg.P - window) & 31);
+        if (lane < PK / 16) scales[st][lane] = make_uchar2(s & 255, s >> 8);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
       }
       __syncwarp();
       if (++at.t == at.tiles) {
@@ -497,7 +521,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       if (lane == 0) mbar_arrive(&empty[st]);
     }
 
-    // the warps' parts meet in shared memory, 32 columns at a time
+    // the warps' parts meet in shared memory, COLS columns at a time
     const float whole_unit = E4M3 ? scale_value(unit) : 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -513,26 +537,26 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
     const bool complete = first_tile == 0 && count == at.tiles;
     const long long slot = 2ll * blockIdx.x + (segment > 0 ? 1 : 0);
 #pragma unroll
-    for (int c0 = 0; c0 < DH; c0 += 32) {
+    for (int c0 = 0; c0 < DH; c0 += COLS) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int y = 0; y < COLS / 16; ++y)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float (&v)[4] = o[c0 / 16 + y][nt];
-          float* mine = slab + (warp * WR + nt * 8 + 2 * tq) * 32 + 16 * y;
+          float* mine = slab + (warp * WR + nt * 8 + 2 * tq) * COLS + 16 * y;
           if (E4M3) {
             *reinterpret_cast<float2*>(mine + 2 * gq) = make_float2(v[0] * whole_unit, v[2] * whole_unit);
-            *reinterpret_cast<float2*>(mine + 32 + 2 * gq) = make_float2(v[1] * whole_unit, v[3] * whole_unit);
+            *reinterpret_cast<float2*>(mine + COLS + 2 * gq) = make_float2(v[1] * whole_unit, v[3] * whole_unit);
           } else {
             mine[gq] = v[0];
             mine[gq + 8] = v[2];
-            mine[32 + gq] = v[1];
-            mine[32 + gq + 8] = v[3];
+            mine[COLS + gq] = v[1];
+            mine[COLS + gq + 8] = v[3];
           }
         }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int e = threadIdx.x; e < rows * 8; e += 128) {
-        const int r = e >> 3, w0 = (r / WR) * PER_TILE, rr = r % WR, c = (e & 7) * 4;
+      asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+      for (int e = threadIdx.x; e < rows * (COLS / 4); e += WARPS * 32) {
+        const int r = e / (COLS / 4), w0 = (r / WR) * PER_TILE, rr = r % WR, c = e % (COLS / 4) * 4;
         float top = part_m[w0][rr];
 #pragma unroll
         for (int w = 1; w < PER_TILE; ++w) top = paged_max(top, part_m[w0 + w][rr]);
@@ -541,7 +565,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
 #pragma unroll
         for (int w = 0; w < PER_TILE; ++w) {
           const float f = part_m[w0 + w][rr] == -INFINITY ? 0.f : exp2f(part_m[w0 + w][rr] - top);
-          const float4 v = *reinterpret_cast<const float4*>(slab + ((w0 + w) * WR + rr) * 32 + c);
+          const float4 v = *reinterpret_cast<const float4*>(slab + ((w0 + w) * WR + rr) * COLS + c);
           s.x += f * v.x;
           s.y += f * v.y;
           s.z += f * v.z;
@@ -561,7 +585,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
           if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(parts.tops + (slot * ROWS + r) * 2) = make_float2(top, sum);
         }
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
     }
     at.t = first_tile + count;
     if (at.t == at.tiles) at.next_segment(a);
@@ -569,15 +593,21 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
   if (!ok && lane == 0) report_status(pg.status, STATUS_TIMEOUT, 184, n);
 }
 
-// One row of one sequence per block: the parts of its key head, in order. Rows of sequences without keys are zero.
+// A row to a warp, or to all four of a block where a row has many parts: the parts of its key head, in order. What they need to know they find out while the first kernel
+// runs. Rows of sequences without keys are zero.
 constexpr int PJ_THREADS = 128;
-template <int DH>
+template <int DH, int WARPS>
 __global__ void __launch_bounds__(PJ_THREADS)
 paged_join_kernel(const __grid_constant__ MdbPagedAttnArgs a, const PagedParts parts, const int grid, const int part_rows) {
-  constexpr int LANES = DH / 4, GROUPS = PJ_THREADS / LANES;
-  __shared__ float tops[GROUPS], sums[GROUPS], slab[GROUPS][DH];
-  const int lane = threadIdx.x & 31, b = blockIdx.y, h = blockIdx.x % a.H, i = blockIdx.x / a.H, rep = a.H / a.pages.Hkv, g = h / rep, r = i * rep + h % rep;
-  const int c = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  constexpr int LANES = DH / 4, IN_WARP = 32 / LANES, GROUPS = WARPS * IN_WARP;
+  __shared__ float tops[4], sums[4];
+  __shared__ float4 slab[4][LANES];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % LANES, group = warp % WARPS * IN_WARP + lane / LANES;
+  const long long row = blockIdx.x * (4ll / WARPS) + warp / WARPS;
+  const int per = a.Sq * a.H;
+  const bool in = row < static_cast<long long>(a.pages.B) * per;
+  const int b = in ? static_cast<int>(row / per) : 0, rest = in ? static_cast<int>(row - static_cast<long long>(b) * per) : 0, h = rest % a.H, i = rest / a.H;
+  const int rep = a.H / a.pages.Hkv, g = h / rep, r = i * rep + h % rep;
   long long before = 0, total = 0;                    // tiles of a key head before this sequence, in all
   for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
     const unsigned n = b0 + lane < a.pages.B ? static_cast<unsigned>(paged_length(a, b0 + lane) + PK - 1) / PK : 0u;
@@ -585,22 +615,21 @@ paged_join_kernel(const __grid_constant__ MdbPagedAttnArgs a, const PagedParts p
     before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0u);
   }
   const int tiles = (paged_length(a, b) + PK - 1) / PK;
-  const long long line = total * a.pages.Hkv, u0 = before * a.pages.Hkv + static_cast<long long>(g) * tiles, u1 = u0 + tiles;
+  const long long line = max(total * a.pages.Hkv, 1ll), u0 = before * a.pages.Hkv + static_cast<long long>(g) * tiles, u1 = u0 + tiles;
   const long long ctas = min(static_cast<long long>(grid), line);
+  // CTA k has the tiles from line k / ctas on
+  const int first = static_cast<int>(((u0 + 1) * ctas - 1) / line), last = static_cast<int>((max(u1, 1ll) * ctas - 1) / line);
+  const bool first_of_all = line * first / ctas == u0;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + b * a.o_strides[0] + i * a.o_strides[1] + h * a.o_strides[2];
   asm volatile("griddepcontrol.wait;" ::: "memory");      // by all: this kernel must not end before the one whose parts it joins
-  if (tiles == 0) {
-    for (int d = threadIdx.x; d < DH / 8; d += PJ_THREADS) *reinterpret_cast<uint4*>(out + d * 8) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  // CTA k has the tiles from line k / ctas on
-  const long long first = ((u0 + 1) * ctas - 1) / line, last = (u1 * ctas - 1) / line;
-  if (first == last) return;
+  if (in && tiles == 0 && group == 0) *reinterpret_cast<uint2*>(out + c * 4) = make_uint2(0, 0);
+  const bool joined = in && tiles > 0 && first < last;
+  if (!joined) return;                                     // the same in a warp, and with four warps to a row in the block
   float top = -INFINITY, sum = 0.f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (long long k = first + group; k <= last; k += GROUPS) {
-    const long long slot = 2 * k + (k == first && line * k / ctas != u0 ? 1 : 0);
+  for (int k = first + group; k <= last; k += GROUPS) {
+    const long long slot = 2ll * k + (k == first && !first_of_all ? 1 : 0);
     const float2 ml = *reinterpret_cast<const float2*>(parts.tops + (slot * part_rows + r) * 2);
     const float4 v = *reinterpret_cast<const float4*>(parts.sums + (slot * part_rows + r) * DH + c * 4);
     if (ml.x == -INFINITY) continue;
@@ -612,28 +641,32 @@ paged_join_kernel(const __grid_constant__ MdbPagedAttnArgs a, const PagedParts p
     sum = sum * f + ml.y * w;
     top = up;
   }
-  if (c == 0) {
-    tops[group] = top;
-    sums[group] = sum;
+  const auto join = [&](float top2, float sum2, float4 v) {
+    const float up = paged_max(top, top2), f = top == -INFINITY ? 0.f : exp2f(top - up), w = top2 == -INFINITY ? 0.f : exp2f(top2 - up);
+    s.x = s.x * f + v.x * w;
+    s.y = s.y * f + v.y * w;
+    s.z = s.z * f + v.z * w;
+    s.w = s.w * f + v.w * w;
+    sum = sum * f + sum2 * w;
+    top = up;
+  };
+  if (IN_WARP == 2) {
+    const float4 v = make_float4(__shfl_down_sync(0xffffffffu, s.x, 16), __shfl_down_sync(0xffffffffu, s.y, 16), __shfl_down_sync(0xffffffffu, s.z, 16), __shfl_down_sync(0xffffffffu, s.w, 16));
+    const float top2 = __shfl_down_sync(0xffffffffu, top, 16), sum2 = __shfl_down_sync(0xffffffffu, sum, 16);
+    if (lane < 16) join(top2, sum2, v);
   }
-  *reinterpret_cast<float4*>(&slab[group][c * 4]) = s;
-  __syncthreads();
-  if (group > 0) return;
-  top = tops[0];
+  if (WARPS > 1) {
+    if (lane < LANES) slab[warp][lane] = s;
+    if (lane == 0) {
+      tops[warp] = top;
+      sums[warp] = sum;
+    }
+    __syncthreads();
+    if (warp > 0) return;
 #pragma unroll
-  for (int k = 1; k < GROUPS; ++k) top = paged_max(top, tops[k]);
-  sum = 0.f;
-  s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int k = 0; k < GROUPS; ++k) {
-    const float w = tops[k] == -INFINITY ? 0.f : exp2f(tops[k] - top);
-    const float4 v = *reinterpret_cast<const float4*>(&slab[k][c * 4]);
-    s.x += w * v.x;
-    s.y += w * v.y;
-    s.z += w * v.z;
-    s.w += w * v.w;
-    sum += w * sums[k];
+    for (int w = 1; w < WARPS; ++w) join(tops[w], sums[w], slab[w][c]);
   }
+  if (lane >= LANES) return;
   uint2 w = make_uint2(0, 0);
   if (top != -INFINITY) {
     const float inv = 1.f / sum;
@@ -661,10 +694,12 @@ static int step_rows(const MdbPagedAttnArgs& a) {
   const int rows = a.Sq * (a.H / a.pages.Hkv);
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
-// Two CTAs per SM, or one per tile where there are fewer
+// One CTA for each sequence and key head, and nothing to join: the longest has four tiles at most. One token over 300 keys of 8 heads of 128 in 8 bits: see below.
+static bool is_whole(const MdbPagedAttnArgs& a) { return a.pages.most <= 4 * PK; }
+// As many CTAs as the SMs hold (see PagedShape), or one per tile where there are fewer
 static int step_ctas(const MdbPagedAttnArgs& a) {
   const long long tiles = static_cast<long long>(a.pages.B) * a.pages.Hkv * ((a.pages.most + PK - 1) / PK);
-  return static_cast<int>(std::max(1ll, std::min(tiles, 2ll * device_sm_count())));
+  return static_cast<int>(std::max(1ll, std::min(tiles, (step_rows(a) == 8 && a.pages.Dh == 64 ? 3ll : 2ll) * device_sm_count())));
 }
 
 template <int DH, bool E4M3, int NT, int RG>
@@ -674,18 +709,25 @@ static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStr
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !ready[dev])) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DH, E4M3>::BYTES);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedShape<DH, E4M3, NT, RG>::BYTES);
     if (e == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (e != cudaSuccess) return static_cast<int>(e);
+  if (is_whole(a)) {
+    kern<<<a.pages.B * a.pages.Hkv, PagedShape<DH, E4M3, NT, RG>::THREADS, PagedShape<DH, E4M3, NT, RG>::BYTES, st>>>(maps, a, PagedParts{nullptr, nullptr});
+    return static_cast<int>(cudaGetLastError());
+  }
   const int ctas = step_ctas(a);
   constexpr int ROWS = 8 * NT * RG;
   const PagedParts parts = {a.ws, a.ws + 2ll * ctas * ROWS * DH};
-  kern<<<ctas, PS_THREADS, PagedShape<DH, E4M3>::BYTES, st>>>(maps, a, parts);
+  kern<<<ctas, PagedShape<DH, E4M3, NT, RG>::THREADS, PagedShape<DH, E4M3, NT, RG>::BYTES, st>>>(maps, a, parts);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t c;
   memset(&c, 0, sizeof(c));
-  c.gridDim = dim3(a.Sq * a.H, a.pages.B);
+  // Four warps to a row where it has more than eight parts on average. One sequence of 8192 keys, 32 / 8 heads of 128 in 8 bits: see below.
+  const bool many = ctas > 8ll * a.pages.B * a.pages.Hkv;
+  const long long all = static_cast<long long>(a.pages.B) * a.Sq * a.H;
+  c.gridDim = dim3(static_cast<unsigned>(many ? all : (all + 3) / 4));
   c.blockDim = dim3(PJ_THREADS);
   c.stream = st;
   cudaLaunchAttribute at;
@@ -693,7 +735,7 @@ static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStr
   at.val.programmaticStreamSerializationAllowed = 1;
   c.attrs = &at;
   c.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&c, paged_join_kernel<DH>, a, parts, ctas, ROWS));
+  return static_cast<int>(cudaLaunchKernelEx(&c, many ? paged_join_kernel<DH, 4> : paged_join_kernel<DH, 1>, a, parts, ctas, ROWS));
 }
 template <int DH, bool E4M3>
 static int launch_paged(const MdbPagedAttnArgs& a, cudaStream_t st) {
@@ -788,6 +830,7 @@ static int launch_gathered(const MdbPagedAttnArgs& a, cudaStream_t st) {
 extern "C" long long mdb_paged_attention_floats(const MdbPagedAttnArgs* a) {
   if (a->pages.most == 0) return 0;
   if (!mdb::is_step(*a)) return mdb::gathered(*a) + 2ll * a->pages.B;
+  if (mdb::is_whole(*a)) return 0;
   return 2ll * mdb::step_ctas(*a) * mdb::step_rows(*a) * (a->pages.Dh + 2);
 }
 extern "C" int mdb_paged_attention(const MdbPagedAttnArgs* a, cudaStream_t st) {

@@ -80,11 +80,14 @@ def use_native(t: torch.Tensor) -> bool:
     return _loaded or load(True)
 
 
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
+
+
 def direct(*tensors: torch.Tensor) -> bool:
     """Whether nothing but the kernels looks at an operation on these tensors: plain tensors outside every functorch transform
     (vmap, grad, jvp), forward-mode AD level, dispatch mode and trace. Ops that also have a form in torch operations keep to it
     otherwise."""
-    return (all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+    return (_PLAIN.issuperset(map(type, tensors))
             and torch._C._functorch.peek_interpreter_stack() is None and forward_ad._current_level < 0
             and torch._C._len_torch_dispatch_stack() == 0 and not torch.jit.is_tracing() and not torch.compiler.is_compiling())
 

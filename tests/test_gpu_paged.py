@@ -149,7 +149,11 @@ def test_attention(case):
     q, kp, vp, ks, vs, table, kd, vd = _attention_inputs(case)
     out = O.paged_attention(q, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs)
     check_attention(out, q, kd, vd, lengths, str(case))
-    assert torch.equal(O.paged_attention(q, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs, max_len=max(lengths)), out)
+    bounded = O.paged_attention(q, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs, max_len=max(lengths))
+    if (max(lengths) <= 512) == (table.shape[1] * kp.shape[2] <= 512):
+        assert torch.equal(bounded, out)
+    else:       # up to 512 positions a sequence's keys are not shared out, so the sums of one result are added in another order: the same bounds, not the same bits
+        check_attention(bounded, q, kd, vd, lengths, str(case))
     strided = torch.stack((q, q), 3)[:, :, :, 0]
     assert torch.equal(O.paged_attention(strided.transpose(1, 2).contiguous().transpose(1, 2), kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs), out)
     assert torch.equal(O.paged_attention(strided, kp, vp, table, _ints(lengths), k_scale=ks, v_scale=vs), out)
