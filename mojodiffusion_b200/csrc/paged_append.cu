@@ -399,12 +399,13 @@ static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
   if (units > 0x7ffffff0) return -8;
   const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
   const int rows = static_cast<int>(std::min<long long>(P, a.T)), H = a.q != nullptr ? a.H : 0, G = a.pages.Hkv;      // rows of a unit, at most
-  // heads of a block: eight and two, fewer where that leaves fewer than six blocks to an SM
-  AppendGrid grid = {static_cast<int>(units), 8, 2};
+  // heads of a block: sixteen and four, fewer where that leaves fewer than six blocks to an SM (11.7 thousand tokens, 32 / 8 heads of 128: 59.4 us, with eight and two 62.3,
+  // four and one 69.6; 4.4 thousand, 28 / 4 heads of 64, bf16 pages: eight and two 20.5 us, eight and one 22.5)
+  AppendGrid grid = {static_cast<int>(units), 16, 4};
   const auto parts = [&]() { return (H + grid.q_heads - 1) / grid.q_heads + 2 * ((G + grid.kv_heads - 1) / grid.kv_heads); };
   while (grid.q_heads > 1 && units * parts() < 6ll * device_sm_count()) {
     grid.q_heads /= 2;
-    grid.kv_heads = 1;
+    grid.kv_heads = std::max(grid.kv_heads / 2, 1);
   }
   const dim3 blocks(static_cast<unsigned>(units) + spare, parts());
   if (rows <= groups) paged_append_kernel<DH, E4M3, 1><<<blocks, PA_THREADS, 0, st>>>(a, grid);
