@@ -342,7 +342,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       const uint8_t* sk = smem + st * 2 * TILE;
       uint8_t* sv = smem + st * 2 * TILE + TILE;
 #pragma unroll 1
-      for (int k32 = part * WK; k32 < part * WK + WK; k32 += 32) {      // row in the stage
+      for (int k32 = part * WK; k32 < part * WK + WK && rg * WR < rows; k32 += 32) {      // row in the stage; a warp without rows only gives the stages back
         const int kb = tile * PK + k32;                                 // key
         if (kb >= end) break;
         if (kb + 32 > end) {
