@@ -872,8 +872,9 @@ MdbPages pages_of(const Tensor& like, const Tensor& k_pages, const Tensor& v_pag
   p.k = k_pages.data_ptr();
   p.v = v_pages.data_ptr();
   p.table = own.back().data_ptr<int>();
-  p.count = (int)k_pages.size(0); p.Hkv = (int)k_pages.size(1); p.P = (int)k_pages.size(2); p.Dh = (int)k_pages.size(3);
+  p.count = (int)k_pages.size(0); p.Hkv = (int)k_pages.size(1); p.P = (int)k_pages.size(2); p.shift = 0; p.Dh = (int)k_pages.size(3);
   PAGED_CHECK(B < 65536 && table.size(1) < (1ll << 30) / p.P, "fewer than 65536 sequences and 2^30 positions");
+  while (1 << p.shift < p.P) ++p.shift;
   p.B = (int)B;
   p.width = (int)table.size(1);
   p.most = (int)std::min<int64_t>(most < 0 ? 1ll << 30 : most, table.size(1) * p.P);
@@ -971,6 +972,8 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.pages = pages_of(q, k_pages, v_pages, table, k_scale, v_scale, q.size(0), max_len.has_value() ? *max_len : -1, own);
   PAGED_CHECK(q.size(2) % a.pages.Hkv == 0, "the pages need a number of heads that divides q's");
   PAGED_CHECK(kv_len.scalar_type() == at::kInt && kv_len.dim() == 1 && kv_len.size(0) == a.pages.B && kv_len.device() == q.device(), "kv_len must be int32 [B] on q's device");
+  // the kernels number the tiles of 128 keys of all sequences and heads in 32 bits
+  PAGED_CHECK((int64_t)a.pages.B * a.pages.Hkv * ((a.pages.most + 127) / 128) < 1ll << 31, "fewer than 2^31 tiles of 128 keys: give max_len");
   const double factor = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3));
   PAGED_CHECK(factor >= 0x1p-126 && factor <= 0x1p126, "scale must be positive, and normal in fp32");
   paged_no_gradient({&q, &k_pages, &v_pages});

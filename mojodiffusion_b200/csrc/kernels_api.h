@@ -253,7 +253,7 @@ typedef struct MdbPages {
   const int* table;                                    // [B, width]
   long long k_strides[2], v_strides[2];                // elements between pages and between heads; a head's [P, Dh] is contiguous
   long long scale_strides[2];                          // between pages, of either
-  int count, width, P, Hkv, Dh, B;
+  int count, width, P, shift, Hkv, Dh, B;              // P = 2^shift
   int most;                                            // positions of a sequence, at most: width * P, or fewer
   int* status;
 } MdbPages;

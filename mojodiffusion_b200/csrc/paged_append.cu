@@ -153,14 +153,14 @@ __device__ __forceinline__ void rows_of(const MdbPagedAppendArgs& a, int b, long
 }
 // By a whole warp: units are numbered sequence after sequence, a page after the other
 __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int unit) {
-  const int lane = threadIdx.x & 31, P = a.pages.P;
+  const int lane = threadIdx.x & 31, P = a.pages.P, shift = a.pages.shift;
   AppendUnit u = {0, 0, 0, 0, 0, 0};
   int before = 0;
   for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
     long long first = 0;
     int length = 0, start = 0;
     if (b0 + lane < a.pages.B) rows_of(a, b0 + lane, first, length, start);
-    const int mine = length > 0 ? (start + length - 1) / P - start / P + 1 : 0;
+    const int mine = length > 0 ? ((start + length - 1) >> shift) - (start >> shift) + 1 : 0;
     int upto = mine;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -175,7 +175,7 @@ __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int
       start = __shfl_sync(0xffffffffu, start, at);
       const int j = unit - before - __shfl_sync(0xffffffffu, upto - mine, at);
       u.b = b0 + at;
-      u.index = start / P + j;
+      u.index = (start >> shift) + j;
       const int from = max(u.index * P, start), to = static_cast<int>(min(static_cast<long long>(u.index + 1) * P, static_cast<long long>(start) + length));
       u.slot = from - u.index * P;
       u.count = to - from;
@@ -338,7 +338,7 @@ paged_append_token_kernel(const __grid_constant__ MdbPagedAppendArgs a) {
   uint4 raw[2];
   if (in) Row::fetch(raw, is_q ? static_cast<const __nv_bfloat16*>(a.q) + b * a.q_strides[0] + g * a.q_strides[1]
                       : is_v ? static_cast<const __nv_bfloat16*>(a.v) + b * a.v_strides[0] + g * a.v_strides[1] : static_cast<const __nv_bfloat16*>(a.k) + b * a.k_strides[0] + g * a.k_strides[1], l);
-  const int page = p >= 0 && p < a.positions ? page_of(a.pages, b, p / a.pages.P) : -1, slot = p & (a.pages.P - 1);
+  const int page = p >= 0 && p < a.positions ? page_of(a.pages, b, p >> a.pages.shift) : -1, slot = p & (a.pages.P - 1);
   unsigned char* scale = E4M3 && page >= 0 && !is_q ? (is_v ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[is_v] + g : nullptr;
   const int before = scale != nullptr && slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
   const void* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;

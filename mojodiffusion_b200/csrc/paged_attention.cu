@@ -28,7 +28,7 @@
 
 namespace mdb {
 
-constexpr int PK = 128;                                       // keys of a tile
+constexpr int PK = 128;                                       // keys of a tile: no more than a page has, or several pages
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 struct alignas(64) PagedMaps {
@@ -39,7 +39,7 @@ struct alignas(64) PagedMaps {
 template <int DH, bool E4M3, int NT, int RG> struct PagedShape {
   static constexpr int WARPS = 4;                                     // that multiply
   static constexpr int THREADS = (WARPS + 1) * 32;
-  static constexpr int COLS = 32;                                     // columns that the warps join at a time
+  static constexpr int COLS = 64 / NT;                                // columns that the warps join at a time
   static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
   static constexpr int CTAS = NT == 1 && DH == 64 ? 3 : 2;            // per SM, with 192 KB of stages
   static constexpr int STAGES = 192 * 1024 / CTAS / (2 * TILE);
@@ -78,21 +78,31 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 
 // ---- the line of tiles: sequence after sequence, key head after key head, tile after tile ----
 __device__ __forceinline__ int paged_length(const MdbPagedAttnArgs& a, int b) { return min(max(a.kv_len[b], 0), a.pages.most); }
-__device__ __forceinline__ long long paged_tiles(const MdbPagedAttnArgs& a) {      // of one key head; by a whole warp
-  long long total = 0;
+__device__ __forceinline__ int paged_tiles(const MdbPagedAttnArgs& a) {      // of one key head; by a whole warp
+  int total = 0;
   for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
     const int b = b0 + (threadIdx.x & 31);
     total += __reduce_add_sync(0xffffffffu, b < a.pages.B ? static_cast<unsigned>(paged_length(a, b) + PK - 1) / PK : 0u);
   }
   return total;
 }
+// The line's shares: `ctas` of them, the first `more` with a tile more than the others. 32-bit divisions only, for they stand before the first load: with those of 64 bits the
+// first tile was there 11300 cycles after a CTA's start, without them 10300 (cold caches), and 32 tokens over 0 to 16384 positions took 87 us instead of 80.
+struct PagedShares {
+  int ctas, each, more;
+  __device__ __forceinline__ PagedShares(int line, int grid) : ctas(min(grid, line)), each(line / max(ctas, 1)), more(line - each * ctas) {}
+  __device__ __forceinline__ int first(int cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ int cta_of(int tile) const {
+    const int early = more * (each + 1);
+    return tile < early ? tile / (each + 1) : more + (tile - early) / each;
+  }
+};
 struct PagedPlace {
   int b, g, t, length, tiles;
   // of tile `at` on the line; by a whole warp
-  __device__ __forceinline__ void seek(const MdbPagedAttnArgs& a, long long at) {
-    const int lane = threadIdx.x & 31;
-    const long long target = at / a.pages.Hkv;
-    long long before = 0;
+  __device__ __forceinline__ void seek(const MdbPagedAttnArgs& a, int at) {
+    const int lane = threadIdx.x & 31, target = at / a.pages.Hkv;
+    int before = 0;
     b = 0;
     length = tiles = 0;
     for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
@@ -114,9 +124,9 @@ struct PagedPlace {
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const long long rest = at - before * a.pages.Hkv;
-    g = tiles > 0 ? static_cast<int>(rest / tiles) : 0;
-    t = tiles > 0 ? static_cast<int>(rest - static_cast<long long>(g) * tiles) : 0;
+    const int rest = at - before * a.pages.Hkv;
+    g = tiles > 0 ? rest / tiles : 0;
+    t = rest - g * tiles;
   }
   __device__ __forceinline__ void next_segment(const MdbPagedAttnArgs& a) {
     t = 0;
@@ -155,6 +165,10 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const MdbPages& pg = a.pages;
+  if (warp == WARPS && lane == 0) {
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], E4M3 ? 2 : 1);      // the copies, and the scales
@@ -181,27 +195,27 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       return;
     }
   } else {
-    const long long line = paged_tiles(a) * pg.Hkv, ctas = min(static_cast<long long>(gridDim.x), line);
-    const long long line_first = blockIdx.x < ctas ? line * blockIdx.x / ctas : 0;
+    const PagedShares shares(paged_tiles(a) * pg.Hkv, gridDim.x);
+    const int cta = blockIdx.x, line_first = cta < shares.ctas ? shares.first(cta) : 0;
     at.seek(a, line_first);
     __syncthreads();
-    if (blockIdx.x >= ctas) return;
-    n = static_cast<int>(line * (blockIdx.x + 1) / ctas - line_first);
+    if (cta >= shares.ctas) return;
+    n = shares.first(cta + 1) - line_first;
   }
 
   if (warp == WARPS) {
-    const int per_tile = max(PK / pg.P, 1), rows = min(pg.P, PK);            // boxes of a tile, keys of a box
+    const int per_tile = PK >> pg.shift, rows = pg.P;            // boxes of a tile, keys of a box
     const uint32_t box_bytes = rows * DH * (E4M3 ? 1 : 2);
     int window = 0, page = -1;                                              // this lane's place of the table: window + lane
     uint32_t sc = 0;
     bool ok = true, fresh = true;
     int i = 0;
     for (; i < n; ++i) {
-      const int first_index = static_cast<int>(static_cast<long long>(at.t) * PK / pg.P);
+      const int first_index = at.t * PK >> pg.shift;
       if (fresh || first_index + per_tile > window + 32) {
         window = first_index;
         const int index = window + lane;
-        const bool needed = index < (at.length + pg.P - 1) / pg.P;
+        const bool needed = index <= (at.length - 1) >> pg.shift;
         page = needed ? page_of(pg, at.b, index) : -1;
         if (needed && page < 0) report_status(pg.status, STATUS_BOUNDS, 182, at.b);
         if (E4M3) {
@@ -216,27 +230,26 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
         if (lane == 0) report_status(pg.status, STATUS_TIMEOUT, 183, i);
         break;
       }
-      const int keys = min(at.length - at.t * PK, PK), boxes = (keys + rows - 1) / rows;
+      const int keys = min(at.length - at.t * PK, PK), boxes = (keys + rows - 1) >> pg.shift;
       const int mine = __shfl_sync(0xffffffffu, page, (first_index - window + min(lane, per_tile - 1)) & 31);
       __syncwarp();
       if (lane == 0) mbar_expect_tx(&full[st], 2 * boxes * box_bytes);
       __syncwarp();
       if (lane < boxes) {
-        const int row = pg.P > PK ? at.t * PK % pg.P : 0;
         uint8_t* to = smem + st * 2 * TILE;
         if (E4M3) {
-          tma_load_4d(to + lane * box_bytes, &maps.k, &full[st], 0, row * DH / 128, at.g, mine);
-          tma_load_4d(to + TILE + lane * box_bytes, &maps.v, &full[st], 0, row * DH / 128, at.g, mine);
+          tma_load_4d(to + lane * box_bytes, &maps.k, &full[st], 0, 0, at.g, mine);
+          tma_load_4d(to + TILE + lane * box_bytes, &maps.v, &full[st], 0, 0, at.g, mine);
         } else {
 #pragma unroll
           for (int d = 0; d < DH / 64; ++d) {
-            tma_load_4d(to + d * BOX + lane * rows * 128, &maps.k, &full[st], d * 64, row, at.g, mine);
-            tma_load_4d(to + TILE + d * BOX + lane * rows * 128, &maps.v, &full[st], d * 64, row, at.g, mine);
+            tma_load_4d(to + d * BOX + lane * rows * 128, &maps.k, &full[st], d * 64, 0, at.g, mine);
+            tma_load_4d(to + TILE + d * BOX + lane * rows * 128, &maps.v, &full[st], d * 64, 0, at.g, mine);
           }
         }
       }
       if (E4M3) {      // behind the copies, which need not wait for them
-        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 7) * 16) / pg.P - window) & 31);
+        const uint32_t s = __shfl_sync(0xffffffffu, sc, ((at.t * PK + (lane & 7) * 16 >> pg.shift) - window) & 31);
         if (lane < PK / 16) scales[st][lane] = make_uchar2(s & 255, s >> 8);
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[st]);
@@ -608,18 +621,16 @@ paged_join_kernel(const __grid_constant__ MdbPagedAttnArgs a, const PagedParts p
   const bool in = row < static_cast<long long>(a.pages.B) * per;
   const int b = in ? static_cast<int>(row / per) : 0, rest = in ? static_cast<int>(row - static_cast<long long>(b) * per) : 0, h = rest % a.H, i = rest / a.H;
   const int rep = a.H / a.pages.Hkv, g = h / rep, r = i * rep + h % rep;
-  long long before = 0, total = 0;                    // tiles of a key head before this sequence, in all
+  int before = 0, total = 0;                          // tiles of a key head before this sequence, in all
   for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
     const unsigned n = b0 + lane < a.pages.B ? static_cast<unsigned>(paged_length(a, b0 + lane) + PK - 1) / PK : 0u;
     total += __reduce_add_sync(0xffffffffu, n);
     before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? n : 0u);
   }
-  const int tiles = (paged_length(a, b) + PK - 1) / PK;
-  const long long line = max(total * a.pages.Hkv, 1ll), u0 = before * a.pages.Hkv + static_cast<long long>(g) * tiles, u1 = u0 + tiles;
-  const long long ctas = min(static_cast<long long>(grid), line);
-  // CTA k has the tiles from line k / ctas on
-  const int first = static_cast<int>(((u0 + 1) * ctas - 1) / line), last = static_cast<int>((max(u1, 1ll) * ctas - 1) / line);
-  const bool first_of_all = line * first / ctas == u0;
+  const int tiles = (paged_length(a, b) + PK - 1) / PK, u0 = before * a.pages.Hkv + g * tiles;
+  const PagedShares shares(max(total * a.pages.Hkv, 1), grid);
+  const int first = shares.cta_of(u0), last = shares.cta_of(u0 + max(tiles, 1) - 1);
+  const bool first_of_all = shares.first(first) == u0;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.o) + b * a.o_strides[0] + i * a.o_strides[1] + h * a.o_strides[2];
   asm volatile("griddepcontrol.wait;" ::: "memory");      // by all: this kernel must not end before the one whose parts it joins
   if (in && tiles == 0 && group == 0) *reinterpret_cast<uint2*>(out + c * 4) = make_uint2(0, 0);
@@ -763,14 +774,14 @@ paged_gather_kernel(const __grid_constant__ MdbPagedAttnArgs a, __nv_bfloat16* _
   }
   for (long long e = blockIdx.x * 256ll + threadIdx.x; e < static_cast<long long>(length) * per_key; e += gridDim.x * 256ll) {
     const int j = static_cast<int>(e / per_key), rest = static_cast<int>(e - static_cast<long long>(j) * per_key), g = rest / LANES, c = rest % LANES * 16;
-    const int page = page_of(pg, b, j / pg.P);
+    const int page = page_of(pg, b, j >> pg.shift);
     if (page < 0) report_status(pg.status, STATUS_BOUNDS, 185, b);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
       if (page >= 0) {
         const long long* s = kv ? pg.v_strides : pg.k_strides;
-        const long long from = page * s[0] + g * s[1] + (j % pg.P) * DH + c;
+        const long long from = page * s[0] + g * s[1] + (j & (pg.P - 1)) * DH + c;
         if (E4M3) {
           const float f = scale_value((kv ? pg.v_scale : pg.k_scale)[page * pg.scale_strides[kv] + g]);
           const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(kv ? pg.v : pg.k) + from);
