@@ -188,18 +188,20 @@ __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int
   return u;
 }
 
-// Heads h0 .. hn - 1 of the rows behind the last sequence come out as zeros; by the blocks from `units` on
+// Heads h0 .. hn - 1 of the rows before the first sequence and behind the last one come out as zeros; by the blocks from `units` on
 template <int DH> __device__ __forceinline__ void clear_rows_of_none(const MdbPagedAppendArgs& a, int units, __nv_bfloat16* to, int heads, int h0, int hn) {
   using Row = AppendRow<DH>;
   constexpr int GROUPS = PA_THREADS / Row::LANES;
-  const long long end = min(max(static_cast<long long>(a.cu[a.pages.B]), 0ll), a.T);
+  const long long first = min(max(static_cast<long long>(a.cu[0]), 0ll), a.T), end = min(max(static_cast<long long>(a.cu[a.pages.B]), first), a.T);
   Row r;
   r.clear();
-  for (long long t = end + (static_cast<long long>(blockIdx.x) - units) * GROUPS + threadIdx.x / Row::LANES; t < a.T; t += static_cast<long long>(gridDim.x - units) * GROUPS)
+  for (long long i = (static_cast<long long>(blockIdx.x) - units) * GROUPS + threadIdx.x / Row::LANES; i < first + a.T - end; i += static_cast<long long>(gridDim.x - units) * GROUPS) {
+    const long long t = i < first ? i : i - first + end;
     for (int h = h0; h < hn; ++h) r.store_bf16(to + (t * heads + h) * DH, threadIdx.x % Row::LANES);
+  }
 }
 
-// grid: units, then rows behind the last sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
+// grid: units, then rows of no sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
 // few heads, so a block has several of them. Queries are turned one row of a group of lanes after the other, two heads at a time; of keys and values a block needs a head's rows
 // of the whole unit at once, for its scale.
 struct AppendGrid {
@@ -397,7 +399,7 @@ static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
   const int B = a.pages.B, P = a.pages.P, groups = PA_THREADS / AppendRow<DH>::LANES;
   const long long units = std::min(a.T, a.T / P + 2ll * B);
   if (units > 0x7ffffff0) return -8;
-  const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 0;      // blocks for rows behind the last sequence
+  const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 0;      // blocks for rows of no sequence
   const int rows = static_cast<int>(std::min<long long>(P, a.T)), H = a.q != nullptr ? a.H : 0, G = a.pages.Hkv;      // rows of a unit, at most
   // heads of a block: sixteen and four, fewer where that leaves fewer than six blocks to an SM (11.7 thousand tokens, 32 / 8 heads of 128: 59.4 us, with eight and two 62.3,
   // four and one 69.6; 4.4 thousand, 28 / 4 heads of 64, bf16 pages: eight and two 20.5 us, eight and one 22.5)

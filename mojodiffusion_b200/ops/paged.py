@@ -66,11 +66,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     these and the normalised, rotated keys [T, Hkv, Dh] in k's type, for the attention of whole prompts.
 
     k, v [T, Hkv, Dh] and q [T, H, Dh] (any strides) hold the sequences' new rows one behind the other: sequence b has the rows
-    cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1]; None: one row each, T = B), which take the positions start[b], start[b] + 1, ... (int32 [B]).
+    cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1], not falling; None: one row each, T = B), which take the positions start[b], start[b] + 1, ... (int32 [B]).
     Per head: root-mean-square norm with the weight ``q_norm`` / ``k_norm`` [Dh] where given (``eps`` inside the root), then the halves (a, b) become
     (a cos - b sin, b cos + a sin) with row p of ``cos`` / ``sin`` [positions, Dh / 2] (fp32) for position p; values stay as they are. All in fp32, rounded once.
     A page that gets its first token takes its scales anew, whatever it held before. Infinities in k or v become NaN in 8 bits and do not count for the scale.
-    Rows behind the last sequence are not read, and zero in the results. A page that tokens go to must belong to one sequence.
+    Rows of no sequence are not read, and zero in the results. A page that tokens go to must belong to one sequence.
     """
     if _kernels(k, k_pages, v, q, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q_norm, k_norm):
         found = native.ops().paged_append(k, v, k_pages, v_pages, block_table, start, cos, sin, cu_seqlens, k_scale, v_scale, q, q_norm, k_norm, eps, keys)
@@ -113,7 +113,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     The pages of sequence b hold ``kv_len[b]`` positions (int32 [B]), those of the queries among them: query row i stands at position kv_len[b] - Sq + i and sees
     the keys up to its own position. Query head h reads key head ``h // (H // Hkv)``. A row before the first position is zero. ``max_len`` (int): no sequence is longer, and
     what lies behind is not seen; parts of prompts take a workspace of this size (all that the table has room for by default). Slots behind a sequence's
-    end are not read: they may hold anything.
+    end are not read: they may hold anything. A value of infinity that a query sees gives NaN.
     """
     if max_len is not None and (type(max_len) is not int or max_len < 0):
         raise ValueError("paged_attention: max_len must be an int of at least 0")

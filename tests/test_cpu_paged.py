@@ -41,6 +41,17 @@ def test_append(case):
     check_append(before, (kp, vp, ks, vs), out, k, v, q, table, start, cu, cos, sin, qn, kn, 1e-6, str(case))
 
 
+def test_append_rows_of_no_sequence():
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(9, n, 16, generator=g) for n in (2, 1, 1))
+    q[[0, 1, 8]] = k[[0, 1, 8]] = torch.nan
+    (kp, ks), (vp, vs) = pool(2, 1, 16, 16, True, "cpu", 2), pool(2, 1, 16, 16, True, "cpu", 3)
+    cos, sin = angles(20, 16, "cpu")
+    out, keys = O.paged_append(k, v, kp, vp, _ints([[1], [0]]), _ints([0, 3]), cos, sin, cu_seqlens=_ints([2, 5, 8]), k_scale=ks, v_scale=vs, q=q, keys=True)
+    for t in (out, keys):
+        assert not t[:2].any() and not t[8:].any() and torch.isfinite(t).all() and t[2:8].all()
+
+
 def test_append_scale_values():
     """Zeros, values at the border of a scale, infinities and NaN; a larger token later, and a new owner of a page."""
     P, D = 16, 16

@@ -79,6 +79,21 @@ def test_append(case):
         assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize("eight", [True, False])
+def test_append_rows_of_no_sequence(eight):
+    q, k, v = (_normal(90, n, 64, seed=n) for n in (6, 2, 2))
+    for t in (q, k, v):
+        t[:20] = t[75:] = torch.nan
+    (kp, ks), (vp, vs) = pool(6, 2, 16, 64, eight, DEV, 2), pool(6, 2, 16, 64, eight, DEV, 3)
+    cos, sin = angles(60, 64, DEV)
+    out, keys = O.paged_append(k, v, kp, vp, _ints([[1, 2, 4, 0], [0, 3, 0, 0]]), _ints([0, 3]), cos, sin, cu_seqlens=_ints([20, 60, 75]), k_scale=ks, v_scale=vs, q=q, keys=True)
+    for t in (out, keys):
+        assert not t[:20].any() and not t[75:].any() and torch.isfinite(t).all()
+    part = O.paged_append(k[20:75], v[20:75], kp, vp, _ints([[1, 2, 4, 0], [0, 3, 0, 0]]), _ints([0, 3]), cos, sin, cu_seqlens=_ints([0, 40, 55]), k_scale=ks, v_scale=vs, q=q[20:75], keys=True)
+    assert torch.equal(part[0], out[20:75]) and torch.equal(part[1], keys[20:75])
+    O.check_status()
+
+
 def test_append_values_that_are_not_finite_and_later_larger_ones():
     P, D, G = 16, 64, 2
     (kp, ks), (vp, vs) = pool(3, G, P, D, True, DEV, 0), pool(3, G, P, D, True, DEV, 1)
