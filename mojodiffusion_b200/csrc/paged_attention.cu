@@ -435,20 +435,23 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
         const bool whole = kb + 31 <= start && kb + 32 <= end;
         bool raise = false;
         float f[NT][2];
+        float2 mul[2][NT];                // of the rows 2 t, 2 t + 1; not 0, for -inf * 0 is not -inf
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+          for (int s = 0; s < 2; ++s) {
+            mul[s][nt] = make_float2(fmaxf(sl2[nt][0] * ks[s], 0x1p-126f), fmaxf(sl2[nt][1] * ks[s], 0x1p-126f));
+            if (!whole) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[s][nt][e] *= sl2[nt][e & 1] * ks[s];
-              if (!whole) {
+              for (int e = 0; e < 4; ++e) {
                 const int j = kb + s * 16 + key_of(gq) + 8 * (e >> 1);
                 if (!(j <= p_row[nt][e & 1] && j < end)) x[s][nt][e] = -INFINITY;
               }
-              top[e & 1] = paged_max(top[e & 1], x[s][nt][e]);
             }
+            top[0] = paged_max(top[0], paged_max(x[s][nt][0], x[s][nt][2]) * mul[s][nt].x);
+            top[1] = paged_max(top[1], paged_max(x[s][nt][1], x[s][nt][3]) * mul[s][nt].y);
+          }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
 #pragma unroll
@@ -477,23 +480,29 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
         // P^T as the B operand: keys 2 t, 2 t + 1 (and 8 more) of row gq, which is the transpose of what the lane has
         uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 less = make_float2(m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]);
+          float2 sum = make_float2(l[nt][0], l[nt][1]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const float p0 = ex2_approx(x[s][nt][2 * y] - (m[nt][0] == -INFINITY ? 0.f : m[nt][0])), p1 = ex2_approx(x[s][nt][2 * y + 1] - (m[nt][1] == -INFINITY ? 0.f : m[nt][1]));
-              l[nt][0] += p0;
-              l[nt][1] += p1;
+              const float2 t = ffma2(make_float2(x[s][nt][2 * y], x[s][nt][2 * y + 1]), mul[s][nt], less);
+              const float2 p = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+              sum = fadd2(sum, p);
               if (E4M3) {
-                ph[s][nt][y] = paged_transpose(pack_f16x2(p0 * into[s], p1 * into[s]));
+                const float2 q2 = fmul2(p, make_float2(into[s], into[s]));
+                ph[s][nt][y] = paged_transpose(pack_f16x2(q2.x, q2.y));
               } else {
-                const uint32_t h = pack_bf16x2(p0, p1);
-                const float2 back = unpack_bf16x2(h);
+                const uint32_t h = pack_bf16x2(p.x, p.y);
+                const float2 low = ffma2(unpack_bf16x2(h), make_float2(-1.f, -1.f), p);
                 ph[s][nt][y] = paged_transpose(h);
-                pl[s][nt][y] = paged_transpose(pack_bf16x2(p0 - back.x, p1 - back.y));
+                pl[s][nt][y] = paged_transpose(pack_bf16x2(low.x, low.y));
               }
             }
+          l[nt][0] = sum.x;
+          l[nt][1] = sum.y;
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int kr = k32 + s * 16;
