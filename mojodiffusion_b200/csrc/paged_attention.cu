@@ -20,6 +20,11 @@
 // bf16: the products are bf16 ones; a probability goes into its product as two bf16 terms, so only the output is rounded.
 //
 // Keys behind the sequence's end are masked and their values zeroed in shared memory before the product (0 * NaN is not 0).
+//
+// What bounds it: memory where sequences are long. 4 tokens over 70001 to 131072 positions, 32 / 8 heads of 128, e4m3: 129 us, 5.95 TB/s (0.91 of the measured rate; bf16, 16 over 16384: 183 us, 5.86 TB/s). 32 over 0 to 16384:
+// 79 us, 4.6 TB/s: 12000 cycles to a CTA's first tile (lengths, table, scales and data one after the other), then 3200 a tile of which it works 1300. Few rows leave latencies: one token over 300
+// positions 7 us on the device. With more than 16 rows the turns of a warp: 40 rows over bf16 pages, heads of 64, 5600 cycles a tile of 128 keys, 26 us for 8 sequences of 17 to 4091.
+// Keys as the rows of the products (S^T) took 131 us in the first case where the queries' as rows took 169, for up to 8 rows fill half of 16.
 #include "gemm_api.h"
 #include "paged.cuh"
 
@@ -41,7 +46,8 @@ template <int DH, bool E4M3, int NT, int RG> struct PagedShape {
   static constexpr int THREADS = (WARPS + 1) * 32;
   static constexpr int COLS = 64 / NT;                                // columns that the warps join at a time
   static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
-  static constexpr int CTAS = NT == 1 && DH == 64 ? 3 : 2;            // per SM, with 192 KB of stages
+  // per SM, with 192 KB of stages. 16 tokens over 16384, 64 / 8 heads of 64: three CTAs 76 us, two 94; 4 over 131072, heads of 128, where three would have two stages each: 150 and 143.
+  static constexpr int CTAS = NT == 1 && DH == 64 ? 3 : 2;
   static constexpr int STAGES = 192 * 1024 / CTAS / (2 * TILE);
   static constexpr int SLAB = WARPS * 8 * NT * COLS * 4;
   static constexpr int BYTES = STAGES * 2 * TILE + SLAB + 1024;
@@ -714,7 +720,8 @@ static int step_rows(const MdbPagedAttnArgs& a) {
   const int rows = a.Sq * (a.H / a.pages.Hkv);
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
-// One CTA for each sequence and key head, and nothing to join: the longest has four tiles at most. One token over 300 keys of 8 heads of 128 in 8 bits: see below.
+// One CTA for each sequence and key head, and nothing to join: the longest has four tiles at most. In us, so / shared out and joined: one token over 300 positions of 8 heads of
+// 128 10.2 / 12.3, 8 over 500 12.3 / 16.4, 64 over 500 28.7 / 30.7, 16 over 300 of 8 heads of 64 10.2 / 14.4; with four tiles, 512 positions, 12.3 / 12.3.
 static bool is_whole(const MdbPagedAttnArgs& a) { return a.pages.most <= 4 * PK; }
 // As many CTAs as the SMs hold (see PagedShape), or one per tile where there are fewer
 static int step_ctas(const MdbPagedAttnArgs& a) {
@@ -744,7 +751,7 @@ static int launch_step(const PagedMaps& maps, const MdbPagedAttnArgs& a, cudaStr
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t c;
   memset(&c, 0, sizeof(c));
-  // Four warps to a row where it has more than eight parts on average. One sequence of 8192 keys, 32 / 8 heads of 128 in 8 bits: see below.
+  // Four warps to a row where it has more than eight parts on average, as one long sequence has: there a warp alone would have ten loads behind one another.
   const bool many = ctas > 8ll * a.pages.B * a.pages.Hkv;
   const long long all = static_cast<long long>(a.pages.B) * a.Sq * a.H;
   c.gridDim = dim3(static_cast<unsigned>(many ? all : (all + 3) / 4));
@@ -815,6 +822,7 @@ paged_gather_kernel(const __grid_constant__ MdbPagedAttnArgs a, __nv_bfloat16* _
   }
 }
 
+// Up to 64 rows. 8 sequences of 4000 positions, 8 key heads of 128, 32 rows: 50 us, where the gather alone has 262 MB to write and to read again.
 static bool is_step(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.Sq) * (a.H / a.pages.Hkv) <= 64; }
 static long long gathered(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.pages.B) * a.pages.most * a.pages.Hkv * a.pages.Dh; }      // values
 

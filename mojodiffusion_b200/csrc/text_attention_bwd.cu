@@ -72,7 +72,7 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
   }
 };
 
-// PACKED: a block is a unit of 128 rows of one sequence
+// PACKED: a block is a unit of 128 rows of one sequence. 4996 rows in nine sequences of 20 to 1531, 32 / 8 heads of 128: dq 141 us, dk and dv 188 (tensor pipe 29 and 42 %)
 template <int DH, bool KEYS, bool BIAS, bool PACKED>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
 text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextParts parts) {

@@ -20,6 +20,11 @@
 //
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
+// PACKED: an item is a unit of one sequence (see text_unit); coordinates and rows count from the sequence's first row. A tile holds rows of one sequence only, at the cost of tiles that are
+// not full: rows of several sequences in a tile would multiply each other's values by zero, and 0 * NaN would carry one sequence's NaN into another. 10155 tokens in six sequences of 301
+// to 4096, 32 / 8 heads of 128: 264 us (872 TFLOP/s; equal lengths take 1.01 to 1.05 of the batched form's time); 16 sequences of 7 to 300, 64 / 8 heads of 64, window 128: 33 us,
+// a CTA with one key tile 6.7 us of which 2.6 before its first scores.
+//
 // What bounds it: the latency of a tile's way from the scores through the softmax to the next product; no unit is busy half of the time. 8192 tokens,
 // 32 / 8 heads of 128, window 1024 with 4 first keys: 162 us, 797 TFLOP/s of visible pairs, 985 with the masked 19 % of the tiles (tensor pipe active 46 % of
 // the cycles, issue slots 43 %, special-function unit 35 %). 8 x 512 tokens, 64 heads of 64 with a table: 80 us, 320 TFLOP/s (17 %, 43 %, 36 %); one CTA
