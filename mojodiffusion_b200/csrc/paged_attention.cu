@@ -822,7 +822,7 @@ paged_gather_kernel(const __grid_constant__ MdbPagedAttnArgs a, __nv_bfloat16* _
   }
 }
 
-// Up to 64 rows. 8 sequences of 4000 positions, 8 key heads of 128, 32 rows: 50 us, where the gather alone has 262 MB to write and to read again.
+// Up to 64 rows. 8 sequences of 4000 positions, 8 key heads of 128, 32 rows: 50 us, where the gather alone has 131 MB to write and to read again.
 static bool is_step(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.Sq) * (a.H / a.pages.Hkv) <= 64; }
 static long long gathered(const MdbPagedAttnArgs& a) { return static_cast<long long>(a.pages.B) * a.pages.most * a.pages.Hkv * a.pages.Dh; }      // values
 
