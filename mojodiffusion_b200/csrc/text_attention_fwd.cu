@@ -20,6 +20,10 @@
 //
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
+// FINE (packed, with a backward pass to come): in items whose rows have few keys a probability goes into its product as two bf16 terms, the second one in the half of the scores' columns that
+// the first leaves free. There ds = p (dp - do . o) is a difference of nearly equal terms, and the rounding of p shows in it through o: dq and dk of 23 sequences of two or three tokens
+// were off by 0.0026 of their size, of three with a window of 2 by 0.0030; the rounding of ds and of the result alone make 0.0024.
+//
 // PACKED: an item is a unit of one sequence (see text_unit); coordinates and rows count from the sequence's first row. A tile holds rows of one sequence only, at the cost of tiles that are
 // not full: rows of several sequences in a tile would multiply each other's values by zero, and 0 * NaN would carry one sequence's NaN into another. 10155 tokens in six sequences of 301
 // to 4096, 32 / 8 heads of 128: 264 us (872 TFLOP/s; equal lengths take 1.01 to 1.05 of the batched form's time); 16 sequences of 7 to 300, 64 / 8 heads of 64, window 128: 33 us,
@@ -32,11 +36,13 @@
 #include "text_attention.cuh"
 #include "gemm_api.h"
 
+#include <algorithm>
 #include <string.h>
 
 namespace mdb {
 
 constexpr int TQ = 128;                              // rows of a query tile
+constexpr int TXT_FEW_KEYS = 256;
 
 template <int DH> struct FwdShape {
   static constexpr int TK = DH == 64 ? 64 : 128;     // keys of a key tile
@@ -66,11 +72,12 @@ struct TextTiles {
 
 // One work item, seen by a whole warp: its query tiles, and the key tiles that any of them visits: [0, ns) and then [lo, lo + n_kv - ns).
 // Lane l looks at query tile l % 2.
-template <int DH, bool BIAS, bool PACKED> struct TextItem {
+template <int DH, bool BIAS, bool PACKED, bool FINE> struct TextItem {
   using Shape = FwdShape<DH>;
   static constexpr int TK = Shape::TK;
   int batch, head, q0;        // of the first tile
   int base, rows;             // packed: first row and length of the sequence; else 0 and Sq
+  bool fine;                  // FINE: no row has more than TXT_FEW_KEYS keys
   TextSight sight;
   TextKeys all;               // keys that any row sees
   int t_lo, t_hi;             // key tiles of this lane's query tile: [t_lo, t_hi), and of [0, ns) those below t_hi
@@ -105,6 +112,7 @@ template <int DH, bool BIAS, bool PACKED> struct TextItem {
       block = l.row_items - 1 - block;
     }
     q0 = block * l.blocks * TQ;
+    fine = FINE && min(a.window, min(q0 + l.blocks * TQ, rows)) <= TXT_FEW_KEYS;
     if (PACKED) sight = {rows, 0};
     else sight = text_sight(a, batch);
     const int t = threadIdx.x & 1, first = tile_q0(q0, t, l);
@@ -131,7 +139,7 @@ template <int N> struct Int {
   static constexpr int value = N;
 };
 
-template <int DH, bool BIAS, bool PACKED>
+template <int DH, bool BIAS, bool PACKED, bool FINE>
 __global__ void __launch_bounds__(FwdShape<DH>::THREADS, FwdShape<DH>::CTAS)
 text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextTiles tiles) {
   using Shape = FwdShape<DH>;
@@ -160,7 +168,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   const int first = RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * blockIdx.x / gridDim.x) : blockIdx.x;
   const int last = ONE ? first + 1 : RANGE ? static_cast<int>(static_cast<long long>(tiles.items) * (blockIdx.x + 1) / gridDim.x) : tiles.items;
   const int step = ONE || RANGE ? 1 : gridDim.x;
-  TextItem<DH, BIAS, PACKED> w;
+  TextItem<DH, BIAS, PACKED, FINE> w;
 
   // The TMA warp makes the barriers and starts loading while the others get ready: nobody else touches either before __syncthreads.
   if (warp == 0) {
@@ -292,6 +300,13 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
           const int kk = part * 4 + k2;
           umma_f16_ts(o_col + u * DH, s_col + u * TK + kk * 8, v_desc + ((st * Shape::K_BYTES + kk * 2048) >> 4), idesc_pv, kk == 0 ? more : 1u);
         }
+        if (FINE && w.fine) {
+#pragma unroll
+          for (int k2 = 0; k2 < 4; ++k2) {
+            const int kk = part * 4 + k2;
+            umma_f16_ts(o_col + u * DH, s_col + u * TK + TK / 2 + kk * 8, v_desc + ((st * Shape::K_BYTES + kk * 2048) >> 4), idesc_pv, 1u);
+          }
+        }
       };
       int n_items = 0, n_tiles = 0;
       uint32_t done[2] = {0, 0}, outs[2] = {0, 0};      // key tiles, and items with keys, that either query tile has behind it
@@ -398,6 +413,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     for (int item = first; item < last; item += step) {
       const int batch = w.batch, head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
       const int base = w.base, rows = w.rows;
+      const bool fine = w.fine;
       if (BIAS && !ONE && head != lut_head) {
         asm volatile("bar.sync 1, 256;" ::: "memory");           // nobody reads the head before
         lut.set(a, head, warp - Shape::SOFT, 8);
@@ -504,30 +520,58 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
         const float m_now = m_used == -INFINITY ? 0.f : m_used < INFINITY ? m_used : NAN;
         float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
         const float2 mul2 = make_float2(mul, mul), nm2 = make_float2(add - m_now, add - m_now);
+        // four neighbours' exponentials, those of columns e and e + 2 in u, of e + 1 and e + 3 in v
+        const auto exps = [&](int c, int e, float2& u, float2& v) {
+          // Half of every second group of four exponentials runs on the FMA pipe, the rest on the special-function unit (1 x 4096 x 37 x 64, all keys
+          // visible: 208 us, 216 without). Beside the biases of heads of 64 instructions are scarcer: all on the unit (232 us, 249 with).
+          const float2 x01 = ffma2(make_float2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), mul2, nm2);
+          const float2 x23 = ffma2(make_float2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), mul2, nm2);
+          u = make_float2(ex2_approx(x01.x), ex2_approx(x23.x));
+          if (!(DH == 64 && BIAS) && (e >> 2) % 2 == 1) v = ex2_poly2(make_float2(x01.y, x23.y), -127.f);
+          else v = make_float2(ex2_approx(x01.y), ex2_approx(x23.y));
+          sum_a = fadd2(sum_a, u);
+          sum_b = fadd2(sum_b, v);
+        };
+        const auto publish = [&](int c) {      // 64 keys
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t][c >> 1]);
+        };
+        if (FINE && fine) {
 #pragma unroll
-        for (int c = 0; c < PIECES; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < PIECES; ++c) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            // Half of every second group of four exponentials runs on the FMA pipe, the rest on the special-function unit (1 x 4096 x 37 x 64, all keys
-            // visible: 208 us, 216 without). Beside the biases of heads of 64 instructions are scarcer: all on the unit (232 us, 249 with).
-            const float2 x01 = ffma2(make_float2(__uint_as_float(sv[c][e]), __uint_as_float(sv[c][e + 1])), mul2, nm2);
-            const float2 x23 = ffma2(make_float2(__uint_as_float(sv[c][e + 2]), __uint_as_float(sv[c][e + 3])), mul2, nm2);
-            const float2 u = make_float2(ex2_approx(x01.x), ex2_approx(x23.x));
-            float2 v;
-            if (!(DH == 64 && BIAS) && (e >> 2) % 2 == 1) v = ex2_poly2(make_float2(x01.y, x23.y), -127.f);
-            else v = make_float2(ex2_approx(x01.y), ex2_approx(x23.y));
-            sum_a = fadd2(sum_a, u);
-            sum_b = fadd2(sum_b, v);
-            pk[e >> 1] = pack_bf16x2(u.x, v.x);
-            pk[(e >> 1) + 1] = pack_bf16x2(u.y, v.y);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[8], low[8];
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) {
+                float2 u, v;
+                exps(c, h * 16 + e, u, v);
+                pk[e >> 1] = pack_bf16x2(u.x, v.x);
+                pk[(e >> 1) + 1] = pack_bf16x2(u.y, v.y);
+                const float2 h0 = unpack_bf16x2(pk[e >> 1]), h1 = unpack_bf16x2(pk[(e >> 1) + 1]);
+                low[e >> 1] = pack_bf16x2(u.x - h0.x, v.x - h0.y);
+                low[(e >> 1) + 1] = pack_bf16x2(u.y - h1.x, v.y - h1.y);
+              }
+              tmem_st_32x32b_x8(s_tile + c * 16 + h * 8, pk);
+              tmem_st_32x32b_x8(s_tile + TK / 2 + c * 16 + h * 8, low);
+            }
+            if (c & 1) publish(c);
           }
-          tmem_st_32x32b_x16(s_tile + c * 16, pk);          // over scores that are in registers by now
-          if (c & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t][c >> 1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float2 u, v;
+              exps(c, e, u, v);
+              pk[e >> 1] = pack_bf16x2(u.x, v.x);
+              pk[(e >> 1) + 1] = pack_bf16x2(u.y, v.y);
+            }
+            tmem_st_32x32b_x16(s_tile + c * 16, pk);          // over scores that are in registers by now
+            if (c & 1) publish(c);
           }
         }
         l_run += (sum_a.x + sum_a.y) + (sum_b.x + sum_b.y);
@@ -623,7 +667,7 @@ static int text_map(CUtensorMap* m, const void* ptr, int B, int S, int H, int Dh
   return mdb_make_tmap(m, ptr, 2, 4, ext, str, box, 1);
 }
 
-template <int DH, bool BIAS, bool PACKED>
+template <int DH, bool BIAS, bool PACKED, bool FINE>
 static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
   const int B = PACKED ? 1 : a.B;
   using Shape = FwdShape<DH>;
@@ -635,7 +679,7 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
   r = text_map(&maps.v, a.v, B, a.Skv, a.Hkv, DH, a.v_strides, Shape::TK);
   if (r) return 3000 + r;
   constexpr int MOST = 226 * 1024;
-  auto kern = text_fwd_kernel<DH, BIAS, PACKED>;
+  auto kern = text_fwd_kernel<DH, BIAS, PACKED, FINE>;
   static bool ready[TXT_DEVICES];
   if ((r = allow_smem(kern, MOST, ready))) return r;
   const int smem = Shape::BYTES + (BIAS ? TextLut::bytes(text_near(a)) : 0);
@@ -664,9 +708,14 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
 }
 
 int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st) {
-  if (a.cu != nullptr) return a.Dh == 128 ? launch_text_fwd<128, false, true>(a, st) : launch_text_fwd<64, false, true>(a, st);
-  if (a.table != nullptr) return a.Dh == 128 ? launch_text_fwd<128, true, false>(a, st) : launch_text_fwd<64, true, false>(a, st);
-  return a.Dh == 128 ? launch_text_fwd<128, false, false>(a, st) : launch_text_fwd<64, false, false>(a, st);
+  if (a.cu != nullptr) {
+    // FINE where sequences or windows are short on average. A training forward pass of 40 x 128 rows, 32 / 8 heads of 128, takes 66 us with it and 58 without, 4 x 1280 112 and 96, where it
+    // makes no difference that shows.
+    if (a.o_low != nullptr && std::min(a.window, a.Sq / a.B) <= 128) return a.Dh == 128 ? launch_text_fwd<128, false, true, true>(a, st) : launch_text_fwd<64, false, true, true>(a, st);
+    return a.Dh == 128 ? launch_text_fwd<128, false, true, false>(a, st) : launch_text_fwd<64, false, true, false>(a, st);
+  }
+  if (a.table != nullptr) return a.Dh == 128 ? launch_text_fwd<128, true, false, false>(a, st) : launch_text_fwd<64, true, false, false>(a, st);
+  return a.Dh == 128 ? launch_text_fwd<128, false, false, false>(a, st) : launch_text_fwd<64, false, false, false>(a, st);
 }
 
 }  // namespace mdb

@@ -58,8 +58,11 @@ def test_values_and_gradients(case):
     value, bound = packed_oracle(clean(q), clean(k), clean(v), cu, D ** -0.5, window, clean(grad), sink)
     with torch.no_grad():
         alone = O.packed_attention(q, k, v, _ints(cu), window, sink_logits=sink)
+    check(dict(out=alone), dict(out=value["out"]), dict(out=bound["out"]), f"{case} without gradients")
     out = O.packed_attention(q, k, v, _ints(cu), window, sink_logits=sink)
-    assert torch.equal(out, alone)
+    assert not alone[:before].any() and not alone[cu[-1]:].any()
+    for lo, hi in zip(cu[:-1], cu[1:]):         # rows of few keys may keep more of the probabilities when a backward pass follows; the others have the same bits
+        assert window is not None and window <= 256 or torch.equal(out[lo + 256:hi], alone[lo + 256:hi])
     got = dict(zip(("dq", "dk", "dv", "dsink"), torch.autograd.grad(out, [q, k, v] + ([sink] if logits else []), grad)))
     check(dict(out=out) | got, value, bound, str(case))
     for t in (out, got["dq"], got["dk"], got["dv"]):
