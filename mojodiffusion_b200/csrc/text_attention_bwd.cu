@@ -124,6 +124,24 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   TextUnit of = {0, KEYS ? a.Skv : a.Sq, block};
   if (PACKED) of = KEYS ? text_unit_of_keys(a, unit, TR) : text_unit(a, unit, TR);
   const int base = of.base, r0 = of.block * TR, out_rows = of.rows, Sq = PACKED ? of.rows : a.Sq;
+  const auto clear_rows = [&](int t, int threads) {      // packed, rows of no sequence: gradients of zero
+    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int line) {
+      for (int e = t; e < DH / 8; e += threads) {
+        const auto clear = [&](void* to, const long long* st) { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(to) + line * st[1] + blockIdx.y * st[2] + e * 8) = make_uint4(0, 0, 0, 0); };
+        if (!KEYS) {
+          clear(a.dq, a.dq_strides);
+          if (e == 0) a.delta[static_cast<long long>(blockIdx.y) * a.Sq + line] = 0.f;
+        } else {
+          clear(a.dk, a.dk_strides);
+          clear(a.dv, a.dv_strides);
+        }
+      }
+    });
+  };
+  if (PACKED && of.rows == 0) {      // no such unit
+    clear_rows(threadIdx.x, TB_THREADS);
+    return;
+  }
   TextSight sight;
   if (PACKED) sight = {of.rows, 0};
   else sight = text_sight(a, batch);
@@ -654,21 +672,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
 
-  if (PACKED && warp >= 2) {      // rows of no sequence: gradients of zero
-    const int t = threadIdx.x - 64;
-    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int line) {
-      for (int e = t; e < DH / 8; e += 256) {
-        const auto clear = [&](void* to, const long long* st) { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(to) + line * st[1] + blockIdx.y * st[2] + e * 8) = make_uint4(0, 0, 0, 0); };
-        if (!KEYS) {
-          clear(a.dq, a.dq_strides);
-          if (e == 0) a.delta[static_cast<long long>(blockIdx.y) * a.Sq + line] = 0.f;
-        } else {
-          clear(a.dk, a.dk_strides);
-          clear(a.dv, a.dv_strides);
-        }
-      }
-    });
-  }
+  if (PACKED && warp >= 2) clear_rows(threadIdx.x - 64, 256);
 
   tc_fence_before();
   __syncthreads();

@@ -88,6 +88,12 @@ template <int DH, bool BIAS, bool PACKED, bool FINE> struct TextItem {
   // the order of the items with BIAS: those of a head follow one another, so that its bias table is made once
   static __device__ __forceinline__ int head_of(const MdbTextAttnArgs& a, int item, const TextTiles& l) { return item / l.row_items / a.B; }
   __device__ __forceinline__ void set(const MdbTextAttnArgs& a, int item, const TextTiles& l) {
+    TextUnit u = {0, a.Sq, 0};
+    if (PACKED) u = text_unit(a, item / (a.H >> l.heads_log), l.blocks * TQ);
+    set(a, item, l, u);
+  }
+  // `u`: packed, the item's unit
+  __device__ __forceinline__ void set(const MdbTextAttnArgs& a, int item, const TextTiles& l, const TextUnit& u) {
     int block;
     base = 0;
     rows = a.Sq;
@@ -95,7 +101,6 @@ template <int DH, bool BIAS, bool PACKED, bool FINE> struct TextItem {
       const int groups = a.H >> l.heads_log, rest = item / groups;
       head = (item - rest * groups) << l.heads_log;
       batch = 0;
-      const TextUnit u = text_unit(a, rest, l.blocks * TQ);
       base = u.base;
       rows = u.rows;
       block = u.block;
@@ -170,6 +175,29 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   const int step = ONE || RANGE ? 1 : gridDim.x;
   TextItem<DH, BIAS, PACKED, FINE> w;
 
+  const auto clear_rows = [&](int thread, int threads) {      // packed, rows of no sequence: zero, and no gradient
+    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int row) {
+      for (int e = thread; e < a.H * (DH / 8); e += threads) {
+        const long long to = row * a.o_strides[1] + e / (DH / 8) * a.o_strides[2] + e % (DH / 8) * 8;
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + to) = make_uint4(0, 0, 0, 0);
+        if (a.o_low != nullptr) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o_low) + to) = make_uint4(0, 0, 0, 0);
+        if (a.lse != nullptr && e < a.H) a.lse[static_cast<long long>(e) * a.Sq + row] = INFINITY;
+      }
+    });
+  };
+  TextUnit only = {0, 0, 0};  // PACKED, one item to a CTA: its unit. There may be fewer units than the grid has room for
+  if (PACKED && ONE) {
+    only = text_unit(a, first / (a.H >> tiles.heads_log), tiles.blocks * TQ);
+    if (only.rows == 0) {
+      clear_rows(threadIdx.x, Shape::THREADS);
+      return;
+    }
+  }
+  const auto set_first = [&](int item) {
+    if (PACKED && ONE) w.set(a, item, tiles, only);
+    else w.set(a, item, tiles);
+  };
+
   // The TMA warp makes the barriers and starts loading while the others get ready: nobody else touches either before __syncthreads.
   if (warp == 0) {
     if (lane == 0) {
@@ -221,7 +249,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   const int rep = a.H / a.Hkv;
   int early = 0;              // key tiles of the first item that are on their way
   if (warp == 0 && first < last) {
-    w.set(a, first, tiles);
+    set_first(first);
     if (w.n_kv > 0) {
       load_q();
 #pragma unroll 1
@@ -312,7 +340,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       uint32_t done[2] = {0, 0}, outs[2] = {0, 0};      // key tiles, and items with keys, that either query tile has behind it
       bool ok = true;
       for (int item = first; ok && item < last; item += step) {
-        w.set(a, item, tiles);
+        set_first(item);
         if (w.n_kv == 0) continue;
         int t_lo[2], t_hi[2];
 #pragma unroll
@@ -409,7 +437,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
     bool ok = true;
     int done = 0, lut_head = -1;
 
-    if (first < last) w.set(a, first, tiles);
+    if (first < last) set_first(first);
     for (int item = first; item < last; item += step) {
       const int batch = w.batch, head = w.tile_head(w.head, t, tiles), row0 = w.tile_q0(w.q0, t, tiles) + quad * 32;      // the warp's first row
       const int base = w.base, rows = w.rows;
@@ -638,17 +666,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       if (a.lse != nullptr && row0 + lane < rows)
         a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + base + row0 + lane] = m_used == -INFINITY || l_run == 0.f ? INFINITY : m_used + log2f(l_run);
     }
-    if (PACKED) {      // rows of no sequence: zero, and no gradient
-      const int groups = a.H * (DH / 8);
-      text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int row) {
-        for (int e = threadIdx.x - Shape::SOFT * 32; e < groups; e += 256) {
-          const long long to = row * a.o_strides[1] + e / (DH / 8) * a.o_strides[2] + e % (DH / 8) * 8;
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + to) = make_uint4(0, 0, 0, 0);
-          if (a.o_low != nullptr) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o_low) + to) = make_uint4(0, 0, 0, 0);
-          if (a.lse != nullptr && e < a.H) a.lse[static_cast<long long>(e) * a.Sq + row] = INFINITY;
-        }
-      });
-    }
+    if (PACKED) clear_rows(threadIdx.x - Shape::SOFT * 32, 256);
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, done);
   }
 

@@ -80,12 +80,12 @@ def use_native(t: torch.Tensor) -> bool:
     return _loaded or load(True)
 
 
-_PLAIN = {torch.Tensor, torch.nn.Parameter}
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 
 
 def direct(*tensors: torch.Tensor) -> bool:
     """Whether nothing but the kernels looks at an operation on these tensors: plain tensors outside every functorch transform
-    (vmap, grad, jvp), forward-mode AD level, dispatch mode and trace. Ops that also have a form in torch operations keep to it
+    (vmap, grad, jvp), forward-mode AD level, dispatch mode and trace. None stands for an operand left out. Ops that also have a form in torch operations keep to it
     otherwise."""
     return (_PLAIN.issuperset(map(type, tensors))
             and torch._C._functorch.peek_interpreter_stack() is None and forward_ad._current_level < 0

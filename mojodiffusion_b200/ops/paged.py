@@ -55,7 +55,7 @@ def _kernels(x, k_pages, *others) -> bool:
     """Whether the kernels cover the call. They check shapes, types and devices themselves, which costs a short call less."""
     if not x.is_cuda or x.dtype is not torch.bfloat16 or k_pages.dim() != 4 or x.shape[-1] not in (64, 128) or k_pages.shape[2] not in _SIZES:
         return False
-    return native.use_native(x) and native.direct(x, k_pages, *[t for t in others if t is not None])
+    return native.use_native(x) and native.direct(x, k_pages, *others)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,

@@ -170,7 +170,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         scale = float(scale)
     if (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 3 and q.shape[2] in (64, 128) and q.shape[0] < _NO_WINDOW and q.shape[1] <= _MOST_BLOCKS and cu_seqlens.numel() <= _MOST_BLOCKS
             and (scale is None or _LEAST_SCALE <= scale <= _MOST_SCALE) and (sink_logits is None or sink_logits.dtype in (torch.bfloat16, torch.float32)) and native.use_native(q)
-            and native.direct(*[t for t in (q, k, v, cu_seqlens, sink_logits) if t is not None])):
+            and native.direct(q, k, v, cu_seqlens, sink_logits)):
         if not _wants_grad(q, k, v, sink_logits):
             return native.ops().packed_attention_fwd(q, k, v, cu_seqlens, window, scale, sink_logits)
         return native.ops().packed_attention(q, k, v, sink_logits, cu_seqlens, window, scale)
