@@ -206,17 +206,19 @@ template <int DH> __device__ __forceinline__ void clear_rows_of_none(const MdbPa
 
 // grid: units, then rows of no sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
 // few heads, so a block has several of them. Queries are turned one row of a group of lanes after the other, two heads at a time; of keys and values a block needs a head's rows
-// of the whole unit at once, for its scale.
+// of the whole unit at once, for its scale. Where a page has fewer rows than the block has groups of lanes, the groups share out the heads
+// (TEAMS; 11.3 thousand tokens in pages of 16, e4m3: 28 / 4 heads of 64 61 -> 39 us, 32 / 8 of 128 92 -> 78; its registers would cost larger pages a tenth).
 struct AppendGrid {
   int units, q_heads, kv_heads;      // heads of a block
 };
-template <int DH, bool E4M3, int ITERS>
+template <int DH, bool E4M3, int ITERS, bool TEAMS>
 __global__ void __launch_bounds__(PA_THREADS, ITERS == 4 ? 2 : 4)
 paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGrid grid) {
   using Row = AppendRow<DH>;
   constexpr int LANES = Row::LANES, GROUPS = PA_THREADS / LANES;
   __shared__ float tops[2][PA_THREADS / 32];
   const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, G = a.pages.Hkv;
+  const int page_rows = TEAMS ? a.pages.P : GROUPS, teams = TEAMS ? GROUPS >> a.pages.shift : 1, team = TEAMS ? group >> a.pages.shift : 0, row = TEAMS ? group & (a.pages.P - 1) : group;      // a team is whole warps
   const int q_parts = a.q != nullptr ? (a.H + grid.q_heads - 1) / grid.q_heads : 0, kv_parts = (G + grid.kv_heads - 1) / grid.kv_heads;
   if (static_cast<int>(blockIdx.y) < q_parts) {
     const int h0 = blockIdx.y * grid.q_heads, hn = min(a.H, h0 + grid.q_heads);
@@ -227,14 +229,14 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
     const AppendUnit u = find_unit(a, blockIdx.x);
     const bool page = u.count > 0 && page_of(a.pages, u.b, u.index) >= 0;
     const int turned = page ? min(u.count, max(a.positions - u.position, 0)) : 0;      // rows that have a place and angles
-    for (int t0 = 0; t0 < u.count; t0 += GROUPS) {
-      const int t = t0 + group;
+    for (int t0 = 0; t0 < u.count; t0 += page_rows) {
+      const int t = t0 + row;
       const bool in = t < u.count, placed = t < turned;
       const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(a.q) + (u.row + t) * a.q_strides[0];
       __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.q_out) + (u.row + t) * a.H * DH;
       Row angles;
       if (placed) angles.set_angles(a.cos + (u.position + t) * static_cast<long long>(DH / 2), a.sin + (u.position + t) * static_cast<long long>(DH / 2), l);
-      for (int h = h0; h < hn; h += 2) {
+      for (int h = h0 + 2 * team; h < hn; h += 2 * teams) {
         uint4 raw[2][2];
         const bool two = h + 1 < hn;
         if (in) Row::fetch(raw[0], from + h * a.q_strides[1], l);
@@ -269,24 +271,27 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
   const long long* ps = kv ? a.pages.v_strides : a.pages.k_strides;
   const __nv_bfloat16* from = static_cast<const __nv_bfloat16*>(kv ? a.v : a.k) + u.row * fs[0];
   const long long at = page * ps[0] + u.slot * DH;
+  const int threads = page_rows * LANES, warps = threads / 32;      // of a team
 #pragma unroll 1
-  for (int h = h0; h < hn; ++h) {
-    unsigned char* scale = E4M3 && page >= 0 ? (kv ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kv] + h : nullptr;
+  for (int turn = 0; h0 + turn * teams < hn; ++turn) {
+    const int h = h0 + turn * teams + team;
+    const bool mine = h < hn;
+    unsigned char* scale = E4M3 && mine && page >= 0 ? (kv ? a.pages.v_scale : a.pages.k_scale) + page * a.pages.scale_strides[kv] + h : nullptr;
     const int before = scale != nullptr && u.slot > 0 ? min(static_cast<int>(*scale), 253) : 0;
     Row r[ITERS];
     uint4 raw[ITERS][2];
 #pragma unroll
     for (int n = 0; n < ITERS; ++n)
-      if (n * GROUPS + group < turned) Row::fetch(raw[n], from + (n * GROUPS + group) * fs[0] + h * fs[1], l);
+      if (mine && n * page_rows + row < turned) Row::fetch(raw[n], from + (n * page_rows + row) * fs[0] + h * fs[1], l);
     float top = 0.f;
 #pragma unroll
     for (int n = 0; n < ITERS; ++n) {
-      const int t = n * GROUPS + group;
+      const int t = n * page_rows + row;
       r[n].set(raw[n]);
       if (kv == 0 && a.k_norm != nullptr) r[n].weigh(a.k_norm, a.k_norm_f32, r[n].norm(a.eps), l);
-      if (t >= turned) {
+      if (!mine || t >= turned) {
         r[n].clear();
-        if (k_out != nullptr && t < u.count) r[n].store_bf16(k_out + ((u.row + t) * G + h) * DH, l);
+        if (k_out != nullptr && mine && t < u.count) r[n].store_bf16(k_out + ((u.row + t) * G + h) * DH, l);
         continue;
       }
       if (kv == 0) {
@@ -298,29 +303,29 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
       if (!E4M3) {
         r[n].store_bf16(static_cast<__nv_bfloat16*>(kv ? a.pages.v : a.pages.k) + at + h * ps[1] + t * DH, l);
       } else {
-        float mine = r[n].most();
-        if (mine == INFINITY) {
+        float size = r[n].most();
+        if (size == INFINITY) {
           r[n].infinite_to_nan();
-          mine = r[n].most();
+          size = r[n].most();
         }
-        top = fmaxf(top, mine);
+        top = fmaxf(top, size);
       }
     }
     if (!E4M3 || turned == 0) continue;
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    if ((threadIdx.x & 31) == 0) tops[h & 1][threadIdx.x >> 5] = top;
-    __syncthreads();      // a head's half of `tops` is written again behind the next one's barrier
-#pragma unroll
-    for (int i = 0; i < PA_THREADS / 32; ++i) top = fmaxf(top, tops[h & 1][i]);
-    const int byte = max(scale_byte(top), before);
+    if ((threadIdx.x & 31) == 0) tops[turn & 1][threadIdx.x >> 5] = top;
+    __syncthreads();      // a turn's half of `tops` is written again behind the next one's barrier
+    if (!mine) continue;
+    for (int i = 0; i < warps; ++i) top = fmaxf(top, tops[turn & 1][team * warps + i]);
+    const int byte = max(scale_byte(top), before), thread = threadIdx.x - team * threads;
     uint8_t* to = static_cast<uint8_t*>(kv ? a.pages.v : a.pages.k) + at + h * ps[1];
-    if (u.slot > 0 && byte > before) rescale(to - u.slot * DH, u.slot * DH, byte - before, threadIdx.x, PA_THREADS);
+    if (u.slot > 0 && byte > before) rescale(to - u.slot * DH, u.slot * DH, byte - before, thread, threads);
     const float f = scale_inverse(byte);
 #pragma unroll
     for (int n = 0; n < ITERS; ++n)
-      if (n * GROUPS + group < turned) r[n].store_e4m3(to + (n * GROUPS + group) * DH, l, f);
-    if (threadIdx.x == 0 && byte != before) *scale = static_cast<unsigned char>(byte);
+      if (n * page_rows + row < turned) r[n].store_e4m3(to + (n * page_rows + row) * DH, l, f);
+    if (thread == 0 && byte != before) *scale = static_cast<unsigned char>(byte);
   }
 }
 
@@ -413,9 +418,10 @@ static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
     grid.kv_heads = std::max(grid.kv_heads / 2, 1);
   }
   const dim3 blocks(static_cast<unsigned>(units) + spare, parts());
-  if (rows <= groups) paged_append_kernel<DH, E4M3, 1><<<blocks, PA_THREADS, 0, st>>>(a, grid);
-  else if (rows <= 2 * groups) paged_append_kernel<DH, E4M3, 2><<<blocks, PA_THREADS, 0, st>>>(a, grid);
-  else paged_append_kernel<DH, E4M3, 4><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  if (P < groups) paged_append_kernel<DH, E4M3, 1, true><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  else if (rows <= groups) paged_append_kernel<DH, E4M3, 1, false><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  else if (rows <= 2 * groups) paged_append_kernel<DH, E4M3, 2, false><<<blocks, PA_THREADS, 0, st>>>(a, grid);
+  else paged_append_kernel<DH, E4M3, 4, false><<<blocks, PA_THREADS, 0, st>>>(a, grid);
   return static_cast<int>(cudaGetLastError());
 }
 
