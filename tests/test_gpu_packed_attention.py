@@ -124,3 +124,32 @@ def test_refuses_what_the_cpu_refuses():
     d, = torch.autograd.grad(out.sum(), a["q"], create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         d.sum().backward()
+
+
+def test_more_than_32_bits_of_elements():
+    """2400 sequences whose rows reach beyond 2^31 elements: the last ones as by themselves."""
+    B, n, H, G, D = 2400, 131, 64, 1, 128
+    T = B * n
+    assert T * H * D > 1 << 31
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV) * n
+    q = torch.zeros(T, H, D, dtype=torch.bfloat16, device=DEV)
+    k, v = _normal(T, G, D, seed=2), _normal(T, G, D, seed=3)
+    grad = torch.zeros(T, H, D, dtype=torch.bfloat16, device=DEV)
+    last = slice(T - 3 * n, T)
+    q[last], grad[last] = _normal(3 * n, H, D, seed=1), _normal(3 * n, H, D, seed=4)
+
+    def run(rows, cu):
+        x = [t[rows].clone().requires_grad_() for t in (q, k, v)]
+        out = O.packed_attention(*x, cu)
+        return out, *torch.autograd.grad(out, x, grad[rows])
+
+    small = run(last, _ints([0, n, 2 * n, 3 * n]))
+    large = run(slice(0, T), cu)
+    with torch.no_grad():
+        alone = O.packed_attention(q, k, v, cu)[last]
+        assert torch.equal(alone, O.packed_attention(q[last], k[last], v[last], _ints([0, n, 2 * n, 3 * n])))
+    # few blocks of keys are shared by several CTAs, many are not: the sums of dk and dv are added in another order
+    assert torch.equal(small[0], large[0][last]) and torch.equal(small[1], large[1][last])
+    value, bound = packed_oracle(q[last], k[last], v[last], [0, n, 2 * n, 3 * n], D ** -0.5, None, grad[last])
+    check(dict(zip(("out", "dq", "dk", "dv"), (t[last] for t in large))), value, bound, "far")
+    O.check_status()

@@ -251,3 +251,71 @@ def test_refuses_what_the_cpu_refuses():
     for a, b in zip(before, (kp, vp, ks, vs)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     O.check_status()
+
+
+@pytest.mark.parametrize("eight", [True, False])
+def test_pools_inside_larger_ones(eight):
+    """Keys and values of one page next to one another, and scales in a larger array: strides of pages and heads of any size."""
+    P, D, G, H, N = 32, 64, 2, 6, 8
+    (kp, ks), (vp, vs) = pool(N, G, P, D, eight, DEV, 2), pool(N, G, P, D, eight, DEV, 3)
+    both = torch.zeros(N, G, 3, P, D, device=DEV).to(kp.dtype)
+    both[:, :, 0], both[:, :, 2] = kp, vp
+    scales = torch.zeros(N, 2 * G + 3, dtype=torch.uint8, device=DEV)
+    if eight:
+        scales[:, 1:1 + G], scales[:, G + 2:2 * G + 2] = ks, vs
+    inner = (both[:, :, 0], both[:, :, 2], *((scales[:, 1:1 + G], scales[:, G + 2:2 * G + 2]) if eight else (None, None)))
+    cos, sin = angles(200, D, DEV)
+    table, start = _ints([[3, 1, 0, 0], [2, 7, 5, 4]]), [20, 60]
+    q, k, v = (_normal(50, n, D, seed=n) for n in (H, G, G))
+    want = O.paged_append(k, v, kp, vp, table, _ints(start), cos, sin, cu_seqlens=_ints([0, 30, 50]), k_scale=ks, v_scale=vs, q=q)
+    got = O.paged_append(k, v, inner[0], inner[1], table, _ints(start), cos, sin, cu_seqlens=_ints([0, 30, 50]), k_scale=inner[2], v_scale=inner[3], q=q)
+    assert torch.equal(got, want)
+    for a, b in zip(inner, (kp, vp, ks, vs)):
+        assert a is None or torch.equal(a.contiguous().view(torch.uint8), b.view(torch.uint8))
+    assert not both[:, :, 1].float().any()
+    for Sq in (1, 3, 30):
+        x = _normal(2, Sq, H, D, seed=9)
+        a = O.paged_attention(x, kp, vp, table, _ints([50, 80]), k_scale=ks, v_scale=vs)
+        assert torch.equal(O.paged_attention(x, inner[0], inner[1], table, _ints([50, 80]), k_scale=inner[2], v_scale=inner[3]), a)
+    O.check_status()
+
+
+@pytest.mark.parametrize("eight", [True, False])
+def test_pools_of_more_than_32_bits(eight):
+    """Pages whose elements lie beyond 2^31."""
+    P, D, G, H = 64, 128, 2, 8
+    N = (1 << 31) // (G * P * D) + 70
+    big = [torch.empty(N, G, P, D, dtype=torch.float8_e4m3fn if eight else torch.bfloat16, device=DEV) for _ in range(2)]
+    scales = [torch.ones(N, G, dtype=torch.uint8, device=DEV) if eight else None for _ in range(2)]
+    (kp, ks), (vp, vs) = pool(6, G, P, D, eight, DEV, 2), pool(6, G, P, D, eight, DEV, 3)
+    far = torch.tensor([N - 1, N - 2, 3, N - 60, 0, N - 9], device=DEV)
+    for t, s, p, c in zip(big, scales, (kp, vp), (ks, vs)):
+        t.view(torch.uint8).index_copy_(0, far, p.view(torch.uint8))
+        if eight:
+            s[far] = c
+    near, distant = _ints([[0, 1, 2], [3, 4, 5]]), far.int().view(2, 3)
+    cos, sin = angles(200, D, DEV)
+    q, k, v = (_normal(90, n, D, seed=n) for n in (H, G, G))
+    calls = [(near, kp, vp, ks, vs), (distant, *big, *scales)]
+    got = [O.paged_append(k, v, p, w, table, _ints([30, 100]), cos, sin, cu_seqlens=_ints([0, 40, 90]), k_scale=c, v_scale=d, q=q) for table, p, w, c, d in calls]
+    assert torch.equal(*got)
+    got = [O.paged_append(k[:2], v[:2], p, w, table, _ints([70, 150]), cos, sin, k_scale=c, v_scale=d, q=q[:2]) for table, p, w, c, d in calls]
+    assert torch.equal(*got)
+    for t, p in zip((*big, *scales), (kp, vp, ks, vs)):
+        assert t is None or torch.equal(t.view(torch.uint8)[far], p.view(torch.uint8))
+    for Sq in (1, 5, 40):
+        x = _normal(2, Sq, H, D, seed=9)
+        got = [O.paged_attention(x, p, w, table, _ints([71, 151]), k_scale=c, v_scale=d) for table, p, w, c, d in calls]
+        assert torch.equal(*got)
+    O.check_status()
+
+
+def test_parts_of_prompts_report_pages_that_are_not_there():
+    P, D, G = 16, 64, 2
+    (kp, ks), (vp, vs) = pool(4, G, P, D, True, DEV, 0), pool(4, G, P, D, True, DEV, 1)
+    q = _normal(2, 40, 4, D, seed=5)
+    good = O.paged_attention(q, kp, vp, _ints([[0, 1], [2, 3]]), _ints([20, 20]), k_scale=ks, v_scale=vs)
+    out = O.paged_attention(q, kp, vp, _ints([[0, 1], [2, -3]]), _ints([20, 20]), k_scale=ks, v_scale=vs)
+    assert torch.equal(out[0], good[0])
+    with pytest.raises(RuntimeError, match="BOUNDS"):
+        O.check_status()
