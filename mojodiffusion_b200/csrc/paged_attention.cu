@@ -9,8 +9,8 @@
 // sequence and head each instead, and there is nothing to join.
 //
 // A warp of its own starts the copies: it knows the pages of the next 32 places of the table and their scales, and brings K and V of a tile in by TMA, one box
-// per page. Four warps multiply, with mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the keys and the columns of V fill the 16 and the rows, of which there
-// are few, the 8. (A 128-row tcgen05 tile would be mostly padding.) Each warp has 32 keys at a time; where there are more than 16 rows the warps share out those.
+// per page. Four or eight warps multiply, with mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, so that the keys and the columns of V fill the 16 and the rows, of which there
+// are few, the 8. (A 128-row tcgen05 tile would be mostly padding.) Each warp has 32 keys at a time; where a warp has no room for all rows the warps share out those.
 //
 // 8 bits: e4m3 values are exact in f16, and two of them take one conversion, so the products are f16 ones. Of a key's row a lane reads 16 bytes as they lie; which
 // of them are columns 2t, 2t + 1 of a k-step is free as long as the queries' registers use the same order, and so no byte is moved. For values ldmatrix transposes pairs of bytes,
@@ -42,12 +42,14 @@ struct alignas(64) PagedMaps {
 
 // A warp has NT tiles of 8 rows; RG warps share the rows, and the others the keys of a tile
 template <int DH, bool E4M3, int NT, int RG> struct PagedShape {
-  static constexpr int WARPS = 4;                                     // that multiply
+  // that multiply. Heads of 128 have room for the queries and sums of 8 rows in a warp; for 16 rows (168 registers, 90 to 110 bytes spilled) 8 sequences of 4000 with 32 rows took 49 us
+  // (bf16 57) with four warps and two CTAs to an SM, with eight warps of 8 rows and one CTA 43 (45). Heads of 64 have room for 16: eight warps took 37 us instead of 33 there.
+  static constexpr int WARPS = DH == 128 && RG > 1 ? 8 : 4;
   static constexpr int THREADS = (WARPS + 1) * 32;
   static constexpr int COLS = 64 / NT;                                // columns that the warps join at a time
   static constexpr int TILE = PK * DH * (E4M3 ? 1 : 2);               // K or V of a stage
   // per SM, with 192 KB of stages. 16 tokens over 16384, 64 / 8 heads of 64: three CTAs 76 us, two 94; 4 over 131072, heads of 128, where three would have two stages each: 150 and 143.
-  static constexpr int CTAS = NT == 1 && DH == 64 ? 3 : 2;
+  static constexpr int CTAS = WARPS == 8 ? 1 : NT == 1 && DH == 64 ? 3 : 2;
   static constexpr int STAGES = 192 * 1024 / CTAS / (2 * TILE);
   static constexpr int SLAB = WARPS * 8 * NT * COLS * 4;
   static constexpr int BYTES = STAGES * 2 * TILE + SLAB + 1024;
@@ -726,7 +728,7 @@ static bool is_whole(const MdbPagedAttnArgs& a) { return a.pages.most <= 4 * PK;
 // As many CTAs as the SMs hold (see PagedShape), or one per tile where there are fewer
 static int step_ctas(const MdbPagedAttnArgs& a) {
   const long long tiles = static_cast<long long>(a.pages.B) * a.pages.Hkv * ((a.pages.most + PK - 1) / PK);
-  return static_cast<int>(std::max(1ll, std::min(tiles, (step_rows(a) == 8 && a.pages.Dh == 64 ? 3ll : 2ll) * device_sm_count())));
+  return static_cast<int>(std::max(1ll, std::min(tiles, (a.pages.Dh == 64 ? (step_rows(a) == 8 ? 3ll : 2ll) : step_rows(a) == 8 ? 2ll : 1ll) * device_sm_count())));
 }
 
 template <int DH, bool E4M3, int NT, int RG>
@@ -772,9 +774,10 @@ static int launch_paged(const MdbPagedAttnArgs& a, cudaStream_t st) {
   r = pages_map(&maps.v, a.pages.v, a.pages, a.pages.v_strides, E4M3);
   if (r) return 3000 + r;
   const int rows = step_rows(a);
+  constexpr int NT = DH == 64 ? 2 : 1;
   if (rows == 8) return launch_step<DH, E4M3, 1, 1>(maps, a, st);
-  if (rows == 16) return launch_step<DH, E4M3, 2, 1>(maps, a, st);
-  return rows == 32 ? launch_step<DH, E4M3, 2, 2>(maps, a, st) : launch_step<DH, E4M3, 2, 4>(maps, a, st);
+  if (rows == 16) return launch_step<DH, E4M3, NT, 2 / NT>(maps, a, st);
+  return rows == 32 ? launch_step<DH, E4M3, NT, 4 / NT>(maps, a, st) : launch_step<DH, E4M3, NT, 8 / NT>(maps, a, st);
 }
 
 // ---- parts of prompts: the pages in one piece, for the kernels of whole prompts ----
