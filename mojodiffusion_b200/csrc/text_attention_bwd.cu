@@ -72,8 +72,9 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
   }
 };
 
+// FINE: P and dS go into their products as two bf16 terms, the second one in the columns of the scores that the first leaves free (see text_is_fine).
 // PACKED: a block is a unit of 128 rows of one sequence. 4996 rows in nine sequences of 20 to 1531, 32 / 8 heads of 128: dq 141 us, dk and dv 188 (tensor pipe 29 and 42 %)
-template <int DH, bool KEYS, bool BIAS, bool PACKED>
+template <int DH, bool KEYS, bool BIAS, bool PACKED, bool FINE>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
 text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextParts parts) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
@@ -311,6 +312,13 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
           for (int kk = 0; kk < TC / 16; ++kk)
             umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk / 2 * 32 + kk % 2 * 8, c2 + (kk * 2048 >> 4), idesc_acc, (first && kk == 0) ? 0u : 1u);
         }
+        if (FINE) {
+#pragma unroll
+          for (int kk = 0; kk < TC / 16; ++kk) {
+            umma_f16_ts(tmem_base + ACC1_COL, tmem_base + Y_COL + buf * TC + kk / 2 * 32 + 16 + kk % 2 * 8, c1 + (kk * 2048 >> 4), idesc_acc, 1u);
+            if (KEYS) umma_f16_ts(tmem_base + ACC2_COL, tmem_base + X_COL + buf * TC + kk / 2 * 32 + 16 + kk % 2 * 8, c2 + (kk * 2048 >> 4), idesc_acc, 1u);
+          }
+        }
       };
       // rows of a key tile that no query of the CTA sees; packed, also rows of a query tile that belong to the next sequence
       const auto clean = [&](int i, int st) {
@@ -503,7 +511,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
           if (uniform) one_bias = d0 > 0 ? lut.behind() : lut.before();
           else b = lut.from(KEYS ? row - b0 - 3 : b0 - row);
         }
-        uint32_t pk[16], dk[16];
+        uint32_t pk[16], dk[16];      // FINE: of 16 columns, [0, 8), and what their rounding left, [8, 16)
         const float2 sl2_2 = make_float2(sl2, sl2);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
@@ -538,10 +546,37 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
           }
           const float2 d01 = fmul2(p01, fadd2(make_float2(__uint_as_float(yr[c][e]), __uint_as_float(yr[c][e + 1])), make_float2(nd[0], nd[1])));
           const float2 d23 = fmul2(p23, fadd2(make_float2(__uint_as_float(yr[c][e + 2]), __uint_as_float(yr[c][e + 3])), make_float2(nd[2], nd[3])));
-          pk[e >> 1] = pack_bf16x2(p01.x, p01.y);
-          pk[(e >> 1) + 1] = pack_bf16x2(p23.x, p23.y);
-          dk[e >> 1] = pack_bf16x2(d01.x, d01.y);
-          dk[(e >> 1) + 1] = pack_bf16x2(d23.x, d23.y);
+          const int at = (FINE ? e & 15 : e) >> 1;
+          pk[at] = pack_bf16x2(p01.x, p01.y);
+          pk[at + 1] = pack_bf16x2(p23.x, p23.y);
+          dk[at] = pack_bf16x2(d01.x, d01.y);
+          dk[at + 1] = pack_bf16x2(d23.x, d23.y);
+          if constexpr (FINE) {
+            const auto rest = [](float2 x, uint32_t rounded) {
+              const float2 h = unpack_bf16x2(rounded);
+              return pack_bf16x2(x.x - h.x, x.y - h.y);
+            };
+            if (KEYS) {
+              pk[at + 8] = rest(p01, pk[at]);
+              pk[at + 9] = rest(p23, pk[at + 1]);
+            }
+            dk[at + 8] = rest(d01, dk[at]);
+            dk[at + 9] = rest(d23, dk[at + 1]);
+            if ((e & 15) == 12) {
+              const auto store = [&](uint32_t to, const uint32_t (&w)[16]) {
+                uint32_t high[8], low[8];
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                  high[m] = w[m];
+                  low[m] = w[m + 8];
+                }
+                tmem_st_32x32b_x8(to, high);
+                tmem_st_32x32b_x8(to + 16, low);
+              };
+              if (KEYS) store(xa + (piece0 + c) * 32 + (e >> 4) * 8, pk);
+              store(ya + (piece0 + c) * 32 + (e >> 4) * 8, dk);
+            }
+          }
           if (BIAS && !KEYS) {
             run[c][e] = d01.x;
             run[c][e + 1] = d01.y;
@@ -549,8 +584,10 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
             run[c][e + 3] = d23.y;
           }
         }
-        if (KEYS) tmem_st_32x32b_x16(xa + (piece0 + c) * 32, pk);      // over scores of this piece: they are in registers by now
-        tmem_st_32x32b_x16(ya + (piece0 + c) * 32, dk);
+        if constexpr (!FINE) {
+          if (KEYS) tmem_st_32x32b_x16(xa + (piece0 + c) * 32, pk);      // over scores of this piece: they are in registers by now
+          tmem_st_32x32b_x16(ya + (piece0 + c) * 32, dk);
+        }
       }
       tmem_wait_st();
       tc_fence_before();
@@ -784,13 +821,13 @@ static long long part_floats(const MdbTextAttnArgs& a, const TextParts& p) {
   return static_cast<long long>(a.cu != nullptr ? 1 : a.B) * a.Hkv * p.blocks * p.count * 2 * TR * a.Dh;
 }
 
-template <int DH, bool KEYS, bool BIAS, bool PACKED>
+template <int DH, bool KEYS, bool BIAS, bool PACKED, bool FINE = false>
 static int launch_text_bwd(const TextBwdMaps& maps, const MdbTextAttnArgs& a, const TextParts& parts, cudaStream_t st) {
   using Shape = TextBwdShape<DH, KEYS, BIAS>;
   constexpr int MOST = 225 * 1024;                 // beside what the kernel declares itself
   const int smem = BIAS ? Shape::bytes(text_near(a), a.buckets) : Shape::bytes(0, 0);
   if (smem > MOST) return -6;
-  auto kern = text_bwd_kernel<DH, KEYS, BIAS, PACKED>;
+  auto kern = text_bwd_kernel<DH, KEYS, BIAS, PACKED, FINE>;
   static bool ready[TXT_DEVICES];
   if (int r = allow_smem(kern, MOST, ready)) return r;
   int blocks = PACKED ? static_cast<int>(text_units(a, TR)) : ((KEYS ? a.Skv : a.Sq) + TR - 1) / TR;
@@ -811,14 +848,15 @@ static int text_backward(const MdbTextAttnArgs& a, const TextParts& parts, cudaS
   if ((r = bwd_map(&maps.r2, a.dout, B, a.Sq, a.H, DH, a.do_strides, TR))) return 1500 + r;
   if ((r = bwd_map(&maps.o, a.o, B, a.Sq, a.H, DH, a.o_strides, TR))) return 1600 + r;
   if (a.o_low != nullptr && (r = bwd_map(&maps.o_low, a.o_low, B, a.Sq, a.H, DH, a.o_strides, TR))) return 1700 + r;
-  if (a.cu != nullptr) r = launch_text_bwd<DH, false, false, true>(maps, a, parts, st);
+  const bool fine = text_is_fine(a);
+  if (a.cu != nullptr) r = fine ? launch_text_bwd<DH, false, false, true, true>(maps, a, parts, st) : launch_text_bwd<DH, false, false, true>(maps, a, parts, st);
   else r = a.table != nullptr ? launch_text_bwd<DH, false, true, false>(maps, a, parts, st) : launch_text_bwd<DH, false, false, false>(maps, a, parts, st);
   if (r) return r;
   if ((r = bwd_map(&maps.r1, a.k, B, a.Skv, a.Hkv, DH, a.k_strides, TR))) return 2000 + r;
   if ((r = bwd_map(&maps.r2, a.v, B, a.Skv, a.Hkv, DH, a.v_strides, TR))) return 2100 + r;
   if ((r = bwd_map(&maps.c1, a.q, B, a.Sq, a.H, DH, a.q_strides, TC))) return 2200 + r;
   if ((r = bwd_map(&maps.c2, a.dout, B, a.Sq, a.H, DH, a.do_strides, TC))) return 2300 + r;
-  if (a.cu != nullptr) return launch_text_bwd<DH, true, false, true>(maps, a, parts, st);
+  if (a.cu != nullptr) return fine ? launch_text_bwd<DH, true, false, true, true>(maps, a, parts, st) : launch_text_bwd<DH, true, false, true>(maps, a, parts, st);
   return a.table != nullptr ? launch_text_bwd<DH, true, true, false>(maps, a, parts, st) : launch_text_bwd<DH, true, false, false>(maps, a, parts, st);
 }
 

@@ -20,9 +20,8 @@
 //
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
-// FINE (packed, with a backward pass to come): in items whose rows have few keys a probability goes into its product as two bf16 terms, the second one in the half of the scores' columns that
-// the first leaves free. There ds = p (dp - do . o) is a difference of nearly equal terms, and the rounding of p shows in it through o: dq and dk of 23 sequences of two or three tokens
-// were off by 0.0026 of their size, of three with a window of 2 by 0.0030; the rounding of ds and of the result alone make 0.0024.
+// FINE (packed, short, with a backward pass to come; see text_is_fine): in items whose rows have few keys a probability goes into its product as two bf16 terms, the second one in the half of
+// the scores' columns that the first leaves free.
 //
 // PACKED: an item is a unit of one sequence (see text_unit); coordinates and rows count from the sequence's first row. A tile holds rows of one sequence only, at the cost of tiles that are
 // not full: rows of several sequences in a tile would multiply each other's values by zero, and 0 * NaN would carry one sequence's NaN into another. 10155 tokens in six sequences of 301
@@ -36,7 +35,6 @@
 #include "text_attention.cuh"
 #include "gemm_api.h"
 
-#include <algorithm>
 #include <string.h>
 
 namespace mdb {
@@ -727,9 +725,7 @@ static int launch_text_fwd(const MdbTextAttnArgs& a, cudaStream_t st) {
 
 int text_attention_prompt(const MdbTextAttnArgs& a, cudaStream_t st) {
   if (a.cu != nullptr) {
-    // FINE where sequences or windows are short on average. A training forward pass of 40 x 128 rows, 32 / 8 heads of 128, takes 66 us with it and 58 without, 4 x 1280 112 and 96, where it
-    // makes no difference that shows.
-    if (a.o_low != nullptr && std::min(a.window, a.Sq / a.B) <= 128) return a.Dh == 128 ? launch_text_fwd<128, false, true, true>(a, st) : launch_text_fwd<64, false, true, true>(a, st);
+    if (a.o_low != nullptr && text_is_fine(a)) return a.Dh == 128 ? launch_text_fwd<128, false, true, true>(a, st) : launch_text_fwd<64, false, true, true>(a, st);
     return a.Dh == 128 ? launch_text_fwd<128, false, true, false>(a, st) : launch_text_fwd<64, false, true, false>(a, st);
   }
   if (a.table != nullptr) return a.Dh == 128 ? launch_text_fwd<128, true, false, false>(a, st) : launch_text_fwd<64, true, false, false>(a, st);
