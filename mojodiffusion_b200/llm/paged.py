@@ -23,8 +23,10 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: at least one page of at least one position")
         L, G, D = cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim
         self.cfg, self.page_size, self.device = cfg, page_size, torch.device(device if device is not None else "cpu")
-        self.k, self.v = (torch.zeros(L, pages, G, page_size, D, device=device).to(dtype) for _ in range(2))
         eight = dtype == torch.float8_e4m3fn
+        self.k, self.v = (torch.zeros(L, pages, G, page_size, D, dtype=torch.uint8 if eight else dtype, device=device) for _ in range(2))
+        if eight:
+            self.k, self.v = self.k.view(dtype), self.v.view(dtype)
         self.k_scale, self.v_scale = (torch.ones(L, pages, G, dtype=torch.uint8, device=device) if eight else None for _ in range(2))
         self.free = list(range(pages))[::-1]
         self.pages: Dict[int, List[int]] = {}
