@@ -15,8 +15,9 @@
 // 8 bits: e4m3 values are exact in f16, and two of them take one conversion, so the products are f16 ones. Of a key's row a lane reads 16 bytes as they lie; which
 // of them are columns 2t, 2t + 1 of a k-step is free as long as the queries' registers use the same order, and so no byte is moved. For values ldmatrix transposes pairs of bytes,
 // and one byte permutation makes two columns of them. Queries are brought to [1, 2) by a power of two per row, which leaves them exact but for those below 2^-14 of
-// the row's largest (2^-25 of it at most). Probabilities are rounded to f16 (2^-11, where the output's rounding is 2^-8); the reference is kept 2^7 below the first maximum, so
-// that also probabilities of 2^-21 have all their bits. The powers of two of values go into the probabilities, relative to the largest met so far.
+// the row's largest (2^-25 of it at most). A value's power of two goes into its probability: the product is of w_ij = p_ij 2^(ev - u_i), rounded to f16 (2^-11, where the output's
+// rounding is 2^-8). The reference m_i is kept 2^7 below the first maximum of x_ij, and the whole number u_i follows so that the largest w_ij is between about 2^6 and 2^15: whatever the
+// pages' units are, weights down to 2^-20 of the largest have all their bits (with one u for all rows, the largest unit met, a page that a row hardly sees took the bits of those that it sees).
 // bf16: the products are bf16 ones; a probability goes into its product as two bf16 terms, so only the output is rounded.
 //
 // Keys behind the sequence's end are masked and their values zeroed in shared memory before the product (0 * NaN is not 0).
@@ -354,7 +355,9 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    int unit = 0;                                                      // byte of the power of two that o is in units of
+    float u[NT][2];                                                    // o is in units of 2^(u - 127), a whole number for each row
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) u[nt][0] = u[nt][1] = 145.f;      // 2^(ev - u) is a number for any ev
 
     for (int tile = first_tile; tile < first_tile + count; ++tile, ++i) {
       const int st = i % STAGES;
@@ -418,35 +421,25 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
             }
           }
         }
-        float ks[2] = {1.f, 1.f}, into[2] = {1.f, 1.f};
+        float ks[2] = {1.f, 1.f}, ev[2] = {0.f, 0.f};                  // unit of the keys, byte of the values' (a page behind the end: 0)
+        bool apart = false;
         if (E4M3) {
           const uchar2 sc[2] = {scales[st][k32 / 16], scales[st][k32 / 16 + 1]};
-          const int top = max(sc[0].y, kb + 16 < end ? sc[1].y : 0);
-          if (top > unit) {                // the same in the whole warp
-            const float f = scale_inverse(127 + min(top - unit, 126));
-            if (unit != 0) {
-#pragma unroll
-              for (int d = 0; d < DM; ++d)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) o[d][nt][e] *= f;
-            }
-            unit = top;
-          }
+          apart = sc[0].y != sc[1].y;      // the same in the whole warp
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             ks[s] = scale_value(sc[s].x);
-            into[s] = scale_inverse(127 + min(unit - sc[s].y, 126));
+            ev[s] = sc[s].y;
           }
         }
         const bool whole = kb + 31 <= start && kb + 32 <= end;
         bool raise = false;
-        float f[NT][2];
+        float top[NT][2], big[NT][2];     // the largest of the scores, and of the scores plus ev
         float2 mul[2][NT];                // of the rows 2 t, 2 t + 1; not 0, for -inf * 0 is not -inf
+        const float most_ev = fmaxf(ev[0], ev[1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float top[2] = {-INFINITY, -INFINITY};
+          top[nt][0] = top[nt][1] = big[nt][0] = big[nt][1] = -INFINITY;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             mul[s][nt] = make_float2(fmaxf(sl2[nt][0] * ks[s], 0x1p-126f), fmaxf(sl2[nt][1] * ks[s], 0x1p-126f));
@@ -457,33 +450,71 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
                 if (!(j <= p_row[nt][e & 1] && j < end)) x[s][nt][e] = -INFINITY;
               }
             }
-            top[0] = paged_max(top[0], paged_max(x[s][nt][0], x[s][nt][2]) * mul[s][nt].x);
-            top[1] = paged_max(top[1], paged_max(x[s][nt][1], x[s][nt][3]) * mul[s][nt].y);
+            const float t[2] = {paged_max(x[s][nt][0], x[s][nt][2]) * mul[s][nt].x, paged_max(x[s][nt][1], x[s][nt][3]) * mul[s][nt].y};
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              top[nt][y] = paged_max(top[nt][y], t[y]);
+              if (E4M3) big[nt][y] = paged_max(big[nt][y], t[y] + ev[s]);
+            }
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
 #pragma unroll
-            for (int z = 4; z < 32; z <<= 1) top[y] = paged_max(top[y], __shfl_xor_sync(0xffffffffu, top[y], z));
-            top[y] -= ABOVE;
-            // the reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept
-            f[nt][y] = 1.f;
-            if (!(top[y] <= m[nt][y] + 8.f)) {
-              f[nt][y] = exp2f(m[nt][y] - top[y]);
-              m[nt][y] = paged_max(m[nt][y], top[y]);
-              raise = true;
-            }
+            for (int z = 4; z < 32; z <<= 1) top[nt][y] = paged_max(top[nt][y], __shfl_xor_sync(0xffffffffu, top[nt][y], z));
+            top[nt][y] -= ABOVE;
+            // The reference is raised when outgrown by more than 2^8, and with the first key that the row sees; NaN is kept. u is set when the weights have outgrown it, and
+            // where m is; it stays within 2^118 of every unit, so that 2^(ev - u) is a number.
+            raise = raise || !(top[nt][y] <= m[nt][y] + 8.f);
           }
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        if (E4M3) {
+          if (apart) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            l[nt][0] *= f[nt][0];
-            l[nt][1] *= f[nt][1];
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+#pragma unroll
+                for (int z = 4; z < 32; z <<= 1) big[nt][y] = paged_max(big[nt][y], __shfl_xor_sync(0xffffffffu, big[nt][y], z));
+                big[nt][y] -= ABOVE;
+              }
+          } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) big[nt][y] = top[nt][y] + ev[0];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) raise = raise || !(big[nt][y] <= m[nt][y] + (u[nt][y] + 8.f)) || most_ev > u[nt][y] + 118.f;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          float fo[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float before = m[nt][y];
+              const bool up = !(top[nt][y] <= before + 8.f);
+              fo[nt][y] = 1.f;
+              if (up) {
+                m[nt][y] = paged_max(before, top[nt][y]);
+                fo[nt][y] = exp2f(before - m[nt][y]);
+                l[nt][y] *= fo[nt][y];
+              }
+              if (E4M3 && m[nt][y] != -INFINITY) {
+                float now = paged_max(up ? ceilf(u[nt][y] + (before - m[nt][y])) : u[nt][y], most_ev - 110.f);
+                if (up || !(big[nt][y] <= m[nt][y] + (now + 8.f))) now = paged_max(now, ceilf(big[nt][y] - m[nt][y]));
+                fo[nt][y] = exp2f((up ? before - m[nt][y] : 0.f) + (u[nt][y] - now));
+                u[nt][y] = now;
+              }
+            }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int d = 0; d < DM; ++d)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[d][nt][e] *= f[nt][e & 1];
-          }
+              for (int e = 0; e < 4; ++e) o[d][nt][e] *= fo[nt][e & 1];
         }
         // P^T as the B operand: keys 2 t, 2 t + 1 (and 8 more) of row gq, which is the transpose of what the lane has
         uint32_t ph[2][NT][2], pl[2][NT][2];
@@ -492,14 +523,15 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
           const float2 less = make_float2(m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]);
           float2 sum = make_float2(l[nt][0], l[nt][1]);
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+          for (int s = 0; s < 2; ++s) {
+            const float2 into = E4M3 ? make_float2(ex2_approx(ev[s] - u[nt][0]), ex2_approx(ev[s] - u[nt][1])) : make_float2(1.f, 1.f);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const float2 t = ffma2(make_float2(x[s][nt][2 * y], x[s][nt][2 * y + 1]), mul[s][nt], less);
               const float2 p = make_float2(ex2_approx(t.x), ex2_approx(t.y));
               sum = fadd2(sum, p);
               if (E4M3) {
-                const float2 q2 = fmul2(p, make_float2(into[s], into[s]));
+                const float2 q2 = fmul2(p, into);
                 ph[s][nt][y] = paged_transpose(pack_f16x2(q2.x, q2.y));
               } else {
                 const uint32_t h = pack_bf16x2(p.x, p.y);
@@ -508,6 +540,7 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
                 pl[s][nt][y] = paged_transpose(pack_bf16x2(low.x, low.y));
               }
             }
+          }
           l[nt][0] = sum.x;
           l[nt][1] = sum.y;
         }
@@ -552,13 +585,21 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
     }
 
     // the warps' parts meet in shared memory, COLS columns at a time
-    const float whole_unit = E4M3 ? scale_value(unit) : 1.f;
+    // 8 bits: divisors are brought to [1, 2), and sums with them, so that these are no larger than the values
+    float less[NT][2], units[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
 #pragma unroll
         for (int z = 4; z < 32; z <<= 1) l[nt][y] += __shfl_xor_sync(0xffffffffu, l[nt][y], z);
+        if (E4M3) {
+          const int e = min(max(static_cast<int>(__float_as_uint(l[nt][y]) >> 23), 1), 253);      // 0 (no key) and NaN stay as they are
+          less[nt][y] = scale_inverse(e);
+          units[nt][y] = exp2f(u[nt][y] - 127.f);
+          l[nt][y] *= less[nt][y];
+          m[nt][y] += e - 127;
+        }
         if (gq == 0) {
           part_m[warp][nt * 8 + 2 * tq + y] = m[nt][y];
           part_l[warp][nt * 8 + 2 * tq + y] = l[nt][y];
@@ -575,8 +616,8 @@ paged_step_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant_
           const float (&v)[4] = o[c0 / 16 + y][nt];
           float* mine = slab + (warp * WR + nt * 8 + 2 * tq) * COLS + 16 * y;
           if (E4M3) {
-            *reinterpret_cast<float2*>(mine + 2 * gq) = make_float2(v[0] * whole_unit, v[2] * whole_unit);
-            *reinterpret_cast<float2*>(mine + COLS + 2 * gq) = make_float2(v[1] * whole_unit, v[3] * whole_unit);
+            *reinterpret_cast<float2*>(mine + 2 * gq) = make_float2(v[0] * less[nt][0] * units[nt][0], v[2] * less[nt][0] * units[nt][0]);
+            *reinterpret_cast<float2*>(mine + COLS + 2 * gq) = make_float2(v[1] * less[nt][1] * units[nt][1], v[3] * less[nt][1] * units[nt][1]);
           } else {
             mine[gq] = v[0];
             mine[gq + 8] = v[2];
