@@ -52,10 +52,11 @@ class PagedKVCache:
         return torch.tensor([self.pages[s] + [0] * (width - len(self.pages[s])) for s in sequences], dtype=torch.int32, device=self.device).reshape(len(sequences), width)
 
     def angles(self, positions: int):
-        """cos and sin [at least ``positions``, head_dim / 2] in fp32, formed in 64 bits: angles of far positions have few bits left in 32."""
+        """cos and sin [at least ``positions``, head_dim / 2] in fp32, formed in 64 bits: angles of far positions have few bits left in 32. The tables grow by doubling, so that
+        a sequence that gets longer token by token rarely waits for new ones."""
         if self._angles is None or self._angles[0].shape[0] < positions:
             inv = scaled_inv_freq(self.cfg.head_dim, self.cfg.rope_theta, self.cfg.rope_scaling).double()
-            a = torch.arange(max(positions, 64), dtype=torch.float64)[:, None] * inv[None]
+            a = torch.arange(1 << (max(positions, 64) - 1).bit_length(), dtype=torch.float64)[:, None] * inv[None]
             self._angles = a.cos().float().to(self.device), a.sin().float().to(self.device)
         return self._angles
 

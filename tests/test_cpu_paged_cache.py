@@ -1,0 +1,27 @@
+"""The pool of pages behind a batch of prompts: its tables of angles."""
+import torch
+
+from mojodiffusion_b200.llm import PagedKVCache, paged_prefill, paged_step
+from mojodiffusion_b200.models.text.qwen3 import Qwen3Config, Qwen3Encoder
+
+
+def _tiny(**more):
+    torch.manual_seed(0)
+    cfg = Qwen3Config(**(dict(vocab_size=97, hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=16, rope_theta=10000.0) | more))
+    return cfg, Qwen3Encoder(cfg, torch.float32, "cpu")
+
+
+def test_angles_are_kept_from_step_to_step():
+    cfg, enc = _tiny()
+    cache = PagedKVCache(cfg, 30, torch.float32, page_size=16)
+    paged_prefill(enc, cache, [0], [[1] * 70])
+    tables = []
+    for _ in range(70):                                        # from 71 positions to 140
+        paged_step(enc, cache, [0], torch.tensor([3]))
+        if not tables or cache.angles(1)[0] is not tables[-1]:
+            tables.append(cache.angles(1)[0])
+    assert [t.shape[0] for t in tables] == [128, 256]
+    inv = 1.0 / 10000.0 ** (torch.arange(0, 16, 2, dtype=torch.float64) / 16)
+    angle = torch.arange(256, dtype=torch.float64)[:, None] * inv.float().double()
+    for t, want in zip(cache.angles(200), (angle.cos(), angle.sin())):
+        assert torch.equal(t, want.float())
