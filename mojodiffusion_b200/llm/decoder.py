@@ -197,9 +197,9 @@ class Qwen3Decoder:
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         h = self.enc.model.norm(hidden)
         w = self.lm_head if self.lm_head is not None else self.enc.model.embed_tokens.weight
-        if (native.use_native(h) and native.direct(h, w) and h.dtype == w.dtype == torch.bfloat16 and h.dim() == w.dim() == 2 and 0 < h.shape[0] <= 8
+        if (native.use_native(h) and native.direct(h, w) and h.dtype == w.dtype == torch.bfloat16 and h.dim() == w.dim() == 2 and h.shape[0] > 0
                 and h.shape[1] == w.shape[1] and h.shape[1] % 8 == 0 and native.ops().bf16_operands_ok([h, w], [-1, 0])):
-            # products of bf16 values are exact in fp32 and the few-row kernel sums in fp32: the table needs no fp32 copy
+            # products of bf16 values are exact in fp32 and the kernels sum in fp32, for any number of rows: the table needs no fp32 copy
             return ops.functional._gemm([h], [w], out_fp32=True)
         return h.float() @ w.float().t()
 
