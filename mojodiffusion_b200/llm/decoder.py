@@ -14,7 +14,7 @@ import torch
 
 from .. import ops
 from ..models.layers import globally_hooked, own_parameters
-from ..models.text.qwen3 import _MLP, _Norm, _W, Qwen3Config, Qwen3Encoder, _rope
+from ..models.text.qwen3 import _MLP, _Norm, _W, Qwen3Config, Qwen3Encoder, _rope, scaled_inv_freq
 from ..ops import native
 from .paged import PagedKVCache, paged_prefill, paged_step
 from .sampler import Rng, SamplerConfig, sample
@@ -56,7 +56,10 @@ class Qwen3Decoder:
 
     def _angles(self, pos: torch.Tensor, dtype):
         c = self.cfg
-        inv = 1.0 / (c.rope_theta ** (torch.arange(0, c.head_dim, 2, device=pos.device).float() / c.head_dim))
+        if c.rope_scaling is None:
+            inv = 1.0 / (c.rope_theta ** (torch.arange(0, c.head_dim, 2, device=pos.device).float() / c.head_dim))
+        else:
+            inv = scaled_inv_freq(c.head_dim, c.rope_theta, c.rope_scaling).to(pos.device)
         ang = pos.float()[:, None] * inv[None]
         emb = torch.cat((ang, ang), dim=-1)
         return emb.cos().to(dtype), emb.sin().to(dtype)
@@ -222,7 +225,8 @@ class Qwen3Decoder:
     @torch.no_grad()
     def generate_batch(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, cfg: SamplerConfig = SamplerConfig(), eos_ids: Sequence[int] = (),
                        device=None, cache: Optional[PagedKVCache] = None, eight_bits: bool = False) -> List[List[int]]:
-        """``generate`` for several prompts at once: a reply for each, every one with a sampler of its own that starts from ``cfg.seed``. Prompts run packed, then one token of
+        """``generate`` for several prompts at once: a reply for each, every one with a sampler of its own that starts from ``cfg.seed``. Angles are fp32 here, where
+        ``generate`` rounds them to the model's type, so in bf16 its logits are nearer to the exact ones and a reply may differ. Prompts run packed, then one token of
         each sequence that has not ended at a time, over pages of bf16 (the model's type) or 8 bits. ``cache``: pages to take and give back, else as many as the prompts need."""
         dev = device or next(self.enc.parameters()).device
         if any(len(p) == 0 for p in prompts):

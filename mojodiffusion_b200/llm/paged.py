@@ -2,7 +2,8 @@
 
 A sequence takes pages as it grows and gives them back when it ends, so that a batch of prompts needs no common length and no padding: prompts run packed one
 behind the other (``ops.packed_attention``), their keys and values go to the pages on the way (``ops.paged_append``), and each step decodes one token of every
-sequence over its pages (``ops.paged_attention``). Per sequence the behaviour is that of the cached decoder for one prompt (serenitymojo/llm/decoder.mojo:1-150)."""
+sequence over its pages (``ops.paged_attention``). Per sequence the behaviour is that of the cached decoder for one prompt (serenitymojo/llm/decoder.mojo:1-150), with
+angles in fp32 instead of the model's type."""
 from __future__ import annotations
 
 from typing import Dict, List, Optional, Sequence
