@@ -44,8 +44,16 @@ class PagedKVCache:
         self.lengths.setdefault(sequence, 0)
 
     def release(self, sequence: int) -> None:
-        self.free += self.pages.pop(sequence)[::-1]
-        del self.lengths[sequence]
+        self.give_back(sequence, None)
+
+    def give_back(self, sequence: int, kept: Optional[int]) -> None:
+        """All pages of a sequence but the first ``kept``; None: the sequence itself ends."""
+        pages = self.pages.pop(sequence)
+        self.free += pages[kept or 0:][::-1]
+        if kept is None:
+            del self.lengths[sequence]
+        else:
+            self.pages[sequence] = pages[:kept]
 
     def table(self, sequences: Sequence[int]) -> torch.Tensor:
         """int32 [B, width]: the pages of the sequences. Places that a shorter sequence does not have name page 0 and are not read."""
@@ -87,9 +95,23 @@ def _layers(enc, x, attend):
 
 @torch.no_grad()
 def paged_prefill(enc, cache: PagedKVCache, sequences: Sequence[int], prompts: Sequence[Sequence[int]]) -> torch.Tensor:
-    """Whole prompts of new sequences, packed -> hidden state of the last token of each [B, hidden]."""
+    """Whole prompts of new sequences, packed -> hidden state of the last token of each [B, hidden]. After an error the cache is as it was: no sequence has begun."""
     if any(len(p) == 0 for p in prompts) or any(cache.lengths.get(s, 0) for s in sequences) or len(set(sequences)) != len(sequences) or len(sequences) != len(prompts):
         raise ValueError("paged_prefill: a prompt of at least one token for each of several new sequences")
+    held = {s: len(cache.pages[s]) for s in sequences if s in cache.pages}
+    try:
+        x = _prefill(enc, cache, sequences, prompts)
+    except BaseException:
+        for s in reversed(sequences):
+            if s in cache.pages:
+                cache.give_back(s, held.get(s))
+        raise
+    for s, p in zip(sequences, prompts):
+        cache.lengths[s] = len(p)
+    return x
+
+
+def _prefill(enc, cache, sequences, prompts):
     dev = cache.device
     for s, p in zip(sequences, prompts):
         cache.reserve(s, len(p))
@@ -105,8 +127,6 @@ def paged_prefill(enc, cache: PagedKVCache, sequences: Sequence[int], prompts: S
         return ops.packed_attention(q, k, v, cu)
 
     x = _layers(enc, enc.model.embed_tokens(torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=dev)), attend)
-    for s, p in zip(sequences, prompts):
-        cache.lengths[s] = len(p)
     return x[cu[1:].long() - 1]
 
 

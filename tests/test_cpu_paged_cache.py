@@ -1,4 +1,5 @@
-"""The pool of pages behind a batch of prompts: its tables of angles."""
+"""The pool of pages behind a batch of prompts: its tables of angles, and pages after an error."""
+import pytest
 import torch
 
 from mojodiffusion_b200.llm import PagedKVCache, paged_prefill, paged_step
@@ -25,3 +26,33 @@ def test_angles_are_kept_from_step_to_step():
     angle = torch.arange(256, dtype=torch.float64)[:, None] * inv.float().double()
     for t, want in zip(cache.angles(200), (angle.cos(), angle.sin())):
         assert torch.equal(t, want.float())
+
+
+def test_a_prefill_that_fails_takes_no_pages():
+    cfg, enc = _tiny()
+    cache = PagedKVCache(cfg, 8, torch.float32, page_size=16)
+    paged_prefill(enc, cache, [0], [[1] * 20])
+    cache.reserve(4, 16)                                       # a new sequence with a page already
+
+    def state():
+        return list(cache.free), {s: list(p) for s, p in cache.pages.items()}, dict(cache.lengths)
+
+    before = state()
+    with pytest.raises(RuntimeError, match="full"):            # five pages are left, the first two prompts take four
+        paged_prefill(enc, cache, [1, 4, 2], [[1] * 32, [2] * 40, [3] * 70])
+    assert state() == before
+    hook = enc.model.layers[1].mlp.register_forward_hook(_fail)
+    with pytest.raises(ArithmeticError):                       # in the model
+        paged_prefill(enc, cache, [1, 4], [[1] * 32, [2] * 40])
+    hook.remove()
+    assert state() == before
+    again = paged_prefill(enc, cache, [1, 4], [[1] * 32, [2] * 40])
+    other = PagedKVCache(cfg, 8, torch.float32, page_size=16)
+    assert torch.equal(again, paged_prefill(enc, other, [1, 4], [[1] * 32, [2] * 40]))
+    for s in (0, 1, 4):
+        cache.release(s)
+    assert sorted(cache.free) == list(range(8)) and not cache.pages and not cache.lengths
+
+
+def _fail(*_):
+    raise ArithmeticError
