@@ -227,10 +227,13 @@ class Qwen3Decoder:
                        device=None, cache: Optional[PagedKVCache] = None, eight_bits: bool = False) -> List[List[int]]:
         """``generate`` for several prompts at once: a reply for each, every one with a sampler of its own that starts from ``cfg.seed``. Angles are fp32 here, where
         ``generate`` rounds them to the model's type, so in bf16 its logits are nearer to the exact ones and a reply may differ. Prompts run packed, then one token of
-        each sequence that has not ended at a time, over pages of bf16 (the model's type) or 8 bits. ``cache``: pages to take and give back, else as many as the prompts need."""
+        each sequence that has not ended at a time, over pages of bf16 (the model's type) or 8 bits. ``cache``: pages to take and give back, else as many as the prompts need; its pages have the type that it was made with, so
+        ``eight_bits`` with a cache of another type is an error."""
         dev = device or next(self.enc.parameters()).device
         if any(len(p) == 0 for p in prompts):
             raise ValueError("generate_batch: every prompt needs a token")
+        if eight_bits and cache is not None and cache.k.dtype != torch.float8_e4m3fn:
+            raise ValueError("generate_batch: eight_bits needs a cache with pages of float8_e4m3fn")
         if cache is None:
             need = sum(-(-(len(p) + max_new_tokens) // 64) for p in prompts)
             cache = PagedKVCache(self.cfg, max(need, 1), torch.float8_e4m3fn if eight_bits else self.enc.model.embed_tokens.weight.dtype, dev)

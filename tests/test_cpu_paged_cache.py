@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from mojodiffusion_b200.llm import PagedKVCache, paged_prefill, paged_step
+from mojodiffusion_b200.llm import PagedKVCache, Qwen3Decoder, SamplerConfig, paged_prefill, paged_step
 from mojodiffusion_b200.models.text.qwen3 import Qwen3Config, Qwen3Encoder
 
 
@@ -56,3 +56,14 @@ def test_a_prefill_that_fails_takes_no_pages():
 
 def _fail(*_):
     raise ArithmeticError
+
+
+def test_eight_bits_and_a_cache_of_another_type():
+    cfg, enc = _tiny()
+    dec = Qwen3Decoder(enc)
+    eight, wide = (PagedKVCache(cfg, 8, t, page_size=16) for t in (torch.float8_e4m3fn, torch.float32))
+    greedy = SamplerConfig(temperature=0.0)
+    want = dec.generate_batch([[1, 2], [3]], 3, greedy, cache=eight)
+    assert dec.generate_batch([[1, 2], [3]], 3, greedy, cache=eight, eight_bits=True) == want
+    with pytest.raises(ValueError, match="eight_bits"):
+        dec.generate_batch([[1, 2], [3]], 3, greedy, cache=wide, eight_bits=True)
