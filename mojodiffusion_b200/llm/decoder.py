@@ -246,6 +246,7 @@ class Qwen3Decoder:
             hidden = paged_prefill(self.enc, cache, [first + i for i in alive], prompts)
             while True:
                 rows = self.logits(hidden).tolist()
+                ops.check_status(hidden)                     # what a kernel gave up is not sampled from
                 for i, row in zip(alive, rows):
                     out[i].append(sample(row, cfg, rngs[i]))
                 ended = [i for i in alive if out[i][-1] in eos_ids or len(out[i]) == max_new_tokens]

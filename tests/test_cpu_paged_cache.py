@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from mojodiffusion_b200 import ops as O
 from mojodiffusion_b200.llm import PagedKVCache, Qwen3Decoder, SamplerConfig, paged_prefill, paged_step
 from mojodiffusion_b200.models.text.qwen3 import Qwen3Config, Qwen3Encoder
 
@@ -67,3 +68,19 @@ def test_eight_bits_and_a_cache_of_another_type():
     assert dec.generate_batch([[1, 2], [3]], 3, greedy, cache=eight, eight_bits=True) == want
     with pytest.raises(ValueError, match="eight_bits"):
         dec.generate_batch([[1, 2], [3]], 3, greedy, cache=wide, eight_bits=True)
+
+
+def test_reports_of_kernels_end_the_generation(monkeypatch):
+    """``ops.check_status`` is asked before tokens are drawn; its error gives the pages back."""
+    cfg, enc = _tiny()
+    cache, asked = PagedKVCache(cfg, 8, torch.float32, page_size=16), []
+
+    def status(like):
+        asked.append(like.shape)
+        if len(asked) == 3:
+            raise RuntimeError("TIMEOUT")
+
+    monkeypatch.setattr(O, "check_status", status)
+    with pytest.raises(RuntimeError, match="TIMEOUT"):
+        Qwen3Decoder(enc).generate_batch([[1, 2], [3]], 6, SamplerConfig(temperature=0.0), cache=cache)
+    assert asked == [(2, 64)] * 3 and sorted(cache.free) == list(range(8)) and not cache.pages

@@ -48,3 +48,16 @@ def test_a_dozen_prompts():
     replies = Qwen3Decoder(enc).generate_batch(prompts, 5, SamplerConfig(temperature=0.0))
     assert [len(r) for r in replies] == [5] * 12
     O.check_status()
+
+
+def test_a_page_that_is_not_there_ends_the_generation():
+    class Wrong(PagedKVCache):
+        def table(self, sequences):
+            return super().table(sequences) + (1000 if max(self.lengths[s] for s in sequences) > 5 else 0)
+
+    cfg, enc, _ = _model()
+    cache = Wrong(cfg, 8, torch.bfloat16, DEV)
+    with pytest.raises(RuntimeError, match="BOUNDS"):
+        Qwen3Decoder(enc).generate_batch([[1, 2], [3]], 9, SamplerConfig(temperature=0.0), cache=cache)
+    assert sorted(cache.free) == list(range(8))
+    O.check_status()
