@@ -146,23 +146,34 @@ struct AppendUnit {
   int b, index, slot, count, position;
   long long row;
 };
-// The rows of sequence b; what the lengths say is held within the T rows
-__device__ __forceinline__ void rows_of(const MdbPagedAppendArgs& a, int b, long long& first, int& length, int& start) {
-  const long long lo = min(max(static_cast<long long>(a.cu[b]), 0ll), a.T), hi = min(max(static_cast<long long>(a.cu[b + 1]), lo), a.T);
-  first = lo;
-  length = static_cast<int>(hi - lo);
-  start = a.start[b];
-  if (start < 0 || start > 1 << 30) start = 1 << 30;      // behind every page: reported like any position without one
-}
+// Sequences are disjoint and lie within the T rows whatever cu says: where it falls the largest end so far counts, and none passes the last one.
+__device__ __forceinline__ int row_within(const MdbPagedAppendArgs& a, int b) { return min(max(a.cu[b], 0), static_cast<int>(a.T)); }
 // By a whole warp: units are numbered sequence after sequence, a page after the other
 __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int unit) {
-  const int lane = threadIdx.x & 31, P = a.pages.P, shift = a.pages.shift;
+  const int lane = threadIdx.x & 31, P = a.pages.P, shift = a.pages.shift, last = row_within(a, a.pages.B);
   AppendUnit u = {0, 0, 0, 0, 0, 0};
-  int before = 0;
+  int before = 0, largest = 0;
+  bool fell = false;
   for (int b0 = 0; b0 < a.pages.B; b0 += 32) {
-    long long first = 0;
-    int length = 0, start = 0;
-    if (b0 + lane < a.pages.B) rows_of(a, b0 + lane, first, length, start);
+    int lo = 0, hi = 0, start = 0;
+    if (b0 + lane < a.pages.B) {
+      lo = row_within(a, b0 + lane);
+      hi = row_within(a, b0 + lane + 1);
+      start = a.start[b0 + lane];
+      if (start < 0 || start > 1 << 30) start = 1 << 30;      // behind every page: reported like any position without one
+    }
+    fell = fell || __any_sync(0xffffffffu, hi < lo);
+    if (fell) {
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, lo, m);
+        if (lane >= m) lo = max(lo, other);
+      }
+      lo = max(lo, largest);
+      hi = max(hi, lo);
+    }
+    largest = __reduce_max_sync(0xffffffffu, hi);
+    int first = min(lo, last), length = min(hi, last) - first;
     const int mine = length > 0 ? ((start + length - 1) >> shift) - (start >> shift) + 1 : 0;
     int upto = mine;
 #pragma unroll
@@ -190,12 +201,17 @@ __device__ __forceinline__ AppendUnit find_unit(const MdbPagedAppendArgs& a, int
   }
   return u;
 }
+// By one block: ends that fall or lie outside the rows
+__device__ __forceinline__ void check_ends(const MdbPagedAppendArgs& a) {
+  for (int b = threadIdx.x; b < a.pages.B; b += PA_THREADS)
+    if (a.cu[b] < 0 || a.cu[b] > a.cu[b + 1] || a.cu[b + 1] > a.T) report_status(a.pages.status, STATUS_BOUNDS, 186, b);
+}
 
 // Heads h0 .. hn - 1 of the rows before the first sequence and behind the last one come out as zeros; by the blocks from `units` on
 template <int DH> __device__ __forceinline__ void clear_rows_of_none(const MdbPagedAppendArgs& a, int units, __nv_bfloat16* to, int heads, int h0, int hn) {
   using Row = AppendRow<DH>;
   constexpr int GROUPS = PA_THREADS / Row::LANES;
-  const long long first = min(max(static_cast<long long>(a.cu[0]), 0ll), a.T), end = min(max(static_cast<long long>(a.cu[a.pages.B]), first), a.T);
+  const long long end = row_within(a, a.pages.B), first = min(static_cast<long long>(row_within(a, 0)), end);
   Row r;
   r.clear();
   for (long long i = (static_cast<long long>(blockIdx.x) - units) * GROUPS + threadIdx.x / Row::LANES; i < first + a.T - end; i += static_cast<long long>(gridDim.x - units) * GROUPS) {
@@ -219,6 +235,7 @@ paged_append_kernel(const __grid_constant__ MdbPagedAppendArgs a, const AppendGr
   __shared__ float tops[2][PA_THREADS / 32];
   const int l = threadIdx.x % LANES, group = threadIdx.x / LANES, G = a.pages.Hkv;
   const int page_rows = TEAMS ? a.pages.P : GROUPS, teams = TEAMS ? GROUPS >> a.pages.shift : 1, team = TEAMS ? group >> a.pages.shift : 0, row = TEAMS ? group & (a.pages.P - 1) : group;      // a team is whole warps
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) check_ends(a);      // behind the units
   const int q_parts = a.q != nullptr ? (a.H + grid.q_heads - 1) / grid.q_heads : 0, kv_parts = (G + grid.kv_heads - 1) / grid.kv_heads;
   if (static_cast<int>(blockIdx.y) < q_parts) {
     const int h0 = blockIdx.y * grid.q_heads, hn = min(a.H, h0 + grid.q_heads);
@@ -407,7 +424,7 @@ static int launch_append(const MdbPagedAppendArgs& a, cudaStream_t st) {
   const int B = a.pages.B, P = a.pages.P, groups = PA_THREADS / AppendRow<DH>::LANES;
   const long long units = std::min(a.T, a.T / P + 2ll * B);
   if (units > 0x7ffffff0) return -8;
-  const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 0;      // blocks for rows of no sequence
+  const int spare = a.q != nullptr || a.k_out != nullptr ? 8 : 1;      // blocks for rows of no sequence and a look at the ends
   const int rows = static_cast<int>(std::min<long long>(P, a.T)), H = a.q != nullptr ? a.H : 0, G = a.pages.Hkv;      // rows of a unit, at most
   // heads of a block: sixteen and four, fewer where that leaves fewer than six blocks to an SM (11.3 thousand tokens, 32 / 8 heads of 128: 59.4 us, with eight and two 62.3,
   // four and one 69.6; 4.2 thousand, 28 / 4 heads of 64, bf16 pages: eight and two 20.5 us, eight and one 22.5)

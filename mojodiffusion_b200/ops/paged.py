@@ -11,7 +11,7 @@ serenitymojo/llm/sqa.mojo:1-116, for a batch of sequences of different lengths).
 
 bf16 tensors with heads of 64 or 128 and pages of 16, 32, 64 or 128 positions run the kernels of ``csrc/paged*.cu`` on a GPU; other types and sizes and the CPU run the torch
 statements of ``ops.reference``. A page number outside the pool, or a position without a page, is an error on the CPU; the kernels skip it and report it
-(``ops.check_status``). Neither operator has a gradient.
+(``ops.check_status``). So they do with ends of sequences that fall or lie outside the rows: there the largest end so far counts, and none passes the last one. Neither operator has a gradient.
 """
 from __future__ import annotations
 

@@ -1,0 +1,57 @@
+"""Ends of packed sequences that fall, or lie outside the rows: sequences stay disjoint and within the rows, and the call is reported."""
+import pytest
+import torch
+
+from mojodiffusion_b200 import ops as O
+from paged_oracle import angles, pool
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _normal(*shape, seed):
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(torch.bfloat16)
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def held(cu, T):
+    """The largest end so far, none beyond the last one, all within T rows."""
+    cu = [min(max(c, 0), T) for c in cu]
+    return [min(max(cu[:i + 1]), cu[-1]) for i in range(len(cu))]
+
+
+# of 60 rows
+ENDS = [[0, 40, 10, 60], [0, 40, 10], [50, 20, 60], [60, 0], [30, 40, 20, 25, 50], [0, 60, 0, 60, 0, 60], list(range(0, 40)) + [5] * 30 + [55, 60]]
+OUTSIDE = [[-5, 30, 70], [70, 80, 90], [0, 1 << 30], [-(1 << 31), 20, 60]]
+
+
+@pytest.mark.parametrize("eight", [True, False])
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 32), (64, 64)])
+@pytest.mark.parametrize("cu", ENDS + OUTSIDE, ids=lambda c: str(c[:6]).replace(" ", ""))
+def test_append(cu, D, P, eight):
+    T, H, G, B = 60, 4, 2, len(cu) - 1
+    width = 80 // P + 1
+    q, k, v = (_normal(T, n, D, seed=n) for n in (H, G, G))
+    start = _ints([(7 * b) % 19 for b in range(B)])
+    table = torch.arange(B * width, dtype=torch.int32, device=DEV).view(B, width)
+    cos, sin = angles(100, D, DEV)
+    O.check_status()
+    found = []
+    for ends in (held(cu, T), cu):
+        (kp, ks), (vp, vs) = pool(B * width, G, P, D, eight, DEV, 2), pool(B * width, G, P, D, eight, DEV, 3)
+        out, keys = O.paged_append(k, v, kp, vp, table, start, cos, sin, cu_seqlens=_ints(ends), k_scale=ks, v_scale=vs, q=q, keys=True)
+        (kp2, ks2), (vp2, vs2) = pool(B * width, G, P, D, eight, DEV, 2), pool(B * width, G, P, D, eight, DEV, 3)
+        if ends is cu:
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+        O.check_status()
+        assert O.paged_append(k, v, kp2, vp2, table, start, cos, sin, cu_seqlens=_ints(ends), k_scale=ks2, v_scale=vs2) is None
+        if ends is cu:
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+        found.append([t.view(torch.uint8) for t in (out, keys, kp, vp, ks, vs, kp2, vp2, ks2, vs2) if t is not None])
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
