@@ -44,15 +44,24 @@ __device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const Te
 struct TextUnit {
   int base, rows, block;      // first row and length of the sequence; rows 0: no unit
 };
-__device__ __forceinline__ int text_first_row(const MdbTextAttnArgs& a, int b) { return min(max(a.cu[b], 0), a.Sq); }
-__device__ __forceinline__ int text_rows_of(const MdbTextAttnArgs& a, int b, int first) { return min(max(a.cu[b + 1], first), a.Sq) - first; }
+// Sequences are disjoint and lie within the rows whatever cu says: where it falls, which is reported, the largest end so far counts, and none passes the last one.
+__device__ __forceinline__ int text_row_within(const MdbTextAttnArgs& a, int b) { return min(max(a.cu[b], 0), a.Sq); }
 __device__ __forceinline__ TextUnit text_unit(const MdbTextAttnArgs& a, int unit, int gran) {
   if (a.units != nullptr) {
     const int4 u = a.units[unit];
     return {u.x, u.y, u.z};
   }
   const int lane = threadIdx.x & 31;
-  const int first = lane < a.B ? text_first_row(a, lane) : 0, rows = lane < a.B ? text_rows_of(a, lane, first) : 0, n = (rows + gran - 1) / gran;
+  int first = lane < a.B ? text_row_within(a, lane) : 0, end = lane < a.B ? text_row_within(a, lane + 1) : 0;
+  if (__any_sync(0xffffffffu, end < first)) {
+    const int last = __shfl_sync(0xffffffffu, end, a.B - 1);
+#pragma unroll 1
+    for (int m = 1; m < 32; m <<= 1) first = max(first, __shfl_up_sync(0xffffffffu, first, m));      // a lane that has none below it reads itself
+    end = min(max(end, first), last);
+    first = min(first, last);
+    if (lane == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
+  }
+  const int rows = lane < a.B ? end - first : 0, n = (rows + gran - 1) / gran;
   const auto from = [&](int level) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - level, 0)))); };      // blocks of this number or a larger one
   int lo = 0, hi = __reduce_max_sync(0xffffffffu, n);      // from(lo) > unit >= from(hi)
   if (unit >= from(0)) return {0, 0, 0};
@@ -84,7 +93,7 @@ int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st);
 
 // rows before the first sequence and behind the last one, in turn
 template <typename F> __device__ __forceinline__ void text_rows_of_none(const MdbTextAttnArgs& a, int from, int step, F f) {
-  const int first = text_first_row(a, 0), last = max(text_first_row(a, a.B), first), n = first + a.Sq - last;
+  const int last = text_row_within(a, a.B), first = min(text_row_within(a, 0), last), n = first + a.Sq - last;
   for (int i = from; i < n; i += step) f(i < first ? i : i - first + last);
 }
 

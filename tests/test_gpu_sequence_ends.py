@@ -24,7 +24,7 @@ def held(cu, T):
 
 
 # of 60 rows
-ENDS = [[0, 40, 10, 60], [0, 40, 10], [50, 20, 60], [60, 0], [30, 40, 20, 25, 50], [0, 60, 0, 60, 0, 60], list(range(0, 40)) + [5] * 30 + [55, 60]]
+ENDS = [[0, 40, 10, 60], [0, 40, 10], [50, 20, 60], [60, 0], [30, 40, 20, 25, 50], [0, 60, 0, 60, 0, 60], list(range(0, 40)) + [5] * 30 + [55, 60], [7 * i % 61 for i in range(1500)] + [50]]
 OUTSIDE = [[-5, 30, 70], [70, 80, 90], [0, 1 << 30], [-(1 << 31), 20, 60]]
 
 
@@ -55,3 +55,34 @@ def test_append(cu, D, P, eight):
         found.append([t.view(torch.uint8) for t in (out, keys, kp, vp, ks, vs, kp2, vp2, ks2, vs2) if t is not None])
     for a, b in zip(*found):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H,G,D", [(4, 2, 64), (4, 2, 128), (3, 1, 128)])
+@pytest.mark.parametrize("scale", [1, 9])
+@pytest.mark.parametrize("cu", ENDS + OUTSIDE, ids=lambda c: str(c[:6]).replace(" ", ""))
+def test_packed_attention(cu, scale, H, G, D):
+    T = 60 * scale                                              # with 9, sequences of several tiles
+    cu = [c * scale if abs(c) < 1 << 20 else c for c in cu]
+    q, k, v, grad, sink = _normal(T, H, D, seed=1), _normal(T, G, D, seed=2), _normal(T, G, D, seed=3), _normal(T, H, D, seed=4), _normal(H, seed=5)
+    O.check_status()
+
+    def reports(ends):
+        inside = [min(max(c, 0), T) for c in ends]
+        if inside != sorted(inside):
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+        O.check_status()
+
+    found = []
+    for ends in (held(cu, T), cu):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, sink)]
+        with torch.no_grad():
+            alone = O.packed_attention(*leaves[:3], _ints(ends), sink_logits=leaves[3])
+        reports(ends)
+        out = O.packed_attention(*leaves[:3], _ints(ends), sink_logits=leaves[3])
+        reports(ends)
+        grads = torch.autograd.grad(out, leaves, grad)
+        reports(ends)
+        found.append((alone, out, *grads))
+    for a, b in zip(*found):
+        assert torch.equal(a, b) and torch.isfinite(b).all()
