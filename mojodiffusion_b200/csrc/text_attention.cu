@@ -29,33 +29,15 @@ static int check_args(const MdbTextAttnArgs* a) {
 // The units of more than 32 sequences, one block of threads: sequence after sequence, the last rows of each first
 constexpr int TU_THREADS = 1024;
 __global__ void __launch_bounds__(TU_THREADS) text_units_kernel(const __grid_constant__ MdbTextAttnArgs a, const int gran, const int units) {
-  __shared__ int sums[TU_THREADS / 32], ends[TU_THREADS / 32], at[TU_THREADS];
+  __shared__ int sums[TU_THREADS / 32], at[TU_THREADS];
   __shared__ int2 rows_of[TU_THREADS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, last = text_row_within(a, a.B);
-  int before = 0, largest = 0;
-  bool fell = false;
-  for (int b0 = 0; b0 < a.B; b0 += TU_THREADS) {
-    const int b = b0 + threadIdx.x;
-    int first = b < a.B ? text_row_within(a, b) : 0, end = b < a.B ? text_row_within(a, b + 1) : 0;
-    if (__syncthreads_or(end < first)) fell = true;
-    if (fell) {
-      int most = max(first, end);
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        first = max(first, __shfl_up_sync(0xffffffffu, first, m));
-        most = max(most, __shfl_up_sync(0xffffffffu, most, m));
-      }
-      if (lane == 31) ends[warp] = most;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) first = max(first, ends[w]);
-      first = max(first, largest);
-      for (int w = 0; w < TU_THREADS / 32; ++w) largest = max(largest, ends[w]);
-      end = min(max(end, first), last);
-      first = min(first, last);
-    } else {
-      largest = text_row_within(a, min(b0 + TU_THREADS, a.B));
-    }
-    const int rows = b < a.B ? end - first : 0, n = (rows + gran - 1) / gran;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bool falls = false;
+  for (int b = threadIdx.x; b < a.B; b += TU_THREADS) falls = falls || text_row_within(a, b + 1) < text_row_within(a, b);
+  const int sequences = __syncthreads_or(falls) ? 0 : a.B;      // where ends fall there is no unit, and the first place says so
+  int before = 0;
+  for (int b0 = 0; b0 < sequences; b0 += TU_THREADS) {
+    const int b = b0 + threadIdx.x, first = b < a.B ? text_row_within(a, b) : 0, rows = b < a.B ? text_row_within(a, b + 1) - first : 0, n = (rows + gran - 1) / gran;
     int upto = n;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -79,8 +61,7 @@ __global__ void __launch_bounds__(TU_THREADS) text_units_kernel(const __grid_con
     }
     before += all;
   }
-  if (fell && threadIdx.x == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
-  for (int i = before + threadIdx.x; i < units; i += TU_THREADS) a.units[i] = make_int4(0, 0, 0, 0);
+  for (int i = before + threadIdx.x; i < units; i += TU_THREADS) a.units[i] = make_int4(0, 0, 0, sequences == 0 ? -1 : 0);
 }
 int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st) {
   if (a.units == nullptr) return 0;

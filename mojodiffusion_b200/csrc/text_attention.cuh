@@ -44,7 +44,7 @@ __device__ __forceinline__ TextKeys text_keys(const MdbTextAttnArgs& a, const Te
 struct TextUnit {
   int base, rows, block;      // first row and length of the sequence; rows 0: no unit
 };
-// Sequences are disjoint and lie within the rows whatever cu says: where it falls, which is reported, the largest end so far counts, and none passes the last one.
+// Ends are held within the rows. Where they fall there is no unit: sequences would have rows in common.
 __device__ __forceinline__ int text_row_within(const MdbTextAttnArgs& a, int b) { return min(max(a.cu[b], 0), a.Sq); }
 __device__ __forceinline__ TextUnit text_unit(const MdbTextAttnArgs& a, int unit, int gran) {
   if (a.units != nullptr) {
@@ -52,16 +52,10 @@ __device__ __forceinline__ TextUnit text_unit(const MdbTextAttnArgs& a, int unit
     return {u.x, u.y, u.z};
   }
   const int lane = threadIdx.x & 31;
-  int first = lane < a.B ? text_row_within(a, lane) : 0, end = lane < a.B ? text_row_within(a, lane + 1) : 0;
-  if (__any_sync(0xffffffffu, end < first)) {
-    const int last = __shfl_sync(0xffffffffu, end, a.B - 1);
-#pragma unroll 1
-    for (int m = 1; m < 32; m <<= 1) first = max(first, __shfl_up_sync(0xffffffffu, first, m));      // a lane that has none below it reads itself
-    end = min(max(end, first), last);
-    first = min(first, last);
-    if (lane == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
-  }
-  const int rows = lane < a.B ? end - first : 0, n = (rows + gran - 1) / gran;
+  const int first = lane < a.B ? text_row_within(a, lane) : 0;
+  int rows = lane < a.B ? text_row_within(a, lane + 1) - first : 0;
+  if (__any_sync(0xffffffffu, rows < 0)) rows = 0;
+  const int n = (rows + gran - 1) / gran;
   const auto from = [&](int level) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - level, 0)))); };      // blocks of this number or a larger one
   int lo = 0, hi = __reduce_max_sync(0xffffffffu, n);      // from(lo) > unit >= from(hi)
   if (unit >= from(0)) return {0, 0, 0};
@@ -91,9 +85,16 @@ constexpr int TXT_FEW_SEQUENCES = 32;
 inline bool text_is_fine(const MdbTextAttnArgs& a) { return a.cu != nullptr && (a.window <= 128 || a.Sq / a.B <= (a.sink_logits != nullptr ? 256 : 128)); }
 int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st);
 
-// rows before the first sequence and behind the last one, in turn
+// rows before the first sequence and behind the last one, in turn, or all rows where ends fall, which is reported; by whole warps
 template <typename F> __device__ __forceinline__ void text_rows_of_none(const MdbTextAttnArgs& a, int from, int step, F f) {
-  const int last = text_row_within(a, a.B), first = min(text_row_within(a, 0), last), n = first + a.Sq - last;
+  const int lane = threadIdx.x & 31;
+  int first = text_row_within(a, 0), last = text_row_within(a, a.B);
+  const bool fell = a.units != nullptr ? a.units[0].w < 0 : lane < a.B && text_row_within(a, lane + 1) < text_row_within(a, lane);
+  if (__any_sync(0xffffffffu, fell)) {
+    if (lane == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
+    first = last = 0;
+  }
+  const int n = first + a.Sq - last;
   for (int i = from; i < n; i += step) f(i < first ? i : i - first + last);
 }
 

@@ -157,8 +157,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Sequence b has the rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32 [B + 1], not falling, on the tensors' device; a length may be zero), and its row i sees its rows
     j with ``j <= i`` and ``i - j < window`` (None: all earlier ones). Query head h reads key / value head ``h // (H // Hkv)``; ``sink_logits`` [H] take part in each row's
     softmax and carry no value. What other sequences hold does not count, NaN neither; rows of no sequence are not read, their output is zero and has no gradient.
-    Ends outside the rows or falling ones are an error on the CPU; the kernels hold ends within the rows, and where they fall the largest so far counts, none passes the
-    last one, and ``ops.check_status`` reports it.
+    Ends outside the rows or falling ones are an error on the CPU; the kernels hold ends within the rows, and where they fall no sequence is seen: all is zero, and
+    ``ops.check_status`` reports it.
     Differentiable in q, k, v and sink_logits, once; with a gradient wanted, rows that see few keys may be rounded less, for it is a difference of nearly equal terms.
     """
     name = "packed_attention"

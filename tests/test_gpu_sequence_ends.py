@@ -1,4 +1,4 @@
-"""Ends of packed sequences that fall, or lie outside the rows: sequences stay disjoint and within the rows, and the call is reported."""
+"""Ends of packed sequences that fall, or lie outside the rows: an append keeps sequences disjoint and within the rows, attention has none where they fall; such calls are reported."""
 import pytest
 import torch
 
@@ -66,23 +66,26 @@ def test_packed_attention(cu, scale, H, G, D):
     q, k, v, grad, sink = _normal(T, H, D, seed=1), _normal(T, G, D, seed=2), _normal(T, G, D, seed=3), _normal(T, H, D, seed=4), _normal(H, seed=5)
     O.check_status()
 
-    def reports(ends):
-        inside = [min(max(c, 0), T) for c in ends]
-        if inside != sorted(inside):
+    inside = [min(max(c, 0), T) for c in cu]
+    falls = inside != sorted(inside)
+
+    def reports(bad):
+        if bad:
             with pytest.raises(RuntimeError, match="BOUNDS"):
                 O.check_status()
         O.check_status()
 
     found = []
-    for ends in (held(cu, T), cu):
+    for ends in (inside, cu):
         leaves = [t.clone().requires_grad_() for t in (q, k, v, sink)]
         with torch.no_grad():
             alone = O.packed_attention(*leaves[:3], _ints(ends), sink_logits=leaves[3])
-        reports(ends)
+        reports(falls)
         out = O.packed_attention(*leaves[:3], _ints(ends), sink_logits=leaves[3])
-        reports(ends)
+        reports(falls)
         grads = torch.autograd.grad(out, leaves, grad)
-        reports(ends)
+        reports(falls)
         found.append((alone, out, *grads))
     for a, b in zip(*found):
         assert torch.equal(a, b) and torch.isfinite(b).all()
+        assert not (falls and b.any())
