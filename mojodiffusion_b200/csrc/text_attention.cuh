@@ -78,11 +78,13 @@ __device__ __forceinline__ TextUnit text_unit_of_keys(const MdbTextAttnArgs& a, 
 // how many units there may be
 inline long long text_units(const MdbTextAttnArgs& a, int gran) { return a.Sq / gran + static_cast<long long>(a.B); }
 constexpr int TXT_FEW_SEQUENCES = 32;
-// Packed and with gradients: whether sequences or windows are short on average. Rows of few keys then make up the result, and the rounding of probabilities and of ds shows in it: P
-// near 1/2 is off by up to 2^-8 of itself where the result's own rounding is off by 2^-9.3 on average, and ds = p (dp - do . o) is a difference of nearly equal terms. They go into their
-// products as two bf16 terms. Relative errors against 64 bits with one term / with two: dq of 23 sequences of two or three tokens 0.0026 / 0.0017, of three with a window of 2 0.0030 / 0.0017; 40 x 128 rows,
-// 32 / 8 heads of 128, 0.0024 / 0.0017, which takes 232 us for a training step instead of 218. Sink logits add up do . o, so they have twice the limit.
-inline bool text_is_fine(const MdbTextAttnArgs& a) { return a.cu != nullptr && (a.window <= 128 || a.Sq / a.B <= (a.sink_logits != nullptr ? 256 : 128)); }
+// Packed and with gradients: whether the rows of a sequence have few keys. The rounding of their probabilities and of ds shows most in the result: P near 1/2 is off by up to
+// 2^-8 of itself where the result's own rounding is off by 2^-9.3 on average, and ds = p (dp - do . o) is a difference of nearly equal terms. They go into their
+// products as two bf16 terms. The sequence alone decides, so that a result's rounding does not depend on what else is packed. Relative errors of dq against 64 bits with one term / with two:
+// sequences of two or three tokens 0.0026 to 0.0030 / 0.0017, of 200 0.0024 / 0.0017, of 1500 0.0024 / 0.0017, where two would take a training step of nine sequences of 20 to 1531
+// (32 / 8 heads of 128) from 413 us to 484; 40 sequences of 128 223 us with two terms, 205 with one; 1500 and 1000 with a window of 200 186 and 168.
+constexpr int TXT_FEW_ROWS = 256, TXT_SHORT_WINDOW = 128;
+__device__ __forceinline__ bool text_is_fine(const MdbTextAttnArgs& a, int rows) { return rows <= TXT_FEW_ROWS || a.window <= TXT_SHORT_WINDOW; }
 int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st);
 
 // rows before the first sequence and behind the last one, in turn, or all rows where ends fall, which is reported; by whole warps

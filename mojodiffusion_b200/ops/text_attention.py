@@ -159,7 +159,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     softmax and carry no value. What other sequences hold does not count, NaN neither; rows of no sequence are not read, their output is zero and has no gradient.
     Ends outside the rows or falling ones are an error on the CPU; the kernels hold ends within the rows, and where they fall no sequence is seen: all is zero, and
     ``ops.check_status`` reports it.
-    Differentiable in q, k, v and sink_logits, once; with a gradient wanted, rows that see few keys may be rounded less, for it is a difference of nearly equal terms.
+    Differentiable in q, k, v and sink_logits, once; with a gradient wanted, sequences of up to 256 rows and windows of up to 128 are rounded less, for it is a difference of nearly equal terms.
     """
     name = "packed_attention"
     if window is None:
