@@ -33,11 +33,10 @@ __global__ void __launch_bounds__(TU_THREADS) text_units_kernel(const __grid_con
   __shared__ int2 rows_of[TU_THREADS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   bool falls = false;
-  for (int b = threadIdx.x; b < a.B; b += TU_THREADS) falls = falls || text_row_within(a, b + 1) < text_row_within(a, b);
-  const int sequences = __syncthreads_or(falls) ? 0 : a.B;      // where ends fall there is no unit, and the first place says so
   int before = 0;
-  for (int b0 = 0; b0 < sequences; b0 += TU_THREADS) {
-    const int b = b0 + threadIdx.x, first = b < a.B ? text_row_within(a, b) : 0, rows = b < a.B ? text_row_within(a, b + 1) - first : 0, n = (rows + gran - 1) / gran;
+  for (int b0 = 0; b0 < a.B; b0 += TU_THREADS) {
+    const int b = b0 + threadIdx.x, first = b < a.B ? text_row_within(a, b) : 0, rows = b < a.B ? text_row_within(a, b + 1) - first : 0, n = max(rows + gran - 1, 0) / gran;
+    falls = falls || rows < 0;
     int upto = n;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -57,11 +56,12 @@ __global__ void __launch_bounds__(TU_THREADS) text_units_kernel(const __grid_con
     __syncthreads();
     for (int i = warp; i < TU_THREADS && b0 + i < a.B; i += TU_THREADS / 32) {
       const int blocks = (rows_of[i].y + gran - 1) / gran;
-      for (int k = lane; k < blocks && at[i] + k < units; k += 32) a.units[at[i] + k] = make_int4(rows_of[i].x, rows_of[i].y, blocks - 1 - k, b0 + i);
+      for (int k = lane; k < blocks && static_cast<unsigned>(at[i] + k) < static_cast<unsigned>(units); k += 32) a.units[at[i] + k] = make_int4(rows_of[i].x, rows_of[i].y, blocks - 1 - k, b0 + i);
     }
     before += all;
   }
-  for (int i = before + threadIdx.x; i < units; i += TU_THREADS) a.units[i] = make_int4(0, 0, 0, sequences == 0 ? -1 : 0);
+  const bool none = __syncthreads_or(falls);      // where ends fall there is no unit, and the first place says so
+  for (int i = (none ? 0 : before) + threadIdx.x; i < units; i += TU_THREADS) a.units[i] = make_int4(0, 0, 0, none ? -1 : 0);
 }
 int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st) {
   if (a.units == nullptr) return 0;

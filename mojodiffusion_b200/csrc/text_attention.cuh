@@ -87,14 +87,16 @@ constexpr int TXT_FEW_ROWS = 256, TXT_SHORT_WINDOW = 128;
 __device__ __forceinline__ bool text_is_fine(const MdbTextAttnArgs& a, int rows) { return rows <= TXT_FEW_ROWS || a.window <= TXT_SHORT_WINDOW; }
 int text_make_units(const MdbTextAttnArgs& a, int gran, cudaStream_t st);
 
-// rows before the first sequence and behind the last one, in turn, or all rows where ends fall, which is reported; by whole warps
-template <typename F> __device__ __forceinline__ void text_rows_of_none(const MdbTextAttnArgs& a, int from, int step, F f) {
-  const int lane = threadIdx.x & 31;
+// rows before the first sequence and behind the last one, in turn; by whole warps. Where ends fall there are no units, so a CTA that had one need not look: then all rows, and a report.
+template <typename F> __device__ __forceinline__ void text_rows_of_none(const MdbTextAttnArgs& a, bool look, int from, int step, F f) {
   int first = text_row_within(a, 0), last = text_row_within(a, a.B);
-  const bool fell = a.units != nullptr ? a.units[0].w < 0 : lane < a.B && text_row_within(a, lane + 1) < text_row_within(a, lane);
-  if (__any_sync(0xffffffffu, fell)) {
-    if (lane == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
-    first = last = 0;
+  if (look) {
+    const int lane = threadIdx.x & 31;
+    const bool fell = a.units != nullptr ? a.units[0].w < 0 : lane < a.B && text_row_within(a, lane + 1) < text_row_within(a, lane);
+    if (__any_sync(0xffffffffu, fell)) {
+      if (lane == 0) report_status(a.status, STATUS_BOUNDS, 187, a.B);
+      first = last = 0;
+    }
   }
   const int n = first + a.Sq - last;
   for (int i = from; i < n; i += step) f(i < first ? i : i - first + last);

@@ -125,8 +125,8 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   TextUnit of = {0, KEYS ? a.Skv : a.Sq, block};
   if (PACKED) of = KEYS ? text_unit_of_keys(a, unit, TR) : text_unit(a, unit, TR);
   const int base = of.base, r0 = of.block * TR, out_rows = of.rows, Sq = PACKED ? of.rows : a.Sq;
-  const auto clear_rows = [&](int t, int threads) {      // packed, rows of no sequence: gradients of zero
-    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int line) {
+  const auto clear_rows = [&](bool look, int t, int threads) {      // packed, rows of no sequence: gradients of zero
+    text_rows_of_none(a, look, blockIdx.x, gridDim.x, [&](int line) {
       for (int e = t; e < DH / 8; e += threads) {
         const auto clear = [&](void* to, const long long* st) { *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(to) + line * st[1] + blockIdx.y * st[2] + e * 8) = make_uint4(0, 0, 0, 0); };
         if (!KEYS) {
@@ -141,7 +141,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
   };
   const bool fine = PACKED && text_is_fine(a, of.rows);
   if (PACKED && of.rows == 0) {      // no such unit
-    clear_rows(threadIdx.x, TB_THREADS);
+    clear_rows(true, threadIdx.x, TB_THREADS);
     return;
   }
   TextSight sight;
@@ -542,7 +542,7 @@ text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant_
     }
   }
 
-  if (PACKED && warp >= 2) clear_rows(threadIdx.x - 64, 256);
+  if (PACKED && warp >= 2) clear_rows(false, threadIdx.x - 64, 256);
 
   tc_fence_before();
   __syncthreads();

@@ -170,8 +170,8 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   const int step = ONE || RANGE ? 1 : gridDim.x;
   TextItem<DH, BIAS, PACKED, FINE> w;
 
-  const auto clear_rows = [&](int thread, int threads) {      // packed, rows of no sequence: zero, and no gradient
-    text_rows_of_none(a, blockIdx.x, gridDim.x, [&](int row) {
+  const auto clear_rows = [&](bool look, int thread, int threads) {      // packed, rows of no sequence: zero, and no gradient
+    text_rows_of_none(a, look, blockIdx.x, gridDim.x, [&](int row) {
       for (int e = thread; e < a.H * (DH / 8); e += threads) {
         const long long to = row * a.o_strides[1] + e / (DH / 8) * a.o_strides[2] + e % (DH / 8) * 8;
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.o) + to) = make_uint4(0, 0, 0, 0);
@@ -184,7 +184,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
   if (PACKED && ONE) {
     only = text_unit(a, first / (a.H >> tiles.heads_log), tiles.blocks * TQ);
     if (only.rows == 0) {
-      clear_rows(threadIdx.x, Shape::THREADS);
+      clear_rows(true, threadIdx.x, Shape::THREADS);
       return;
     }
   }
@@ -532,7 +532,7 @@ text_fwd_kernel(const __grid_constant__ TextMaps maps, const __grid_constant__ M
       if (a.lse != nullptr && row0 + lane < rows)
         a.lse[(static_cast<long long>(batch) * a.H + head) * a.Sq + base + row0 + lane] = m_used == -INFINITY || l_run == 0.f ? INFINITY : m_used + log2f(l_run);
     }
-    if (PACKED) clear_rows(threadIdx.x - Shape::SOFT * 32, 256);
+    if (PACKED) clear_rows(!ONE, threadIdx.x - Shape::SOFT * 32, 256);
     if (!ok && lane == 0) report_status(a.status, STATUS_TIMEOUT, 131 + t, done);
   }
 
