@@ -8,7 +8,9 @@
 // rounded, what was there is brought to it by the same block, and every element has one writer.
 //
 // What bounds it: memory, and the latency of its loads. 11.3 thousand tokens of sixteen prompts, 32 / 8 heads of 128, e4m3: 53 us a pass, 4.9 TB/s of what has to move (0.75 of the
-// measured rate; 32 warps to an SM, issue slots 48 %). With 80 registers and 24 warps 63.5 us instead of 62.3, with four heads held in fp32 (168 registers) 178. A token of each of 128 sequences: 7 us.
+// measured rate; 32 warps to an SM, issue slots 48 %). With 80 registers and 24 warps 63.5 us instead of 62.3, with four heads held in fp32 (168 registers) 178.
+// At 64 registers, with which 32 warps fit, the forms of one or two rows to a group spill 100 to 244 bytes: the queries' path, with two rows and their angles, and the keys' share them.
+// A token of each of 128 sequences: 7 us.
 //
 // A row (one head of one token) is held by Dh / 16 lanes, each with 8 values of either half: the halves of a rotated pair meet in one thread, the sum of squares takes
 // two or three shuffles, and loads and stores are 16 bytes a lane.
@@ -223,7 +225,7 @@ template <int DH> __device__ __forceinline__ void clear_rows_of_none(const MdbPa
 // grid: units, then rows of no sequence; parts of the heads: of the queries, of the keys, of the values. Finding the unit and its page takes as long as a
 // few heads, so a block has several of them. Queries are turned one row of a group of lanes after the other, two heads at a time; of keys and values a block needs a head's rows
 // of the whole unit at once, for its scale. Where a page has fewer rows than the block has groups of lanes, the groups share out the heads
-// (TEAMS; 11.3 thousand tokens in pages of 16, e4m3: 28 / 4 heads of 64 61 -> 39 us, 32 / 8 of 128 92 -> 78; its registers would cost larger pages a tenth).
+// (TEAMS; 11.3 thousand tokens in pages of 16, e4m3: 28 / 4 heads of 64 61 -> 39 us, 32 / 8 of 128 92 -> 76; its registers would cost larger pages a tenth).
 struct AppendGrid {
   int units, q_heads, kv_heads;      // heads of a block
 };

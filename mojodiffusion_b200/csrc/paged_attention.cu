@@ -22,9 +22,10 @@
 //
 // Keys behind the sequence's end are masked and their values zeroed in shared memory before the product (0 * NaN is not 0).
 //
-// What bounds it: memory where sequences are long. 4 tokens over 70001 to 131072 positions, 32 / 8 heads of 128, e4m3: 129 us, 5.95 TB/s (0.91 of the measured rate; bf16, 16 over 16384: 183 us, 5.86 TB/s). 32 over 0 to 16384:
-// 79 us, 4.6 TB/s: 12000 cycles to a CTA's first tile (lengths, table, scales and data one after the other), then 3200 a tile of which it works 1300. Few rows leave latencies: one token over 300
-// positions 7 us on the device. With more than 16 rows the turns of a warp: 40 rows over bf16 pages, heads of 64, 5600 cycles a tile of 128 keys, 26 us for 8 sequences of 17 to 4091.
+// What bounds it: memory where sequences are long. 4 tokens over 70001 to 131072 positions, 32 / 8 heads of 128, e4m3: 129 us, 5.95 TB/s (0.91 of the measured rate; bf16, 16 over 16384: 182 us, 5.9 TB/s). 32 over 0 to 16384:
+// 82 us, 4.4 TB/s: 12000 cycles to a CTA's first tile (lengths, table, scales and data one after the other), then 3200 a tile of which it works 1300. Few rows leave latencies: one token over 300
+// positions 7 us on the device. With more than 16 rows the turns of a warp: 40 rows over bf16 pages, heads of 64, 5600 cycles a tile of 128 keys, 27 us for 8 sequences of 17 to 4091; 32 rows over 8 bits, heads of 128,
+// 8 sequences of 4000, 46 us.
 // Keys as the rows of the products (S^T) took 131 us in the first case where the queries' as rows took 169, for up to 8 rows fill half of 16.
 #include "gemm_api.h"
 #include "paged.cuh"

@@ -73,7 +73,7 @@ template <int DH, bool KEYS, bool BIAS> struct TextBwdShape {
 };
 
 // PACKED: in sequences whose rows have few keys (see text_is_fine) P and dS go into their products as two bf16 terms, the second one in the columns of the scores that the first leaves free.
-// A block is a unit of 128 rows of one sequence. 4996 rows in nine sequences of 20 to 1531, 32 / 8 heads of 128: dq 141 us, dk and dv 188 (tensor pipe 29 and 42 %)
+// A block is a unit of 128 rows of one sequence. 4996 rows in nine sequences of 20 to 1531, 32 / 8 heads of 128: dq 134 us, dk and dv 185 (tensor pipe 30 and 42 %)
 template <int DH, bool KEYS, bool BIAS, bool PACKED>
 __global__ void __launch_bounds__(TB_THREADS, TextBwdShape<DH, KEYS, BIAS>::CTAS)
 text_bwd_kernel(const __grid_constant__ TextBwdMaps maps, const __grid_constant__ MdbTextAttnArgs a, const TextParts parts) {

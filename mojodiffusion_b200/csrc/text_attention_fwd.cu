@@ -20,12 +20,14 @@
 //
 // Rows of V that no row of the CTA sees are zeroed in shared memory before the product, for 0 * NaN is not 0.
 //
+// Probabilities go into their product as one bf16 term: they are off by 2^-9 of themselves at most, each in its own direction, as much as the output's own rounding (relative errors against 64
+// bits 0.0020 with one term, 0.0016 with two or with fp32). A second term is a second product of the same size: six prompts (below) would take 361 us instead of 268, captions 39.3 instead of 36.5.
 // FINE (packed, with a backward pass to come): in sequences whose rows have few keys (see text_is_fine) a probability goes into its product as two bf16 terms, the second one in the half of
 // the scores' columns that the first leaves free.
 //
 // PACKED: an item is a unit of one sequence (see text_unit); coordinates and rows count from the sequence's first row. A tile holds rows of one sequence only, at the cost of tiles that are
 // not full: rows of several sequences in a tile would multiply each other's values by zero, and 0 * NaN would carry one sequence's NaN into another. 10155 tokens in six sequences of 301
-// to 4096, 32 / 8 heads of 128: 264 us (872 TFLOP/s; equal lengths take 1.01 to 1.05 of the batched form's time); 16 sequences of 7 to 300, 64 / 8 heads of 64, window 128: 33 us,
+// to 4096, 32 / 8 heads of 128: 294 us among other passes, 268 by itself (784 and 860 TFLOP/s; equal lengths take 1.01 to 1.05 of the batched form's time; 396 bytes spilled, 340 without sequences); 16 sequences of 7 to 300, 64 / 8 heads of 64, window 128: 33 us,
 // a CTA with one key tile 6.7 us of which 2.6 before its first scores.
 //
 // What bounds it: the latency of a tile's way from the scores through the softmax to the next product; no unit is busy half of the time. 8192 tokens,
