@@ -89,3 +89,67 @@ def test_packed_attention(cu, scale, H, G, D):
     for a, b in zip(*found):
         assert torch.equal(a, b) and torch.isfinite(b).all()
         assert not (falls and b.any())
+
+
+@pytest.mark.parametrize("B", [20, 45])
+def test_captured_training_step_follows_the_ends(B):
+    """A captured step replayed with other ends, falling ones among them: what an eager call gives."""
+    T, H, G, D = 700, 4, 2, 128
+    q, k, v, grad = (_normal(T, n, D, seed=n + i) for i, n in enumerate((H, G, G, H)))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=DEV)
+
+    def step():
+        out = O.packed_attention(*leaves, cu)
+        return (out.detach(), *torch.autograd.grad(out, leaves, grad))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    O.check_status()
+    g = torch.Generator().manual_seed(3)
+    for n in range(12):
+        ends = torch.sort(torch.randint(0, T + 1, (B + 1,), generator=g)).values.int()
+        if n % 4 == 1:
+            ends = torch.where(torch.rand(B + 1, generator=g) < 0.7, 650, ends).sort().values.int()      # a long one and short ones
+        if n % 4 == 3:
+            ends[B // 2] = 0
+            ends[0] = 1
+        cu.copy_(ends)
+        graph.replay()
+        if n % 4 == 3:
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+        O.check_status()
+        want = step()
+        if n % 4 == 3:
+            with pytest.raises(RuntimeError, match="BOUNDS"):
+                O.check_status()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), n
+
+
+def test_many_sequences_on_several_streams():
+    """Each call has its own list of units."""
+    cases = []
+    for i in range(3):
+        lengths = [(j * (7 + i)) % 60 for j in range(40 + 300 * i)]
+        cu = _ints([sum(lengths[:j]) for j in range(len(lengths) + 1)])
+        cases.append((*(_normal(sum(lengths), n, 64, seed=10 * i + n) for n in (4, 2)), _normal(sum(lengths), 2, 64, seed=10 * i + 9), cu))
+    want = [O.packed_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(10):
+        got = []
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(O.packed_attention(*c))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    O.check_status()
