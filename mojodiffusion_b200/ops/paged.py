@@ -113,7 +113,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     The pages of sequence b hold ``kv_len[b]`` positions (int32 [B]), those of the queries among them: query row i stands at position kv_len[b] - Sq + i and sees
     the keys up to its own position. Query head h reads key head ``h // (H // Hkv)``. A row before the first position is zero. ``max_len`` (int): no sequence is longer, and
     what lies behind is not seen; parts of prompts take a workspace of this size (all that the table has room for by default). Slots behind a sequence's
-    end are not read: they may hold anything. A value of infinity that a query sees gives NaN.
+    end are not read: they may hold anything. A value of infinity that a query sees gives NaN, and a value that is not finite may reach the other queries of its sequence in the same call.
     """
     if max_len is not None and (type(max_len) is not int or max_len < 0):
         raise ValueError("paged_attention: max_len must be an int of at least 0")
